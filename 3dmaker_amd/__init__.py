@@ -19,11 +19,19 @@ LIB_PATH = os.path.join(_HERE, "lib3dmaker_amd.so")
 
 __all__ = [
     "LIB_PATH", "lib", "launch", "MLPOption", "MLPGridOptions", "HashGrid", "Net",
-    "OUT_ACT_NONE", "OUT_ACT_SIGMOID", "ptr", "check", "Float3", "Uint3", "NerfOptions", "Nerf", "NerfTrainer", "NtrConfig", "NtrStats",
+    "OUT_ACT_NONE", "OUT_ACT_SIGMOID", "ptr", "check", "RouteOption", "Fp8QuantOption", "Fp8ProductOption", "NormGateOption",
+    "DATA_F32", "DATA_F16", "DATA_BF16", "ROUTE_SOFTMAX", "ROUTE_SIGMOID", "PRODUCT_DENSE", "PRODUCT_ROWS", "PRODUCT_SUM",
+    "NORM_NONE", "NORM_RMS", "NORM_LAYER", "fp8_pitch", "fp8_scale_pitch", "Float3", "Uint3", "NerfOptions", "Nerf", "NerfTrainer", "NtrConfig", "NtrStats",
 ]
 
 OUT_ACT_NONE = 0
 OUT_ACT_SIGMOID = 1
+
+# include/experts_abi.h
+DATA_F32, DATA_F16, DATA_BF16 = 0, 1, 2
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
+PRODUCT_DENSE, PRODUCT_ROWS, PRODUCT_SUM = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 
 
 class MLPOption(C.Structure):
@@ -95,6 +103,44 @@ class NtrStats(C.Structure):
                 ("lr", C.c_float), ("epochs", C.c_float), ("msPerStep", C.c_float), ("etaSeconds", C.c_float)]
 
 
+class RouteOption(C.Structure):
+    """include/experts_abi.h RouteOption"""
+    _fields_ = [("numExperts", C.c_int), ("topK", C.c_int), ("scoreType", C.c_int), ("numGroups", C.c_int),
+                ("topGroups", C.c_int), ("groupScore", C.c_int), ("renormalize", C.c_int), ("scale", C.c_float),
+                ("logitsType", C.c_int)]
+
+
+class Fp8QuantOption(C.Structure):
+    """include/experts_abi.h Fp8QuantOption"""
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("batch", C.c_int), ("blockRows", C.c_int), ("srcType", C.c_int),
+                ("slotsPerRow", C.c_int), ("srcRows", C.c_int), ("srcStride", C.c_longlong),
+                ("srcBatchStride", C.c_longlong), ("gateStride", C.c_longlong)]
+
+
+class Fp8ProductOption(C.Structure):
+    """include/experts_abi.h Fp8ProductOption"""
+    _fields_ = [("m", C.c_int), ("n", C.c_int), ("k", C.c_int), ("numExperts", C.c_int), ("grouping", C.c_int),
+                ("scaleRowsB", C.c_int), ("activation", C.c_int), ("outType", C.c_int), ("outStride", C.c_longlong)]
+
+
+class NormGateOption(C.Structure):
+    """include/experts_abi.h NormGateOption"""
+    _fields_ = [("dim", C.c_int), ("postNorm", C.c_int), ("preNorm", C.c_int), ("gateRows", C.c_int),
+                ("residualScale", C.c_float), ("blockScale", C.c_float), ("epsilon", C.c_float), ("dataType", C.c_int),
+                ("strideX", C.c_longlong), ("strideF", C.c_longlong), ("strideGate", C.c_longlong),
+                ("strideY", C.c_longlong), ("strideH", C.c_longlong)]
+
+
+def fp8_pitch(cols: int) -> int:
+    """Bytes between the rows of an 8-bit matrix of `cols` columns (include/experts_abi.h)."""
+    return -(-cols // 128) * 128
+
+
+def fp8_scale_pitch(cols: int) -> int:
+    """Scale bytes between its rows of blocks."""
+    return -(-fp8_pitch(cols) // 512) * 4
+
+
 class StepBuffers(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in (
         "num_steps", "ray_offsets", "positions", "ray_indices", "t_sorted", "density_out", "color_input",
@@ -108,6 +154,7 @@ class RefreshBuffers(C.Structure):
         [("last_count", C.c_int), ("density_stride", C.c_int), ("density_order", C.c_void_p)]
 
 
+_ll = C.c_longlong
 _vp, _i, _f, _u = C.c_void_p, C.c_int, C.c_float, C.c_uint
 _u32 = C.c_uint32
 
@@ -129,6 +176,17 @@ SIGNATURES = {
     "launchHashTableBackwardKernelNoAlloc": (None, [_vp, _vp, _vp, _i, _i, _i, _f, _i, _i, _vp]),
     "launchAdamHashGridOptim": (None, [_vp, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _f, _f, _f, _vp]),
     "launchHashEncodeKernel": (None, [_vp, _vp, _vp, _i, _vp, _i, _vp]),
+    # include/experts_abi.h (mixture-of-experts block)
+    "launchRouteExperts": (None, [_vp, _vp, _ll, _vp, _vp, _vp, _i, _vp]),
+    "launchRouteExpertsBackward": (None, [_vp, _vp, _ll, _vp, _vp, _vp, _ll, _i, _vp]),
+    "routePlanCapacity": (_ll, [_i, _i, _i, _i]),
+    "launchRoutePlan": (None, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "launchFp8Quantize": (None, [_vp] * 10),
+    "launchFp8Product": (None, [_vp] * 8),
+    "launchExpertCombine": (None, [_i, _i, _vp, _i, _ll, _vp, _vp, _vp, _ll, _i, _i, _vp]),
+    "launchExpertCombineBackward": (None, [_i, _i, _vp, _i, _ll, _vp, _vp, _ll, _vp, _i, _i, _vp]),
+    "launchNormGateResidual": (None, [_vp] * 10 + [_i, _vp]),
+    "launchNormGateResidualBackward": (None, [_vp] * 17 + [_i, _vp]),
     "tinymlp_last_error": (_i, []),
     "tinymlp_last_error_message": (C.c_char_p, []),
     # include/tinymlp_capi.h (flat handle API)

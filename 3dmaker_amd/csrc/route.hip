@@ -1,0 +1,662 @@
+// Routing of tokens to experts and the plan of the experts' rows, for gfx950.
+//
+//   s = softmax(z) or sigmoid(z),  c = s + b;  the best groups by c, then the
+//   k largest c in them, ties to the lowest index;  w = scale s / (sum s + 1e-20)
+//
+// A token lies on LPT lanes of a wave, every group of experts on LG of them,
+// a lane's V experts next to each other, so that lane order is index order: the
+// largest key of all lanes by a butterfly, then the lowest lane that has it and
+// that lane's first place with it are the lowest index.
+#include "experts.h"
+#include "lanes.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace graft {
+
+namespace {
+
+constexpr int kRouteThreads = 256;
+constexpr int kMaxExperts = 1024;
+
+struct RouteArgs {
+    const void* logits;
+    long long stride;
+    const float* bias;
+    int* indices;
+    float* weights;
+    int tokens, experts, topk, groups, kept, group_size, lanes_group, group_best;
+    int type;
+    bool sigmoid, renorm, vec;
+    float scale;
+    // backward
+    const float* dweights;
+    void* dlogits;
+    long long dstride;
+};
+
+// Larger float, larger integer; 0 is below every number (an unavailable expert).
+__device__ __forceinline__ uint32_t key_of(float c)
+{
+    const uint32_t u = __builtin_bit_cast(uint32_t, c);
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+
+__device__ __forceinline__ float of_key(uint32_t k)
+{
+    return __builtin_bit_cast(float, k ^ ((k & 0x80000000u) ? 0x80000000u : 0xffffffffu));
+}
+
+// e^x for x <= 0 to about an ulp: 2^t with the rounding error of t = x log2(e)
+// put back (t's error alone would be |x| ulps).  Below e^-100 it is 0.
+__device__ __forceinline__ float exp_neg(float x)
+{
+    x = fmaxf(x, -120.0f);
+    const float t = x * 1.44269504f;
+    const float r = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, r * 0.693147181f, e);
+}
+
+template <class T, int V>
+__device__ __forceinline__ void load_v(float (&z)[V], const T* p, int n, bool vec)
+{
+    if (vec) {
+        constexpr int N = 16 / sizeof(T) < V ? 16 / sizeof(T) : V;
+#pragma unroll
+        for (int i = 0; i < V; i += N) {
+            const Vec<T, N> v = *reinterpret_cast<const Vec<T, N>*>(p + i);
+#pragma unroll
+            for (int j = 0; j < N; j++) z[i + j] = (float)v[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) z[i] = i < n ? (float)p[i] : 0.0f;
+    }
+}
+
+// The lane's V logits: experts first .. first + n of the token (others and
+// unavailable ones: live bit 0).
+template <int V>
+__device__ __forceinline__ uint32_t load_logits(float (&z)[V], const RouteArgs& a, int token, int first, int n)
+{
+    if (n > 0) {
+        const long long at = (long long)token * a.stride + first;
+        if (a.type == DATA_F32) load_v(z, (const float*)a.logits + at, n, a.vec);
+        else if (a.type == DATA_F16) load_v(z, (const _Float16*)a.logits + at, n, a.vec);
+        else load_v(z, (const __bf16*)a.logits + at, n, a.vec);
+    }
+    uint32_t live = 0;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const bool ok = i < n && z[i] > -INFINITY;  // false for NaN
+        live |= ok ? 1u << i : 0u;
+        z[i] = ok ? fminf(z[i], 3.402823466e38f) : 0.0f;
+    }
+    return live;
+}
+
+// Scores of the lane's experts (0 where not live).  For the sigmoid q is 1 - s.
+template <int V, int LPT>
+__device__ __forceinline__ void scores_of(float (&s)[V], const float (&z)[V], uint32_t live, bool sigmoid)
+{
+    if (sigmoid) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float t = exp_neg(-fabsf(z[i]));
+            const float r = __builtin_amdgcn_rcpf(1.0f + t);
+            s[i] = live >> i & 1 ? (z[i] >= 0.0f ? r : t * r) : 0.0f;
+        }
+    } else {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < V; i++) m = live >> i & 1 ? fmaxf(m, z[i]) : m;
+        m = lanes_max<LPT>(m);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            s[i] = live >> i & 1 ? exp_neg(z[i] - m) : 0.0f;
+            sum += s[i];
+        }
+        sum = lanes_sum<LPT>(sum);
+        const float r = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; i++) s[i] *= r;
+    }
+}
+
+// Lanes of the token below this one that are set in the wave's mask.
+template <int LPT>
+__device__ __forceinline__ bool first_of(uint64_t mask, int lane)
+{
+    const uint64_t below = (1ull << lane) - 1;
+    const uint64_t token = LPT == 64 ? ~0ull : ((1ull << LPT) - 1) << (lane & ~(LPT - 1));
+    return (mask & token & below) == 0;
+}
+
+template <int V, int LPT>
+__global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a)
+{
+    constexpr int kTokens = kRouteThreads / LPT;
+    constexpr int kPicked = V == 4 ? 1024 : kTokens * 32;  // at most min(LPT V, 32) slots a token
+    __shared__ int picked_i[kPicked];
+    __shared__ float picked_s[kPicked];
+    __shared__ uint32_t group_key[kRouteThreads];
+    const int lane = threadIdx.x & 63, sub = threadIdx.x & (LPT - 1), local = threadIdx.x / LPT;
+    const int token = blockIdx.x * kTokens + local;
+    const int group = sub / a.lanes_group, in_group = (sub & (a.lanes_group - 1)) * V;
+    const int first = group * a.group_size + in_group;
+    const int n = token < a.tokens && group < a.groups ? min(V, a.group_size - in_group) : 0;
+    float z[V], s[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) z[i] = 0.0f;
+    uint32_t live = load_logits(z, a, token, first, n);
+    scores_of<V, LPT>(s, z, live, a.sigmoid);
+    uint32_t key[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const float c = s[i] + (a.bias && i < n ? a.bias[first + i] : 0.0f);
+        key[i] = (live >> i & 1) && c > -INFINITY ? key_of(c) : 0u;
+    }
+    if (a.groups > 1) {
+        uint32_t b1 = 0, b2 = 0;  // keys of the best two
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            b2 = max(b2, min(b1, key[i]));
+            b1 = max(b1, key[i]);
+        }
+        for (int w = 1; w < a.lanes_group; w <<= 1) {
+            const uint32_t o1 = __shfl_xor(b1, w), o2 = __shfl_xor(b2, w);
+            b2 = max(min(b1, o1), max(b2, o2));
+            b1 = max(b1, o1);
+        }
+        uint32_t g = b1;
+        if (a.group_best == 2 && b2 != 0) g = key_of(of_key(b1) + of_key(b2));
+        if ((sub & (a.lanes_group - 1)) == 0) group_key[local * LPT + group] = g;
+        __syncthreads();
+        int ahead = 0;
+        for (int o = 0; o < a.groups; o++) {
+            const uint32_t k = group_key[local * LPT + o];
+            ahead += k > g || (k == g && o < group);
+        }
+        if (ahead >= a.kept) {
+#pragma unroll
+            for (int i = 0; i < V; i++) key[i] = 0;
+        }
+    }
+    for (int j = 0; j < a.topk; j++) {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < V; i++) best = max(best, key[i]);
+        const uint32_t top = lanes_umax<LPT>(best);
+        const bool mine = best == top && top != 0;
+        const uint64_t mask = __ballot(mine);
+        if (mine && first_of<LPT>(mask, lane)) {
+            int at = 0;
+            float sc = 0.0f;
+#pragma unroll
+            for (int i = V - 1; i >= 0; i--) {
+                const bool here = key[i] == top;
+                at = here ? i : at;
+                sc = here ? s[i] : sc;
+            }
+#pragma unroll
+            for (int i = 0; i < V; i++) key[i] = i == at ? 0u : key[i];
+            picked_i[local * a.topk + j] = first + at;
+            picked_s[local * a.topk + j] = sc;
+        } else if (top == 0 && sub == 0) {
+            picked_i[local * a.topk + j] = -1;
+            picked_s[local * a.topk + j] = 0.0f;
+        }
+    }
+    __syncthreads();
+    float sum = 0.0f;
+    for (int j = sub; j < a.topk; j += LPT) sum += picked_s[local * a.topk + j];
+    sum = lanes_sum<LPT>(sum);
+    const float factor = a.renorm ? a.scale / (sum + 1e-20f) : a.scale;
+    if (token >= a.tokens) return;
+    for (int j = sub; j < a.topk; j += LPT) {
+        const long long at = (long long)token * a.topk + j;
+        a.indices[at] = picked_i[local * a.topk + j];
+        a.weights[at] = picked_s[local * a.topk + j] * factor;
+    }
+}
+
+// ds of the selected experts from dw, then the score function's derivative:
+//   renorm: ds_i = scale (g_i - sum_j g_j s_j / S) / S, S = sum_j s_j + 1e-20
+//   softmax dz = s (ds - sum s ds), sigmoid dz = ds s (1 - s)
+template <int V, int LPT>
+__global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteArgs a)
+{
+    constexpr int kTokens = kRouteThreads / LPT;
+    const int sub = threadIdx.x & (LPT - 1), token = blockIdx.x * kTokens + threadIdx.x / LPT;
+    const int first = sub * V;
+    const int n = token < a.tokens ? max(0, min(V, a.experts - first)) : 0;
+    float z[V], s[V], g[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) z[i] = 0.0f, g[i] = 0.0f;
+    const uint32_t live = load_logits(z, a, token, first, n);
+    scores_of<V, LPT>(s, z, live, a.sigmoid);
+    uint32_t chosen = 0;
+    if (n > 0) {
+        for (int j = 0; j < a.topk; j++) {
+            const long long at = (long long)token * a.topk + j;
+            const int i = a.indices[at] - first;
+            const float d = a.dweights[at];
+#pragma unroll
+            for (int q = 0; q < V; q++) {
+                g[q] = q == i ? d : g[q];
+                chosen |= q == i && q < n ? 1u << q : 0u;
+            }
+        }
+    }
+    float total = 0.0f, dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const float c = chosen >> i & 1 ? s[i] : 0.0f;
+        total += c;
+        dot = fmaf(c, g[i], dot);
+    }
+    total = lanes_sum<LPT>(total) + 1e-20f;
+    dot = lanes_sum<LPT>(dot);
+    const float r = a.renorm ? 1.0f / total : 1.0f;
+    const float shift = a.renorm ? dot * r : 0.0f;
+    float back = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        g[i] = chosen >> i & 1 ? a.scale * (g[i] - shift) * r : 0.0f;
+        back = fmaf(g[i], s[i], back);
+    }
+    back = lanes_sum<LPT>(back);
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        float q = g[i] - back;
+        if (a.sigmoid) {
+            const float t = exp_neg(-fabsf(z[i]));  // 1 - s without cancellation
+            const float rest = __builtin_amdgcn_rcpf(1.0f + t);
+            q = g[i] * (z[i] >= 0.0f ? t * rest : rest);
+        }
+        g[i] = live >> i & 1 ? q * s[i] : 0.0f;
+    }
+    if (n <= 0) return;
+    const long long at = (long long)token * a.dstride + first;
+    auto store = [&](auto zero) {
+        using T = decltype(zero);
+        T* p = (T*)a.dlogits + at;
+        if (a.vec) {
+            constexpr int N = 16 / (int)sizeof(T) < V ? 16 / (int)sizeof(T) : V;
+#pragma unroll
+            for (int i = 0; i < V; i += N) {
+                Vec<T, N> v;
+#pragma unroll
+                for (int j = 0; j < N; j++) v[j] = (T)g[i + j];
+                *reinterpret_cast<Vec<T, N>*>(p + i) = v;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (i < n) p[i] = (T)g[i];
+        }
+    };
+    if (a.type == DATA_F32) store(float{});
+    else if (a.type == DATA_F16) store((_Float16)0);
+    else store((__bf16)0.0f);
+}
+
+int pow2_from(int n)
+{
+    int p = 1;
+    while (p < n) p *= 2;
+    return p;
+}
+
+// Four experts a lane as long as a wave holds the token, then 8, 16 or 32.
+template <class F>
+void with_layout(int lanes, int per_lane, F&& f)
+{
+    using std::integral_constant;
+    if (per_lane <= 4) {
+        switch (lanes) {
+            case 1: f(integral_constant<int, 4>{}, integral_constant<int, 1>{}); break;
+            case 2: f(integral_constant<int, 4>{}, integral_constant<int, 2>{}); break;
+            case 4: f(integral_constant<int, 4>{}, integral_constant<int, 4>{}); break;
+            case 8: f(integral_constant<int, 4>{}, integral_constant<int, 8>{}); break;
+            case 16: f(integral_constant<int, 4>{}, integral_constant<int, 16>{}); break;
+            case 32: f(integral_constant<int, 4>{}, integral_constant<int, 32>{}); break;
+            default: f(integral_constant<int, 4>{}, integral_constant<int, 64>{}); break;
+        }
+    } else if (per_lane <= 8) f(integral_constant<int, 8>{}, integral_constant<int, 64>{});
+    else if (per_lane <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 64>{});
+    else f(integral_constant<int, 32>{}, integral_constant<int, 64>{});
+}
+
+void check_route(const RouteOption& o, const void* logits, long long stride, int tokens)
+{
+    require(o.numExperts >= 1 && o.numExperts <= kMaxExperts, "numExperts must be 1..1024");
+    require(o.topK >= 1 && o.topK <= 32 && o.topK <= o.numExperts, "topK must be 1..32 and at most numExperts");
+    require(o.scoreType == ROUTE_SOFTMAX || o.scoreType == ROUTE_SIGMOID, "unknown scoreType");
+    require(o.numGroups >= 1 && o.numGroups <= 64 && o.numExperts % o.numGroups == 0,
+            "numGroups must be 1..64 and divide numExperts");
+    require(o.topGroups >= 1 && o.topGroups <= o.numGroups, "topGroups must be 1..numGroups");
+    require(o.numGroups == 1 || o.groupScore == 1 || o.groupScore == 2, "groupScore must be 1 or 2");
+    require(std::isfinite(o.scale), "scale must be finite");
+    require_type(o.logitsType);
+    require(tokens >= 0 && tokens <= kMaxRows, "numTokens must be 0..2^30");
+    require(stride >= o.numExperts, "logitsStride must be at least numExperts");
+    require(tokens == 0 || logits, "null argument");
+}
+
+RouteArgs route_args(const RouteOption& o, const void* logits, long long stride, int tokens)
+{
+    RouteArgs a{};
+    a.logits = logits;
+    a.stride = stride;
+    a.tokens = tokens;
+    a.experts = o.numExperts;
+    a.topk = o.topK;
+    a.type = o.logitsType;
+    a.sigmoid = o.scoreType == ROUTE_SIGMOID;
+    a.renorm = o.renormalize != 0;
+    a.scale = o.scale;
+    return a;
+}
+
+// Whole lanes of V from addresses that their vector loads take.
+bool can_vec(const void* p, long long stride, int per_group, int V, int type)
+{
+    const int bytes = std::min(16, V * data_bytes(type));
+    return per_group % V == 0 && (uintptr_t)p % bytes == 0 && stride * data_bytes(type) % bytes == 0;
+}
+
+}  // namespace
+
+void route_experts(const RouteOption& o, const void* logits, long long stride, const float* bias, int* indices,
+                   float* weights, int tokens, hipStream_t s)
+{
+    check_route(o, logits, stride, tokens);
+    if (tokens == 0) return;
+    require(indices && weights, "null argument");
+    RouteArgs a = route_args(o, logits, stride, tokens);
+    a.bias = bias;
+    a.indices = indices;
+    a.weights = weights;
+    a.groups = o.numGroups;
+    a.kept = o.topGroups;
+    a.group_size = o.numExperts / o.numGroups;
+    a.group_best = o.groupScore;
+    const int slots = pow2_from(o.numGroups);
+    a.lanes_group = std::min(64 / slots, pow2_from((a.group_size + 3) / 4));
+    const int lanes = slots * a.lanes_group, per_lane = (a.group_size + a.lanes_group - 1) / a.lanes_group;
+    with_layout(lanes, per_lane, [&](auto V, auto LPT) {
+        a.vec = can_vec(logits, stride, a.group_size, V, a.type);
+        const int per_wg = kRouteThreads / LPT;
+        route_kernel<decltype(V)::value, decltype(LPT)::value><<<(tokens + per_wg - 1) / per_wg, kRouteThreads, 0, s>>>(a);
+    });
+    GRAFT_LAUNCH_CHECK();
+}
+
+void route_experts_backward(const RouteOption& o, const void* logits, long long stride, const int* indices,
+                            const float* dweights, void* dlogits, long long dstride, int tokens, hipStream_t s)
+{
+    check_route(o, logits, stride, tokens);
+    require(dstride >= o.numExperts, "dlogitsStride must be at least numExperts");
+    if (tokens == 0) return;
+    require(indices && dweights && dlogits, "null argument");
+    RouteArgs a = route_args(o, logits, stride, tokens);
+    a.indices = const_cast<int*>(indices);
+    a.dweights = dweights;
+    a.dlogits = dlogits;
+    a.dstride = dstride;
+    const int lanes = std::min(64, pow2_from((o.numExperts + 3) / 4)), per_lane = (o.numExperts + lanes - 1) / lanes;
+    with_layout(lanes, per_lane, [&](auto V, auto LPT) {
+        a.vec = can_vec(logits, stride, o.numExperts, V, a.type) && can_vec(dlogits, dstride, o.numExperts, V, a.type);
+        const int per_wg = kRouteThreads / LPT;
+        route_backward_kernel<decltype(V)::value, decltype(LPT)::value><<<(tokens + per_wg - 1) / per_wg, kRouteThreads, 0, s>>>(a);
+    });
+    GRAFT_LAUNCH_CHECK();
+}
+
+// ---------------------------------------------------------------------------
+// the plan: a stable counting sort of the slots by expert
+// ---------------------------------------------------------------------------
+
+namespace {
+
+constexpr int kPlanThreads = 256;
+constexpr int kPlanWaves = kPlanThreads / 64;
+constexpr int kPlanChunk = 4096;  // slots of a workgroup
+
+struct PlanArgs {
+    const int* indices;
+    int slots, experts, align, capacity, blocks;
+    int* offsets;
+    int* order;
+    int* position;
+    int* counts;  // [experts][blocks]: a block's slots of an expert, then the row of its first
+    int* ends;    // [experts]: the row behind an expert's last slot
+};
+
+__device__ __forceinline__ int expert_of(const PlanArgs& a, int slot, int end)
+{
+    const int e = slot < end ? a.indices[slot] : -1;
+    return (unsigned)e < (unsigned)a.experts ? e : -1;
+}
+
+// Rows of the waves of the block in front of each other: hist [waves][experts]
+// counts of each wave's quarter of the chunk.
+__device__ __forceinline__ void plan_count(const PlanArgs& a, int* hist, int begin, int end, int wave, int lane, int waves)
+{
+    for (int i = threadIdx.x; i < waves * a.experts; i += blockDim.x) hist[i] = 0;
+    __syncthreads();
+    const int span = ((end - begin + waves * 64 - 1) / (waves * 64)) * 64;
+    const int w0 = begin + wave * span, w1 = min(end, w0 + span);
+    for (int i = w0 + lane; i < w1; i += 64) {
+        const int e = expert_of(a, i, end);
+        if (e >= 0) atomicAdd(&hist[wave * a.experts + e], 1);
+    }
+    __syncthreads();
+}
+
+// The slots of a wave's part in order: rank among the wave's lanes of the same
+// expert from one ballot per bit of the expert's number.
+__device__ __forceinline__ void plan_place(const PlanArgs& a, int* next, int begin, int end, int wave, int lane, int waves,
+                                           int bits)
+{
+    const int span = ((end - begin + waves * 64 - 1) / (waves * 64)) * 64;
+    const int w0 = begin + wave * span, w1 = min(end, w0 + span);
+    int* mine = next + wave * a.experts;
+    for (int i0 = w0; i0 < w1; i0 += 64) {
+        const int i = i0 + lane;
+        const int e = expert_of(a, i, w1);
+        uint64_t same = __ballot(e >= 0);
+        for (int b = 0; b < bits; b++) {
+            const uint64_t m = __ballot(e >> b & 1);
+            same &= (e >> b & 1) ? m : ~m;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        int row = -1;
+        if (e >= 0) {
+            row = mine[e] + rank;
+            a.order[row] = i;
+        }
+        if (i < w1) a.position[i] = row;
+        __builtin_amdgcn_wave_barrier();
+        if (e >= 0 && rank == 0) mine[e] += __popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+__global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(PlanArgs a)
+{
+    extern __shared__ int hist[];
+    const int begin = blockIdx.x * kPlanChunk, end = min(a.slots, begin + kPlanChunk);
+    plan_count(a, hist, begin, end, threadIdx.x / 64, threadIdx.x & 63, kPlanWaves);
+    for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) {
+        int n = 0;
+        for (int w = 0; w < kPlanWaves; w++) n += hist[w * a.experts + e];
+        a.counts[(size_t)e * a.blocks + blockIdx.x] = n;
+    }
+}
+
+// Inclusive sum over the wave.
+__device__ __forceinline__ int wave_scan(int v, int lane)
+{
+    for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(v, d);
+        v += lane >= d ? o : 0;
+    }
+    return v;
+}
+
+// One workgroup: offsets from the experts' counts in LDS (total, then overwritten
+// with the segment's first row).
+__device__ __forceinline__ void plan_offsets(const PlanArgs& a, int* total, int lane, int wave)
+{
+    if (wave == 0) {
+        int base = 0;
+        for (int e0 = 0; e0 < a.experts; e0 += 64) {
+            const int e = e0 + lane;
+            const int n = e < a.experts ? (total[e] + a.align - 1) / a.align * a.align : 0;
+            const int up = wave_scan(n, lane);
+            if (e < a.experts) {
+                a.ends[e] = base + up - n + total[e];
+                total[e] = base + up - n;
+                a.offsets[e] = base + up - n;
+            }
+            base += __shfl(up, 63);
+        }
+        if (lane == 0) a.offsets[a.experts] = base;
+    }
+    __syncthreads();
+}
+
+__global__ __launch_bounds__(1024) void plan_scan_kernel(PlanArgs a)
+{
+    __shared__ int total[kMaxExperts];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    for (int e = wave; e < a.experts; e += 16) {
+        int* c = a.counts + (size_t)e * a.blocks;
+        int sum = 0;
+        for (int b0 = 0; b0 < a.blocks; b0 += 64) {
+            const int b = b0 + lane, n = b < a.blocks ? c[b] : 0;
+            const int up = wave_scan(n, lane);
+            if (b < a.blocks) c[b] = sum + up - n;
+            sum += __shfl(up, 63);
+        }
+        if (lane == 0) total[e] = sum;
+    }
+    __syncthreads();
+    plan_offsets(a, total, lane, wave);
+}
+
+// Blocks 0 .. blocks - 1 place their slots; those behind them fill the rows
+// that no slot has.
+__global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(PlanArgs a, int bits)
+{
+    extern __shared__ int next[];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    if ((int)blockIdx.x >= a.blocks) {
+        const int fill = blockIdx.x - a.blocks, fills = gridDim.x - a.blocks;
+        for (int e = fill; e < a.experts; e += fills)
+            for (int r = a.ends[e] + threadIdx.x; r < a.offsets[e + 1]; r += kPlanThreads) a.order[r] = -1;
+        const int last = a.offsets[a.experts];
+        for (long long r = last + (long long)fill * kPlanThreads + threadIdx.x; r < a.capacity; r += fills * kPlanThreads)
+            a.order[r] = -1;
+        return;
+    }
+    const int begin = blockIdx.x * kPlanChunk, end = min(a.slots, begin + kPlanChunk);
+    plan_count(a, next, begin, end, wave, lane, kPlanWaves);
+    for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) {
+        int at = a.offsets[e] + a.counts[(size_t)e * a.blocks + blockIdx.x];
+        for (int w = 0; w < kPlanWaves; w++) {
+            const int n = next[w * a.experts + e];
+            next[w * a.experts + e] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+    plan_place(a, next, begin, end, wave, lane, kPlanWaves, bits);
+}
+
+// Few slots: one workgroup does all of it.
+__global__ __launch_bounds__(kPlanThreads) void plan_small_kernel(PlanArgs a, int bits)
+{
+    extern __shared__ int lds[];
+    int* next = lds;                               // [waves][experts]
+    int* total = lds + kPlanWaves * a.experts;     // [experts]
+    a.ends = total + a.experts;                    // [experts], in LDS too
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    plan_count(a, next, 0, a.slots, wave, lane, kPlanWaves);
+    for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) {
+        int n = 0;
+        for (int w = 0; w < kPlanWaves; w++) n += next[w * a.experts + e];
+        total[e] = n;
+    }
+    __syncthreads();
+    plan_offsets(a, total, lane, wave);
+    for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) {
+        int at = total[e];
+        for (int w = 0; w < kPlanWaves; w++) {
+            const int n = next[w * a.experts + e];
+            next[w * a.experts + e] = at;
+            at += n;
+        }
+        for (int r = a.ends[e]; r < total[e] + (a.ends[e] - total[e] + a.align - 1) / a.align * a.align; r++) a.order[r] = -1;
+    }
+    __syncthreads();
+    const int e = a.experts - 1;
+    const int last = total[e] + (a.ends[e] - total[e] + a.align - 1) / a.align * a.align;
+    for (int r = last + threadIdx.x; r < a.capacity; r += kPlanThreads) a.order[r] = -1;
+    plan_place(a, next, 0, a.slots, wave, lane, kPlanWaves, bits);
+}
+
+}  // namespace
+
+long long route_plan_capacity(int tokens, int topK, int experts, int align)
+{
+    if (tokens < 0 || tokens > kMaxRows || topK < 1 || topK > 32 || experts < 1 || experts > kMaxExperts || align < 1 || align > 128) return -1;
+    const long long slots = (long long)tokens * topK;
+    const long long rows = slots + std::min<long long>(experts, slots) * (align - 1);
+    const long long capacity = round_up<long long>(rows, align);
+    return capacity <= kMaxRows ? capacity : -1;
+}
+
+void route_plan(const int* indices, int tokens, int topK, int experts, int align, int capacity, int* offsets, int* order,
+                int* position, hipStream_t s)
+{
+    const long long need = route_plan_capacity(tokens, topK, experts, align);
+    require(need >= 0, "numTokens must be >= 0, topK 1..32, numExperts 1..1024, align 1..128, and the rows at most 2^30");
+    require(capacity >= need, "capacity is less than routePlanCapacity()");
+    require(offsets && (capacity == 0 || order) && (tokens == 0 || (indices && position)), "null argument");
+    PlanArgs a{};
+    a.indices = indices;
+    a.slots = tokens * topK;
+    a.experts = experts;
+    a.align = align;
+    a.capacity = capacity;
+    a.offsets = offsets;
+    a.order = order;
+    a.position = position;
+    int bits = 0;
+    while ((1 << bits) < experts) bits++;
+    if (a.slots <= kPlanChunk) {
+        plan_small_kernel<<<1, kPlanThreads, (kPlanWaves + 2) * experts * sizeof(int), s>>>(a, bits);
+        GRAFT_LAUNCH_CHECK();
+        return;
+    }
+    a.blocks = (a.slots + kPlanChunk - 1) / kPlanChunk;
+    Workspace& ws = stream_workspace(s);
+    a.counts = (int*)ws.get(((size_t)a.blocks + 1) * experts * sizeof(int));
+    a.ends = a.counts + (size_t)a.blocks * experts;
+    const size_t lds = kPlanWaves * experts * sizeof(int);
+    plan_count_kernel<<<a.blocks, kPlanThreads, lds, s>>>(a);
+    GRAFT_LAUNCH_CHECK();
+    plan_scan_kernel<<<1, 1024, 0, s>>>(a);
+    GRAFT_LAUNCH_CHECK();
+    plan_place_kernel<<<a.blocks + 64, kPlanThreads, lds, s>>>(a, bits);
+    GRAFT_LAUNCH_CHECK();
+}
+
+}  // namespace graft
