@@ -16,6 +16,8 @@
 #include "experts.h"
 
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 namespace graft {
 
@@ -38,11 +40,6 @@ struct ProductArgs {
     int tiles_m, tiles_n;
 };
 
-__device__ __forceinline__ f4 mfma_scaled(i8v a, int sa, i8v b, int sb, f4 c)
-{
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
-}
-
 // Eight e4m3 values times 2^(scale - 127) as bf16 (exact: e4m3 has 4 bits).
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ bf16x8 widen(int lo, int hi, float scale)
@@ -56,214 +53,397 @@ __device__ __forceinline__ bf16x8 widen(int lo, int hi, float scale)
 
 __device__ __forceinline__ float scale_of(int byte) { return __builtin_bit_cast(float, byte << 23); }
 
-// 16 bytes a lane from global memory to consecutive LDS addresses of the wave.
-__device__ __forceinline__ void load_lds16(const uint8_t* from, uint8_t* to)
+// f(integral_constant<int, 0>) .. f(integral_constant<int, N - 1>)
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F& f, std::integer_sequence<int, I...>)
 {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f)
+{
+    each_of(f, std::make_integer_sequence<int, N>{});
 }
 
-// A segment's rows and the expert they belong to: tile `t` of all experts' row
-// tiles of `tm` rows, or no rows.  Every wave finds it by itself.
-__device__ __forceinline__ void find_rows(const ProductArgs& a, int t, int tm, int& expert, int& row0, int& row1)
+// The workgroup meets when its waves' memory counters have come down to COUNTS
+// (an s_waitcnt operand); no memory access moves across.
+constexpr int kAllDone = 0x0070, kLdsDone = 0xc07f;
+template <int COUNTS>
+__device__ __forceinline__ void meet()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(COUNTS);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Where a segment's row tiles begin: starts[e] for e in 0..experts, from the
+// offsets, by the first wave; the last one is their number.
+template <int TM>
+__device__ __forceinline__ void row_tiles(const ProductArgs& a, int* starts)
 {
     const int lane = threadIdx.x & 63;
-    int before = 0;
-    row0 = row1 = 0;
-    expert = 0;
-    for (int e0 = 0; e0 < a.experts; e0 += 64) {
-        const int e = e0 + lane;
-        int lo = 0, hi = 0;
-        if (e < a.experts) {
-            lo = min(max(a.offsets[e], 0), a.m);
-            hi = min(max(a.offsets[e + 1], lo), a.m);
+    if (threadIdx.x < 64) {
+        int before = 0;
+        for (int e0 = 0; e0 < a.experts; e0 += 64) {
+            const int e = e0 + lane;
+            int n = 0;
+            if (e < a.experts) {
+                const int lo = min(max(a.offsets[e], 0), a.m), hi = min(max(a.offsets[e + 1], lo), a.m);
+                n = (hi - lo + TM - 1) / TM;
+            }
+            int up = n;
+            for (int d = 1; d < 64; d *= 2) {
+                const int o = __shfl_up(up, d);
+                up += lane >= d ? o : 0;
+            }
+            if (e < a.experts) starts[e] = before + up - n;
+            before += __shfl(up, 63);
         }
-        const int tiles = (hi - lo + tm - 1) / tm;
-        int up = tiles;
-        for (int d = 1; d < 64; d *= 2) {
-            const int o = __shfl_up(up, d);
-            up += lane >= d ? o : 0;
-        }
-        const uint64_t found = __ballot(before + up > t);
-        if (found) {
-            const int l = __ffsll((unsigned long long)found) - 1;
-            const int first = before + __shfl(up - tiles, l);
-            expert = e0 + l;
-            row0 = __shfl(lo, l) + (t - first) * tm;
-            row1 = __shfl(hi, l);
-            return;
-        }
-        before += __shfl(up, 63);
+        if (lane == 0) starts[a.experts] = before;
+    }
+    __syncthreads();
+}
+
+// The expert whose row tiles hold tile t < starts[experts].
+__device__ __forceinline__ int expert_of_tile(const int* starts, int experts, int t)
+{
+    const int lane = threadIdx.x & 63;
+    for (int e0 = 0;; e0 += 64) {
+        const uint64_t found = __ballot(e0 + lane < experts && starts[e0 + lane + 1] > t);
+        if (found) return e0 + __ffsll((unsigned long long)found) - 1;
     }
 }
 
-__device__ __forceinline__ void store4(const ProductArgs& a, long long at, int n, f4 v)
+template <class T>
+__device__ __forceinline__ T finish(float v, bool relu)
 {
-    if (a.relu) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = v[j] < 0.0f ? 0.0f : v[j];  // NaN stays
-    }
-    const int left = a.n - n;
-    auto put = [&](auto zero) {
-        using T = decltype(zero);
-        T* p = (T*)a.out + at + n;
-        if (a.vec && left >= 4) {
-            *reinterpret_cast<Vec<T, 4>*>(p) = Vec<T, 4>{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (j < left) p[j] = (T)v[j];
-        }
-    };
-    if (a.out_type == DATA_F32) put(float{});
-    else if (a.out_type == DATA_F16) put((_Float16)0);
-    else put((__bf16)0.0f);
+    return (T)(relu && v < 0.0f ? 0.0f : v);  // NaN stays
 }
 
-// Tiles of TM x TN, WM x WN waves.  Both operands of a block of k go through
-// two LDS stages, rows of 128 bytes whose 16-byte pieces are permuted by the
-// row's low bits (the permutation is in the global addresses: the copy to LDS
-// is linear), so that 8 rows' pieces of one column lie in different banks.
-template <int TM, int TN, int WM, int WN, bool WIDE>
-__global__ __launch_bounds__(WM* WN * 64) void product_kernel(ProductArgs a)
+// N consecutive results from column n on.
+template <class T, int N>
+__device__ __forceinline__ void store_row(const ProductArgs& a, T* row, int n, const float (&v)[N])
 {
-    constexpr int kWaves = WM * WN, MT = TM / WM / 16, NT = TN / WN / 16;
-    constexpr int kStage = (TM + TN) * 128, kLoads = (TM + TN) / 8 / kWaves;
-    static_assert((TM + TN) % (8 * kWaves) == 0 && TM % 8 == 0, "whole wave loads");
-    __shared__ __attribute__((aligned(128))) uint8_t lds[2 * kStage];
+    constexpr int P = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+    if (a.vec && n + N <= a.n) {
+#pragma unroll
+        for (int i = 0; i < N; i += P) {
+            Vec<T, P> o;
+#pragma unroll
+            for (int j = 0; j < P; j++) o[j] = finish<T>(v[i + j], a.relu);
+            *reinterpret_cast<Vec<T, P>*>(row + n + i) = o;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (n + i < a.n) row[n + i] = finish<T>(v[i], a.relu);
+    }
+}
+
+// Large products: TM x TN tiles by four waves, persistent workgroups.
+//
+// A block of k of both operands lies in one of two LDS stages, rows of 128
+// bytes whose 16-byte pieces are permuted by a key of the row, so that the 16
+// rows of a fragment are read from all banks; the copy to LDS is linear, so the
+// permutation is in its global addresses.  It is a buffer load, which gives rows
+// behind the tile's last as zeros.
+//
+// A wave's tile is worked through in quadrants of its two halves of A's and of
+// B's fragments.  The next quadrant's half is read from LDS, and the block after
+// the next copied to it, between this one's matrix instructions: a copy or read
+// that is issued in a burst holds the wave's matrix instructions up (8192 x
+// 5120 x 4096: 207 us with bursts, 170 spread).  The order is held by the empty
+// asm on the accumulators and the scheduling barriers.  The one barrier of a
+// block stands behind its last LDS read, half a block before its last matrix
+// instruction.
+//
+// B's row of fragment i and lane column c is (i / 2) 32 + (c / 4) 8 + (i % 2) 4 +
+// c % 4: a lane ends with eight consecutive columns of two fragments, one 16-byte
+// store of 16-bit results.
+//
+// The scales of 32 blocks lie in LDS in the order in which a lane takes them:
+// one read gives four fragments' bytes, which the matrix instruction selects.
+//
+// Tile sizes: a block costs a CU (TM + TN) 128 bytes of copies at 64 a clock and
+// (TM WN + TN WM) 128 of LDS reads at 128 a clock besides writes, for TM TN / 512
+// clocks of matrix work.  256 x 256 has most room (2.5 PFLOP/s at 8192^3) but one
+// workgroup a CU; two of 128 x 128 fit (2.2 PFLOP/s) and lose less to a last round
+// of tiles.
+template <class T, int TM, int TN, bool WIDE>
+__global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kernel(ProductArgs a)
+{
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass needs the kernel's name alone
+    using std::integral_constant;
+    constexpr int WM = 2, WN = 2, kWaves = 4, MT = TM / WM / 16, NT = TN / WN / 16, MH = MT / 2, NH = NT / 2;
+    constexpr int kStage = (TM + TN) * 128, kLoads = (TM + TN) / 8 / kWaves, kScaleRow = TM + TN;
+    static_assert(TM % (8 * kWaves) == 0 && MT % 4 == 0 && NT % 4 == 0, "whole fragments and copies");
+    // One array: with two, the compiler waits for all copies before each LDS read.
+    __shared__ __attribute__((aligned(128))) uint8_t lds[2 * kStage + 32 * kScaleRow + 1028 * 4];
+    int* const starts = reinterpret_cast<int*>(lds + 2 * kStage + 32 * kScaleRow);
+    uint8_t* const scale_lds = lds + 2 * kStage;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    int tm, tn, expert = 0, row0, row1, kb0 = 0, kb1 = a.pitch / 128;
-    if (a.grouping == PRODUCT_SUM) {
-        const int per = a.tiles_m * a.tiles_n;
-        expert = blockIdx.x / per;
-        tm = blockIdx.x % per / a.tiles_n;
-        tn = blockIdx.x % a.tiles_n;
-        kb0 = min(max(a.offsets[expert] / 128, 0), kb1);
-        kb1 = min(max(a.offsets[expert + 1] / 128, kb0), kb1);
+    const int wm = wave / WN, wn = wave % WN, col = lane & 15, quad = lane >> 4;
+
+    int total = a.tiles_m * a.tiles_n;
+    if (a.grouping == PRODUCT_SUM) total *= a.experts;
+    int row_tile_count = a.tiles_m;
+    if (a.grouping == PRODUCT_ROWS) {
+        row_tiles<TM>(a, starts);
+        row_tile_count = __builtin_amdgcn_readfirstlane(starts[a.experts]);
+        total = row_tile_count * a.tiles_n;
+    }
+    // Workgroups go round the XCDs: each XCD works through a range of its own.
+    const int xcd = blockIdx.x & 7, x0 = xcd * (total / 8) + min(xcd, total % 8), xn = total / 8 + (xcd < total % 8);
+    const int stride = (gridDim.x + 7 - xcd) / 8;
+    int at = blockIdx.x >> 3;
+    if (at >= xn) return;
+
+    int row0, row1, n0, kb0, kb1;
+    long long out0;
+    const uint8_t *SA, *SB;
+    __amdgpu_buffer_rsrc_t ra, rb;
+    auto place = [&](int t) {  // four row tiles by all columns at a time: what an XCD has in flight shares its L2
+        int expert = 0;
+        if (a.grouping == PRODUCT_SUM) {
+            expert = t / (a.tiles_m * a.tiles_n);
+            t -= expert * a.tiles_m * a.tiles_n;
+        }
+        const int group = t / (4 * a.tiles_n), first = group * 4, rows = min(4, row_tile_count - first);
+        const int in = t - first * a.tiles_n, tm = first + in % rows;
+        n0 = in / rows * TN;
+        kb0 = 0;
+        kb1 = a.pitch / 128;
         row0 = tm * TM;
         row1 = a.m;
-    } else {
-        tm = blockIdx.x / a.tiles_n;
-        tn = blockIdx.x % a.tiles_n;
+        const uint8_t* B = a.b;
+        SB = a.bs;
+        out0 = 0;
         if (a.grouping == PRODUCT_ROWS) {
-            find_rows(a, tm, TM, expert, row0, row1);
-            if (row0 >= row1) return;
-        } else {
-            row0 = tm * TM;
-            row1 = a.m;
+            expert = __builtin_amdgcn_readfirstlane(expert_of_tile(starts, a.experts, tm));
+            const int lo = min(max(a.offsets[expert], 0), a.m);
+            row0 = lo + (tm - starts[expert]) * TM;
+            row1 = min(max(a.offsets[expert + 1], lo), a.m);
+            row0 = __builtin_amdgcn_readfirstlane(row0);
+            row1 = __builtin_amdgcn_readfirstlane(row1);
+            B += expert * a.b_size;
+            SB += expert * a.bs_size;
+        } else if (a.grouping == PRODUCT_SUM) {
+            kb0 = __builtin_amdgcn_readfirstlane(min(max(a.offsets[expert] / 128, 0), kb1));
+            kb1 = __builtin_amdgcn_readfirstlane(min(max(a.offsets[expert + 1] / 128, kb0), kb1));
+            out0 = (long long)expert * a.m * a.out_stride;
         }
-    }
-    const int n0 = tn * TN;
-    const long long be = a.grouping == PRODUCT_ROWS ? expert : 0;
-    const uint8_t* A = a.a + (long long)row0 * a.pitch;
-    const uint8_t* B = a.b + be * a.b_size + (long long)n0 * a.pitch;
-    const uint8_t* SA = a.as + (long long)row0 * a.spitch;
-    const uint8_t* SB = a.bs + be * a.bs_size + (long long)(n0 >> a.scale_shift) * a.spitch;
-
-    // The wave's pieces of a stage: 8 rows by 128 bytes each.
-    uint32_t from[kLoads];
-    bool of_a[kLoads];
-#pragma unroll
-    for (int i = 0; i < kLoads; i++) {
-        const int r = (i * kWaves + wave) * 8 + (lane >> 3);
-        const int piece = (lane & 7) ^ (r & 7);
-        of_a[i] = (i * kWaves + wave) * 8 < TM;
-        const int row = of_a[i] ? min(r, row1 - row0 - 1) : min(r - TM, a.n - n0 - 1);
-        from[i] = (uint32_t)row * a.pitch + piece * 16;
-    }
-    auto fetch = [&](int kb, int stage) {
-#pragma unroll
-        for (int i = 0; i < kLoads; i++)
-            load_lds16((of_a[i] ? A : B) + (long long)kb * 128 + from[i], lds + stage * kStage + (i * kWaves + wave) * 1024);
+        const int flags = 0x00020000;
+        ra = __builtin_amdgcn_make_buffer_rsrc((void*)(a.a + (long long)row0 * a.pitch), 0, min(TM, row1 - row0) * a.pitch,
+                                               flags);
+        rb = __builtin_amdgcn_make_buffer_rsrc((void*)(B + (long long)n0 * a.pitch), 0, min(TN, a.n - n0) * a.pitch, flags);
+        SA = a.as + (long long)row0 * a.spitch;
+        SB += (long long)(n0 >> a.scale_shift) * a.spitch;
     };
 
-    const int wm = wave / WN, wn = wave % WN, col = lane & 15, quad = lane >> 4;
-    uint32_t sa_at[MT], sb_at[NT];
+    uint32_t from[kLoads];  // the lane's piece of each copy: 8 rows of 128 bytes a wave
 #pragma unroll
-    for (int i = 0; i < MT; i++) sa_at[i] = min(wm * (TM / WM) + i * 16 + col, row1 - row0 - 1) * a.spitch;
+    for (int i = 0; i < kLoads; i++) {
+        const bool of_a = i * kWaves * 8 < TM;
+        const int r = (i * kWaves + wave) * 8 + (lane >> 3) - (of_a ? 0 : TM);
+        const int key = of_a ? r & 7 : (r & 3) | (r >> 1 & 4);
+        from[i] = (uint32_t)r * a.pitch + ((lane & 7) ^ key) * 16;
+    }
+    auto copy = [&](int kb, int stage, int i) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(i * kWaves * 8 < TM ? ra : rb,
+                                                 (__attribute__((address_space(3))) void*)(lds + stage * kStage +
+                                                                                           (i * kWaves + wave) * 1024),
+                                                 16, from[i], kb * 128, 0, 0);
+    };
+    auto copy_first = [&] {
 #pragma unroll
-    for (int i = 0; i < NT; i++)
-        sb_at[i] = (uint32_t)((min(n0 + wn * (TN / WN) + i * 16 + col, a.n - 1) >> a.scale_shift) - (n0 >> a.scale_shift)) *
-                   a.spitch;
+        for (int i = 0; i < kLoads; i++) copy(kb0, 0, i);
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) copy(min(kb0 + 1, kb1 - 1), 1, i);
+    };
+    // Scale bytes of blocks kb .. kb + 31 (kb a multiple of 4) to
+    // [block][the fragments' bytes of a wave and lane column together].
+    auto copy_scales = [&](int kb) {
+        const int words = min(8, (kb1 - kb + 3) / 4);
+        for (int r = threadIdx.x; r < TM + TN; r += 256) {
+            const bool of_a = r < TM;
+            const int row = of_a ? min(r, row1 - row0 - 1)
+                                 : (min(n0 + r - TM, a.n - 1) >> a.scale_shift) - (n0 >> a.scale_shift);
+            const uint8_t* p = (of_a ? SA : SB) + (uint32_t)row * a.spitch + kb;
+            const int w = of_a ? r : r - TM, in = w % (of_a ? TM / WM : TN / WN);
+            const int to = of_a ? w - in + (in & 15) * MT + (in >> 4)
+                                : TM + w - in + ((in >> 3 & 3) * 4 + (in & 3)) * NT + (in >> 5) * 2 + (in >> 2 & 1);
+            for (int d = 0; d < words; d++) {
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(p + d * 4);
+#pragma unroll
+                for (int q = 0; q < 4; q++) scale_lds[(d * 4 + q) * kScaleRow + to] = (uint8_t)(v >> (8 * q));
+            }
+        }
+    };
 
     f4 acc[NT][MT];
+    i8v a0[MH], a1[MH], b0[NH], b1[NH];
+    bf16x8 wa[WIDE ? MH : 1][4], w0[WIDE ? NH : 1][4], w1[WIDE ? NH : 1][4];
+    int sa[MT / 4], sb[NT / 4];
+    auto scales = [&](int slot) {
+        const uint8_t* p = scale_lds + (slot & 31) * kScaleRow;
 #pragma unroll
-    for (int i = 0; i < NT; i++)
+        for (int i = 0; i < MT / 4; i++) sa[i] = *reinterpret_cast<const int*>(p + wm * (TM / WM) + col * MT + i * 4);
 #pragma unroll
-        for (int j = 0; j < MT; j++) acc[i][j] = f4zero();
-
-    if (kb0 < kb1) fetch(kb0, 0);
-    __syncthreads();
-    for (int kb = kb0; kb < kb1; kb++) {
-        const int stage = (kb - kb0) & 1;
-        if (kb + 1 < kb1) fetch(kb + 1, stage ^ 1);
-        int sa[MT], sb[NT];
+        for (int i = 0; i < NT / 4; i++) sb[i] = *reinterpret_cast<const int*>(p + TM + wn * (TN / WN) + col * NT + i * 4);
+    };
+    // Half h (pieces quad or quad + 4) of fragment i.
+    const int a_at = (wm * (TM / WM) + col) * 128, b_at = (TM + wn * (TN / WN) + (col >> 2) * 8 + (col & 3)) * 128;
+    const int a_key = col & 7, b_key = col & 7;  // of rows 16 i + col; of B's rows (row & 3) | (row >> 1 & 4)
+    auto read_half = [&](i8v& f, int address, int h, int key) {
+        const i4v v = *reinterpret_cast<const i4v*>(lds + address + (((quad + 4 * h) ^ key) * 16));
 #pragma unroll
-        for (int i = 0; i < MT; i++) sa[i] = SA[sa_at[i] + kb];
+        for (int j = 0; j < 4; j++) f[4 * h + j] = v[j];
+    };
+    auto read_a = [&](i8v& f, int stage, int i, int h) { read_half(f, stage * kStage + a_at + i * 2048, h, a_key); };
+    auto read_b = [&](i8v& f, int stage, int i, int h) {
+        read_half(f, stage * kStage + b_at + (i >> 1) * 4096 + (i & 1) * 512, h, b_key);
+    };
+    auto widen_all = [&](auto& w, auto& f, const int* s, int first) {
+        each<sizeof(f) / sizeof(f[0])>([&](auto I) {
+            constexpr int i = decltype(I)::value;
+            const float scale = scale_of(s[(first + i) / 4] >> (8 * ((first + i) % 4)) & 0xff);
 #pragma unroll
-        for (int i = 0; i < NT; i++) sb[i] = SB[sb_at[i] + kb];
-        const uint8_t* base = lds + stage * kStage;
-        auto fragment = [&](int r) {  // row r of the stage, pieces quad and quad + 4
-            const uint8_t* p = base + r * 128;
-            const i4v lo = *reinterpret_cast<const i4v*>(p + ((quad ^ (r & 7)) * 16));
-            const i4v hi = *reinterpret_cast<const i4v*>(p + (((quad + 4) ^ (r & 7)) * 16));
-            return i8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        };
-        if constexpr (WIDE) {
-            bf16x8 fa[MT][4];
+            for (int q = 0; q < 4; q++) w[i][q] = widen(f[i][2 * q], f[i][2 * q + 1], scale);
+        });
+    };
+    // One quadrant; between(m) behind its m-th fragment pair.
+    auto quadrant = [&](auto& x, auto& wx, auto MO, auto& y, auto& wy, auto NO, auto between) {
+        constexpr int mo = decltype(MO)::value, no = decltype(NO)::value;
+        each<NH>([&](auto I) {
+            each<MH>([&](auto J) {
+                constexpr int i = decltype(I)::value, j = decltype(J)::value;
+                f4& c = acc[no + i][mo + j];
+                if constexpr (WIDE) {
 #pragma unroll
-            for (int j = 0; j < MT; j++) {
-                const i8v f = fragment(wm * (TM / WM) + j * 16 + col);
-#pragma unroll
-                for (int q = 0; q < 4; q++) fa[j][q] = widen(f[2 * q], f[2 * q + 1], scale_of(sa[j]));
-            }
-#pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const i8v f = fragment(TM + wn * (TN / WN) + i * 16 + col);
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const bf16x8 fb = widen(f[2 * q], f[2 * q + 1], scale_of(sb[i]));
-#pragma unroll
-                    for (int j = 0; j < MT; j++)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, fa[j][q], acc[i][j], 0, 0, 0);
+                    for (int q = 0; q < 4; q++) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wy[i][q], wx[j][q], c, 0, 0, 0);
+                } else {
+                    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(y[i], x[j], c, 0, 0, (no + i) % 4, sb[(no + i) / 4],
+                                                                         (mo + j) % 4, sa[(mo + j) / 4]);
                 }
+                asm volatile("" : "+v"(c));
+                between(integral_constant<int, i * MH + j>{});
+                __builtin_amdgcn_sched_barrier(0);
+            });
+        });
+    };
+    // f(0) .. f(N - 1) spread over a quadrant's MH * NH places.
+    auto spread = [&](auto N, auto M, auto f) {
+        constexpr int n = decltype(N)::value, m = decltype(M)::value, places = MH * NH;
+        constexpr int lo = (m * n + places - 1) / places, hi = ((m + 1) * n + places - 1) / places;
+        each<hi - lo>([&](auto Q) { f(lo + decltype(Q)::value); });
+    };
+    // Block kb in `stage`: A's first half and B's half X have been read; leaves the
+    // next block's first half of A and half Y of B read, Y its X.
+    auto block = [&](int kb, int stage, auto& bx, auto& wx, auto X, auto& by, auto& wy, auto Y) {
+        constexpr int xo = decltype(X)::value, yo = decltype(Y)::value;
+        const integral_constant<int, 0> lower{};
+        const integral_constant<int, MH> upper{};
+        const integral_constant<int, 2 * MH> a_reads{};
+        const integral_constant<int, 2 * NH> b_reads{};
+        const integral_constant<int, kLoads / 2> copies{};
+        if constexpr (WIDE) {
+            widen_all(wa, a0, sa, 0);
+            widen_all(wx, bx, sb, xo);
+        }
+        quadrant(a0, wa, lower, bx, wx, X, [&](auto m) {
+            spread(b_reads, m, [&](int q) { read_b(by[q / 2], stage, yo + q / 2, q % 2); });
+        });
+        if constexpr (WIDE) widen_all(wy, by, sb, yo);
+        quadrant(a0, wa, lower, by, wy, Y, [&](auto m) {
+            spread(a_reads, m, [&](int q) { read_a(a1[q / 2], stage, MH + q / 2, q % 2); });
+        });
+        meet<kAllDone>();  // the next block is here, this one is read
+        const int after = min(kb + 2, kb1 - 1);  // behind the last block: copied again, and not read
+        if constexpr (WIDE) widen_all(wa, a1, sa, MH);
+        quadrant(a1, wa, upper, by, wy, Y, [&](auto m) {
+            spread(a_reads, m, [&](int q) { read_a(a0[q / 2], stage ^ 1, q / 2, q % 2); });
+            spread(copies, m, [&](int q) { copy(after, stage, q); });
+        });
+        quadrant(a1, wa, upper, bx, wx, X, [&](auto m) {
+            spread(b_reads, m, [&](int q) { read_b(by[q / 2], stage ^ 1, yo + q / 2, q % 2); });
+            spread(copies, m, [&](int q) { copy(after, stage, kLoads / 2 + q); });
+        });
+        const int slot = kb + 1 - (kb0 & ~3);
+        if ((slot & 31) == 0 && kb + 1 < kb1) {
+            meet<kLdsDone>();
+            copy_scales(kb + 1);
+            meet<kLdsDone>();
+        }
+        scales(slot);
+    };
+
+    place(x0 + at);
+    if (kb0 < kb1) copy_first();
+    copy_scales(kb0 & ~3);
+    for (;;) {
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int j = 0; j < MT; j++) acc[i][j] = f4zero();
+        const int r0 = row0, r1 = row1, c0 = n0;
+        const long long o0 = out0;
+        meet<kAllDone>();
+        if (kb0 < kb1) {
+            scales(kb0 & 3);
+#pragma unroll
+            for (int i = 0; i < 2 * MH; i++) read_a(a0[i / 2], 0, i / 2, i % 2);
+#pragma unroll
+            for (int i = 0; i < 2 * NH; i++) read_b(b0[i / 2], 0, i / 2, i % 2);
+            const integral_constant<int, 0> lower{};
+            const integral_constant<int, NH> upper{};
+            int kb = kb0;
+            for (; kb + 1 < kb1; kb += 2) {
+                block(kb, 0, b0, w0, lower, b1, w1, upper);
+                block(kb + 1, 1, b1, w1, upper, b0, w0, lower);
             }
-        } else {
-            i8v fa[MT];
+            if (kb < kb1) block(kb, 0, b0, w0, lower, b1, w1, upper);
+        }
+        at += stride;
+        const bool more = at < xn;
+        // Copies behind the last block end here at the latest.  The next tile's are
+        // under way while this one's results are stored.
+        meet<kAllDone>();
+        if (more) {
+            place(x0 + at);
+            if (kb0 < kb1) copy_first();
+            copy_scales(kb0 & ~3);
+        }
 #pragma unroll
-            for (int j = 0; j < MT; j++) fa[j] = fragment(wm * (TM / WM) + j * 16 + col);
+        for (int j = 0; j < MT; j++) {
+            const int r = r0 + wm * (TM / WM) + j * 16 + col;
+            if (r >= r1) continue;
+            T* row = (T*)a.out + o0 + (long long)r * a.out_stride;
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                const i8v fb = fragment(TM + wn * (TN / WN) + i * 16 + col);
-#pragma unroll
-                for (int j = 0; j < MT; j++) acc[i][j] = mfma_scaled(fb, sb[i], fa[j], sa[j], acc[i][j]);
+            for (int i = 0; i < NT; i += 2) {
+                const f4 u = acc[i][j], w = acc[i + 1][j];
+                const float v[8] = {u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]};
+                const int n = c0 + wn * (TN / WN) + (i >> 1) * 32 + quad * 8;
+                if (n < a.n) store_row<T, 8>(a, row, n, v);
             }
         }
-        __syncthreads();
+        if (!more) break;
     }
-#pragma unroll
-    for (int j = 0; j < MT; j++) {
-        const int r = wm * (TM / WM) + j * 16 + col;
-        if (row0 + r >= row1) continue;
-        const long long at = ((a.grouping == PRODUCT_SUM ? (long long)expert * a.m : 0) + row0 + r) * a.out_stride;
-#pragma unroll
-        for (int i = 0; i < NT; i++) {
-            const int n = n0 + wn * (TN / WN) + i * 16 + quad * 4;
-            if (n < a.n) store4(a, at, n, acc[i][j]);
-        }
-    }
+#endif
 }
 
-template <int TM, int TN, int WM, int WN, bool WIDE>
+template <class T, int TM, int TN, bool WIDE>
 void product_launch(ProductArgs& a, hipStream_t s)
 {
     a.tiles_n = (a.n + TN - 1) / TN;
     a.tiles_m = (a.m + TM - 1) / TM;
-    long long grid = (long long)a.tiles_m * a.tiles_n;
-    if (a.grouping == PRODUCT_ROWS) grid = ((long long)a.m / TM + a.experts) * a.tiles_n;
-    if (a.grouping == PRODUCT_SUM) grid *= a.experts;
-    require(grid <= 0x7fffffffll, "too many tiles for one call");
-    product_kernel<TM, TN, WM, WN, WIDE><<<(unsigned)grid, WM * WN * 64, 0, s>>>(a);
+    long long tiles = (long long)a.tiles_m * a.tiles_n;
+    if (a.grouping == PRODUCT_ROWS) tiles = ((long long)a.m / TM + a.experts) * a.tiles_n;
+    if (a.grouping == PRODUCT_SUM) tiles *= a.experts;
+    require(tiles <= 0x7fffffffll, "too many tiles for one call");
+    const long long slots = (long long)num_cus() * (TM * TN > 128 * 128 ? 1 : 2);
+    product_kernel<T, TM, TN, WIDE><<<(unsigned)std::min(tiles, slots), 256, 0, s>>>(a);
     GRAFT_LAUNCH_CHECK();
 }
 
@@ -306,11 +486,25 @@ void fp8_product(const Fp8ProductOption& o, const uint8_t* a, const uint8_t* a_s
     p.out_stride = o.outStride;
     p.out_type = o.outType;
     p.relu = o.activation == 1;
-    p.vec = (uintptr_t)out % (4 * data_bytes(o.outType)) == 0 && o.outStride % 4 == 0;
-    // Up to two blocks of k the output's bytes bound the product, and widening
-    // costs nothing.
-    if (o.outType == DATA_F32 || p.pitch <= 256) product_launch<128, 128, 2, 2, true>(p, s);
-    else product_launch<128, 128, 2, 2, false>(p, s);
+    p.vec = aligned16(out) && o.outStride * data_bytes(o.outType) % 16 == 0;
+    with_type(o.outType, [&](auto zero) {
+        using T = decltype(zero);
+        // fp32 results, weight gradients of any type, and products of up to two
+        // blocks of k, which their output's bytes bound: there widening costs nothing.
+        if (std::is_same_v<T, float> || o.grouping == PRODUCT_SUM || p.pitch <= 256) return product_launch<T, 128, 128, true>(p, s);
+        if constexpr (!std::is_same_v<T, float>) {
+            // Rounds of tiles over the CUs, by what a round takes: 256 x 256 at 2.5
+            // PFLOP/s, two 128 x 128 a CU at 2.2.
+            const long long cus = num_cus(), experts = o.grouping == PRODUCT_DENSE ? 0 : o.numExperts;
+            auto tiles = [&](int t) {
+                const long long n = (o.n + t - 1) / t, m = (o.m + t - 1) / t;
+                return o.grouping == PRODUCT_ROWS ? (o.m / t + experts) * n : m * n;
+            };
+            const long long large = (tiles(256) + cus - 1) / cus, small = (tiles(128) + 2 * cus - 1) / (2 * cus);
+            if (large * 4 * 22 < small * 2 * 25) product_launch<T, 256, 256, false>(p, s);
+            else product_launch<T, 128, 128, false>(p, s);
+        }
+    });
 }
 
 }  // namespace graft

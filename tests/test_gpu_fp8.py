@@ -157,7 +157,7 @@ def option(m, n, k, experts=1, grouping=0, rows_b=128, act=0, code=0, stride=Non
     (31, 96, 5000, 0, 1, 0, 0, 0), (33, 64, 640, 1, 128, 1, 4, 0), (64, 1000, 1024, 2, 128, 0, 0, 0),
     (65, 31, 384, 0, 128, 0, 1, 0), (100, 300, 900, 0, 1, 0, 0, 0), (128, 128, 256, 1, 128, 0, 0, 0),
     (129, 1290, 127, 0, 128, 0, 0, 0), (257, 513, 1000, 2, 1, 1, 0, 2), (300, 2048, 512, 1, 128, 0, 8, 0),
-    (1000, 700, 700, 0, 128, 0, 0, 0), (2049, 1025, 260, 2, 128, 0, 0, 0), (4100, 2100, 128, 1, 1, 0, 0, 0)])
+    (1000, 700, 700, 0, 128, 0, 0, 0), (4096, 4090, 700, 2, 128, 0, 0, 0), (4090, 4096, 4300, 1, 1, 1, 8, 0), (2049, 1025, 260, 2, 128, 0, 0, 0), (4100, 2100, 128, 1, 1, 0, 0, 0)])
 def test_dense_product(m, n, k, code, rows_b, act, pad, shift):
     print(f"[product] m={m} n={n} k={k} type={code}", flush=True)
     g = R.gen(m + n + k)
@@ -184,7 +184,7 @@ def segments(lengths, align):
 @pytest.mark.parametrize("lengths,align,n,k,code,rows_b", [
     ([5], 1, 40, 100, 0, 128), ([0, 3, 0, 0, 130, 1], 1, 200, 300, 1, 128), ([128, 0, 300, 77], 128, 640, 512, 2, 128),
     ([0, 0, 0], 128, 64, 64, 0, 1), ([1] * 20 + [0] * 60 + [7] * 5, 1, 136, 260, 0, 1), ([700, 10, 513], 128, 300, 384, 2, 128),
-    ([2, 1, 3, 0, 2], 16, 1030, 1000, 1, 128), ([20, 40, 60, 17], 16, 256, 640, 0, 128), ([1500, 2000], 128, 520, 130, 1, 1)])
+    ([4000, 60, 1, 0, 3000], 128, 2050, 300, 2, 128), ([2, 1, 3, 0, 2], 16, 1030, 1000, 1, 128), ([20, 40, 60, 17], 16, 256, 640, 0, 128), ([1500, 2000], 128, 520, 130, 1, 1)])
 def test_rows_product(lengths, align, n, k, code, rows_b):
     print(f"[rows product] {lengths} n={n} k={k}", flush=True)
     E = len(lengths)
@@ -206,7 +206,7 @@ def test_rows_product(lengths, align, n, k, code, rows_b):
 
 @pytest.mark.parametrize("lengths,m,n,code,rows_b", [
     ([100], 40, 60, 0, 1), ([0, 128, 0, 300, 1], 130, 257, 0, 1), ([1000, 0, 129], 300, 200, 2, 1), ([0, 0], 33, 20, 1, 128),
-    ([5, 6, 7, 8], 512, 640, 0, 1), ([], 8, 8, 0, 1), ([2500, 130], 64, 1000, 1, 1)])
+    ([5, 6, 7, 8], 512, 640, 0, 1), ([5, 4300, 7, 8], 512, 640, 0, 1), ([0, 700, 384, 5], 2050, 2100, 1, 1), ([], 8, 8, 0, 1), ([2500, 130], 64, 1000, 1, 1)])
 def test_sum_product(lengths, m, n, code, rows_b):
     print(f"[sum product] {lengths} m={m} n={n}", flush=True)
     lengths = lengths or [0]
