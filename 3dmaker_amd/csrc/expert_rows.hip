@@ -52,36 +52,43 @@ __global__ __launch_bounds__(kRowThreads) void combine_kernel(RowArgs a)
     *reinterpret_cast<Vec<T, N>*>((T*)a.out + t * a.out_stride + col) = o;
 }
 
-// A wave: four slots of a token at a time.
-template <class T, int N>
+// A wave: K slots of a token at a time, their rows' loads under way together.
+// Positions outside read row 0 and count for nothing.
+template <class T, int N, int K>
 __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(RowArgs a)
 {
-    const long long t = (long long)blockIdx.x * (kRowThreads / 64) + threadIdx.x / 64;
+    const long long t = (long long)blockIdx.x * (kRowThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int lane = threadIdx.x & 63;
     if (t >= a.tokens) return;
     const T* d = (const T*)a.dout + t * a.out_stride;
-    for (int j0 = 0; j0 < a.topk; j0 += 4) {
-        const T* row[4];
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j0 = 0; j0 < a.topk; j0 += K) {
+        const T* row[K];
+        bool there[K];
+        float acc[K];
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
+        for (int q = 0; q < K; q++) {
             const int p = j0 + q < a.topk ? a.position[t * a.topk + j0 + q] : -1;
-            row[q] = (unsigned)p < (unsigned)a.num_rows ? (const T*)a.rows + (long long)p * a.row_stride : nullptr;
+            there[q] = (unsigned)p < (unsigned)a.num_rows;
+            row[q] = (const T*)a.rows + (there[q] ? (long long)p * a.row_stride : 0);
+            acc[q] = 0.0f;
         }
-        for (int c = lane * N; c < a.dim; c += 64 * N) {
-            const Vec<T, N> dv = *reinterpret_cast<const Vec<T, N>*>(d + c);
+        if (a.num_rows > 0) {
+#pragma unroll 2
+            for (int c = lane * N; c < a.dim; c += 64 * N) {
+                const Vec<T, N> dv = *reinterpret_cast<const Vec<T, N>*>(d + c);
+                Vec<T, N> rv[K];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (!row[q]) continue;
-                const Vec<T, N> rv = *reinterpret_cast<const Vec<T, N>*>(row[q] + c);
+                for (int q = 0; q < K; q++) rv[q] = *reinterpret_cast<const Vec<T, N>*>(row[q] + c);
 #pragma unroll
-                for (int i = 0; i < N; i++) acc[q] = fmaf((float)dv[i], (float)rv[i], acc[q]);
+                for (int q = 0; q < K; q++)
+#pragma unroll
+                    for (int i = 0; i < N; i++) acc[q] = fmaf((float)dv[i], (float)rv[q][i], acc[q]);
             }
         }
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
+        for (int q = 0; q < K; q++) {
             const float sum = lanes_sum<64>(acc[q]);
-            if (lane == 0 && j0 + q < a.topk) a.dweights[t * a.topk + j0 + q] = sum;
+            if (lane == 0 && j0 + q < a.topk) a.dweights[t * a.topk + j0 + q] = there[q] ? sum : 0.0f;
         }
     }
 }
@@ -152,8 +159,12 @@ void expert_combine_backward(int dim, int type, const void* rows, int num_rows, 
     a.dout = dout;
     a.dweights = dweights;
     with_vec(type, row_vec(a, dout, data_bytes(type)), [&](auto zero, auto N) {
-        combine_backward_kernel<decltype(zero), decltype(N)::value>
-            <<<(unsigned)((tokens + 3ll) / 4), kRowThreads, 0, s>>>(a);
+        using T = decltype(zero);
+        constexpr int n = decltype(N)::value;
+        const unsigned wgs = (unsigned)((tokens + 3ll) / 4);
+        if (topK == 1) combine_backward_kernel<T, n, 1><<<wgs, kRowThreads, 0, s>>>(a);
+        else if (topK == 2) combine_backward_kernel<T, n, 2><<<wgs, kRowThreads, 0, s>>>(a);
+        else combine_backward_kernel<T, n, 4><<<wgs, kRowThreads, 0, s>>>(a);
     });
     GRAFT_LAUNCH_CHECK();
 }

@@ -26,7 +26,7 @@ struct QuantArgs {
     int rows, cols, slots_per_row, src_rows;
     int pitch, spitch, pitch_t, spitch_t;
     long long stride, batch_stride, gate_stride;
-    bool vec;  // source (and gate) rows take 16-byte loads
+    bool vec;  // source rows are whole 16-byte pieces of eight columns
 };
 
 __device__ __forceinline__ uint32_t magnitude(float v)
@@ -59,91 +59,125 @@ __device__ __forceinline__ uint32_t fp8x4(const float* v, float inverse)
     return (uint32_t)w;
 }
 
-// Eight consecutive values of a row, zero from `n` on.
-template <class T>
-__device__ __forceinline__ void load8(float (&v)[8], const T* p, int n, bool vec)
+// Where a quantised row comes from; weight 0 and no source where there is none.
+struct Source {
+    long long row;
+    float weight;
+    bool there;
+};
+
+__device__ __forceinline__ Source source_of(const QuantArgs& a, int row)
 {
-    if (vec && n >= 8) {
-        constexpr int N = 16 / sizeof(T);
+    Source s{row, 1.0f, row < a.rows};
+    if (a.order) {
+        const int slot = s.there ? a.order[row] : -1;
+        s.row = slot / a.slots_per_row;
+        s.there = slot >= 0 && s.row < a.src_rows;
+        if (a.weights && s.there) s.weight = a.weights[slot];
+    }
+    if (!s.there) s.row = 0;
+    return s;
+}
+
+// Columns col .. col + 7 of R quantised rows: all rows' loads are under way
+// before the first is used (rows without a source load the first row, columns
+// behind the last the first ones).
+template <class T, int R>
+__device__ __forceinline__ void load_rows(float (&v)[R][8], const QuantArgs& a, const T* src, const int (&row)[R],
+                                          const int (&col)[R])
+{
+    Source s[R];
 #pragma unroll
-        for (int i = 0; i < 8; i += N) {
-            const Vec<T, N> w = *reinterpret_cast<const Vec<T, N>*>(p + i);
+    for (int i = 0; i < R; i++) s[i] = source_of(a, row[i]);
+    if (a.vec) {
+        constexpr int N = 16 / sizeof(T), P = 8 / N;
+        Vec<T, N> raw[R][P];
 #pragma unroll
-            for (int j = 0; j < N; j++) v[i + j] = (float)w[j];
-        }
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int q = 0; q < P; q++)
+                raw[i][q] = *reinterpret_cast<const Vec<T, N>*>(src + s[i].row * a.stride + (col[i] < a.cols ? col[i] : 0) + q * N);
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[i][j] = s[i].there && col[i] < a.cols ? (float)raw[i][j / N][j % N] : 0.0f;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = i < n ? (float)p[i] : 0.0f;
-    }
-}
-
-// Columns col .. col + 7 of quantised row `row`: gathered, weighted, gated.
-template <class T>
-__device__ __forceinline__ void load_row8(float (&v)[8], const QuantArgs& a, const T* src, int row, int col)
-{
-    const int n = a.cols - col;
-    long long from = row;
-    float w = 1.0f;
-    bool there = row < a.rows && n > 0;
-    if (there && a.order) {
-        const int slot = a.order[row];
-        from = slot / a.slots_per_row;
-        there = slot >= 0 && from < a.src_rows;
-        if (there && a.weights) w = a.weights[slot];
-    }
-    if (!there) {
+        for (int i = 0; i < R; i++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = 0.0f;
-        return;
+            for (int j = 0; j < 8; j++)
+                v[i][j] = s[i].there && col[i] + j < a.cols ? (float)src[s[i].row * a.stride + col[i] + j] : 0.0f;
     }
-    load8(v, src + from * a.stride + col, n, a.vec);
     if (a.weights) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= w;
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[i][j] = s[i].there ? v[i][j] * s[i].weight : 0.0f;
     }
     if (a.gate) {
-        float g[8];
-        load8(g, (const T*)a.gate + (long long)row * a.gate_stride + col, n, a.vec);
+        const T* gate = (const T*)a.gate;
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = g[i] > 0.0f ? v[i] : 0.0f;
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                v[i][j] = s[i].there && col[i] + j < a.cols &&
+                                  (float)gate[(long long)row[i] * a.gate_stride + col[i] + j] > 0.0f
+                              ? v[i][j] : 0.0f;
     }
 }
 
-// Rows only: 16 lanes a (row, block).
-template <class T>
+// Rows only: 16 lanes a (row, block), UNITS of them 16 apart.  Four at a time
+// once there are enough for all CUs (65,536 x 1,024 bf16 gathered: 50 us with
+// one, whose loads wait for one another's row numbers).
+template <class T, int UNITS>
 __global__ __launch_bounds__(kQuantThreads) void quant_rows_kernel(QuantArgs a)
 {
-    const int blocks = a.pitch / 128;
-    const long long unit = (long long)blockIdx.x * (kQuantThreads / 16) + threadIdx.x / 16;
-    const int row = (int)(unit / blocks), block = (int)(unit % blocks), col = block * 128 + (threadIdx.x & 15) * 8;
+    const uint32_t blocks = a.pitch / 128;
+    const unsigned long long first = (unsigned long long)blockIdx.x * (16 * UNITS);
+    const uint32_t row0 = (uint32_t)(first / blocks), in0 = (uint32_t)(first % blocks);
     const T* src = (const T*)a.src + (long long)blockIdx.y * a.batch_stride;
-    float v[8];
-    load_row8(v, a, src, row, col);
-    uint32_t top = 0;
+    float v[UNITS][8];
+    int row[UNITS], col[UNITS];
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, magnitude(v[i]));
-    const int byte = scale_byte(lanes_umax<16>(top));
-    if (row >= a.rows) return;
-    const float inv = inverse_scale(byte);
-    const long long r = (long long)blockIdx.y * a.rows + row;
-    *reinterpret_cast<Vec<uint32_t, 2>*>(a.q + r * a.pitch + col) = Vec<uint32_t, 2>{fp8x4(v, inv), fp8x4(v + 4, inv)};
-    if ((threadIdx.x & 15) == 0) a.scales[r * a.spitch + block] = (uint8_t)byte;
+    for (int u = 0; u < UNITS; u++) {
+        const uint32_t in = in0 + u * 16 + threadIdx.x / 16, down = in / blocks;
+        row[u] = (int)(row0 + down);
+        col[u] = (int)(in - down * blocks) * 128 + (threadIdx.x & 15) * 8;
+    }
+    load_rows(v, a, src, row, col);
+#pragma unroll
+    for (int u = 0; u < UNITS; u++) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, magnitude(v[u][j]));
+        const int byte = scale_byte(lanes_umax<16>(top));
+        if (row[u] >= a.rows) continue;
+        const float inv = inverse_scale(byte);
+        const long long r = (long long)blockIdx.y * a.rows + row[u];
+        *reinterpret_cast<Vec<uint32_t, 2>*>(a.q + r * a.pitch + col[u]) =
+            Vec<uint32_t, 2>{fp8x4(v[u], inv), fp8x4(v[u] + 4, inv)};
+        if ((threadIdx.x & 15) == 0) a.scales[r * a.spitch + col[u] / 128] = (uint8_t)byte;
+    }
 }
 
 // A tile of 128 x 128 in registers (thread: 8 rows by 8 columns), as rows,
-// as columns or both.
+// as columns or both.  The transposed bytes cross LDS in pieces of 8, piece ty of
+// column c at ty ^ (c / 8): a wave's writes, one column of every eight, spread
+// over the banks.
 template <class T, bool BLOCKS>
 __global__ __launch_bounds__(kQuantThreads) void quant_tile_kernel(QuantArgs a)
 {
     __shared__ uint32_t tops[16][128];
     __shared__ uint32_t wave_top[4];
-    __shared__ __attribute__((aligned(16))) uint8_t tile[128][144];  // transposed bytes, rows 16-byte aligned
+    __shared__ __attribute__((aligned(16))) uint8_t tile[128 * 128];
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int r0 = blockIdx.x * 128, c0 = blockIdx.y * 128;
     const T* src = (const T*)a.src + (long long)blockIdx.z * a.batch_stride;
     float v[8][8];
+    int row_of[8], col_of[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) load_row8(v[i], a, src, r0 + ty * 8 + i, c0 + tx * 8);
+    for (int i = 0; i < 8; i++) row_of[i] = r0 + ty * 8 + i, col_of[i] = c0 + tx * 8;
+    load_rows(v, a, src, row_of, col_of);
     int block_byte = 0;
     if (BLOCKS) {
         uint32_t top = 0;
@@ -159,7 +193,6 @@ __global__ __launch_bounds__(kQuantThreads) void quant_tile_kernel(QuantArgs a)
     if (a.q) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int row = r0 + ty * 8 + i;
             int byte = block_byte;
             if (!BLOCKS) {
                 uint32_t top = 0;
@@ -167,9 +200,9 @@ __global__ __launch_bounds__(kQuantThreads) void quant_tile_kernel(QuantArgs a)
                 for (int j = 0; j < 8; j++) top = max(top, magnitude(v[i][j]));
                 byte = scale_byte(lanes_umax<16>(top));
             }
-            if (row >= a.rows) continue;
+            if (row_of[i] >= a.rows) continue;
             const float inv = inverse_scale(byte);
-            const long long r = (long long)blockIdx.z * a.rows + row;
+            const long long r = (long long)blockIdx.z * a.rows + row_of[i];
             *reinterpret_cast<Vec<uint32_t, 2>*>(a.q + r * a.pitch + c0 + tx * 8) =
                 Vec<uint32_t, 2>{fp8x4(v[i], inv), fp8x4(v[i] + 4, inv)};
             if (!BLOCKS && tx == 0) a.scales[r * a.spitch + blockIdx.y] = (uint8_t)byte;
@@ -184,7 +217,7 @@ __global__ __launch_bounds__(kQuantThreads) void quant_tile_kernel(QuantArgs a)
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) top = max(top, magnitude(v[i][j]));
-            tops[ty][tx * 8 + j] = top;
+            tops[ty][j * 16 + tx] = top;  // column tx * 8 + j
         }
         __syncthreads();
         if (threadIdx.x < 128) {
@@ -197,10 +230,11 @@ __global__ __launch_bounds__(kQuantThreads) void quant_tile_kernel(QuantArgs a)
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const int byte = BLOCKS ? block_byte : scale_byte(tops[0][tx * 8 + j]);
+        const int byte = BLOCKS ? block_byte : scale_byte(tops[0][j * 16 + tx]);
         const float inv = inverse_scale(byte);
         const float c[8] = {v[0][j], v[1][j], v[2][j], v[3][j], v[4][j], v[5][j], v[6][j], v[7][j]};
-        *reinterpret_cast<Vec<uint32_t, 2>*>(&tile[tx * 8 + j][ty * 8]) = Vec<uint32_t, 2>{fp8x4(c, inv), fp8x4(c + 4, inv)};
+        *reinterpret_cast<Vec<uint32_t, 2>*>(&tile[(tx * 8 + j) * 128 + ((ty ^ tx) * 8)]) =
+            Vec<uint32_t, 2>{fp8x4(c, inv), fp8x4(c + 4, inv)};
         const int col = c0 + tx * 8 + j;
         if (!BLOCKS && ty == 0 && col < a.cols)
             a.scalesT[((long long)blockIdx.z * a.cols + col) * a.spitch_t + blockIdx.x] = (uint8_t)byte;
@@ -210,10 +244,12 @@ __global__ __launch_bounds__(kQuantThreads) void quant_tile_kernel(QuantArgs a)
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int unit = i * kQuantThreads + threadIdx.x, c = unit >> 3, at = (unit & 7) * 16;
-        if (c0 + c < a.cols)
-            *reinterpret_cast<Vec<uint32_t, 4>*>(a.qt + ((long long)blockIdx.z * a.cols + c0 + c) * a.pitch_t + r0 + at) =
-                *reinterpret_cast<const Vec<uint32_t, 4>*>(&tile[c][at]);
+        const int unit = i * kQuantThreads + threadIdx.x, c = unit >> 3, piece = (unit & 7) * 2, key = c >> 3;
+        if (c0 + c >= a.cols) continue;
+        const Vec<uint32_t, 4> w = *reinterpret_cast<const Vec<uint32_t, 4>*>(&tile[c * 128 + (((piece ^ key) & ~1) * 8)]);
+        const Vec<uint32_t, 4> swapped{w[2], w[3], w[0], w[1]};
+        *reinterpret_cast<Vec<uint32_t, 4>*>(a.qt + ((long long)blockIdx.z * a.cols + c0 + c) * a.pitch_t + r0 + piece * 8) =
+            key & 1 ? swapped : w;
     }
 }
 
@@ -260,17 +296,20 @@ void fp8_quantize(const Fp8QuantOption& o, const void* src, const int* order, co
     a.gate_stride = o.gateStride;
     const int bytes = data_bytes(o.srcType);
     auto fits = [&](const void* p, long long stride) { return aligned16(p) && stride * bytes % 16 == 0; };
-    a.vec = fits(src, o.srcStride) && (o.batch == 1 || o.srcBatchStride * bytes % 16 == 0) &&
-            (!gate || fits(gate, o.gateStride));
+    a.vec = o.srcRows > 0 && o.cols % 8 == 0 && fits(src, o.srcStride) &&
+            (o.batch == 1 || o.srcBatchStride * bytes % 16 == 0);
     const int cb = a.pitch / 128, rb = a.pitch_t / 128;
     with_type(o.srcType, [&](auto zero) {
         using T = decltype(zero);
         if (o.blockRows == 128) quant_tile_kernel<T, true><<<dim3(rb, cb, o.batch), kQuantThreads, 0, s>>>(a);
         else if (qt) quant_tile_kernel<T, false><<<dim3(rb, cb, o.batch), kQuantThreads, 0, s>>>(a);
         else {
-            const long long units = (long long)o.rows * cb, wgs = (units + kQuantThreads / 16 - 1) / (kQuantThreads / 16);
-            require(wgs <= 0x7fffffffll, "too many blocks for one call");
-            quant_rows_kernel<T><<<dim3((unsigned)wgs, o.batch), kQuantThreads, 0, s>>>(a);
+            const long long units = (long long)o.rows * cb;
+            require(units / 64 < 0x7fffffffll, "too many blocks for one call");
+            if (units * o.batch >= 64ll * 8 * num_cus())
+                quant_rows_kernel<T, 4><<<dim3((unsigned)((units + 63) / 64), o.batch), kQuantThreads, 0, s>>>(a);
+            else
+                quant_rows_kernel<T, 1><<<dim3((unsigned)((units + 15) / 16), o.batch), kQuantThreads, 0, s>>>(a);
         }
     });
     GRAFT_LAUNCH_CHECK();

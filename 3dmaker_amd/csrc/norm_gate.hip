@@ -18,7 +18,6 @@ namespace graft {
 namespace {
 
 constexpr int kMaxDim = 8192;
-constexpr int kMaxParts = 1024;  // workgroups of a backward, each with its sums over rows
 
 struct NormArgs {
     const void *x, *f, *gate;
@@ -26,7 +25,7 @@ struct NormArgs {
     void *y, *h;
     long long sx, sf, sg, sy, sh;
     int rows, dim, gate_rows, post, pre;
-    float alpha, beta, eps;
+    float alpha, beta, eps, inv_dim;
     // backward
     const void *dy, *dh;
     void *dx, *df, *dgate;
@@ -76,61 +75,147 @@ struct Row {
     }
 };
 
+// A row's pieces as they lie in memory: what is fetched ahead.
+template <class T, int VEC, int THREADS, int PER>
+struct Raw {
+    Vec<T, VEC> v[PER];
+
+    __device__ __forceinline__ void load(const T* p, int sub, int dim)
+    {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int c = (i * THREADS + sub) * VEC;
+            if (c < dim) v[i] = *reinterpret_cast<const Vec<T, VEC>*>(p + c);
+        }
+    }
+    __device__ __forceinline__ void widen(float (&to)[VEC * PER], int sub, int dim) const
+    {
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) to[i * VEC + j] = (i * THREADS + sub) * VEC < dim ? (float)v[i][j] : 0.0f;
+    }
+};
+
+// The thread's elements of a parameter (fp32), `none` where there is no
+// parameter.  In pieces of 16 bytes where the rows' are.
+template <int VEC, int THREADS, int PER>
+struct Param {
+    float v[VEC * PER];
+
+    __device__ __forceinline__ void load(const float* p, float none, int sub, int dim)
+    {
+#pragma unroll
+        for (int i = 0; i < VEC * PER; i++) v[i] = none;
+        if (!p) return;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int c = (i * THREADS + sub) * VEC;
+            if (c < dim) {
+                constexpr int P = VEC < 4 ? VEC : 4;
+#pragma unroll
+                for (int j = 0; j < VEC; j += P) {
+                    const Vec<float, P> w = *reinterpret_cast<const Vec<float, P>*>(p + c + j);
+#pragma unroll
+                    for (int q = 0; q < P; q++) v[i * VEC + j + q] = w[q];
+                }
+            }
+        }
+    }
+};
+
+// f(element, column) over the thread's pieces that lie in the row (a piece is
+// whole: rows in pieces of more than one element are multiples of it).
 template <int VEC, int THREADS, int PER, class F>
 __device__ __forceinline__ void each(int sub, int dim, F&& f)
 {
 #pragma unroll
-    for (int i = 0; i < PER; i++)
+    for (int i = 0; i < PER; i++) {
+        const int c = (i * THREADS + sub) * VEC;
+        if (c < dim) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) {
-            const int c = (i * THREADS + sub) * VEC + j;
-            if (c < dim) f(i * VEC + j, c);
+            for (int j = 0; j < VEC; j++) f(i * VEC + j, c + j);
         }
+    }
 }
 
-// Sum over the THREADS of a row, in the same order for all of them.
+// Sums over the THREADS of a row, in the same order for all of them.  Calls that
+// follow each other use different slots: the barrier of one is what keeps the
+// next use of another's slot behind its last read.
 template <int THREADS>
-__device__ __forceinline__ float row_sum(float v, float* lds)
+__device__ __forceinline__ float row_sum(float v, float (*lds)[THREADS / 64], int slot)
 {
     v = lanes_sum<64>(v);
     if constexpr (THREADS > 64) {
         constexpr int W = THREADS / 64;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        if ((threadIdx.x & 63) == 0) lds[slot][threadIdx.x >> 6] = v;
         __syncthreads();
         v = 0.0f;
 #pragma unroll
-        for (int i = 0; i < W; i++) v += lds[i];
+        for (int i = 0; i < W; i++) v += lds[slot][i];
     }
     return v;
+}
+
+template <int THREADS>
+__device__ __forceinline__ void row_sum2(float& u, float& v, float (*lds)[THREADS / 64], int slot)
+{
+    u = lanes_sum<64>(u);
+    v = lanes_sum<64>(v);
+    if constexpr (THREADS > 64) {
+        constexpr int W = THREADS / 64;
+        if ((threadIdx.x & 63) == 0) lds[slot][threadIdx.x >> 6] = u, lds[slot + 1][threadIdx.x >> 6] = v;
+        __syncthreads();
+        u = v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; i++) u += lds[slot][i], v += lds[slot + 1][i];
+    }
 }
 
 // n = normalised v (in place) and 1 / its deviation; v's elements behind the
 // row stay zero.
 template <int VEC, int THREADS, int PER>
-__device__ __forceinline__ float normalise(float (&v)[VEC * PER], int kind, int sub, int dim, float eps, float* lds)
+__device__ __forceinline__ float normalise(float (&v)[VEC * PER], int kind, int sub, int dim, float inv_dim, float eps,
+                                           float (*lds)[THREADS / 64], int slot)
 {
     if (kind == NORM_NONE) return 1.0f;
     if (kind == NORM_LAYER) {
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < VEC * PER; i++) sum += v[i];
-        const float mean = row_sum<THREADS>(sum, lds) / (float)dim;
+        const float mean = row_sum<THREADS>(sum, lds, slot) * inv_dim;
         each<VEC, THREADS, PER>(sub, dim, [&](int i, int) { v[i] -= mean; });
     }
     float sq = 0.0f;
 #pragma unroll
     for (int i = 0; i < VEC * PER; i++) sq = fmaf(v[i], v[i], sq);
-    const float r = 1.0f / sqrtf(row_sum<THREADS>(sq, lds) / (float)dim + eps);
+    const float r = rsqrtf(row_sum<THREADS>(sq, lds, slot + 1) * inv_dim + eps);
 #pragma unroll
     for (int i = 0; i < VEC * PER; i++) v[i] *= r;
     return r;
 }
 
+// v = v w + b
+template <int VEC, int THREADS, int PER>
+__device__ __forceinline__ void affine(float (&v)[VEC * PER], const float* w, const float* b, int sub, int dim)
+{
+    Param<VEC, THREADS, PER> p;
+    if (w) {
+        p.load(w, 1.0f, sub, dim);
+#pragma unroll
+        for (int i = 0; i < VEC * PER; i++) v[i] *= p.v[i];
+    }
+    if (b) {
+        p.load(b, 0.0f, sub, dim);
+#pragma unroll
+        for (int i = 0; i < VEC * PER; i++) v[i] += p.v[i];
+    }
+}
+
 template <class T, int VEC, int THREADS, int PER>
 __global__ __launch_bounds__(256) void norm_gate_kernel(NormArgs a)
 {
-    __shared__ float lds[4];
+    __shared__ float lds[4][THREADS / 64];
     using R = Row<T, VEC, THREADS, PER>;
     const int sub = threadIdx.x & (THREADS - 1);
     const long long row = (long long)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
@@ -140,11 +225,8 @@ __global__ __launch_bounds__(256) void norm_gate_kernel(NormArgs a)
     if (a.f) {
         R u;
         u.load((const T*)a.f + row * a.sf, sub, a.dim);
-        normalise<VEC, THREADS, PER>(u.v, a.post, sub, a.dim, a.eps, lds);
-        each<VEC, THREADS, PER>(sub, a.dim, [&](int i, int c) {
-            if (a.post_w) u.v[i] *= a.post_w[c];
-            if (a.post_b) u.v[i] += a.post_b[c];
-        });
+        normalise<VEC, THREADS, PER>(u.v, a.post, sub, a.dim, a.inv_dim, a.eps, lds, 0);
+        affine<VEC, THREADS, PER>(u.v, a.post_w, a.post_b, sub, a.dim);
         if (a.gate) {
             R g;
             g.load((const T*)a.gate + row / a.gate_rows * a.sg, sub, a.dim);
@@ -159,55 +241,61 @@ __global__ __launch_bounds__(256) void norm_gate_kernel(NormArgs a)
     }
     if (a.y) y.store((T*)a.y + row * a.sy, sub, a.dim);
     if (!a.h) return;
-    normalise<VEC, THREADS, PER>(y.v, a.pre, sub, a.dim, a.eps, lds);
-    each<VEC, THREADS, PER>(sub, a.dim, [&](int i, int c) {
-        if (a.pre_w) y.v[i] *= a.pre_w[c];
-        if (a.pre_b) y.v[i] += a.pre_b[c];
-    });
+    normalise<VEC, THREADS, PER>(y.v, a.pre, sub, a.dim, a.inv_dim, a.eps, lds, 2);
+    affine<VEC, THREADS, PER>(y.v, a.pre_w, a.pre_b, sub, a.dim);
     y.store((T*)a.h + row * a.sh, sub, a.dim);
 }
 
 // dL/dinput (in place of d) of a norm whose normalised input is n and 1 /
-// deviation r; the parameters' sums of this row added.
+// deviation r; the parameters' sums of this row added.  w: its weights.
 template <int VEC, int THREADS, int PER>
 __device__ __forceinline__ void norm_back(float (&d)[VEC * PER], const float (&n)[VEC * PER], float r, int kind,
-                                          const float* w, float (&dw)[VEC * PER], float (&db)[VEC * PER], int sub, int dim,
-                                          float* lds)
+                                          const float (&w)[VEC * PER], float (&dw)[VEC * PER], float (&db)[VEC * PER],
+                                          int sub, int dim, float inv_dim, float (*lds)[THREADS / 64], int slot)
 {
+    constexpr int N = VEC * PER;
     if (kind == NORM_NONE) return;
     float m = 0.0f, p = 0.0f;
-    each<VEC, THREADS, PER>(sub, dim, [&](int i, int c) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {  // d and n are zero behind the row
         dw[i] = fmaf(d[i], n[i], dw[i]);
         db[i] += d[i];
-        if (w) d[i] *= w[c];
+        d[i] *= w[i];
         m += d[i];
         p = fmaf(d[i], n[i], p);
-    });
-    m = kind == NORM_LAYER ? row_sum<THREADS>(m, lds) / (float)dim : 0.0f;
-    p = row_sum<THREADS>(p, lds) / (float)dim;
+    }
+    row_sum2<THREADS>(m, p, lds, slot);
+    m = kind == NORM_LAYER ? m * inv_dim : 0.0f;
+    p *= inv_dim;
     each<VEC, THREADS, PER>(sub, dim, [&](int i, int) { d[i] = r * (d[i] - m - n[i] * p); });
 }
 
-// A workgroup: `chunk` rows of a span, its row groups (waves for THREADS 64)
-// in turn; sums over its rows go to sums[part], or for one part to the outputs.
+// A workgroup: `chunk` rows of a span, its row groups (waves for THREADS 64) in
+// turn; sums over its rows go to sums[part], or for one part to the outputs.  The
+// next row is fetched while this one is worked on: without that a row waits for
+// four tensors one after the other (16,389 x 1,280 fp16: 237 us, 16 % of the
+// copy rate).
 template <class T, int VEC, int THREADS, int PER, int WG>
 __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
 {
-    constexpr int kGroups = WG / THREADS;
+    constexpr int kGroups = WG / THREADS, N = VEC * PER;
+    constexpr bool kKeep = WG <= 512;  // parameters in registers for all rows, where there are enough
     using R = Row<T, VEC, THREADS, PER>;
-    __shared__ float lds[WG / 64];
-    __shared__ float join[kGroups > 1 ? kGroups : 1][kGroups > 1 ? THREADS * VEC * PER : 1];
-    const int sub = threadIdx.x & (THREADS - 1), group = threadIdx.x / THREADS;
+    using W = Raw<T, VEC, THREADS, PER>;
+    using P = Param<VEC, THREADS, PER>;
+    __shared__ float lds[8][THREADS / 64];
+    __shared__ float join[kGroups > 1 ? kGroups : 1][kGroups > 1 ? THREADS * N : 1];
+    const int sub = threadIdx.x % THREADS, group = __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
     const long long span0 = (long long)(blockIdx.x / a.per_span) * a.span;
     const long long begin = span0 + (long long)(blockIdx.x % a.per_span) * a.chunk;
     const int span_end = (int)(span0 + a.span < a.rows ? span0 + a.span : a.rows);
     const int r0 = (int)(begin < span_end ? begin : span_end), r1 = r0 + a.chunk < span_end ? r0 + a.chunk : span_end;
-    float dw1[R::N], db1[R::N], dw2[R::N], db2[R::N], dg[R::N];
+    float dw1[N], db1[N], dw2[N], db2[N], dg[N];
 #pragma unroll
-    for (int i = 0; i < R::N; i++) dw1[i] = db1[i] = dw2[i] = db2[i] = dg[i] = 0.0f;
+    for (int i = 0; i < N; i++) dw1[i] = db1[i] = dw2[i] = db2[i] = dg[i] = 0.0f;
 
     // The groups' sums of a column array, in group order; the first group has them.
-    auto joined = [&](float (&v)[R::N]) {
+    auto joined = [&](float (&v)[N]) {
         if constexpr (kGroups > 1) {
             __syncthreads();
             each<VEC, THREADS, PER>(sub, a.dim, [&](int i, int c) { join[group][c] = v[i]; });
@@ -221,72 +309,85 @@ __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
                 });
         }
     };
+    W rx, rf, rg, rdy, rdh;
+    auto fetch = [&](int row) {
+        rx.load((const T*)a.x + (long long)row * a.sx, sub, a.dim);
+        if (a.f) rf.load((const T*)a.f + (long long)row * a.sf, sub, a.dim);
+        if (a.gate) rg.load((const T*)a.gate + (long long)(row / a.gate_rows) * a.sg, sub, a.dim);
+        if (a.dh) rdh.load((const T*)a.dh + (long long)row * a.sh, sub, a.dim);
+        if (a.dy) rdy.load((const T*)a.dy + (long long)row * a.sy, sub, a.dim);
+    };
+    P w1, b1, w2;
+    auto parameters = [&] {
+        w1.load(a.post_w, 1.0f, sub, a.dim);
+        b1.load(a.post_b, 0.0f, sub, a.dim);
+        w2.load(a.pre_w, 1.0f, sub, a.dim);
+    };
+    if (kKeep) parameters();
 
+    int row = r0 + group;
+    if (row < r1) fetch(row);
     int next_flush = a.gate_mode == kGateWhole ? r0 + a.gate_rows : 0x7fffffff;
     for (int base = r0; base < r1;) {
         const int stop = next_flush < r1 ? next_flush : r1;
-        for (int row = base + group; row < stop; row += kGroups) {
-            R n1, n2, d;
+        while (row < stop) {
+            float n1[N], n2[N], d[N], g[N], dy[N];
+            rx.widen(n2, sub, a.dim);
+            if (a.f) rf.widen(n1, sub, a.dim);
+            if (a.gate) rg.widen(g, sub, a.dim);
+            if (a.dh) rdh.widen(d, sub, a.dim);
+            if (a.dy) rdy.widen(dy, sub, a.dim);
+            if (row + kGroups < r1) fetch(row + kGroups);
+            if (!kKeep) parameters();
             float r_1 = 1.0f;
-            n2.load((const T*)a.x + (long long)row * a.sx, sub, a.dim);
-            const T* grow = a.gate ? (const T*)a.gate + (long long)(row / a.gate_rows) * a.sg : nullptr;
             if (a.f) {
-                n1.load((const T*)a.f + (long long)row * a.sf, sub, a.dim);
-                r_1 = normalise<VEC, THREADS, PER>(n1.v, a.post, sub, a.dim, a.eps, lds);
-                R g;
-                if (grow) g.load(grow, sub, a.dim);
-                each<VEC, THREADS, PER>(sub, a.dim, [&](int i, int c) {
-                    float u = n1.v[i];
-                    if (a.post_w) u *= a.post_w[c];
-                    if (a.post_b) u += a.post_b[c];
-                    if (grow) u *= g.v[i];
-                    n2.v[i] = fmaf(a.alpha, n2.v[i], a.beta * u);
-                });
+                r_1 = normalise<VEC, THREADS, PER>(n1, a.post, sub, a.dim, a.inv_dim, a.eps, lds, 0);
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const float u = n1[i] * w1.v[i] + b1.v[i];
+                    n2[i] = fmaf(a.alpha, n2[i], a.beta * (a.gate ? u * g[i] : u));
+                }
             } else {
 #pragma unroll
-                for (int i = 0; i < R::N; i++) n2.v[i] *= a.alpha;
+                for (int i = 0; i < N; i++) n2[i] *= a.alpha;
             }
             if (a.dh) {
-                const float r_2 = normalise<VEC, THREADS, PER>(n2.v, a.pre, sub, a.dim, a.eps, lds);
-                d.load((const T*)a.dh + (long long)row * a.sh, sub, a.dim);
-                norm_back<VEC, THREADS, PER>(d.v, n2.v, r_2, a.pre, a.pre_w, dw2, db2, sub, a.dim, lds);
+                const float r_2 = normalise<VEC, THREADS, PER>(n2, a.pre, sub, a.dim, a.inv_dim, a.eps, lds, 2);
+                norm_back<VEC, THREADS, PER>(d, n2, r_2, a.pre, w2.v, dw2, db2, sub, a.dim, a.inv_dim, lds, 4);
             } else {
 #pragma unroll
-                for (int i = 0; i < R::N; i++) d.v[i] = 0.0f;
+                for (int i = 0; i < N; i++) d[i] = 0.0f;
             }
             if (a.dy) {
-                R e;
-                e.load((const T*)a.dy + (long long)row * a.sy, sub, a.dim);
 #pragma unroll
-                for (int i = 0; i < R::N; i++) d.v[i] += e.v[i];
+                for (int i = 0; i < N; i++) d[i] += dy[i];
             }
+            R out;
             if (a.dx) {
-                R e;
 #pragma unroll
-                for (int i = 0; i < R::N; i++) e.v[i] = a.alpha * d.v[i];
-                e.store((T*)a.dx + (long long)row * a.sx, sub, a.dim);
+                for (int i = 0; i < N; i++) out.v[i] = a.alpha * d[i];
+                out.store((T*)a.dx + (long long)row * a.sx, sub, a.dim);
             }
-            if (!a.f) continue;
-            if (grow) {
-                R g, own;
-                g.load(grow, sub, a.dim);
+            if (a.f) {
 #pragma unroll
-                for (int i = 0; i < R::N; i++) own.v[i] = 0.0f;
-                each<VEC, THREADS, PER>(sub, a.dim, [&](int i, int c) {
-                    float u = n1.v[i];
-                    if (a.post_w) u *= a.post_w[c];
-                    if (a.post_b) u += a.post_b[c];
-                    own.v[i] = a.beta * d.v[i] * u;
-                    dg[i] += own.v[i];
-                    d.v[i] *= a.beta * g.v[i];
-                });
-                if (a.gate_mode == kGateRow) own.store((T*)a.dgate + (long long)row * a.sg, sub, a.dim);
-            } else {
+                for (int i = 0; i < N; i++) d[i] *= a.beta;
+                if (a.gate) {
 #pragma unroll
-                for (int i = 0; i < R::N; i++) d.v[i] *= a.beta;
+                    for (int i = 0; i < N; i++) {
+                        out.v[i] = d[i] * (n1[i] * w1.v[i] + b1.v[i]);
+                        dg[i] += out.v[i];
+                        d[i] *= g[i];
+                    }
+                    if (a.gate_mode == kGateRow) out.store((T*)a.dgate + (long long)row * a.sg, sub, a.dim);
+                }
+                norm_back<VEC, THREADS, PER>(d, n1, r_1, a.post, w1.v, dw1, db1, sub, a.dim, a.inv_dim, lds, 6);
+                if (a.df) {
+#pragma unroll
+                    for (int i = 0; i < N; i++) out.v[i] = d[i];
+                    out.store((T*)a.df + (long long)row * a.sf, sub, a.dim);
+                }
             }
-            norm_back<VEC, THREADS, PER>(d.v, n1.v, r_1, a.post, a.post_w, dw1, db1, sub, a.dim, lds);
-            if (a.df) d.store((T*)a.df + (long long)row * a.sf, sub, a.dim);
+            row += kGroups;
         }
         base = stop;
         if (a.gate_mode == kGateWhole) {
@@ -294,16 +395,16 @@ __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
             if (group == 0) {
                 R out;
 #pragma unroll
-                for (int i = 0; i < R::N; i++) out.v[i] = dg[i];
+                for (int i = 0; i < N; i++) out.v[i] = dg[i];
                 out.store((T*)a.dgate + (long long)((stop - 1) / a.gate_rows) * a.sg, sub, a.dim);
             }
 #pragma unroll
-            for (int i = 0; i < R::N; i++) dg[i] = 0.0f;
+            for (int i = 0; i < N; i++) dg[i] = 0.0f;
             next_flush = stop + a.gate_rows;
         }
     }
     float* own = a.sums + (long long)blockIdx.x * 4 * a.dim;
-    auto finish = [&](float (&v)[R::N], int k) {
+    auto finish = [&](float (&v)[N], int k) {
         if (!a.dst[k]) return;
         joined(v);
         float* to = a.parts > 1 ? own + (long long)k * a.dim : a.dst[k];
@@ -321,33 +422,43 @@ __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
     }
 }
 
-// Sums of `parts` rows of src (stride apart) in a fixed order: 64 columns a
-// workgroup, four interleaved quarters of the parts.
+// Sums of `parts` rows of src (stride apart) in a fixed order: 16 columns a
+// workgroup, 16 interleaved shares of the parts.
+constexpr int kSumColumns = 16;
 template <class T>
 __device__ __forceinline__ void sum_parts(const float* src, long long stride, int parts, int dim, T* out, int column0)
 {
-    __shared__ float quarter[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = column0 + lane;
-    float s = 0.0f;
-    if (c < dim)
-        for (int p = w; p < parts; p += 4) s += src[p * stride + c];
-    quarter[w][lane] = s;
+    __shared__ float share[16][kSumColumns];
+    const int lane = threadIdx.x & 15, w = threadIdx.x >> 4, c = column0 + lane;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < dim) {
+        int p = w;
+        for (; p + 48 < parts; p += 64)
+#pragma unroll
+            for (int q = 0; q < 4; q++) s[q] += src[(p + 16 * q) * stride + c];
+        for (; p < parts; p += 16) s[0] += src[p * stride + c];
+    }
+    share[w][lane] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
-    if (w == 0 && c < dim) out[c] = (T)(quarter[0][lane] + quarter[1][lane] + quarter[2][lane] + quarter[3][lane]);
+    if (w == 0 && c < dim) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) sum += share[i][lane];
+        out[c] = (T)sum;
+    }
 }
 
+// blockIdx.y: the parameters' four arrays, then the gate's groups (one launch:
+// the two would run one after the other, 9 and 5 us at 1,037 parts of 1,280).
+template <class T>
 __global__ __launch_bounds__(256) void norm_sum_kernel(NormArgs a)
 {
-    float* dst = a.dst[blockIdx.y];
-    if (!dst) return;
-    sum_parts(a.sums + (long long)blockIdx.y * a.dim, 4ll * a.dim, a.parts, a.dim, dst, blockIdx.x * 64);
-}
-
-template <class T>
-__global__ __launch_bounds__(256) void gate_sum_kernel(NormArgs a)
-{
-    sum_parts(a.gate_sums + (long long)blockIdx.y * a.per_span * a.dim, (long long)a.dim, a.per_span, a.dim,
-              (T*)a.dgate + (long long)blockIdx.y * a.sg, blockIdx.x * 64);
+    const int y = blockIdx.y, column = blockIdx.x * kSumColumns;
+    if (y >= 4)
+        sum_parts(a.gate_sums + (y - 4ll) * a.per_span * a.dim, (long long)a.dim, a.per_span, a.dim,
+                  (T*)a.dgate + (y - 4ll) * a.sg, column);
+    else if (a.dst[y] && a.parts > 1)
+        sum_parts(a.sums + (long long)y * a.dim, 4ll * a.dim, a.parts, a.dim, a.dst[y], column);
 }
 
 NormArgs norm_args(const NormGateOption& o, const NormGateTensors& t, int rows)
@@ -387,6 +498,7 @@ NormArgs norm_args(const NormGateOption& o, const NormGateTensors& t, int rows)
     a.alpha = o.residualScale;
     a.beta = o.blockScale;
     a.eps = o.epsilon;
+    a.inv_dim = (float)(1.0 / o.dim);
     return a;
 }
 
@@ -397,7 +509,7 @@ struct Access {
 
 bool norm_vec(int dim, int bytes, std::initializer_list<Access> all)
 {
-    bool ok = dim * bytes % 16 == 0;
+    bool ok = dim * bytes % 16 == 0;  // then the parameters' pieces are whole too
     for (const Access& x : all) ok = ok && (!x.p || (aligned16(x.p) && x.stride * bytes % 16 == 0));
     return ok;
 }
@@ -428,18 +540,31 @@ void backward_launch(const NormArgs& a, hipStream_t s)
     norm_gate_backward_kernel<T, VEC, THREADS, PER, WG><<<a.parts, WG, 0, s>>>(a);
 }
 
-// Sixteen elements a thread at most: five sums over rows and the row's own
-// arrays stay in registers.
+// Eight elements a thread: the five sums over rows, the row's own arrays and the
+// next row stay in registers.  Whole waves, as few as hold the row.  Twelve waves a CU are resident, which is how
+// many workgroups the rows are dealt to.
+int backward_threads(int dim, int vec)
+{
+    const int lanes = ((dim + vec - 1) / vec + 8 / vec - 1) / (8 / vec);
+    for (int t : {64, 128, 192, 256, 384}) {
+        if (lanes <= t) return t;
+    }
+    return lanes <= 512 ? 512 : 1024;
+}
+
 template <class T, int VEC>
 void backward_rows(const NormArgs& a, hipStream_t s)
 {
-    const int pieces = (a.dim + VEC - 1) / VEC;
-    constexpr int P = 16 / VEC;
-    if (pieces <= 32 * P) backward_launch<T, VEC, 64, P / 2, 256>(a, s);
-    else if (pieces <= 64 * P) backward_launch<T, VEC, 64, P, 256>(a, s);
-    else if (pieces <= 128 * P) backward_launch<T, VEC, 256, P / 2, 256>(a, s);
-    else if (pieces <= 256 * P) backward_launch<T, VEC, 256, P, 256>(a, s);
-    else backward_launch<T, VEC, 512, P, 512>(a, s);
+    constexpr int P = 8 / VEC;
+    switch (backward_threads(a.dim, VEC)) {
+        case 64: return backward_launch<T, VEC, 64, P, 256>(a, s);
+        case 128: return backward_launch<T, VEC, 128, P, 128>(a, s);
+        case 192: return backward_launch<T, VEC, 192, P, 192>(a, s);
+        case 256: return backward_launch<T, VEC, 256, P, 256>(a, s);
+        case 384: return backward_launch<T, VEC, 384, P, 384>(a, s);
+        case 512: return backward_launch<T, VEC, 512, P, 512>(a, s);
+        default: return backward_launch<T, VEC, 1024, P, 1024>(a, s);
+    }
 }
 
 }  // namespace
@@ -453,7 +578,8 @@ void norm_gate(const NormGateOption& o, const NormGateTensors& t, void* y, void*
     a.y = y;
     a.h = h;
     const int bytes = data_bytes(o.dataType);
-    const bool vec = norm_vec(o.dim, bytes, {{t.x, a.sx}, {t.f, a.sf}, {t.gate, a.sg}, {y, a.sy}, {h, a.sh}});
+    const bool vec = norm_vec(o.dim, bytes, {{t.x, a.sx}, {t.f, a.sf}, {t.gate, a.sg}, {y, a.sy}, {h, a.sh}, {t.post_w, 16}, {t.post_b, 16},
+                                               {t.pre_w, 16}, {t.pre_b, 16}});
     with_type(o.dataType, [&](auto zero) {
         using T = decltype(zero);
         if (vec) forward_rows<T, 16 / (int)sizeof(T)>(a, s);
@@ -480,11 +606,16 @@ void norm_gate_backward(const NormGateOption& o, const NormGateTensors& t, const
     a.dst[1] = g.dpost_b;
     a.dst[2] = g.dpre_w;
     a.dst[3] = g.dpre_b;
+    const int bytes = data_bytes(o.dataType);
+    const bool vec = norm_vec(o.dim, bytes,
+                              {{t.x, a.sx}, {t.f, a.sf}, {t.gate, a.sg}, {dy, a.sy}, {dh, a.sh}, {g.dx, a.sx}, {g.df, a.sf},
+                               {g.dgate, a.sg}, {t.post_w, 16}, {t.post_b, 16}, {t.pre_w, 16}, {t.pre_b, 16}});
     const bool sums = g.dpost_w || g.dpost_b || g.dpre_w || g.dpre_b;
     // Rows of a workgroup: whole groups of the gate, or an even part of one, so
     // that no workgroup has rows of two gates whose sums it cannot finish; the
     // same ones whether the gate's gradient is asked for or not.
-    const int most = std::min(kMaxParts, std::max(1, rows / 4));
+    const int threads = backward_threads(o.dim, vec ? 16 / bytes : 1), wg = threads == 64 ? 256 : threads;
+    const int most = std::min(num_cus() * std::max(1, 768 / wg), std::max(1, rows / 4));
     int chunk = std::max(1, (rows + most - 1) / most);
     a.gate_mode = !t.gate ? kGateNone : a.gate_rows == 1 ? kGateRow : kGateWhole;
     if (a.gate_mode != kGateWhole || a.gate_rows >= rows) {
@@ -511,18 +642,13 @@ void norm_gate_backward(const NormGateOption& o, const NormGateTensors& t, const
         a.sums = (float*)stream_workspace(s).get(columns * 5 * sizeof(float));
         a.gate_sums = a.sums + columns * 4;
     }
-    const int bytes = data_bytes(o.dataType);
-    const bool vec = norm_vec(o.dim, bytes,
-                              {{t.x, a.sx}, {t.f, a.sf}, {t.gate, a.sg}, {dy, a.sy}, {dh, a.sh}, {g.dx, a.sx}, {g.df, a.sf},
-                               {g.dgate, a.sg}});
     with_type(o.dataType, [&](auto zero) {
         using T = decltype(zero);
         if (vec) backward_rows<T, 16 / (int)sizeof(T)>(a, s);
         else backward_rows<T, 1>(a, s);
         GRAFT_LAUNCH_CHECK();
-        const int columns = (a.dim + 63) / 64;
-        if (sums && a.parts > 1) norm_sum_kernel<<<dim3(columns, 4), 256, 0, s>>>(a);
-        if (a.gate_mode == kGatePart) gate_sum_kernel<T><<<dim3(columns, spans), 256, 0, s>>>(a);
+        const int columns = (a.dim + kSumColumns - 1) / kSumColumns;
+        if (to_scratch) norm_sum_kernel<T><<<dim3(columns, 4 + (a.gate_mode == kGatePart ? spans : 0)), 256, 0, s>>>(a);
     });
     GRAFT_LAUNCH_CHECK();
 }
