@@ -14,6 +14,7 @@
 // four consecutive n of one row m.  Its two operands are read with the same
 // order of k within the block, whatever it is.
 #include "experts.h"
+#include "lanes.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -78,6 +79,35 @@ __device__ __forceinline__ void meet()
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// Row tile `t` of tm rows among all experts' segments: its expert and rows, or
+// none.  Every wave finds it by itself.
+__device__ __forceinline__ void find_rows(const ProductArgs& a, int t, int tm, int& expert, int& row0, int& row1)
+{
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    row0 = row1 = expert = 0;
+    for (int e0 = 0; e0 < a.experts; e0 += 64) {
+        const int e = e0 + lane;
+        int lo = 0, hi = 0;
+        if (e < a.experts) {
+            lo = min(max(a.offsets[e], 0), a.m);
+            hi = min(max(a.offsets[e + 1], lo), a.m);
+        }
+        const int tiles = (hi - lo + tm - 1) / tm;
+        const int up = lanes_scan(tiles);
+        const uint64_t found = __ballot(before + up > t);
+        if (found) {
+            const int l = __ffsll((unsigned long long)found) - 1;
+            const int first = before + __shfl(up - tiles, l);
+            expert = __builtin_amdgcn_readfirstlane(e0 + l);
+            row0 = __builtin_amdgcn_readfirstlane(__shfl(lo, l) + (t - first) * tm);
+            row1 = __builtin_amdgcn_readfirstlane(__shfl(hi, l));
+            return;
+        }
+        before += __shfl(up, 63);
+    }
+}
+
 // Where a segment's row tiles begin: starts[e] for e in 0..experts, from the
 // offsets, by the first wave; the last one is their number.
 template <int TM>
@@ -93,11 +123,7 @@ __device__ __forceinline__ void row_tiles(const ProductArgs& a, int* starts)
                 const int lo = min(max(a.offsets[e], 0), a.m), hi = min(max(a.offsets[e + 1], lo), a.m);
                 n = (hi - lo + TM - 1) / TM;
             }
-            int up = n;
-            for (int d = 1; d < 64; d *= 2) {
-                const int o = __shfl_up(up, d);
-                up += lane >= d ? o : 0;
-            }
+            const int up = lanes_scan(n);
             if (e < a.experts) starts[e] = before + up - n;
             before += __shfl(up, 63);
         }
@@ -433,6 +459,97 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
 #endif
 }
 
+// Few rows of A: up to 16 MT rows by 16 rows of B a workgroup, its waves sharing
+// out k, four blocks at a time, and their sums joined in LDS in wave order.  B's
+// bytes bound it, so both operands go straight from memory to registers, all of
+// a wave's four blocks under way at once, and are widened (one row by 4096 x
+// 4096: 21 us through the tiles above, whose 32 workgroups wait for one block
+// after the other).
+constexpr int kFewWaves = 8;
+template <class T, int MT>
+__global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(ProductArgs a)
+{
+    __shared__ f4 sums[kFewWaves][MT][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int waves = blockDim.x >> 6, col = lane & 15, quad = lane >> 4;
+    const int tm = blockIdx.x / a.tiles_n, n0 = blockIdx.x % a.tiles_n * 16;
+    int expert = 0, row0 = tm * 16 * MT, row1 = a.m;
+    if (a.grouping == PRODUCT_ROWS) {
+        find_rows(a, tm, 16 * MT, expert, row0, row1);
+        if (row0 >= row1) return;
+    }
+    const int brow = min(n0 + col, a.n - 1);
+    const uint8_t* B = a.b + expert * a.b_size + (long long)brow * a.pitch + quad * 16;
+    const uint8_t* SB = a.bs + expert * a.bs_size + (long long)(brow >> a.scale_shift) * a.spitch;
+    const uint8_t *A[MT], *SA[MT];
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+        const long long r = min(row0 + j * 16 + col, row1 - 1);
+        A[j] = a.a + r * a.pitch + quad * 16;
+        SA[j] = a.as + r * a.spitch;
+    }
+    f4 acc[MT];
+#pragma unroll
+    for (int j = 0; j < MT; j++) acc[j] = f4zero();
+    const int blocks = a.pitch / 128;
+    for (int kb = wave * 4; kb < blocks; kb += waves * 4) {
+        const uint32_t sb = *reinterpret_cast<const uint32_t*>(SB + kb);
+        uint32_t sa[MT];
+        i4v b[4][2], x[4][MT][2];
+#pragma unroll
+        for (int j = 0; j < MT; j++) sa[j] = *reinterpret_cast<const uint32_t*>(SA[j] + kb);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int at = min(kb + q, blocks - 1) * 128;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                b[q][h] = *reinterpret_cast<const i4v*>(B + at + h * 64);
+#pragma unroll
+                for (int j = 0; j < MT; j++) x[q][j][h] = *reinterpret_cast<const i4v*>(A[j] + at + h * 64);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if (kb + q >= blocks) break;
+            const float fb = scale_of(sb >> (8 * q) & 0xff);
+            float fa[MT];
+#pragma unroll
+            for (int j = 0; j < MT; j++) fa[j] = scale_of(sa[j] >> (8 * q) & 0xff);
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    const bf16x8 wb = widen(b[q][h][2 * p], b[q][h][2 * p + 1], fb);
+#pragma unroll
+                    for (int j = 0; j < MT; j++)
+                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            wb, widen(x[q][j][h][2 * p], x[q][j][h][2 * p + 1], fa[j]), acc[j], 0, 0, 0);
+                }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < MT; j++) sums[wave][j][lane] = acc[j];
+    __syncthreads();
+    for (int j = wave; j < MT; j += waves) {
+        f4 v = sums[0][j][lane];
+        for (int w = 1; w < waves; w++) v += sums[w][j][lane];
+        const int r = row0 + j * 16 + col, n = n0 + quad * 4;
+        const float o[4] = {v[0], v[1], v[2], v[3]};
+        if (r < row1 && n < a.n) store_row<T, 4>(a, (T*)a.out + (long long)r * a.out_stride, n, o);
+    }
+}
+
+template <class T, int MT>
+void few_launch(ProductArgs& a, hipStream_t s)
+{
+    a.tiles_n = (a.n + 15) / 16;
+    const long long row_tiles = a.grouping == PRODUCT_ROWS ? a.m / (16 * MT) + a.experts : (a.m + 16 * MT - 1) / (16 * MT);
+    require(row_tiles * a.tiles_n <= 0x7fffffffll, "too many tiles for one call");
+    const int waves = std::min(kFewWaves, std::max(1, (a.pitch / 128 + 3) / 4));
+    product_few_kernel<T, MT><<<(unsigned)(row_tiles * a.tiles_n), waves * 64, 0, s>>>(a);
+    GRAFT_LAUNCH_CHECK();
+}
+
 template <class T, int TM, int TN, bool WIDE>
 void product_launch(ProductArgs& a, hipStream_t s)
 {
@@ -486,9 +603,17 @@ void fp8_product(const Fp8ProductOption& o, const uint8_t* a, const uint8_t* a_s
     p.out_stride = o.outStride;
     p.out_type = o.outType;
     p.relu = o.activation == 1;
+    // stores of up to 16 bytes
     p.vec = aligned16(out) && o.outStride * data_bytes(o.outType) % 16 == 0;
     with_type(o.outType, [&](auto zero) {
         using T = decltype(zero);
+        // Few rows, or few to an expert on average.
+        if (o.grouping != PRODUCT_SUM) {
+            const long long rows = (o.m + o.numExperts - 1ll) / o.numExperts;
+            if (rows <= 16) return few_launch<T, 1>(p, s);
+            if (rows <= 32) return few_launch<T, 2>(p, s);
+            if (rows <= 64) return few_launch<T, 4>(p, s);
+        }
         // fp32 results, weight gradients of any type, and products of up to two
         // blocks of k, which their output's bytes bound: there widening costs nothing.
         if (std::is_same_v<T, float> || o.grouping == PRODUCT_SUM || p.pitch <= 256) return product_launch<T, 128, 128, true>(p, s);

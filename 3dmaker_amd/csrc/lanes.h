@@ -56,4 +56,16 @@ __device__ __forceinline__ uint32_t lanes_umax(uint32_t v)
     return lanes_reduce<W>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
+// Inclusive sum over the wave: row shifts, then the rows' last values onward.
+__device__ __forceinline__ int lanes_scan(int v)
+{
+    v += (int)dpp_mov<0x111>((uint32_t)v);  // row_shr:1, zero at the row's start
+    v += (int)dpp_mov<0x112>((uint32_t)v);
+    v += (int)dpp_mov<0x114>((uint32_t)v);
+    v += (int)dpp_mov<0x118>((uint32_t)v);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 to rows 2 and 3
+    return v;
+}
+
 }  // namespace graft

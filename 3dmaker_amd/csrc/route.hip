@@ -26,7 +26,7 @@ struct RouteArgs {
     const float* bias;
     int* indices;
     float* weights;
-    int tokens, experts, topk, groups, kept, group_size, lanes_group, group_best;
+    int tokens, experts, topk, groups, kept, group_size, lanes_group, lanes_group_bits, group_best;
     int type;
     bool sigmoid, renorm, vec;
     float scale;
@@ -126,54 +126,117 @@ __device__ __forceinline__ void scores_of(float (&s)[V], const float (&z)[V], ui
     }
 }
 
-// Lanes of the token below this one that are set in the wave's mask.
+// The largest key of a token's lanes.  A whole wave's is left in its last lane by
+// the row broadcasts (six instructions, against ten for one that all lanes hold)
+// and read from there.
 template <int LPT>
-__device__ __forceinline__ bool first_of(uint64_t mask, int lane)
+__device__ __forceinline__ uint32_t largest(uint32_t v)
 {
-    const uint64_t below = (1ull << lane) - 1;
-    const uint64_t token = LPT == 64 ? ~0ull : ((1ull << LPT) - 1) << (lane & ~(LPT - 1));
-    return (mask & token & below) == 0;
+    if constexpr (LPT < 64) return lanes_umax<LPT>(v);
+    v = lanes_umax<16>(v);
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x142, 0xa, 0xf, false));  // row_bcast:15
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x143, 0xc, 0xf, false));  // row_bcast:31
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
+// Whether a lane is the lowest of its token's in the wave's mask.
+template <int LPT>
+__device__ __forceinline__ bool lowest_of(uint64_t mask, int lane)
+{
+    if constexpr (LPT == 64) return __ffsll((unsigned long long)mask) - 1 == lane;
+    const uint64_t below = ((1ull << lane) - 1) & (((1ull << LPT) - 1) << (lane & ~(LPT - 1)));  // the same for all picks
+    return (mask & below) == 0;
+}
+
+// The best two keys of the LG lanes of a group.
+template <int LG>
+__device__ __forceinline__ void best_two(uint32_t& b1, uint32_t& b2)
+{
+    auto join = [&](uint32_t o1, uint32_t o2) {
+        b2 = max(min(b1, o1), max(b2, o2));
+        b1 = max(b1, o1);
+    };
+    if constexpr (LG >= 2) join(dpp_mov<0xB1>(b1), dpp_mov<0xB1>(b2));
+    if constexpr (LG >= 4) join(dpp_mov<0x4E>(b1), dpp_mov<0x4E>(b2));
+    if constexpr (LG >= 8) join(dpp_mov<0x141>(b1), dpp_mov<0x141>(b2));
+    if constexpr (LG >= 16) join(dpp_mov<0x140>(b1), dpp_mov<0x140>(b2));
+    if constexpr (LG >= 32) join(__shfl_xor(b1, 16), __shfl_xor(b2, 16));
+}
+
+// Keys sorted downwards with their places, equal ones in their order.
+template <int V>
+__device__ __forceinline__ void sort_down(uint32_t (&key)[V], int (&place)[V])
+{
+#pragma unroll
+    for (int end = V - 1; end > 0; end--)
+#pragma unroll
+        for (int i = 0; i < end; i++) {
+            const bool swap = key[i + 1] > key[i];
+            const uint32_t hi = max(key[i], key[i + 1]), lo = min(key[i], key[i + 1]);
+            const int p = swap ? place[i + 1] : place[i], q = swap ? place[i] : place[i + 1];
+            key[i] = hi;
+            key[i + 1] = lo;
+            place[i] = p;
+            place[i + 1] = q;
+        }
+}
+
+// Four experts a lane are sorted once, and a pick takes the lane's first; more
+// are searched at each pick.  A pick's score comes back from LDS at the end.
 template <int V, int LPT>
 __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a)
 {
     constexpr int kTokens = kRouteThreads / LPT;
     constexpr int kPicked = V == 4 ? 1024 : kTokens * 32;  // at most min(LPT V, 32) slots a token
-    __shared__ int picked_i[kPicked];
-    __shared__ float picked_s[kPicked];
+    __shared__ int picked[kPicked];                        // lane of the token * V + its place, or -1
+    __shared__ __attribute__((aligned(16))) float score[kRouteThreads * V];
     __shared__ uint32_t group_key[kRouteThreads];
     const int lane = threadIdx.x & 63, sub = threadIdx.x & (LPT - 1), local = threadIdx.x / LPT;
     const int token = blockIdx.x * kTokens + local;
-    const int group = sub / a.lanes_group, in_group = (sub & (a.lanes_group - 1)) * V;
+    const int lg = a.lanes_group, lg_bits = a.lanes_group_bits;
+    const int group = sub >> lg_bits, in_group = (sub & (lg - 1)) * V;
     const int first = group * a.group_size + in_group;
     const int n = token < a.tokens && group < a.groups ? min(V, a.group_size - in_group) : 0;
     float z[V], s[V];
 #pragma unroll
     for (int i = 0; i < V; i++) z[i] = 0.0f;
     uint32_t live = load_logits(z, a, token, first, n);
+    float bias[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) bias[i] = a.bias && i < n ? a.bias[first + i] : 0.0f;
     scores_of<V, LPT>(s, z, live, a.sigmoid);
     uint32_t key[V];
+    int place[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const float c = s[i] + (a.bias && i < n ? a.bias[first + i] : 0.0f);
+        const float c = s[i] + bias[i];
         key[i] = (live >> i & 1) && c > -INFINITY ? key_of(c) : 0u;
+        place[i] = i;
+        score[threadIdx.x * V + i] = s[i];
     }
+    if (V == 4) sort_down(key, place);
     if (a.groups > 1) {
-        uint32_t b1 = 0, b2 = 0;  // keys of the best two
+        uint32_t b1 = key[0], b2 = key[1];  // keys of the best two
+        if (V != 4) {
+            b2 = min(key[0], key[1]);
+            b1 = max(key[0], key[1]);
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            b2 = max(b2, min(b1, key[i]));
-            b1 = max(b1, key[i]);
+            for (int i = 2; i < V; i++) {
+                b2 = max(b2, min(b1, key[i]));
+                b1 = max(b1, key[i]);
+            }
         }
-        for (int w = 1; w < a.lanes_group; w <<= 1) {
-            const uint32_t o1 = __shfl_xor(b1, w), o2 = __shfl_xor(b2, w);
-            b2 = max(min(b1, o1), max(b2, o2));
-            b1 = max(b1, o1);
+        switch (lg) {
+            case 1: break;
+            case 2: best_two<2>(b1, b2); break;
+            case 4: best_two<4>(b1, b2); break;
+            case 8: best_two<8>(b1, b2); break;
+            case 16: best_two<16>(b1, b2); break;
+            default: best_two<32>(b1, b2); break;
         }
         uint32_t g = b1;
         if (a.group_best == 2 && b2 != 0) g = key_of(of_key(b1) + of_key(b2));
-        if ((sub & (a.lanes_group - 1)) == 0) group_key[local * LPT + group] = g;
+        if ((sub & (lg - 1)) == 0) group_key[local * LPT + group] = g;
         __syncthreads();
         int ahead = 0;
         for (int o = 0; o < a.groups; o++) {
@@ -185,41 +248,47 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a)
             for (int i = 0; i < V; i++) key[i] = 0;
         }
     }
+    int* const mine_picked = picked + local * a.topk;
     for (int j = 0; j < a.topk; j++) {
         uint32_t best = key[0];
+        if (V != 4) {
 #pragma unroll
-        for (int i = 1; i < V; i++) best = max(best, key[i]);
-        const uint32_t top = lanes_umax<LPT>(best);
+            for (int i = 1; i < V; i++) best = max(best, key[i]);
+        }
+        const uint32_t top = largest<LPT>(best);
         const bool mine = best == top && top != 0;
-        const uint64_t mask = __ballot(mine);
-        if (mine && first_of<LPT>(mask, lane)) {
-            int at = 0;
-            float sc = 0.0f;
+        if (mine && lowest_of<LPT>(__ballot(mine), lane)) {
+            int at = place[0];
+            if (V == 4) {
 #pragma unroll
-            for (int i = V - 1; i >= 0; i--) {
-                const bool here = key[i] == top;
-                at = here ? i : at;
-                sc = here ? s[i] : sc;
+                for (int i = 0; i + 1 < V; i++) key[i] = key[i + 1], place[i] = place[i + 1];
+                key[V - 1] = 0;
+            } else {
+                at = 0;
+#pragma unroll
+                for (int i = V - 1; i >= 0; i--) at = key[i] == top ? i : at;
+#pragma unroll
+                for (int i = 0; i < V; i++) key[i] = i == at ? 0u : key[i];
             }
-#pragma unroll
-            for (int i = 0; i < V; i++) key[i] = i == at ? 0u : key[i];
-            picked_i[local * a.topk + j] = first + at;
-            picked_s[local * a.topk + j] = sc;
+            mine_picked[j] = sub * V + at;
         } else if (top == 0 && sub == 0) {
-            picked_i[local * a.topk + j] = -1;
-            picked_s[local * a.topk + j] = 0.0f;
+            mine_picked[j] = -1;
         }
     }
     __syncthreads();
     float sum = 0.0f;
-    for (int j = sub; j < a.topk; j += LPT) sum += picked_s[local * a.topk + j];
-    sum = lanes_sum<LPT>(sum);
+    for (int j = sub; j < a.topk; j += LPT) {
+        const int p = mine_picked[j];
+        sum += p >= 0 ? score[local * LPT * V + p] : 0.0f;
+    }
+    if (a.renorm) sum = lanes_sum<LPT>(sum);
     const float factor = a.renorm ? a.scale / (sum + 1e-20f) : a.scale;
     if (token >= a.tokens) return;
     for (int j = sub; j < a.topk; j += LPT) {
+        const int p = mine_picked[j], l = p / V;
         const long long at = (long long)token * a.topk + j;
-        a.indices[at] = picked_i[local * a.topk + j];
-        a.weights[at] = picked_s[local * a.topk + j] * factor;
+        a.indices[at] = p >= 0 ? (l >> lg_bits) * a.group_size + (l & (lg - 1)) * V + p % V : -1;
+        a.weights[at] = p >= 0 ? score[local * LPT * V + p] * factor : 0.0f;
     }
 }
 
@@ -230,33 +299,42 @@ template <int V, int LPT>
 __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteArgs a)
 {
     constexpr int kTokens = kRouteThreads / LPT;
+    // The tokens' gradients at their experts' places; kNone (a NaN that no
+    // gradient is written as) at those that were not selected.
+    constexpr uint32_t kNone = 0xffffffffu;
+    __shared__ __attribute__((aligned(16))) uint32_t dense[kRouteThreads * V];
     const int sub = threadIdx.x & (LPT - 1), token = blockIdx.x * kTokens + threadIdx.x / LPT;
     const int first = sub * V;
     const int n = token < a.tokens ? max(0, min(V, a.experts - first)) : 0;
+#pragma unroll
+    for (int i = 0; i < V; i++) dense[threadIdx.x * V + i] = kNone;
     float z[V], s[V], g[V];
 #pragma unroll
-    for (int i = 0; i < V; i++) z[i] = 0.0f, g[i] = 0.0f;
+    for (int i = 0; i < V; i++) z[i] = 0.0f;
     const uint32_t live = load_logits(z, a, token, first, n);
+    __syncthreads();
+    const long long slot0 = (long long)blockIdx.x * kTokens * a.topk;
+    const int slots = min(kTokens, a.tokens - (int)blockIdx.x * kTokens) * a.topk;
+    for (int i = threadIdx.x; i < slots; i += kRouteThreads) {
+        const int e = a.indices[slot0 + i];
+        const uint32_t d = __builtin_bit_cast(uint32_t, a.dweights[slot0 + i]);
+        if ((unsigned)e < (unsigned)a.experts) dense[i / a.topk * (LPT * V) + e] = d == kNone ? 0x7fc00000u : d;
+    }
+    __syncthreads();
     scores_of<V, LPT>(s, z, live, a.sigmoid);
     uint32_t chosen = 0;
-    if (n > 0) {
-        for (int j = 0; j < a.topk; j++) {
-            const long long at = (long long)token * a.topk + j;
-            const int i = a.indices[at] - first;
-            const float d = a.dweights[at];
 #pragma unroll
-            for (int q = 0; q < V; q++) {
-                g[q] = q == i ? d : g[q];
-                chosen |= q == i && q < n ? 1u << q : 0u;
-            }
-        }
+    for (int i = 0; i < V; i++) {
+        const uint32_t d = dense[threadIdx.x * V + i];
+        chosen |= d != kNone ? 1u << i : 0u;
+        g[i] = __builtin_bit_cast(float, d);
     }
     float total = 0.0f, dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const float c = chosen >> i & 1 ? s[i] : 0.0f;
-        total += c;
-        dot = fmaf(c, g[i], dot);
+        const bool in = chosen >> i & 1;
+        total += in ? s[i] : 0.0f;
+        dot += in ? s[i] * g[i] : 0.0f;
     }
     total = lanes_sum<LPT>(total) + 1e-20f;
     dot = lanes_sum<LPT>(dot);
@@ -387,6 +465,7 @@ void route_experts(const RouteOption& o, const void* logits, long long stride, c
     a.group_best = o.groupScore;
     const int slots = pow2_from(o.numGroups);
     a.lanes_group = std::min(64 / slots, pow2_from((a.group_size + 3) / 4));
+    while ((1 << a.lanes_group_bits) < a.lanes_group) a.lanes_group_bits++;
     const int lanes = slots * a.lanes_group, per_lane = (a.group_size + a.lanes_group - 1) / a.lanes_group;
     with_layout(lanes, per_lane, [&](auto V, auto LPT) {
         a.vec = can_vec(logits, stride, a.group_size, V, a.type);
@@ -425,7 +504,8 @@ namespace {
 
 constexpr int kPlanThreads = 256;
 constexpr int kPlanWaves = kPlanThreads / 64;
-constexpr int kPlanChunk = 4096;  // slots of a workgroup
+constexpr int kPlanSmall = 4096;  // slots that one workgroup places alone
+constexpr int kPlanChunk = 1024;  // of a workgroup otherwise: four rounds a wave
 
 struct PlanArgs {
     const int* indices;
@@ -433,8 +513,8 @@ struct PlanArgs {
     int* offsets;
     int* order;
     int* position;
-    int* counts;  // [experts][blocks]: a block's slots of an expert, then the row of its first
-    int* ends;    // [experts]: the row behind an expert's last slot
+    int* counts;  // [experts][blocks]: a block's slots of an expert, then those in front of them
+    int* totals;  // [experts]: an expert's slots
 };
 
 __device__ __forceinline__ int expert_of(const PlanArgs& a, int slot, int end)
@@ -500,76 +580,68 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(PlanArgs a)
     }
 }
 
-// Inclusive sum over the wave.
-__device__ __forceinline__ int wave_scan(int v, int lane)
-{
-    for (int d = 1; d < 64; d *= 2) {
-        const int o = __shfl_up(v, d);
-        v += lane >= d ? o : 0;
-    }
-    return v;
-}
-
-// One workgroup: offsets from the experts' counts in LDS (total, then overwritten
-// with the segment's first row).
-__device__ __forceinline__ void plan_offsets(const PlanArgs& a, int* total, int lane, int wave)
+// A workgroup: each expert's segment from its slots in LDS (total, overwritten
+// with the segment's first row; ends with the row behind its last slot), by the
+// first wave.  Returns the rows of all.
+__device__ __forceinline__ void plan_offsets(const PlanArgs& a, int* total, int* ends, int lane, int wave)
 {
     if (wave == 0) {
         int base = 0;
         for (int e0 = 0; e0 < a.experts; e0 += 64) {
             const int e = e0 + lane;
-            const int n = e < a.experts ? (total[e] + a.align - 1) / a.align * a.align : 0;
-            const int up = wave_scan(n, lane);
+            const int own = e < a.experts ? total[e] : 0, n = (own + a.align - 1) / a.align * a.align;
+            const int up = lanes_scan(n);
             if (e < a.experts) {
-                a.ends[e] = base + up - n + total[e];
                 total[e] = base + up - n;
-                a.offsets[e] = base + up - n;
+                ends[e] = base + up - n + own;
             }
             base += __shfl(up, 63);
         }
-        if (lane == 0) a.offsets[a.experts] = base;
+        if (lane == 0) total[a.experts] = base;
     }
     __syncthreads();
 }
 
-__global__ __launch_bounds__(1024) void plan_scan_kernel(PlanArgs a)
+// A wave: an expert's slots of the blocks in front of each block, and in all.
+// (One workgroup for all experts took 26 us for 256 of 129 blocks.)
+__global__ __launch_bounds__(64) void plan_scan_kernel(PlanArgs a)
 {
-    __shared__ int total[kMaxExperts];
-    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    for (int e = wave; e < a.experts; e += 16) {
-        int* c = a.counts + (size_t)e * a.blocks;
-        int sum = 0;
-        for (int b0 = 0; b0 < a.blocks; b0 += 64) {
-            const int b = b0 + lane, n = b < a.blocks ? c[b] : 0;
-            const int up = wave_scan(n, lane);
-            if (b < a.blocks) c[b] = sum + up - n;
-            sum += __shfl(up, 63);
-        }
-        if (lane == 0) total[e] = sum;
+    const int lane = threadIdx.x;
+    int* c = a.counts + (size_t)blockIdx.x * a.blocks;
+    const int per = (a.blocks + 63) / 64, b0 = min(a.blocks, lane * per), b1 = min(a.blocks, b0 + per);
+    int sum = 0;
+    for (int b = b0; b < b1; b++) sum += c[b];
+    const int up = lanes_scan(sum);
+    int at = up - sum;
+    for (int b = b0; b < b1; b++) {
+        const int n = c[b];
+        c[b] = at;
+        at += n;
     }
-    __syncthreads();
-    plan_offsets(a, total, lane, wave);
+    if (lane == 63) a.totals[blockIdx.x] = up;
 }
 
-// Blocks 0 .. blocks - 1 place their slots; those behind them fill the rows
-// that no slot has.
-__global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(PlanArgs a, int bits)
+// Rows that no slot has: behind the segments' last slots and behind all
+// segments, by workgroup `fill` of `fills`.
+__device__ __forceinline__ void plan_fill(const PlanArgs& a, const int* starts, const int* ends, int fill, int fills)
 {
-    extern __shared__ int next[];
-    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    if ((int)blockIdx.x >= a.blocks) {
-        const int fill = blockIdx.x - a.blocks, fills = gridDim.x - a.blocks;
-        for (int e = fill; e < a.experts; e += fills)
-            for (int r = a.ends[e] + threadIdx.x; r < a.offsets[e + 1]; r += kPlanThreads) a.order[r] = -1;
-        const int last = a.offsets[a.experts];
-        for (long long r = last + (long long)fill * kPlanThreads + threadIdx.x; r < a.capacity; r += fills * kPlanThreads)
-            a.order[r] = -1;
-        return;
+    if (a.align > 1) {
+        constexpr int kWaves = kPlanThreads / 64;
+        for (int e = fill * kWaves + threadIdx.x / 64; e < a.experts; e += fills * kWaves)
+            for (int r = ends[e] + (threadIdx.x & 63); r < starts[e + 1]; r += 64) a.order[r] = -1;
     }
-    const int begin = blockIdx.x * kPlanChunk, end = min(a.slots, begin + kPlanChunk);
-    plan_count(a, next, begin, end, wave, lane, kPlanWaves);
+    for (long long r = starts[a.experts] + (long long)fill * kPlanThreads + threadIdx.x; r < a.capacity;
+         r += (long long)fills * kPlanThreads)
+        a.order[r] = -1;
+}
+
+// The waves' first rows of each expert from their counts; add: what lies in
+// front of the workgroup's.
+template <class F>
+__device__ __forceinline__ void plan_waves(const PlanArgs& a, int* next, F add)
+{
     for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) {
-        int at = a.offsets[e] + a.counts[(size_t)e * a.blocks + blockIdx.x];
+        int at = add(e);
         for (int w = 0; w < kPlanWaves; w++) {
             const int n = next[w * a.experts + e];
             next[w * a.experts + e] = at;
@@ -577,6 +649,30 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(PlanArgs a, in
         }
     }
     __syncthreads();
+}
+
+// Blocks 0 .. blocks - 1 place their slots; those behind them fill the other
+// rows.  Every one forms the offsets for itself.
+__global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(PlanArgs a, int bits)
+{
+    extern __shared__ int lds[];
+    int* next = lds;                            // [waves][experts]
+    int* starts = next + kPlanWaves * a.experts;  // [experts + 1]
+    int* ends = starts + a.experts + 1;         // [experts]
+    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) starts[e] = a.totals[e];
+    __syncthreads();
+    plan_offsets(a, starts, ends, lane, wave);
+    if ((int)blockIdx.x >= a.blocks) {
+        const int fill = blockIdx.x - a.blocks;
+        if (fill == 0)
+            for (int e = threadIdx.x; e <= a.experts; e += kPlanThreads) a.offsets[e] = starts[e];
+        plan_fill(a, starts, ends, fill, gridDim.x - a.blocks);
+        return;
+    }
+    const int begin = blockIdx.x * kPlanChunk, end = min(a.slots, begin + kPlanChunk);
+    plan_count(a, next, begin, end, wave, lane, kPlanWaves);
+    plan_waves(a, next, [&](int e) { return starts[e] + a.counts[(size_t)e * a.blocks + blockIdx.x]; });
     plan_place(a, next, begin, end, wave, lane, kPlanWaves, bits);
 }
 
@@ -584,31 +680,21 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(PlanArgs a, in
 __global__ __launch_bounds__(kPlanThreads) void plan_small_kernel(PlanArgs a, int bits)
 {
     extern __shared__ int lds[];
-    int* next = lds;                               // [waves][experts]
-    int* total = lds + kPlanWaves * a.experts;     // [experts]
-    a.ends = total + a.experts;                    // [experts], in LDS too
+    int* next = lds;
+    int* starts = next + kPlanWaves * a.experts;
+    int* ends = starts + a.experts + 1;
     const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
     plan_count(a, next, 0, a.slots, wave, lane, kPlanWaves);
     for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) {
         int n = 0;
         for (int w = 0; w < kPlanWaves; w++) n += next[w * a.experts + e];
-        total[e] = n;
+        starts[e] = n;
     }
     __syncthreads();
-    plan_offsets(a, total, lane, wave);
-    for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) {
-        int at = total[e];
-        for (int w = 0; w < kPlanWaves; w++) {
-            const int n = next[w * a.experts + e];
-            next[w * a.experts + e] = at;
-            at += n;
-        }
-        for (int r = a.ends[e]; r < total[e] + (a.ends[e] - total[e] + a.align - 1) / a.align * a.align; r++) a.order[r] = -1;
-    }
-    __syncthreads();
-    const int e = a.experts - 1;
-    const int last = total[e] + (a.ends[e] - total[e] + a.align - 1) / a.align * a.align;
-    for (int r = last + threadIdx.x; r < a.capacity; r += kPlanThreads) a.order[r] = -1;
+    plan_offsets(a, starts, ends, lane, wave);
+    for (int e = threadIdx.x; e <= a.experts; e += kPlanThreads) a.offsets[e] = starts[e];
+    plan_fill(a, starts, ends, 0, 1);
+    plan_waves(a, next, [&](int e) { return starts[e]; });
     plan_place(a, next, 0, a.slots, wave, lane, kPlanWaves, bits);
 }
 
@@ -641,19 +727,19 @@ void route_plan(const int* indices, int tokens, int topK, int experts, int align
     a.position = position;
     int bits = 0;
     while ((1 << bits) < experts) bits++;
-    if (a.slots <= kPlanChunk) {
-        plan_small_kernel<<<1, kPlanThreads, (kPlanWaves + 2) * experts * sizeof(int), s>>>(a, bits);
+    const size_t lds = ((kPlanWaves + 2) * experts + 1) * sizeof(int);
+    if (a.slots <= kPlanSmall) {
+        plan_small_kernel<<<1, kPlanThreads, lds, s>>>(a, bits);
         GRAFT_LAUNCH_CHECK();
         return;
     }
     a.blocks = (a.slots + kPlanChunk - 1) / kPlanChunk;
     Workspace& ws = stream_workspace(s);
     a.counts = (int*)ws.get(((size_t)a.blocks + 1) * experts * sizeof(int));
-    a.ends = a.counts + (size_t)a.blocks * experts;
-    const size_t lds = kPlanWaves * experts * sizeof(int);
-    plan_count_kernel<<<a.blocks, kPlanThreads, lds, s>>>(a);
+    a.totals = a.counts + (size_t)a.blocks * experts;
+    plan_count_kernel<<<a.blocks, kPlanThreads, kPlanWaves * experts * sizeof(int), s>>>(a);
     GRAFT_LAUNCH_CHECK();
-    plan_scan_kernel<<<1, 1024, 0, s>>>(a);
+    plan_scan_kernel<<<experts, 64, 0, s>>>(a);
     GRAFT_LAUNCH_CHECK();
     plan_place_kernel<<<a.blocks + 64, kPlanThreads, lds, s>>>(a, bits);
     GRAFT_LAUNCH_CHECK();
