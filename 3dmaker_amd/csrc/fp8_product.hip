@@ -68,7 +68,7 @@ __device__ __forceinline__ void each(F&& f)
 
 // The workgroup meets when its waves' memory counters have come down to COUNTS
 // (an s_waitcnt operand); no memory access moves across.
-constexpr int kAllDone = 0x0070, kLdsDone = 0xc07f;
+constexpr int kAllDone = 0x0070, kLdsDone = 0xc07f, kCopiesDone = 0x0f70;
 template <int COUNTS>
 __device__ __forceinline__ void meet()
 {
@@ -130,6 +130,27 @@ __device__ __forceinline__ void row_tiles(const ProductArgs& a, int* starts)
         if (lane == 0) starts[a.experts] = before;
     }
     __syncthreads();
+}
+
+// Experts in the order of their columns, most first (equal ones in their own
+// order), up to 128 of them; more balance themselves.
+__device__ __forceinline__ void by_length(const ProductArgs& a, int* order)
+{
+    int* length = order + a.experts;
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+        order[e] = e;
+        if (a.experts <= 128) length[e] = a.offsets[e + 1] - a.offsets[e];
+    }
+    __syncthreads();
+    if (a.experts <= 128) {
+        const int e = threadIdx.x;
+        if (e < a.experts) {
+            int rank = 0;
+            for (int o = 0; o < a.experts; o++) rank += length[o] > length[e] || (length[o] == length[e] && o < e);
+            order[rank] = e;
+        }
+        __syncthreads();
+    }
 }
 
 // The expert whose row tiles hold tile t < starts[experts].
@@ -220,11 +241,27 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
         row_tile_count = __builtin_amdgcn_readfirstlane(starts[a.experts]);
         total = row_tile_count * a.tiles_n;
     }
-    // Workgroups go round the XCDs: each XCD works through a range of its own.
+    // Workgroups go round the XCDs.  Each XCD works through a range of tiles of its
+    // own; but where experts' k differ (SUM), a range of one expert's would leave
+    // the XCDs of small ones idle (experts of 1,700 to 11,000 columns: 200 us): there
+    // the workgroups take the tiles of the experts of most k first, every second
+    // round backwards, and an expert's tiles are dealt to all XCDs in ranges.
+    const int per = a.tiles_m * a.tiles_n;
+    if (a.grouping == PRODUCT_SUM) by_length(a, starts);
     const int xcd = blockIdx.x & 7, x0 = xcd * (total / 8) + min(xcd, total % 8), xn = total / 8 + (xcd < total % 8);
-    const int stride = (gridDim.x + 7 - xcd) / 8;
-    int at = blockIdx.x >> 3;
-    if (at >= xn) return;
+    int round = 0;
+    auto tile_of_round = [&]() -> int {  // -1: none left
+        if (a.grouping == PRODUCT_SUM) {
+            const int t = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            if (t >= total) return -1;
+            const int rank = t / per, q = t - rank * per;
+            return starts[rank] * per + (per % 8 == 0 ? q % 8 * (per / 8) + q / 8 : q);
+        }
+        const int at = (blockIdx.x >> 3) + round * ((gridDim.x + 7 - xcd) / 8);
+        return at < xn ? x0 + at : -1;
+    };
+    int tile = __builtin_amdgcn_readfirstlane(tile_of_round());
+    if (tile < 0) return;
 
     int row0, row1, n0, kb0, kb1;
     long long out0;
@@ -233,8 +270,8 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
     auto place = [&](int t) {  // four row tiles by all columns at a time: what an XCD has in flight shares its L2
         int expert = 0;
         if (a.grouping == PRODUCT_SUM) {
-            expert = t / (a.tiles_m * a.tiles_n);
-            t -= expert * a.tiles_m * a.tiles_n;
+            expert = t / per;
+            t -= expert * per;
         }
         const int group = t / (4 * a.tiles_n), first = group * 4, rows = min(4, row_tile_count - first);
         const int in = t - first * a.tiles_n, tm = first + in % rows;
@@ -385,7 +422,8 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
         quadrant(a0, wa, lower, by, wy, Y, [&](auto m) {
             spread(a_reads, m, [&](int q) { read_a(a1[q / 2], stage, MH + q / 2, q % 2); });
         });
-        meet<kAllDone>();  // the next block is here, this one is read
+        if (kb != kb0) __builtin_amdgcn_s_waitcnt(kCopiesDone);  // the next block is here (the second was before the first)
+        meet<kLdsDone>();                                        // this one is read
         const int after = min(kb + 2, kb1 - 1);  // behind the last block: copied again, and not read
         if constexpr (WIDE) widen_all(wa, a1, sa, MH);
         quadrant(a1, wa, upper, by, wy, Y, [&](auto m) {
@@ -405,9 +443,14 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
         scales(slot);
     };
 
-    place(x0 + at);
-    if (kb0 < kb1) copy_first();
-    copy_scales(kb0 & ~3);
+    // What a tile needs before its first block; done when this returns.
+    auto begin = [&] {
+        place(tile);
+        if (kb0 < kb1) copy_first();
+        copy_scales(kb0 & ~3);
+        __builtin_amdgcn_s_waitcnt(kCopiesDone);
+    };
+    begin();
     for (;;) {
 #pragma unroll
         for (int i = 0; i < NT; i++)
@@ -415,7 +458,7 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
             for (int j = 0; j < MT; j++) acc[i][j] = f4zero();
         const int r0 = row0, r1 = row1, c0 = n0;
         const long long o0 = out0;
-        meet<kAllDone>();
+        meet<kLdsDone>();
         if (kb0 < kb1) {
             scales(kb0 & 3);
 #pragma unroll
@@ -431,16 +474,13 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
             }
             if (kb < kb1) block(kb, 0, b0, w0, lower, b1, w1, upper);
         }
-        at += stride;
-        const bool more = at < xn;
+        round++;
+        tile = __builtin_amdgcn_readfirstlane(tile_of_round());
         // Copies behind the last block end here at the latest.  The next tile's are
-        // under way while this one's results are stored.
+        // here before this one's results are stored, so that its first block need
+        // not wait for the stores.
         meet<kAllDone>();
-        if (more) {
-            place(x0 + at);
-            if (kb0 < kb1) copy_first();
-            copy_scales(kb0 & ~3);
-        }
+        if (tile >= 0) begin();
 #pragma unroll
         for (int j = 0; j < MT; j++) {
             const int r = r0 + wm * (TM / WM) + j * 16 + col;
@@ -454,7 +494,7 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
                 if (n < a.n) store_row<T, 8>(a, row, n, v);
             }
         }
-        if (!more) break;
+        if (tile < 0) break;
     }
 #endif
 }
