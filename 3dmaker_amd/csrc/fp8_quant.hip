@@ -29,10 +29,23 @@ struct QuantArgs {
     bool vec;  // source rows are whole 16-byte pieces of eight columns
 };
 
-__device__ __forceinline__ uint32_t magnitude(float v)
+// Bits of |v|: larger floats have larger ones.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+
+constexpr uint32_t kInfinity = 0x7f800000u;
+
+// Largest of a thread's values with infinities and NaN left out: only where a
+// block's largest is one, which it seldom is.
+template <int N, class F>
+__device__ __forceinline__ uint32_t largest_finite(F&& value)
 {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
-    return u < 0x7f800000u ? u : 0u;  // infinities and NaN do not set the scale
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t m = magnitude(value(i));
+        top = m < kInfinity ? max(top, m) : top;
+    }
+    return top;
 }
 
 // Scale byte of a block from the bits of its largest finite magnitude.
@@ -47,16 +60,29 @@ __device__ __forceinline__ float inverse_scale(int byte)
     return __builtin_bit_cast(float, (uint32_t)(254 - byte) << 23);
 }
 
-__device__ __forceinline__ float fp8_operand(float v, float inverse)
-{
-    return fabsf(v) < INFINITY ? v * inverse : __builtin_nanf("");
-}
-
+// Infinities and NaN become NaN: the conversion has no infinity, and nothing
+// finite is above 448 here.
 __device__ __forceinline__ uint32_t fp8x4(const float* v, float inverse)
 {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_operand(v[0], inverse), fp8_operand(v[1], inverse), 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_operand(v[2], inverse), fp8_operand(v[3], inverse), w, true);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inverse, v[1] * inverse, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inverse, v[3] * inverse, w, true);
     return (uint32_t)w;
+}
+
+// Scale byte of the 128 values of 16 lanes, eight each.
+__device__ __forceinline__ int row_byte(const float (&v)[8])
+{
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) top = max(top, magnitude(v[j]));
+    top = lanes_umax<16>(top);
+    if (top >= kInfinity) {
+        top = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = max(top, magnitude(v[j]) < kInfinity ? magnitude(v[j]) : 0u);
+        top = lanes_umax<16>(top);
+    }
+    return scale_byte(top);
 }
 
 // Where a quantised row comes from; weight 0 and no source where there is none.
@@ -98,9 +124,18 @@ __device__ __forceinline__ void load_rows(float (&v)[R][8], const QuantArgs& a, 
             for (int q = 0; q < P; q++)
                 raw[i][q] = *reinterpret_cast<const Vec<T, N>*>(src + s[i].row * a.stride + (col[i] < a.cols ? col[i] : 0) + q * N);
 #pragma unroll
-        for (int i = 0; i < R; i++)
+        for (int i = 0; i < R; i++) {
+            const bool there = s[i].there && col[i] < a.cols;
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[i][j] = s[i].there && col[i] < a.cols ? (float)raw[i][j / N][j % N] : 0.0f;
+            for (int q = 0; q < P; q++) {
+                const Vec<uint32_t, 4> bits = __builtin_bit_cast(Vec<uint32_t, 4>, raw[i][q]);
+                const Vec<uint32_t, 4> kept{there ? bits[0] : 0u, there ? bits[1] : 0u, there ? bits[2] : 0u,
+                                            there ? bits[3] : 0u};
+                const Vec<T, N> w = __builtin_bit_cast(Vec<T, N>, kept);
+#pragma unroll
+                for (int j = 0; j < N; j++) v[i][q * N + j] = (float)w[j];
+            }
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < R; i++)
@@ -112,7 +147,7 @@ __device__ __forceinline__ void load_rows(float (&v)[R][8], const QuantArgs& a, 
 #pragma unroll
         for (int i = 0; i < R; i++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[i][j] = s[i].there ? v[i][j] * s[i].weight : 0.0f;
+            for (int j = 0; j < 8; j++) v[i][j] *= s[i].weight;  // 1 where there is no source, and zeros
     }
     if (a.gate) {
         const T* gate = (const T*)a.gate;
@@ -147,10 +182,7 @@ __global__ __launch_bounds__(kQuantThreads) void quant_rows_kernel(QuantArgs a)
     load_rows(v, a, src, row, col);
 #pragma unroll
     for (int u = 0; u < UNITS; u++) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) top = max(top, magnitude(v[u][j]));
-        const int byte = scale_byte(lanes_umax<16>(top));
+        const int byte = row_byte(v[u]);
         if (row[u] >= a.rows) continue;
         const float inv = inverse_scale(byte);
         const long long r = (long long)blockIdx.y * a.rows + row[u];
@@ -185,6 +217,7 @@ __global__ __launch_bounds__(kQuantThreads) void quant_tile_kernel(QuantArgs a)
         for (int i = 0; i < 8; i++)
 #pragma unroll
             for (int j = 0; j < 8; j++) top = max(top, magnitude(v[i][j]));
+        if (lanes_umax<64>(top) >= kInfinity) top = largest_finite<64>([&](int i) { return v[i / 8][i % 8]; });
         top = lanes_umax<64>(top);
         if ((threadIdx.x & 63) == 0) wave_top[threadIdx.x >> 6] = top;
         __syncthreads();
@@ -194,12 +227,7 @@ __global__ __launch_bounds__(kQuantThreads) void quant_tile_kernel(QuantArgs a)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             int byte = block_byte;
-            if (!BLOCKS) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int j = 0; j < 8; j++) top = max(top, magnitude(v[i][j]));
-                byte = scale_byte(lanes_umax<16>(top));
-            }
+            if (!BLOCKS) byte = row_byte(v[i]);
             if (row_of[i] >= a.rows) continue;
             const float inv = inverse_scale(byte);
             const long long r = (long long)blockIdx.z * a.rows + row_of[i];
@@ -217,6 +245,7 @@ __global__ __launch_bounds__(kQuantThreads) void quant_tile_kernel(QuantArgs a)
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 8; i++) top = max(top, magnitude(v[i][j]));
+            if (top >= kInfinity) top = largest_finite<8>([&](int i) { return v[i][j]; });
             tops[ty][j * 16 + tx] = top;  // column tx * 8 + j
         }
         __syncthreads();
