@@ -236,9 +236,21 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
     int total = a.tiles_m * a.tiles_n;
     if (a.grouping == PRODUCT_SUM) total *= a.experts;
     int row_tile_count = a.tiles_m;
+    // The segments: up to 64 of them lane by lane (rows, and the row tiles up to
+    // their end), more through LDS and memory.
+    int seg_lo = 0, seg_hi = 0, seg_end = 0;
     if (a.grouping == PRODUCT_ROWS) {
-        row_tiles<TM>(a, starts);
-        row_tile_count = __builtin_amdgcn_readfirstlane(starts[a.experts]);
+        if (a.experts <= 64) {
+            if (lane < a.experts) {
+                seg_lo = min(max(a.offsets[lane], 0), a.m);
+                seg_hi = min(max(a.offsets[lane + 1], seg_lo), a.m);
+            }
+            seg_end = lanes_scan((seg_hi - seg_lo + TM - 1) / TM);
+            row_tile_count = __builtin_amdgcn_readlane(seg_end, 63);
+        } else {
+            row_tiles<TM>(a, starts);
+            row_tile_count = __builtin_amdgcn_readfirstlane(starts[a.experts]);
+        }
         total = row_tile_count * a.tiles_n;
     }
     // Workgroups go round the XCDs.  Each XCD works through a range of tiles of its
@@ -284,12 +296,17 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
         SB = a.bs;
         out0 = 0;
         if (a.grouping == PRODUCT_ROWS) {
-            expert = __builtin_amdgcn_readfirstlane(expert_of_tile(starts, a.experts, tm));
-            const int lo = min(max(a.offsets[expert], 0), a.m);
-            row0 = lo + (tm - starts[expert]) * TM;
-            row1 = min(max(a.offsets[expert + 1], lo), a.m);
-            row0 = __builtin_amdgcn_readfirstlane(row0);
-            row1 = __builtin_amdgcn_readfirstlane(row1);
+            if (a.experts <= 64) {
+                expert = __ffsll((unsigned long long)__ballot(seg_end > tm)) - 1;
+                row1 = __builtin_amdgcn_readlane(seg_hi, expert);
+                row0 = __builtin_amdgcn_readlane(seg_lo, expert);
+                row0 += (tm - __builtin_amdgcn_readlane(seg_end, expert) + (row1 - row0 + TM - 1) / TM) * TM;
+            } else {
+                expert = __builtin_amdgcn_readfirstlane(expert_of_tile(starts, a.experts, tm));
+                const int lo = min(max(a.offsets[expert], 0), a.m);
+                row0 = __builtin_amdgcn_readfirstlane(lo + (tm - starts[expert]) * TM);
+                row1 = __builtin_amdgcn_readfirstlane(min(max(a.offsets[expert + 1], lo), a.m));
+            }
             B += expert * a.b_size;
             SB += expert * a.bs_size;
         } else if (a.grouping == PRODUCT_SUM) {
