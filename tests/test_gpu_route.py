@@ -157,7 +157,7 @@ def test_route_backward(T, E, k, sigmoid, renorm, code, pad):
 
 @pytest.mark.parametrize("T,k,E,align", [
     (0, 2, 4, 128), (1, 1, 1, 1), (1, 8, 256, 128), (7, 2, 16, 16), (300, 3, 5, 128), (1365, 3, 1024, 1), (2048, 2, 8, 128),
-    (2049, 2, 8, 128), (5000, 4, 60, 64), (9000, 8, 1024, 128), (40000, 1, 2, 7), (70000, 2, 1, 128)])
+    (2049, 2, 8, 128), (5000, 4, 60, 64), (9000, 8, 1024, 128), (40000, 1, 2, 7), (70000, 2, 1, 128), (70001, 2, 700, 16)])
 @pytest.mark.parametrize("holes", [False, True])
 def test_plan(T, k, E, align, holes):
     print(f"[plan] T={T} k={k} E={E} align={align}", flush=True)
