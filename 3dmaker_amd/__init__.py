@@ -355,10 +355,10 @@ def launch(name: str, *args):
 
     Objects with data_ptr() are passed as their device pointer; ctypes
     structures should be passed by reference (ctypes.byref)."""
-    L = lib()
-    conv = [ptr(a) if hasattr(a, "data_ptr") else a for a in args]
-    getattr(L, name)(*conv)
-    check()
+    L = _LIB or lib()
+    getattr(L, name)(*[a.data_ptr() if hasattr(a, "data_ptr") else a for a in args])
+    if L.tinymlp_last_error():
+        check()
 
 
 class HashGrid:
