@@ -329,17 +329,20 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteArgs
         chosen |= d != kNone ? 1u << i : 0u;
         g[i] = __builtin_bit_cast(float, d);
     }
-    float total = 0.0f, dot = 0.0f;
+    float total = 0.0f, shift = 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        const bool in = chosen >> i & 1;
-        total += in ? s[i] : 0.0f;
-        dot += in ? s[i] * g[i] : 0.0f;
-    }
+    for (int i = 0; i < V; i++) total += chosen >> i & 1 ? s[i] : 0.0f;
     total = lanes_sum<LPT>(total) + 1e-20f;
-    dot = lanes_sum<LPT>(dot);
     const float r = a.renorm ? 1.0f / total : 1.0f;
-    const float shift = a.renorm ? dot * r : 0.0f;
+    if (a.renorm) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            // s / total to the last bit: one expert's weight is 1, its gradient 0
+            const float w = s[i] * r;
+            shift += chosen >> i & 1 ? g[i] * fmaf(fmaf(-w, total, s[i]), r, w) : 0.0f;
+        }
+        shift = lanes_sum<LPT>(shift);
+    }
     float back = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; i++) {

@@ -155,6 +155,19 @@ def test_route_backward(T, E, k, sigmoid, renorm, code, pad):
     assert abs(float(diff - got)) <= float(size) * (8 * REL + 2 * R.HALF[code] + 1e-6)
 
 
+@pytest.mark.parametrize("sigmoid", [0, 1])
+def test_one_renormalised_expert_has_no_gradient(sigmoid):
+    """Its weight is s / (s + 1e-20) = 1 in fp32, whatever its logit."""
+    T, E = 500, 24
+    g = R.gen(6)
+    z, dw = R.randn(g, T, E) * 2, R.randn(g, T, 1)
+    idx = torch.randint(0, E, (T, 1), generator=g, device="cuda").int()
+    out = torch.full((T, E), 9.0, device="cuda")
+    R.launch("launchRouteExpertsBackward", C.byref(option(E, 1, sigmoid)), z, E, idx, dw, out, E, T, R.stream())
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+
+
 @pytest.mark.parametrize("T,k,E,align", [
     (0, 2, 4, 128), (1, 1, 1, 1), (1, 8, 256, 128), (7, 2, 16, 16), (300, 3, 5, 128), (1365, 3, 1024, 1), (2048, 2, 8, 128),
     (2049, 2, 8, 128), (5000, 4, 60, 64), (9000, 8, 1024, 128), (40000, 1, 2, 7), (70000, 2, 1, 128), (70001, 2, 700, 16)])
