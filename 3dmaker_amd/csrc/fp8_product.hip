@@ -4,11 +4,11 @@
 // Two matrix instructions carry it.  v_mfma_scale_f32_16x16x128_f8f6f4 takes 128
 // of k, one block, and both scales; its accumulators are fp32, but it adds eight
 // products at a time and cuts them below 2^-13 of the largest (measured: a 15
-// beside 65536 counts as 8), which leaves sums of normal values 1.5e-5 off (of
-// their 2-norm).  That is a sixteenth of an fp16 output's own rounding, so 16-bit
-// outputs take it.  fp32 outputs (weight gradients) take
-// v_mfma_f32_16x16x32_bf16 on operands widened with their scales, which is exact:
-// products and sums in fp32 (4e-8), at half the rate.
+// beside 65536 counts as 8), which leaves sums of normal values 1.5e-5 off and of
+// values spread over all of e4m3 5e-5 (of their 2-norm).  That is a fifth of an
+// fp16 output's own rounding, so 16-bit outputs take it.  fp32 outputs and weight
+// gradients take v_mfma_f32_16x16x32_bf16 on operands widened with their scales,
+// which is exact: products and sums in fp32 (4e-8), at half the rate.
 //
 // The first MFMA operand is B's rows, the second A's, so that a lane ends with
 // four consecutive n of one row m.  Its two operands are read with the same
@@ -615,7 +615,7 @@ void product_launch(ProductArgs& a, hipStream_t s)
     long long tiles = (long long)a.tiles_m * a.tiles_n;
     if (a.grouping == PRODUCT_ROWS) tiles = ((long long)a.m / TM + a.experts) * a.tiles_n;
     if (a.grouping == PRODUCT_SUM) tiles *= a.experts;
-    require(tiles <= 0x7fffffffll, "too many tiles for one call");
+    require(tiles <= 0x7fff0000ll, "too many tiles for one call");
     const long long slots = (long long)num_cus() * (TM * TN > 128 * 128 ? 1 : 2);
     product_kernel<T, TM, TN, WIDE><<<(unsigned)std::min(tiles, slots), 256, 0, s>>>(a);
     GRAFT_LAUNCH_CHECK();

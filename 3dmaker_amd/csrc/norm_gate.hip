@@ -75,10 +75,11 @@ struct Row {
     }
 };
 
-// A row's pieces as they lie in memory: what is fetched ahead.
+// A row's pieces as they lie in memory: what is fetched ahead.  Pieces behind the
+// row are never loaded and stay zero.
 template <class T, int VEC, int THREADS, int PER>
 struct Raw {
-    Vec<T, VEC> v[PER];
+    Vec<T, VEC> v[PER] = {};
 
     __device__ __forceinline__ void load(const T* p, int sub, int dim)
     {
@@ -88,12 +89,12 @@ struct Raw {
             if (c < dim) v[i] = *reinterpret_cast<const Vec<T, VEC>*>(p + c);
         }
     }
-    __device__ __forceinline__ void widen(float (&to)[VEC * PER], int sub, int dim) const
+    __device__ __forceinline__ void widen(float (&to)[VEC * PER]) const
     {
 #pragma unroll
         for (int i = 0; i < PER; i++)
 #pragma unroll
-            for (int j = 0; j < VEC; j++) to[i * VEC + j] = (i * THREADS + sub) * VEC < dim ? (float)v[i][j] : 0.0f;
+            for (int j = 0; j < VEC; j++) to[i * VEC + j] = (float)v[i][j];
     }
 };
 
@@ -265,9 +266,9 @@ __device__ __forceinline__ void norm_back(float (&d)[VEC * PER], const float (&n
         p = fmaf(d[i], n[i], p);
     }
     row_sum2<THREADS>(m, p, lds, slot);
-    m = kind == NORM_LAYER ? m * inv_dim : 0.0f;
-    p *= inv_dim;
-    each<VEC, THREADS, PER>(sub, dim, [&](int i, int) { d[i] = r * (d[i] - m - n[i] * p); });
+    m = kind == NORM_LAYER ? m * inv_dim * r : 0.0f;
+    p *= inv_dim * r;
+    each<VEC, THREADS, PER>(sub, dim, [&](int i, int) { d[i] = fmaf(-n[i], p, fmaf(d[i], r, -m)); });
 }
 
 // A workgroup: `chunk` rows of a span, its row groups (waves for THREADS 64) in
@@ -332,11 +333,11 @@ __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
         const int stop = next_flush < r1 ? next_flush : r1;
         while (row < stop) {
             float n1[N], n2[N], d[N], g[N], dy[N];
-            rx.widen(n2, sub, a.dim);
-            if (a.f) rf.widen(n1, sub, a.dim);
-            if (a.gate) rg.widen(g, sub, a.dim);
-            if (a.dh) rdh.widen(d, sub, a.dim);
-            if (a.dy) rdy.widen(dy, sub, a.dim);
+            rx.widen(n2);
+            if (a.f) rf.widen(n1);
+            if (a.gate) rg.widen(g);
+            if (a.dh) rdh.widen(d);
+            if (a.dy) rdy.widen(dy);
             if (row + kGroups < r1) fetch(row + kGroups);
             if (!kKeep) parameters();
             float r_1 = 1.0f;
@@ -344,8 +345,8 @@ __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
                 r_1 = normalise<VEC, THREADS, PER>(n1, a.post, sub, a.dim, a.inv_dim, a.eps, lds, 0);
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    const float u = n1[i] * w1.v[i] + b1.v[i];
-                    n2[i] = fmaf(a.alpha, n2[i], a.beta * (a.gate ? u * g[i] : u));
+                    g[i] = a.gate ? a.beta * g[i] : a.beta;  // the block's factor
+                    n2[i] = fmaf(g[i], fmaf(n1[i], w1.v[i], b1.v[i]), a.alpha * n2[i]);
                 }
             } else {
 #pragma unroll
@@ -369,17 +370,17 @@ __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
                 out.store((T*)a.dx + (long long)row * a.sx, sub, a.dim);
             }
             if (a.f) {
+                if (a.gate) {  // beta comes in where the sums are stored
 #pragma unroll
-                for (int i = 0; i < N; i++) d[i] *= a.beta;
-                if (a.gate) {
+                    for (int i = 0; i < N; i++) dg[i] = fmaf(d[i], fmaf(n1[i], w1.v[i], b1.v[i]), dg[i]);
+                    if (a.gate_mode == kGateRow) {
 #pragma unroll
-                    for (int i = 0; i < N; i++) {
-                        out.v[i] = d[i] * (n1[i] * w1.v[i] + b1.v[i]);
-                        dg[i] += out.v[i];
-                        d[i] *= g[i];
+                        for (int i = 0; i < N; i++) out.v[i] = a.beta * dg[i], dg[i] = 0.0f;
+                        out.store((T*)a.dgate + (long long)row * a.sg, sub, a.dim);
                     }
-                    if (a.gate_mode == kGateRow) out.store((T*)a.dgate + (long long)row * a.sg, sub, a.dim);
                 }
+#pragma unroll
+                for (int i = 0; i < N; i++) d[i] *= g[i];
                 norm_back<VEC, THREADS, PER>(d, n1, r_1, a.post, w1.v, dw1, db1, sub, a.dim, a.inv_dim, lds, 6);
                 if (a.df) {
 #pragma unroll
@@ -395,7 +396,7 @@ __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
             if (group == 0) {
                 R out;
 #pragma unroll
-                for (int i = 0; i < N; i++) out.v[i] = dg[i];
+                for (int i = 0; i < N; i++) out.v[i] = a.beta * dg[i];
                 out.store((T*)a.dgate + (long long)((stop - 1) / a.gate_rows) * a.sg, sub, a.dim);
             }
 #pragma unroll
@@ -418,32 +419,32 @@ __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
         joined(dg);
         if (group == 0)
             each<VEC, THREADS, PER>(sub, a.dim,
-                                    [&](int i, int c) { a.gate_sums[(long long)blockIdx.x * a.dim + c] = dg[i]; });
+                                    [&](int i, int c) { a.gate_sums[(long long)blockIdx.x * a.dim + c] = a.beta * dg[i]; });
     }
 }
 
-// Sums of `parts` rows of src (stride apart) in a fixed order: 16 columns a
-// workgroup, 16 interleaved shares of the parts.
-constexpr int kSumColumns = 16;
+// Sums of `parts` rows of src (stride apart) in a fixed order: 32 columns (a line)
+// a workgroup, 8 interleaved shares of the parts.
+constexpr int kSumColumns = 32, kSumShares = 256 / kSumColumns;
 template <class T>
 __device__ __forceinline__ void sum_parts(const float* src, long long stride, int parts, int dim, T* out, int column0)
 {
-    __shared__ float share[16][kSumColumns];
-    const int lane = threadIdx.x & 15, w = threadIdx.x >> 4, c = column0 + lane;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    __shared__ float share[kSumShares][kSumColumns];
+    const int lane = threadIdx.x % kSumColumns, w = threadIdx.x / kSumColumns, c = column0 + lane;
+    float s[8] = {};
     if (c < dim) {
         int p = w;
-        for (; p + 48 < parts; p += 64)
+        for (; p + 7 * kSumShares < parts; p += 8 * kSumShares)
 #pragma unroll
-            for (int q = 0; q < 4; q++) s[q] += src[(p + 16 * q) * stride + c];
-        for (; p < parts; p += 16) s[0] += src[p * stride + c];
+            for (int q = 0; q < 8; q++) s[q] += src[(p + kSumShares * q) * stride + c];
+        for (; p < parts; p += kSumShares) s[0] += src[p * stride + c];
     }
-    share[w][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+    share[w][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
     if (w == 0 && c < dim) {
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; i++) sum += share[i][lane];
+        for (int i = 0; i < kSumShares; i++) sum += share[i][lane];
         out[c] = (T)sum;
     }
 }

@@ -140,8 +140,9 @@ typedef struct Fp8ProductOption {
  * DENSE); SUM needs them to be multiples of 128 (align 128), and gives an
  * expert without columns zeros.  ROWS leaves rows outside all segments as they
  * are.  NaN in a row's values makes that row's results NaN.  fp32 results are
- * sums of exact products in fp32; 16-bit results may come from the matrix
- * cores' 8-bit sums, which are within 2^-15 of the size of the terms (2-norm). */
+ * sums of exact products in fp32, and so are all of SUM; other 16-bit results
+ * may come from the matrix cores' 8-bit sums, which are within 2^-14 of the
+ * exact ones (2-norm), below their own rounding. */
 void launchFp8Product(const Fp8ProductOption* opt, const uint8_t* d_a, const uint8_t* d_aScales, const uint8_t* d_b,
                       const uint8_t* d_bScales, const int* d_offsets, void* d_out, hipStream_t stream);
 
