@@ -201,7 +201,7 @@ __device__ __forceinline__ void store_row(const ProductArgs& a, T* row, int n, c
 // B's fragments.  The next quadrant's half is read from LDS, and the block after
 // the next copied to it, between this one's matrix instructions: a copy or read
 // that is issued in a burst holds the wave's matrix instructions up (8192 x
-// 5120 x 4096: 207 us with bursts, 170 spread).  The order is held by the empty
+// 5120 x 4096 in tiles of 256: 207 us with bursts, 197 spread; of 128: 176 and 168).  The order is held by the empty
 // asm on the accumulators and the scheduling barriers.  The one barrier of a
 // block stands behind its last LDS read, half a block before its last matrix
 // instruction.
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
 // bytes bound it, so both operands go straight from memory to registers, all of
 // a wave's four blocks under way at once, and are widened (one row by 4096 x
 // 4096: 21 us through the tiles above, whose 32 workgroups wait for one block
-// after the other).
+// after the other; 5.7 us here).
 constexpr int kFewWaves = 8;
 template <class T, int MT>
 __global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(ProductArgs a)

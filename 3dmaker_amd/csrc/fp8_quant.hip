@@ -162,8 +162,8 @@ __device__ __forceinline__ void load_rows(float (&v)[R][8], const QuantArgs& a, 
 }
 
 // Rows only: 16 lanes a (row, block), UNITS of them 16 apart.  Four at a time
-// once there are enough for all CUs (65,536 x 1,024 bf16 gathered: 50 us with
-// one, whose loads wait for one another's row numbers).
+// once there are enough for all CUs (65,536 x 1,024 bf16 gathered: 45 us, 4.5 TB/s
+// of its 201 MB; 50 with one, whose loads wait for one another's row numbers).
 template <class T, int UNITS>
 __global__ __launch_bounds__(kQuantThreads) void quant_rows_kernel(QuantArgs a)
 {
@@ -195,7 +195,8 @@ __global__ __launch_bounds__(kQuantThreads) void quant_rows_kernel(QuantArgs a)
 // A tile of 128 x 128 in registers (thread: 8 rows by 8 columns), as rows,
 // as columns or both.  The transposed bytes cross LDS in pieces of 8, piece ty of
 // column c at ty ^ (c / 8): a wave's writes, one column of every eight, spread
-// over the banks.
+// over the banks.  33,792 x 2,048 fp16 gathered and weighted, both ways: 64 us,
+// 4.2 TB/s of its 272 MB.
 template <class T, bool BLOCKS>
 __global__ __launch_bounds__(kQuantThreads) void quant_tile_kernel(QuantArgs a)
 {

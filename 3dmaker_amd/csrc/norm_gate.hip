@@ -213,6 +213,8 @@ __device__ __forceinline__ void affine(float (&v)[VEC * PER], const float* w, co
     }
 }
 
+// A wave or a workgroup a row, which is read once (32,769 x 2,048 bf16: 117 us,
+// 4.6 TB/s; with the parameters read element by element 322).
 template <class T, int VEC, int THREADS, int PER>
 __global__ __launch_bounds__(256) void norm_gate_kernel(NormArgs a)
 {
@@ -274,8 +276,9 @@ __device__ __forceinline__ void norm_back(float (&d)[VEC * PER], const float (&n
 // A workgroup: `chunk` rows of a span, its row groups (waves for THREADS 64) in
 // turn; sums over its rows go to sums[part], or for one part to the outputs.  The
 // next row is fetched while this one is worked on: without that a row waits for
-// four tensors one after the other (16,389 x 1,280 fp16: 237 us, 16 % of the
-// copy rate).
+// four tensors one after the other (16,389 x 1,280 fp16, layer norms: 237 us;
+// 67 now, 3.8 TB/s).  Bound by about 600 instructions a thread and row, at three
+// waves a SIMD: 168 registers are the most for these.
 template <class T, int VEC, int THREADS, int PER, int WG>
 __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
 {
