@@ -514,7 +514,7 @@ namespace {
 constexpr int kPlanThreads = 256;
 constexpr int kPlanWaves = kPlanThreads / 64;
 constexpr int kPlanSmall = 4096;  // slots that one workgroup places alone
-constexpr int kPlanChunk = 1024;  // of a workgroup otherwise: four rounds a wave
+constexpr int kPlanRounds = 4, kPlanChunk = kPlanRounds * kPlanThreads;  // of a workgroup otherwise
 
 struct PlanArgs {
     const int* indices;
@@ -527,38 +527,50 @@ struct PlanArgs {
     bool scanned;
 };
 
-__device__ __forceinline__ int expert_of(const PlanArgs& a, int slot, int end)
-{
-    const int e = slot < end ? a.indices[slot] : -1;
-    return (unsigned)e < (unsigned)a.experts ? e : -1;
-}
+// A wave's slots of a workgroup's, up to R rounds of 64: their experts (-1: none),
+// all loaded before the first is used.
+template <int R>
+struct PlanSlots {
+    int first, rounds;
+    int expert[R];
 
-// Rows of the waves of the block in front of each other: hist [waves][experts]
-// counts of each wave's quarter of the chunk.
-__device__ __forceinline__ void plan_count(const PlanArgs& a, int* hist, int begin, int end, int wave, int lane, int waves)
-{
-    for (int i = threadIdx.x; i < waves * a.experts; i += blockDim.x) hist[i] = 0;
-    __syncthreads();
-    const int span = ((end - begin + waves * 64 - 1) / (waves * 64)) * 64;
-    const int w0 = begin + wave * span, w1 = min(end, w0 + span);
-    for (int i = w0 + lane; i < w1; i += 64) {
-        const int e = expert_of(a, i, end);
-        if (e >= 0) atomicAdd(&hist[wave * a.experts + e], 1);
+    __device__ __forceinline__ PlanSlots(const PlanArgs& a, int begin, int rounds) : rounds(rounds)
+    {
+        first = begin + (threadIdx.x >> 6) * (rounds * 64);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int i = first + r * 64 + (threadIdx.x & 63);
+            expert[r] = r < rounds && i < a.slots ? a.indices[i] : -1;
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) expert[r] = (unsigned)expert[r] < (unsigned)a.experts ? expert[r] : -1;
     }
+};
+
+// hist [waves][experts]: each wave's slots of an expert.
+template <int R>
+__device__ __forceinline__ void plan_count(const PlanArgs& a, int* hist, const PlanSlots<R>& slots)
+{
+    for (int i = threadIdx.x; i < kPlanWaves * a.experts; i += kPlanThreads) hist[i] = 0;
+    __syncthreads();
+    int* const mine = hist + (threadIdx.x >> 6) * a.experts;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+        if (slots.expert[r] >= 0) atomicAdd(&mine[slots.expert[r]], 1);
     __syncthreads();
 }
 
-// The slots of a wave's part in order: rank among the wave's lanes of the same
-// expert from one ballot per bit of the expert's number.
-__device__ __forceinline__ void plan_place(const PlanArgs& a, int* next, int begin, int end, int wave, int lane, int waves,
-                                           int bits)
+// The wave's slots in order, from next [waves][experts]: rank among the round's
+// slots of the same expert from one ballot per bit of the expert's number.
+template <int R>
+__device__ __forceinline__ void plan_place(const PlanArgs& a, int* next, const PlanSlots<R>& slots, int bits)
 {
-    const int span = ((end - begin + waves * 64 - 1) / (waves * 64)) * 64;
-    const int w0 = begin + wave * span, w1 = min(end, w0 + span);
-    int* mine = next + wave * a.experts;
-    for (int i0 = w0; i0 < w1; i0 += 64) {
-        const int i = i0 + lane;
-        const int e = expert_of(a, i, w1);
+    const int lane = threadIdx.x & 63;
+    int* const mine = next + (threadIdx.x >> 6) * a.experts;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        if (r >= slots.rounds) continue;
+        const int i = slots.first + r * 64 + lane, e = slots.expert[r];
         uint64_t same = __ballot(e >= 0);
         for (int b = 0; b < bits; b++) {
             const uint64_t m = __ballot(e >> b & 1);
@@ -570,7 +582,7 @@ __device__ __forceinline__ void plan_place(const PlanArgs& a, int* next, int beg
             row = mine[e] + rank;
             a.order[row] = i;
         }
-        if (i < w1) a.position[i] = row;
+        if (i < a.slots) a.position[i] = row;
         __builtin_amdgcn_wave_barrier();
         if (e >= 0 && rank == 0) mine[e] += __popcll(same);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -581,8 +593,7 @@ __device__ __forceinline__ void plan_place(const PlanArgs& a, int* next, int beg
 __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(PlanArgs a)
 {
     extern __shared__ int hist[];
-    const int begin = blockIdx.x * kPlanChunk, end = min(a.slots, begin + kPlanChunk);
-    plan_count(a, hist, begin, end, threadIdx.x / 64, threadIdx.x & 63, kPlanWaves);
+    plan_count(a, hist, PlanSlots<kPlanRounds>(a, blockIdx.x * kPlanChunk, kPlanRounds));
     for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) {
         int n = 0;
         for (int w = 0; w < kPlanWaves; w++) n += hist[w * a.experts + e];
@@ -689,8 +700,9 @@ __device__ __forceinline__ void plan_waves(const PlanArgs& a, int* next, F add)
 
 // Blocks 0 .. blocks - 1 place their slots; those behind them fill the other
 // rows.  Every one forms the offsets for itself.  Latency: four rounds of 64
-// slots a wave behind the offsets (7 us for 131,128 slots of 256 experts; chunks
-// of 4,096 slots instead of 1,024 took 15).
+// slots a wave behind the offsets, whose loads are issued ahead of them (5.4 us
+// for 131,128 slots of 256 experts, 7.2 with a load in each round; chunks of
+// 4,096 slots instead of 1,024 took 15).
 __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(PlanArgs a, int bits)
 {
     extern __shared__ int lds[];
@@ -699,6 +711,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(PlanArgs a, in
     int* ends = starts + a.experts + 1;         // [experts]
     int* before = ends + a.experts;             // [experts]
     const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const PlanSlots<kPlanRounds> slots(a, blockIdx.x * kPlanChunk, kPlanRounds);
     plan_totals(a, blockIdx.x, starts, before);
     plan_offsets(a, starts, ends, lane, wave);
     if ((int)blockIdx.x >= a.blocks) {
@@ -708,13 +721,13 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(PlanArgs a, in
         plan_fill(a, starts, ends, fill, gridDim.x - a.blocks);
         return;
     }
-    const int begin = blockIdx.x * kPlanChunk, end = min(a.slots, begin + kPlanChunk);
-    plan_count(a, next, begin, end, wave, lane, kPlanWaves);
+    plan_count(a, next, slots);
     plan_waves(a, next, [&](int e) { return starts[e] + before[e]; });
-    plan_place(a, next, begin, end, wave, lane, kPlanWaves, bits);
+    plan_place(a, next, slots, bits);
 }
 
-// Few slots: one workgroup does all of it.
+// Few slots, up to 256 R: one workgroup does all of it.
+template <int R>
 __global__ __launch_bounds__(kPlanThreads) void plan_small_kernel(PlanArgs a, int bits)
 {
     extern __shared__ int lds[];
@@ -722,7 +735,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_small_kernel(PlanArgs a, in
     int* starts = next + kPlanWaves * a.experts;
     int* ends = starts + a.experts + 1;
     const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    plan_count(a, next, 0, a.slots, wave, lane, kPlanWaves);
+    const PlanSlots<R> slots(a, 0, (a.slots + kPlanThreads - 1) / kPlanThreads);
+    plan_count(a, next, slots);
     for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) {
         int n = 0;
         for (int w = 0; w < kPlanWaves; w++) n += next[w * a.experts + e];
@@ -733,7 +747,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_small_kernel(PlanArgs a, in
     for (int e = threadIdx.x; e <= a.experts; e += kPlanThreads) a.offsets[e] = starts[e];
     plan_fill(a, starts, ends, 0, 1);
     plan_waves(a, next, [&](int e) { return starts[e]; });
-    plan_place(a, next, 0, a.slots, wave, lane, kPlanWaves, bits);
+    plan_place(a, next, slots, bits);
 }
 
 }  // namespace
@@ -767,7 +781,8 @@ void route_plan(const int* indices, int tokens, int topK, int experts, int align
     while ((1 << bits) < experts) bits++;
     const size_t lds = ((kPlanWaves + 3) * experts + 1) * sizeof(int);
     if (a.slots <= kPlanSmall) {
-        plan_small_kernel<<<1, kPlanThreads, lds, s>>>(a, bits);
+        if (a.slots <= 4 * kPlanThreads) plan_small_kernel<4><<<1, kPlanThreads, lds, s>>>(a, bits);
+        else plan_small_kernel<kPlanSmall / kPlanThreads><<<1, kPlanThreads, lds, s>>>(a, bits);
         GRAFT_LAUNCH_CHECK();
         return;
     }
