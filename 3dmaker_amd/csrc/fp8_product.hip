@@ -607,6 +607,29 @@ void few_launch(ProductArgs& a, hipStream_t s)
     GRAFT_LAUNCH_CHECK();
 }
 
+// 16-row tiles a workgroup where sharing out k is the faster way, 0 where the
+// 128 x 128 tiles are: the time of a block of k on a CU, in units of 10 ns, times
+// the rounds of workgroups over the CUs.  A few-rows workgroup's goes by the rows
+// of A beside its 16 of B, a tile's by the form of its products (dense, k = 4096,
+// sharing against tiles: 65 x 512 fp32 7 and 34 us, 128 x 2048 bf16 12.7 and
+// 17.0, 300 x 2048 fp32 29.6 and 34.9; 64 x 65536 bf16 164 and 45, 1024 x 2048
+// bf16 79 and 23).  Experts are taken to be of equal length, without the empty
+// ones that a short plan is bound to have.
+int few_tiles(const Fp8ProductOption& o, bool wide)
+{
+    const long long cus = num_cus(), experts = o.grouping == PRODUCT_DENSE ? 1 : std::min(o.numExperts, o.m);
+    const long long rows = (o.m + experts - 1) / experts;
+    const long long tiles = experts * ((rows + 127) / 128) * ((o.n + 127) / 128);
+    double best = (double)((tiles + cus - 1) / cus) * (wide ? 95 : 45);
+    int chosen = 0;
+    for (int mt = 1; mt <= 4; mt *= 2) {
+        const long long groups = experts * ((rows + 16 * mt - 1) / (16 * mt)) * ((o.n + 15) / 16);
+        const double cost = std::max(1.0, (double)groups / cus) * (7 + 0.37 * std::min<long long>(rows, 16 * mt));
+        if (cost < best) best = cost, chosen = mt;
+    }
+    return chosen;
+}
+
 template <class T, int TM, int TN, bool WIDE>
 void product_launch(ProductArgs& a, hipStream_t s)
 {
@@ -664,23 +687,26 @@ void fp8_product(const Fp8ProductOption& o, const uint8_t* a, const uint8_t* a_s
     p.vec = aligned16(out) && o.outStride * data_bytes(o.outType) % 16 == 0;
     with_type(o.outType, [&](auto zero) {
         using T = decltype(zero);
-        // Few rows, or few to an expert on average.
-        if (o.grouping != PRODUCT_SUM) {
-            const long long rows = (o.m + o.numExperts - 1ll) / o.numExperts;
-            if (rows <= 16) return few_launch<T, 1>(p, s);
-            if (rows <= 32) return few_launch<T, 2>(p, s);
-            if (rows <= 64) return few_launch<T, 4>(p, s);
-        }
         // fp32 results, weight gradients of any type, and products of up to two
         // blocks of k, which their output's bytes bound: there widening costs nothing.
-        if (std::is_same_v<T, float> || o.grouping == PRODUCT_SUM || p.pitch <= 256) return product_launch<T, 128, 128, true>(p, s);
+        const bool wide = std::is_same_v<T, float> || o.grouping == PRODUCT_SUM || p.pitch <= 256;
+        if (o.grouping != PRODUCT_SUM) {
+            const int few = few_tiles(o, wide);
+            if (few == 1) return few_launch<T, 1>(p, s);
+            if (few == 2) return few_launch<T, 2>(p, s);
+            if (few == 4) return few_launch<T, 4>(p, s);
+        }
+        if (wide) return product_launch<T, 128, 128, true>(p, s);
         if constexpr (!std::is_same_v<T, float>) {
             // Rounds of tiles over the CUs, by what a round takes: 256 x 256 at 2.5
-            // PFLOP/s, two 128 x 128 a CU at 2.2.
-            const long long cus = num_cus(), experts = o.grouping == PRODUCT_DENSE ? 0 : o.numExperts;
+            // PFLOP/s, two 128 x 128 a CU at 2.2.  Of rows by expert every segment may end
+            // inside a tile, which costs the large ones: they are counted with all such
+            // ends, the small ones without (128 rows of one in 32 experts, 2048 x 1024:
+            // 20 and 8 us).
+            const long long cus = num_cus(), experts = o.numExperts;
             auto tiles = [&](int t) {
                 const long long n = (o.n + t - 1) / t, m = (o.m + t - 1) / t;
-                return o.grouping == PRODUCT_ROWS ? (o.m / t + experts) * n : m * n;
+                return (t == 256 && o.grouping == PRODUCT_ROWS ? o.m / t + experts : m) * n;
             };
             const long long large = (tiles(256) + cus - 1) / cus, small = (tiles(128) + 2 * cus - 1) / (2 * cus);
             if (large * 4 * 22 < small * 2 * 25) product_launch<T, 256, 256, false>(p, s);

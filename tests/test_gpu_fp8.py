@@ -174,6 +174,15 @@ def test_dense_product(m, n, k, code, rows_b, act, pad, shift):
         assert torch.equal(whole.view(m, n + pad)[:, n:], guard.view(m, n + pad)[:, n:])
 
 
+@pytest.mark.parametrize("m,n,k,code,rows_b,act,pad,shift", [
+    (65, 64, 4096, 0, 128, 0, 0, 0), (300, 511, 4000, 1, 1, 1, 1, 1), (1025, 64, 2000, 2, 128, 0, 0, 0), (130, 2048, 1024, 2, 1, 0, 8, 0),
+    (4099, 40, 900, 0, 128, 0, 0, 0), (129, 5121, 1300, 0, 128, 0, 0, 0), (64, 20480, 700, 2, 128, 0, 0, 0),
+    (17, 30001, 1030, 0, 128, 1, 0, 0), (1, 65537, 600, 1, 128, 0, 0, 0), (33, 40000, 200, 1, 1, 0, 0, 0)])
+def test_dense_product_either_form(m, n, k, code, rows_b, act, pad, shift):
+    """Many rows by few columns with a long k, whose waves share k, and few rows by many columns, in tiles."""
+    test_dense_product(m, n, k, code, rows_b, act, pad, shift)
+
+
 def segments(lengths, align):
     off = [0]
     for n in lengths:
@@ -202,6 +211,14 @@ def test_rows_product(lengths, align, n, k, code, rows_b):
         r = slice(off[e], off[e + 1])
         check_product(out[r], av[r] @ parts[e][2].t().contiguous(), av[r].abs() @ parts[e][2].abs().t().contiguous(), k, code)
     assert (out[off[-1]:] == 7.0).all()
+
+
+@pytest.mark.parametrize("lengths,align,n,k,code,rows_b", [
+    ([200, 0, 90, 17], 1, 64, 2000, 0, 1), ([300, 129], 128, 100, 4100, 1, 128), ([70, 1, 0, 64], 16, 33, 1500, 2, 128),
+    ([3, 0, 1, 5, 2, 0, 9, 4], 1, 8193, 384, 2, 128), ([40, 2, 0, 130], 1, 16384, 300, 0, 128)])
+def test_rows_product_either_form(lengths, align, n, k, code, rows_b):
+    """The same with experts: segments that end inside a tile, an empty one, and one much longer than the others."""
+    test_rows_product(lengths, align, n, k, code, rows_b)
 
 
 @pytest.mark.parametrize("lengths,m,n,code,rows_b", [
