@@ -516,12 +516,12 @@ __global__ __launch_bounds__(256, TM * TN > 128 * 128 ? 1 : 2) void product_kern
 #endif
 }
 
-// Few rows of A: up to 16 MT rows by 16 rows of B a workgroup, its waves sharing
-// out k, four blocks at a time, and their sums joined in LDS in wave order.  B's
-// bytes bound it, so both operands go straight from memory to registers, all of
-// a wave's four blocks under way at once, and are widened (one row by 4096 x
-// 4096: 21 us through the tiles above, whose 32 workgroups wait for one block
-// after the other; 5.7 us here).
+// Few rows of A, or few tiles with a long k: up to 16 MT rows by 16 rows of B a
+// workgroup, its waves sharing out k, four blocks at a time, and their sums joined
+// in LDS in wave order.  With few rows B's bytes bound it, so both operands go
+// straight from memory to registers, all of a wave's four blocks under way at
+// once, and are widened (one row by 4096 x 4096: 21 us through the tiles above,
+// whose 32 workgroups wait for one block after the other; 5.7 us here).
 constexpr int kFewWaves = 8;
 template <class T, int MT>
 __global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(ProductArgs a)
