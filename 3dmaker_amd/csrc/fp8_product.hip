@@ -3,12 +3,15 @@
 //   out[m, n] = sum_kb 2^(sa[m, kb] + sb[n, kb] - 254) sum_{k in kb} a[m, k] b[n, k]
 // Two matrix instructions carry it.  v_mfma_scale_f32_16x16x128_f8f6f4 takes 128
 // of k, one block, and both scales; its accumulators are fp32, but it adds eight
-// products at a time and cuts them below 2^-13 of the largest (measured: a 15
-// beside 65536 counts as 8), which leaves sums of normal values 1.5e-5 off and of
-// values spread over all of e4m3 5e-5 (of their 2-norm).  That is a fifth of an
-// fp16 output's own rounding, so 16-bit outputs take it.  fp32 outputs and weight
-// gradients take v_mfma_f32_16x16x32_bf16 on operands widened with their scales,
-// which is exact: products and sums in fp32 (4e-8), at half the rate.
+// products at a time and cuts each towards zero to a multiple of 2^-13 of the
+// largest one's power of two (measured: a 15 beside 65536 counts as 8; between the
+// eights and with the accumulator nothing is cut).  Sums of normal values come out
+// 1.5e-5 off (2-norm; non-negative ones 3e-6), of values spread over all of e4m3
+// 7e-5, below an fp16 output's own rounding of 1.4e-4; but the error goes by the
+// largest product of an eight, not by the sum.  So 16-bit outputs take it unless
+// the caller asks for exact sums.  Those, fp32 outputs and weight gradients take
+// v_mfma_f32_16x16x32_bf16 on operands widened with their scales, which is exact:
+// products and sums in fp32 (4e-8), at half the rate.
 //
 // The first MFMA operand is B's rows, the second A's, so that a lane ends with
 // four consecutive n of one row m.  Its two operands are read with the same
@@ -36,7 +39,6 @@ struct ProductArgs {
     int scale_shift;           // rows of B a scale, as a shift: 7 or 0
     long long b_size, bs_size; // of one expert's B and scales
     long long out_stride;
-    int out_type;
     bool relu, vec;
     int tiles_m, tiles_n;
 };
@@ -657,7 +659,8 @@ void fp8_product(const Fp8ProductOption& o, const uint8_t* a, const uint8_t* a_s
             "numExperts must be 1..1024, and 1 for a dense product");
     require(o.scaleRowsB == 1 || o.scaleRowsB == 128, "scaleRowsB must be 1 or 128");
     require(o.activation == 0 || o.activation == 1, "unknown activation");
-    require_type(o.outType);
+    const int type = o.outType & ~PRODUCT_EXACT;
+    require_type(type);
     require(o.outStride >= o.n, "outStride must be at least n");
     require((o.grouping == PRODUCT_DENSE) == !offsets, "offsets go with grouped products");
     if (o.m == 0) return;
@@ -681,15 +684,15 @@ void fp8_product(const Fp8ProductOption& o, const uint8_t* a, const uint8_t* a_s
     p.b_size = (long long)o.n * p.pitch;
     p.bs_size = (long long)((o.n + o.scaleRowsB - 1) / o.scaleRowsB) * p.spitch;
     p.out_stride = o.outStride;
-    p.out_type = o.outType;
     p.relu = o.activation == 1;
     // stores of up to 16 bytes
-    p.vec = aligned16(out) && o.outStride * data_bytes(o.outType) % 16 == 0;
-    with_type(o.outType, [&](auto zero) {
+    p.vec = aligned16(out) && o.outStride * data_bytes(type) % 16 == 0;
+    with_type(type, [&](auto zero) {
         using T = decltype(zero);
-        // fp32 results, weight gradients of any type, and products of up to two
-        // blocks of k, which their output's bytes bound: there widening costs nothing.
-        const bool wide = std::is_same_v<T, float> || o.grouping == PRODUCT_SUM || p.pitch <= 256;
+        // fp32 results, weight gradients of any type, what is asked for, and products
+        // of up to two blocks of k, which their output's bytes bound: there widening
+        // costs nothing.
+        const bool wide = std::is_same_v<T, float> || o.grouping == PRODUCT_SUM || (o.outType & PRODUCT_EXACT) || p.pitch <= 256;
         if (o.grouping != PRODUCT_SUM) {
             const int few = few_tiles(o, wide);
             if (few == 1) return few_launch<T, 1>(p, s);
