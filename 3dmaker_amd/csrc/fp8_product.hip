@@ -11,7 +11,8 @@
 // largest product of an eight, not by the sum.  So 16-bit outputs take it unless
 // the caller asks for exact sums.  Those, fp32 outputs and weight gradients take
 // v_mfma_f32_16x16x32_bf16 on operands widened with their scales, which is exact:
-// products and sums in fp32 (4e-8), at half the rate.
+// products and sums in fp32 (4e-8), at half the rate (8191 x 5120 x 4096 bf16: 307
+// us and 195, 65,536 rows by eight experts of 2048 x 1024 280 and 189).
 //
 // The first MFMA operand is B's rows, the second A's, so that a lane ends with
 // four consecutive n of one row m.  Its two operands are read with the same
@@ -43,7 +44,8 @@ struct ProductArgs {
     int tiles_m, tiles_n;
 };
 
-// Eight e4m3 values times 2^(scale - 127) as bf16 (exact: e4m3 has 4 bits).
+// Eight e4m3 values times 2^(scale - 127) as bf16: exact, as e4m3 has 4 bits, where
+// the smallest and largest are in bf16's range (2^-9 and 448 times 2^-110 to 2^119).
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ bf16x8 widen(int lo, int hi, float scale)
 {

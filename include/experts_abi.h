@@ -145,8 +145,11 @@ typedef struct Fp8ProductOption {
  * are.  NaN in a row's values makes that row's results NaN.
  *
  * fp32 results are sums of exact products in fp32, and so are all of SUM and all
- * with PRODUCT_EXACT.  Other 16-bit results may come from the matrix cores' 8-bit
- * sums, about twice as fast; which calls take them goes by m, n and k.  Those add
+ * with PRODUCT_EXACT, as far as the values are bf16 numbers: with scales of 2^-110
+ * to 2^119 (bytes 17 to 246) they all are; of smaller scales' values what lies
+ * below 2^-133 is lost, and values of 2^128 and more are infinite.  Other 16-bit
+ * results may come from the matrix cores' 8-bit sums, 1.5 times as fast; which
+ * calls take them goes by m, n and k.  Those add
  * eight products (of consecutive k) at a time and cut each towards zero to a
  * multiple of 2^-13 of the largest one's power of two, and add the eights in
  * fp32: a result is within 7 * 2^-13 of the sum of the eights' largest |a b|,

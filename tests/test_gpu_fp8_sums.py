@@ -159,3 +159,22 @@ def test_exact_sums_are_an_option_of_the_results_type():
     for code in (0, 1, 2):
         assert error(option(0, 8, 100, code | EXACT)) == ""
     assert "type" in error(option(0, 8, 100, 3 | EXACT)) and "type" in error(option(0, 8, 100, 2 * EXACT))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", [0, 2])
+@pytest.mark.parametrize("m,n,k", [(4, 64, 512), (1024, 512, 512)])
+@pytest.mark.parametrize("low_a", [True, False])
+def test_scales_at_the_ends_of_their_range(m, n, k, code, low_a):
+    """Scales of 2^-110 beside 2^93 and of 2^119 beside 2^-107: every value is a bf16 number, and no bit is lost."""
+    g = R.gen(21)
+    a, as_, _ = stored(g, m, k, "wide")
+    b, bs, _ = stored(g, n, k, "wide")
+    as_.fill_(17 if low_a else 246)
+    bs.fill_(220 if low_a else 20)
+    av, bv = R.values(a, as_, k), R.values(b, bs, k)
+    out = torch.empty(m, n, device="cuda", dtype=R.DT[code])
+    R.launch("launchFp8Product", C.byref(option(m, n, k, code | EXACT)), a, as_, b, bs, None, out, R.stream())
+    torch.cuda.synchronize()
+    want = av @ bv.t().contiguous()
+    assert ((out.double() - want).abs() <= allowed(av, bv, want, code, True)).all()
