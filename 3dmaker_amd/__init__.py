@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(_HERE, "lib3dmaker_amd.so")
 __all__ = [
     "LIB_PATH", "lib", "launch", "MLPOption", "MLPGridOptions", "HashGrid", "Net",
     "OUT_ACT_NONE", "OUT_ACT_SIGMOID", "ptr", "check", "RouteOption", "Fp8QuantOption", "Fp8ProductOption", "NormGateOption",
-    "DATA_F32", "DATA_F16", "DATA_BF16", "ROUTE_SOFTMAX", "ROUTE_SIGMOID", "PRODUCT_DENSE", "PRODUCT_ROWS", "PRODUCT_SUM", "PRODUCT_EXACT",
+    "DATA_F32", "DATA_F16", "DATA_BF16", "ROUTE_SOFTMAX", "ROUTE_SIGMOID", "PRODUCT_DENSE", "PRODUCT_ROWS", "PRODUCT_SUM", "PRODUCT_EXACT", "COMBINE_ROWS_F32",
     "NORM_NONE", "NORM_RMS", "NORM_LAYER", "fp8_pitch", "fp8_scale_pitch", "Float3", "Uint3", "NerfOptions", "Nerf", "NerfTrainer", "NtrConfig", "NtrStats",
 ]
 
@@ -32,6 +32,7 @@ DATA_F32, DATA_F16, DATA_BF16 = 0, 1, 2
 ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 PRODUCT_DENSE, PRODUCT_ROWS, PRODUCT_SUM = 0, 1, 2
 PRODUCT_EXACT = 0x100
+COMBINE_ROWS_F32 = 0x100
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 
 

@@ -162,15 +162,21 @@ void launchFp8Product(const Fp8ProductOption* opt, const uint8_t* d_a, const uin
 
 /* ---- the experts' rows back to tokens --------------------------------------- */
 
+/* Or'ed to the dataType of the two launchers below: rows are fp32 whatever the
+ * tokens' type, so that nothing is rounded between the experts' products
+ * (outType DATA_F32) and the tokens. */
+#define COMBINE_ROWS_F32 0x100
+
 /* out[t] = sum_j weights[t, j] * rows[position[t, j]] in fp32, rounded once
  * (weights NULL: 1 each; a position outside 0..numRows-1 adds nothing).
- * rows [numRows x dim], out [numTokens x dim], both of dataType. */
+ * rows [numRows x dim], out [numTokens x dim], both of dataType (rows fp32 with
+ * COMBINE_ROWS_F32). */
 void launchExpertCombine(int dim, int dataType, const void* d_rows, int numRows, long long rowStride,
                          const int* d_position, const float* d_weights, void* d_out, long long outStride,
                          int numTokens, int topK, hipStream_t stream);
 
 /* dL/dweights [numTokens x topK] (fp32) = <dout[t], rows[position[t, j]]>, 0 for
- * positions outside.  The rows' own gradient is weights * dout, which
+ * positions outside; types as above, dout's as out's.  The rows' own gradient is weights * dout, which
  * launchFp8Quantize forms from dout, the order and the weights. */
 void launchExpertCombineBackward(int dim, int dataType, const void* d_rows, int numRows, long long rowStride,
                                  const int* d_position, const void* d_dout, long long doutStride, float* d_dweights,
