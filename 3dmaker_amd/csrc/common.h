@@ -110,6 +110,8 @@ private:
 
 // The workspace of (current device, stream), for callers without an owner of
 // their own (the extern "C" launchers); kept until the process ends.
+// hipStreamPerThread names another stream in every thread: there it is the
+// calling thread's, kept until that ends.
 Workspace& stream_workspace(hipStream_t s);
 
 // One Workspace per (device, stream) that its callers work on, for callers that

@@ -415,6 +415,10 @@ Workspace& stream_workspace(hipStream_t s)
 {
     int dev = 0;
     GRAFT_HIP_CHECK(hipGetDevice(&dev));
+    if (s == hipStreamPerThread) {
+        thread_local std::map<int, Workspace> own;
+        return own[dev];
+    }
     std::lock_guard<std::mutex> lk(g_ws_mu);
     static std::map<std::pair<int, hipStream_t>, std::unique_ptr<Workspace>>* cache =
         new std::map<std::pair<int, hipStream_t>, std::unique_ptr<Workspace>>();  // outlives static destructors

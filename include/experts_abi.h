@@ -12,9 +12,10 @@
  * any device call.  A batch of zero tokens or rows is valid and does nothing
  * (a plan of it is written: no rows).  Results do not depend on the order in
  * which the GPU runs workgroups: repeated calls give the same bits.  Strides
- * count elements; tokens and rows of a call are at most 2^30.  Scratch, where a call needs any, belongs to (device,
- * stream) as for the other launchers, so calls of several host threads on one
- * stream have to be serialised by the caller; it grows with hipMalloc on a
+ * count elements; tokens and rows of a call are at most 2^30.  Scratch, where a
+ * call needs any, belongs to (device, stream) as for the other launchers
+ * (hipStreamPerThread: to each thread's own), so calls of several host threads on
+ * one stream have to be serialised by the caller; it grows with hipMalloc on a
  * larger call than before, so a call that is captured into a graph has to be
  * made once before.
  */
