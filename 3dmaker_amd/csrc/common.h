@@ -12,6 +12,7 @@
 #include <stdexcept>
 #include <string>
 #include <utility>
+#include <vector>
 
 #define GRAFT_HIP_CHECK(expr)                                                          \
     do {                                                                               \
@@ -87,7 +88,9 @@ __device__ __forceinline__ uint32_t dense_index(int cx, int cy, int cz, int N_l)
 // extern "C" launchers): grown on demand, never shrunk, freed with the owner.
 // Kernels of one owner run in stream order, so they never share it with
 // another owner's work in flight.  Growing frees the old buffer with
-// hipFree, which waits for the device first.
+// hipFree, which waits for the device first; but a graph that was captured on
+// the owner's stream keeps the address, so from its first capture on the owner
+// keeps what it has outgrown.
 class Workspace {
 public:
     Workspace() = default;
@@ -99,12 +102,15 @@ public:
     // for callers that have another way.  mutex() is theirs to hold while they
     // enqueue what uses it.
     void* try_get(size_t bytes);
+    void keep_for_graphs() { in_graphs_ = true; }
     std::mutex& mutex() { return mu_; }
     size_t size() const { return bytes_; }
 
 private:
     void* p_ = nullptr;
     size_t bytes_ = 0;
+    bool in_graphs_ = false;
+    std::vector<void*> outgrown_;
     std::mutex mu_;
 };
 

@@ -347,12 +347,14 @@ int max_lds_per_block()
 Workspace::~Workspace()
 {
     if (p_) (void)hipFree(p_);
+    for (void* p : outgrown_) (void)hipFree(p);
 }
 
 void* Workspace::get(size_t bytes)
 {
     if (bytes > bytes_) {
-        if (p_) GRAFT_HIP_CHECK(hipFree(p_));
+        if (p_ && in_graphs_) outgrown_.push_back(p_);
+        else if (p_) GRAFT_HIP_CHECK(hipFree(p_));
         p_ = nullptr;
         bytes_ = 0;
         const size_t nb = std::max(bytes, (size_t)1 << 16);
@@ -370,7 +372,8 @@ void* Workspace::try_get(size_t bytes)
         (void)hipGetLastError();
         return nullptr;
     }
-    if (p_) (void)hipFree(p_);
+    if (p_ && in_graphs_) outgrown_.push_back(p_);
+    else if (p_) (void)hipFree(p_);
     p_ = p;
     bytes_ = bytes;
     return p_;
@@ -415,8 +418,12 @@ Workspace& stream_workspace(hipStream_t s)
 {
     int dev = 0;
     GRAFT_HIP_CHECK(hipGetDevice(&dev));
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    const bool capturing = hipStreamIsCapturing(s, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
+    if (capturing) (void)hipGetLastError();
     if (s == hipStreamPerThread) {
         thread_local std::map<int, Workspace> own;
+        if (capturing) own[dev].keep_for_graphs();
         return own[dev];
     }
     std::lock_guard<std::mutex> lk(g_ws_mu);
@@ -424,6 +431,7 @@ Workspace& stream_workspace(hipStream_t s)
         new std::map<std::pair<int, hipStream_t>, std::unique_ptr<Workspace>>();  // outlives static destructors
     auto& w = (*cache)[{dev, s}];
     if (!w) w.reset(new Workspace());
+    if (capturing) w->keep_for_graphs();
     return *w;
 }
 

@@ -17,7 +17,9 @@
  * (hipStreamPerThread: to each thread's own), so calls of several host threads on
  * one stream have to be serialised by the caller; it grows with hipMalloc on a
  * larger call than before, so a call that is captured into a graph has to be
- * made once before.
+ * made once before.  The graph keeps that scratch, which stays allocated however
+ * large later calls on the stream are; its replays have to be ordered with the
+ * stream's other calls, as those are among themselves.
  */
 #ifndef GRAFT_EXPERTS_ABI_H
 #define GRAFT_EXPERTS_ABI_H

@@ -78,3 +78,37 @@ def test_streams_of_several_threads():
             t.join()
         assert not errors, errors
     jobs[0][0].check()
+
+
+@pytest.mark.parametrize("job,larger", [
+    (lambda: Plan(50, 9000, 2, 60), lambda: Plan(51, 400000, 2, 200)),
+    (lambda: NormBackward(52, 2000, 200), lambda: NormBackward(53, 8000, 2000))])
+def test_a_graph_outlives_larger_calls(job, larger):
+    """Captured on a stream whose scratch then grows: what replays use is still theirs."""
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    j, big = job(), larger()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        j.run(s.cuda_stream)  # its scratch
+        s.synchronize()
+        want = [t.clone() for t in j.out]
+        graph = torch.cuda.CUDAGraph()
+        s.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            j.run(s.cuda_stream)
+        for i in range(4):
+            big.run(s.cuda_stream)
+            s.synchronize()
+            # whatever was given back is somebody else's now
+            others = [torch.full((1 << 18,), -1, dtype=torch.int32, device="cuda") for _ in range(64)]
+            for t in j.out:
+                t.fill_(-9)
+            graph.replay()
+            s.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(j.out, want)), i
+            assert all(bool((t == -1).all()) for t in others), i
+            j.run(s.cuda_stream)
+            s.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(j.out, want)), i
+            del others
