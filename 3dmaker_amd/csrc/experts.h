@@ -7,6 +7,8 @@
 #include "common.h"
 #include "experts_abi.h"
 
+#include <algorithm>
+
 namespace graft {
 
 template <class T, int N>
@@ -35,6 +37,18 @@ void with_type(int type, F&& f)
     if (type == DATA_F32) f(float{});
     else if (type == DATA_F16) f((_Float16)0);
     else f((__bf16)0.0f);
+}
+
+// f(first, number) over `wgs` workgroups in launches of less than 2^32 threads,
+// which is what a grid can have.
+template <class F>
+void in_launches(long long wgs, int threads, F&& f)
+{
+    const long long most = 0xffffffffll / threads;
+    for (long long first = 0; first < wgs; first += most) {
+        f(first, (unsigned)std::min(most, wgs - first));
+        GRAFT_LAUNCH_CHECK();
+    }
 }
 
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }

@@ -26,6 +26,7 @@ struct NormArgs {
     long long sx, sf, sg, sy, sh;
     int rows, dim, gate_rows, post, pre;
     float alpha, beta, eps, inv_dim;
+    long long row0;  // the launch's first row (forward)
     // backward
     const void *dy, *dh;
     void *dx, *df, *dgate;
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(256) void norm_gate_kernel(NormArgs a)
     __shared__ float lds[4][THREADS / 64];
     using R = Row<T, VEC, THREADS, PER>;
     const int sub = threadIdx.x & (THREADS - 1);
-    const long long row = (long long)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
+    const long long row = a.row0 + (long long)blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
     if (row >= a.rows) return;  // a row's threads return together; only whole workgroups meet at a barrier
     R y;
     y.load((const T*)a.x + row * a.sx, sub, a.dim);
@@ -519,10 +520,13 @@ bool norm_vec(int dim, int bytes, std::initializer_list<Access> all)
 }
 
 template <class T, int VEC, int THREADS, int PER>
-void forward_launch(const NormArgs& a, hipStream_t s)
+void forward_launch(NormArgs a, hipStream_t s)
 {
-    const int per_wg = 256 / THREADS;
-    norm_gate_kernel<T, VEC, THREADS, PER><<<(a.rows + per_wg - 1) / per_wg, 256, 0, s>>>(a);
+    constexpr int kPerWg = 256 / THREADS;
+    in_launches((a.rows + kPerWg - 1) / kPerWg, 256, [&](long long first, unsigned wgs) {
+        a.row0 = first * kPerWg;
+        norm_gate_kernel<T, VEC, THREADS, PER><<<wgs, 256, 0, s>>>(a);
+    });
 }
 
 // A wave holds a row of up to 32 elements a lane; longer rows take a workgroup.
@@ -589,7 +593,6 @@ void norm_gate(const NormGateOption& o, const NormGateTensors& t, void* y, void*
         if (vec) forward_rows<T, 16 / (int)sizeof(T)>(a, s);
         else forward_rows<T, 1>(a, s);
     });
-    GRAFT_LAUNCH_CHECK();
 }
 
 void norm_gate_backward(const NormGateOption& o, const NormGateTensors& t, const void* dy, const void* dh,

@@ -1,0 +1,64 @@
+"""Calls of more workgroups than one launch can have (2^32 threads): rows and tokens up to 2^30 are valid."""
+import ctypes as C
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import experts_ref as R  # noqa: E402
+from helpers import pkg  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def give_back():
+    yield
+    torch.cuda.empty_cache()
+
+
+def pattern(rows, cols, dtype, period=1009):
+    """[rows, cols] that repeats a random block of an odd number of rows, which does not line up with a launch."""
+    p = R.randn(R.gen(period), period, cols).to(dtype)
+    x = torch.empty(rows, cols, dtype=dtype, device="cuda")
+    whole = rows // period * period
+    x[:whole].view(-1, period, cols).copy_(p)
+    x[whole:] = p[:rows - whole]
+    return x
+
+
+def repeats(y, period=1009):
+    """Whether every block of rows has the first one's bits."""
+    for r in range(0, y.shape[0], period << 10):
+        part = y[r:r + (period << 10)]
+        whole = part.shape[0] // period * period
+        if not (bool((part[:whole].view(-1, period, *y.shape[1:]) == y[:period]).all()) and torch.equal(part[whole:], y[:part.shape[0] - whole])):
+            return False
+    return True
+
+
+def norm_option(dim, pre):
+    return pkg().NormGateOption(dim=dim, postNorm=0, preNorm=pre, gateRows=0, residualScale=0.5, blockScale=1.0, epsilon=1e-6,
+                                dataType=1, strideX=dim, strideF=dim, strideGate=dim, strideY=dim, strideH=dim)
+
+
+def test_norm_rows_of_a_wave():
+    rows, dim = (1 << 26) + 5, 2
+    x = pattern(rows, dim, torch.float16)
+    h = torch.full((rows, dim), 3.0, dtype=torch.float16, device="cuda")
+    R.launch("launchNormGateResidual", C.byref(norm_option(dim, 1)), x, None, None, None, None, None, None, None, h, rows, R.stream())
+    torch.cuda.synchronize()
+    want = R.norm(0.5 * x[:1009].double(), 1, None, None, 1e-6)
+    err = (h[:1009].double() - want).abs()
+    assert (err <= R.HALF[1] * want.abs() + 2.0 ** -19 * want.abs().amax(1, keepdim=True) + R.TINY[1]).all()
+    assert repeats(h)
+
+
+def test_norm_rows_of_a_workgroup():
+    rows, dim = (1 << 24) + 3, 2056
+    x = pattern(rows, dim, torch.float16)  # 69 GB: in place
+    first = x[:1009].clone()
+    R.launch("launchNormGateResidual", C.byref(norm_option(dim, 0)), x, None, None, None, None, None, None, x, None, rows, R.stream())
+    torch.cuda.synchronize()
+    assert torch.equal(x[:1009], 0.5 * first)
+    assert repeats(x)
