@@ -29,6 +29,7 @@ struct RowArgs {
     long long out_stride;    // of out or dout
     float* dweights;
     int dim, num_rows, tokens, topk;
+    long long wg0;           // the launch's first workgroup
 };
 
 // N consecutive elements, in 16-byte loads where they are whole ones.
@@ -51,7 +52,7 @@ template <class R, class T, int N>
 __global__ __launch_bounds__(kRowThreads) void combine_kernel(RowArgs a)
 {
     const int chunks = (a.dim + N - 1) / N;
-    const long long unit = (long long)blockIdx.x * kRowThreads + threadIdx.x;
+    const long long unit = (a.wg0 + blockIdx.x) * kRowThreads + threadIdx.x;
     const long long t = unit / chunks;
     const int col = (int)(unit % chunks) * N;
     if (t >= a.tokens) return;
@@ -79,7 +80,7 @@ __global__ __launch_bounds__(kRowThreads) void combine_kernel(RowArgs a)
 template <class R, class T, int N, int K>
 __global__ __launch_bounds__(kRowThreads) void combine_backward_kernel(RowArgs a)
 {
-    const long long t = (long long)blockIdx.x * (kRowThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const long long t = (a.wg0 + blockIdx.x) * (kRowThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int lane = threadIdx.x & 63;
     if (t >= a.tokens) return;
     const T* d = (const T*)a.dout + t * a.out_stride;
@@ -168,11 +169,12 @@ void expert_combine(int dim, int type, const void* rows, int num_rows, long long
     a.out = out;
     with_vec(type, a, out, [&](auto row, auto zero, auto N) {
         constexpr int n = decltype(N)::value;
-        const long long units = (long long)tokens * ((dim + n - 1) / n), wgs = (units + kRowThreads - 1) / kRowThreads;
-        require(wgs <= 0x7fffffffll, "too many elements for one call");
-        combine_kernel<decltype(row), decltype(zero), n><<<(unsigned)wgs, kRowThreads, 0, s>>>(a);
+        const long long units = (long long)tokens * ((dim + n - 1) / n);
+        in_launches((units + kRowThreads - 1) / kRowThreads, kRowThreads, [&](long long first, unsigned wgs) {
+            a.wg0 = first;
+            combine_kernel<decltype(row), decltype(zero), n><<<wgs, kRowThreads, 0, s>>>(a);
+        });
     });
-    GRAFT_LAUNCH_CHECK();
 }
 
 void expert_combine_backward(int dim, int type, const void* rows, int num_rows, long long row_stride, const int* position,
@@ -187,12 +189,13 @@ void expert_combine_backward(int dim, int type, const void* rows, int num_rows, 
         using R = decltype(row);
         using T = decltype(zero);
         constexpr int n = decltype(N)::value;
-        const unsigned wgs = (unsigned)((tokens + 3ll) / 4);
-        if (topK == 1) combine_backward_kernel<R, T, n, 1><<<wgs, kRowThreads, 0, s>>>(a);
-        else if (topK == 2) combine_backward_kernel<R, T, n, 2><<<wgs, kRowThreads, 0, s>>>(a);
-        else combine_backward_kernel<R, T, n, 4><<<wgs, kRowThreads, 0, s>>>(a);
+        in_launches((tokens + 3ll) / 4, kRowThreads, [&](long long first, unsigned wgs) {
+            a.wg0 = first;
+            if (topK == 1) combine_backward_kernel<R, T, n, 1><<<wgs, kRowThreads, 0, s>>>(a);
+            else if (topK == 2) combine_backward_kernel<R, T, n, 2><<<wgs, kRowThreads, 0, s>>>(a);
+            else combine_backward_kernel<R, T, n, 4><<<wgs, kRowThreads, 0, s>>>(a);
+        });
     });
-    GRAFT_LAUNCH_CHECK();
 }
 
 }  // namespace graft

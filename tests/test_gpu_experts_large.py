@@ -62,3 +62,30 @@ def test_norm_rows_of_a_workgroup():
     torch.cuda.synchronize()
     assert torch.equal(x[:1009], 0.5 * first)
     assert repeats(x)
+
+
+def test_combine_of_many_elements():
+    """More than 2^32 elements, each a thread's: rows that are not whole 16-byte pieces."""
+    T, dim, k, rows = (1 << 20) + 3, 4099, 2, 1009
+    r = R.randn(R.gen(1), rows, dim).half()
+    pos = torch.stack([torch.arange(T, device="cuda") % 1009, (torch.arange(T, device="cuda") % 1009 * 7 + 3) % 1009], 1).int()
+    out = torch.full((T, dim), 3.0, dtype=torch.float16, device="cuda")
+    R.launch("launchExpertCombine", dim, 1, r, rows, dim, pos.contiguous(), None, out, dim, T, k, R.stream())
+    torch.cuda.synchronize()
+    want = (r.double()[pos[:1009, 0].long()] + r.double()[pos[:1009, 1].long()])
+    assert ((out[:1009].double() - want).abs() <= R.HALF[1] * want.abs() + R.TINY[1]).all()
+    assert repeats(out)
+
+
+@pytest.mark.parametrize("k", [1, 3])
+def test_combine_backward_of_many_tokens(k):
+    T, dim, rows = (1 << 26) + 5, 1, 1009
+    r = R.randn(R.gen(2), rows, dim).half()
+    pos = ((torch.arange(T, device="cuda") % 1009)[:, None] * (5 + torch.arange(k, device="cuda")) % 1009).int()
+    dout = pattern(T, dim, torch.float16)
+    dw = torch.full((T, k), 3.0, device="cuda")
+    R.launch("launchExpertCombineBackward", dim, 1, r, rows, dim, pos, dout, dim, dw, T, k, R.stream())
+    torch.cuda.synchronize()
+    want = r.float()[pos[:1009].long(), 0] * dout[:1009].float()
+    assert torch.equal(dw[:1009], want)  # one product of two 11-bit numbers each
+    assert repeats(dw)
