@@ -30,6 +30,7 @@ struct RouteArgs {
     int type;
     bool sigmoid, renorm, vec;
     float scale;
+    int token0;  // the launch's first token
     // backward
     const float* dweights;
     void* dlogits;
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_kernel(RouteArgs a)
     __shared__ __attribute__((aligned(16))) float score[kRouteThreads * V];
     __shared__ uint32_t group_key[kRouteThreads];
     const int lane = threadIdx.x & 63, sub = threadIdx.x & (LPT - 1), local = threadIdx.x / LPT;
-    const int token = blockIdx.x * kTokens + local;
+    const int token = a.token0 + (int)blockIdx.x * kTokens + local;
     const int lg = a.lanes_group, lg_bits = a.lanes_group_bits;
     const int group = sub >> lg_bits, in_group = (sub & (lg - 1)) * V;
     const int first = group * a.group_size + in_group;
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteArgs
     // gradient is written as) at those that were not selected.
     constexpr uint32_t kNone = 0xffffffffu;
     __shared__ __attribute__((aligned(16))) uint32_t dense[kRouteThreads * V];
-    const int sub = threadIdx.x & (LPT - 1), token = blockIdx.x * kTokens + threadIdx.x / LPT;
+    const int sub = threadIdx.x & (LPT - 1), token0 = a.token0 + (int)blockIdx.x * kTokens, token = token0 + (int)threadIdx.x / LPT;
     const int first = sub * V;
     const int n = token < a.tokens ? max(0, min(V, a.experts - first)) : 0;
 #pragma unroll
@@ -319,8 +320,8 @@ __global__ __launch_bounds__(kRouteThreads) void route_backward_kernel(RouteArgs
     for (int i = 0; i < V; i++) z[i] = 0.0f;
     const uint32_t live = load_logits(z, a, token, first, n);
     __syncthreads();
-    const long long slot0 = (long long)blockIdx.x * kTokens * a.topk;
-    const int slots = min(kTokens, a.tokens - (int)blockIdx.x * kTokens) * a.topk;
+    const long long slot0 = (long long)token0 * a.topk;
+    const int slots = min(kTokens, a.tokens - token0) * a.topk;
     for (int i = threadIdx.x; i < slots; i += kRouteThreads) {
         const int e = a.indices[slot0 + i];
         const uint32_t d = __builtin_bit_cast(uint32_t, a.dweights[slot0 + i]);
@@ -478,10 +479,12 @@ void route_experts(const RouteOption& o, const void* logits, long long stride, c
     const int lanes = slots * a.lanes_group, per_lane = (a.group_size + a.lanes_group - 1) / a.lanes_group;
     with_layout(lanes, per_lane, [&](auto V, auto LPT) {
         a.vec = can_vec(logits, stride, a.group_size, V, a.type);
-        const int per_wg = kRouteThreads / LPT;
-        route_kernel<decltype(V)::value, decltype(LPT)::value><<<(tokens + per_wg - 1) / per_wg, kRouteThreads, 0, s>>>(a);
+        constexpr int kPerWg = kRouteThreads / decltype(LPT)::value;
+        in_launches((tokens + kPerWg - 1) / kPerWg, kRouteThreads, [&](long long first, unsigned wgs) {
+            a.token0 = (int)(first * kPerWg);
+            route_kernel<decltype(V)::value, decltype(LPT)::value><<<wgs, kRouteThreads, 0, s>>>(a);
+        });
     });
-    GRAFT_LAUNCH_CHECK();
 }
 
 void route_experts_backward(const RouteOption& o, const void* logits, long long stride, const int* indices,
@@ -499,10 +502,12 @@ void route_experts_backward(const RouteOption& o, const void* logits, long long 
     const int lanes = std::min(64, pow2_from((o.numExperts + 3) / 4)), per_lane = (o.numExperts + lanes - 1) / lanes;
     with_layout(lanes, per_lane, [&](auto V, auto LPT) {
         a.vec = can_vec(logits, stride, o.numExperts, V, a.type) && can_vec(dlogits, dstride, o.numExperts, V, a.type);
-        const int per_wg = kRouteThreads / LPT;
-        route_backward_kernel<decltype(V)::value, decltype(LPT)::value><<<(tokens + per_wg - 1) / per_wg, kRouteThreads, 0, s>>>(a);
+        constexpr int kPerWg = kRouteThreads / decltype(LPT)::value;
+        in_launches((tokens + kPerWg - 1) / kPerWg, kRouteThreads, [&](long long first, unsigned wgs) {
+            a.token0 = (int)(first * kPerWg);
+            route_backward_kernel<decltype(V)::value, decltype(LPT)::value><<<wgs, kRouteThreads, 0, s>>>(a);
+        });
     });
-    GRAFT_LAUNCH_CHECK();
 }
 
 // ---------------------------------------------------------------------------

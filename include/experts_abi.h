@@ -68,7 +68,7 @@ void launchRouteExperts(const RouteOption* opt, const void* d_logits, long long 
 
 /* dL/dlogits (type of the logits) from dL/dweights, for indices that
  * launchRouteExperts gave (distinct in a row; others than 0..E-1 are skipped).
- * The bias has no gradient. */
+ * The bias has no gradient.  d_dlogits may be d_logits, with the same stride. */
 void launchRouteExpertsBackward(const RouteOption* opt, const void* d_logits, long long logitsStride,
                                 const int* d_indices, const float* d_dweights, void* d_dlogits,
                                 long long dlogitsStride, int numTokens, hipStream_t stream);

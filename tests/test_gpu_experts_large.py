@@ -89,3 +89,36 @@ def test_combine_backward_of_many_tokens(k):
     want = r.float()[pos[:1009].long(), 0] * dout[:1009].float()
     assert torch.equal(dw[:1009], want)  # one product of two 11-bit numbers each
     assert repeats(dw)
+
+
+def test_routing_of_many_tokens():
+    """A wave a token: 33 groups of one expert."""
+    T, E, k = (1 << 26) + 5, 33, 2
+    z = pattern(T, E, torch.float16)
+    o = pkg().RouteOption(numExperts=E, topK=k, scoreType=0, numGroups=33, topGroups=33, groupScore=1, renormalize=1, scale=1.0,
+                          logitsType=1)
+    idx, w = torch.full((T, k), -7, dtype=torch.int32, device="cuda"), torch.full((T, k), -7.0, device="cuda")
+    R.launch("launchRouteExperts", C.byref(o), z, E, None, idx, w, T, R.stream())
+    torch.cuda.synchronize()
+    ri, rw, _ = R.route(z[:1009], None, k, 0, 1, 1, 1, 1, 1.0)
+    assert torch.equal(idx[:1009].cpu(), ri)
+    assert ((w[:1009].cpu().double() - rw).abs() <= 2.0 ** -20 * rw.abs()).all()
+    assert repeats(idx) and repeats(w)
+
+
+def test_routing_gradient_of_many_tokens():
+    T, E = (1 << 26) + 5, 129
+    z = pattern(T, E, torch.float16)
+    first = z[:1009].clone()
+    idx = (torch.arange(T, device="cuda") % 1009 * 31 % E).int()
+    dw = pattern(T, 1, torch.float32)
+    o = pkg().RouteOption(numExperts=E, topK=1, scoreType=0, numGroups=1, topGroups=1, groupScore=1, renormalize=0, scale=1.0,
+                          logitsType=1)
+    R.launch("launchRouteExpertsBackward", C.byref(o), z, E, idx, dw, z, E, T, R.stream())  # 17 GB: in place
+    torch.cuda.synchronize()
+    s = torch.softmax(first.double(), 1)
+    picked = s.gather(1, idx[:1009, None].long())
+    hot = torch.nn.functional.one_hot(idx[:1009].long(), E)
+    want = dw[:1009].double() * picked * (hot - s)
+    assert ((z[:1009].double() - want).abs() <= 8 * 2.0 ** -20 * dw[:1009].double().abs() * s + R.HALF[1] * want.abs() + R.TINY[1]).all()
+    assert repeats(z)
