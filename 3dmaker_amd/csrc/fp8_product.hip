@@ -605,8 +605,9 @@ void few_launch(ProductArgs& a, hipStream_t s)
 {
     a.tiles_n = (a.n + 15) / 16;
     const long long row_tiles = a.grouping == PRODUCT_ROWS ? a.m / (16 * MT) + a.experts : (a.m + 16 * MT - 1) / (16 * MT);
-    require(row_tiles * a.tiles_n <= 0x7fffffffll, "too many tiles for one call");
     const int waves = std::min(kFewWaves, std::max(1, (a.pitch / 128 + 3) / 4));
+    // fewer than 2^32 threads, which is what a grid can have
+    require(row_tiles * a.tiles_n <= 0xffffffffll / (waves * 64), "too many tiles for one call");
     product_few_kernel<T, MT><<<(unsigned)(row_tiles * a.tiles_n), waves * 64, 0, s>>>(a);
     GRAFT_LAUNCH_CHECK();
 }

@@ -26,6 +26,7 @@ struct QuantArgs {
     int rows, cols, slots_per_row, src_rows;
     int pitch, spitch, pitch_t, spitch_t;
     long long stride, batch_stride, gate_stride;
+    long long wg0;  // the launch's first workgroup (rows only)
     bool vec;  // source rows are whole 16-byte pieces of eight columns
 };
 
@@ -168,7 +169,7 @@ template <class T, int UNITS>
 __global__ __launch_bounds__(kQuantThreads) void quant_rows_kernel(QuantArgs a)
 {
     const uint32_t blocks = a.pitch / 128;
-    const unsigned long long first = (unsigned long long)blockIdx.x * (16 * UNITS);
+    const unsigned long long first = (unsigned long long)(a.wg0 + blockIdx.x) * (16 * UNITS);
     const uint32_t row0 = (uint32_t)(first / blocks), in0 = (uint32_t)(first % blocks);
     const T* src = (const T*)a.src + (long long)blockIdx.y * a.batch_stride;
     float v[UNITS][8];
@@ -335,11 +336,12 @@ void fp8_quantize(const Fp8QuantOption& o, const void* src, const int* order, co
         else if (qt) quant_tile_kernel<T, false><<<dim3(rb, cb, o.batch), kQuantThreads, 0, s>>>(a);
         else {
             const long long units = (long long)o.rows * cb;
-            require(units / 64 < 0x7fffffffll, "too many blocks for one call");
-            if (units * o.batch >= 64ll * 8 * num_cus())
-                quant_rows_kernel<T, 4><<<dim3((unsigned)((units + 63) / 64), o.batch), kQuantThreads, 0, s>>>(a);
-            else
-                quant_rows_kernel<T, 1><<<dim3((unsigned)((units + 15) / 16), o.batch), kQuantThreads, 0, s>>>(a);
+            const bool many = units * o.batch >= 64ll * 8 * num_cus();
+            in_launches((units + (many ? 63 : 15)) / (many ? 64 : 16), kQuantThreads, [&](long long first, unsigned wgs) {
+                a.wg0 = first;
+                if (many) quant_rows_kernel<T, 4><<<dim3(wgs, o.batch), kQuantThreads, 0, s>>>(a);
+                else quant_rows_kernel<T, 1><<<dim3(wgs, o.batch), kQuantThreads, 0, s>>>(a);
+            });
         }
     });
     GRAFT_LAUNCH_CHECK();

@@ -122,3 +122,23 @@ def test_routing_gradient_of_many_tokens():
     want = dw[:1009].double() * picked * (hot - s)
     assert ((z[:1009].double() - want).abs() <= 8 * 2.0 ** -20 * dw[:1009].double().abs() * s + R.HALF[1] * want.abs() + R.TINY[1]).all()
     assert repeats(z)
+
+
+def test_quantize_many_blocks():
+    """2^30 blocks of 128 and more: gathered from a small source by an order."""
+    P = pkg()
+    rows, cols, period = (1 << 29) + 5, 129, 1009
+    if torch.cuda.mem_get_info()[0] < 160 << 30:
+        pytest.skip("needs 150 GB")
+    x = R.randn(R.gen(7), period, cols).half()
+    order = torch.arange(period, dtype=torch.int32, device="cuda").repeat(rows // period + 1)[:rows].contiguous()
+    q = torch.empty(rows, P.fp8_pitch(cols), dtype=torch.uint8, device="cuda")
+    s = torch.zeros(rows, P.fp8_scale_pitch(cols), dtype=torch.uint8, device="cuda")
+    o = P.Fp8QuantOption(rows=rows, cols=cols, batch=1, blockRows=1, srcType=1, slotsPerRow=1, srcRows=period, srcStride=cols,
+                         srcBatchStride=0, gateStride=0)
+    R.launch("launchFp8Quantize", C.byref(o), x, order, None, None, q, s, None, None, R.stream())
+    torch.cuda.synchronize()
+    want_q, want_s = R.quantize(x)
+    assert torch.equal(q[:period, :cols].contiguous().view(torch.float8_e4m3fn).double(), want_q)
+    assert (q[:period, cols:] == 0).all() and torch.equal(s[:period, :2], want_s)
+    assert repeats(q) and repeats(s)
