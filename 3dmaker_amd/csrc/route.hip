@@ -50,14 +50,17 @@ __device__ __forceinline__ float of_key(uint32_t k)
 }
 
 // e^x for x <= 0 to about an ulp: 2^t with the rounding error of t = x log2(e)
-// put back (t's error alone would be |x| ulps).  Below e^-100 it is 0.
+// put back (t's error alone would be |x| ulps).  The instruction gives no subnormal
+// numbers, so below 2^-126 it works 2^64 higher: experts far behind the first one
+// still differ, down to 2^-149; below that they are 0, and equal.
 __device__ __forceinline__ float exp_neg(float x)
 {
     x = fmaxf(x, -120.0f);
     const float t = x * 1.44269504f;
     const float r = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
-    const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, r * 0.693147181f, e);
+    const bool low = t < -126.0f;
+    const float e = __builtin_amdgcn_exp2f(low ? t + 64.0f : t);
+    return fmaf(e, r * 0.693147181f, e) * (low ? 0x1p-64f : 1.0f);
 }
 
 template <class T, int V>
