@@ -583,6 +583,7 @@ void norm_gate(const NormGateOption& o, const NormGateTensors& t, void* y, void*
     require((!y || o.strideY >= o.dim) && (!h || o.strideH >= o.dim), "strides must be at least dim");
     if (rows == 0) return;
     require(y || h, "y and h are both NULL");
+    require(y != t.x || o.strideY == o.strideX, "y in x's place needs x's stride");
     a.y = y;
     a.h = h;
     const int bytes = data_bytes(o.dataType);

@@ -8,18 +8,19 @@
  *
  * Conventions are those of tinymlp_abi.h: device pointers unless stated, a
  * trailing stream, void launchers that report through tinymlp_last_error()
- * and tinymlp_last_error_message().  Every argument error is reported before
- * any device call.  A batch of zero tokens or rows is valid and does nothing
- * (a plan of it is written: no rows).  Results do not depend on the order in
- * which the GPU runs workgroups: repeated calls give the same bits.  Strides
- * count elements; tokens and rows of a call are at most 2^30.  Scratch, where a
- * call needs any, belongs to (device, stream) as for the other launchers
- * (hipStreamPerThread: to each thread's own), so calls of several host threads on
- * one stream have to be serialised by the caller; it grows with hipMalloc on a
- * larger call than before, so a call that is captured into a graph has to be
- * made once before.  The graph keeps that scratch, which stays allocated however
- * large later calls on the stream are; its replays have to be ordered with the
- * stream's other calls, as those are among themselves.
+ * and tinymlp_last_error_message().  Every argument error is reported before any
+ * device call.  A batch of zero tokens or rows is valid and does nothing (but a
+ * plan of it is written, with no rows, and the norms' parameters' gradients, of
+ * zeros).  Results do not depend on the order in which the GPU runs workgroups:
+ * repeated calls give the same bits.  Strides count elements; tokens and rows of
+ * a call are at most 2^30.  Scratch, where a call needs any, belongs to (device,
+ * stream) as for the other launchers (hipStreamPerThread: to each thread's own),
+ * so calls of several host threads on one stream have to be serialised by the
+ * caller; it grows with hipMalloc on a larger call than before, so a call that is
+ * captured into a graph has to be made once before.  The graph keeps that
+ * scratch, which stays allocated however large later calls on the stream are; its
+ * replays have to be ordered with the stream's other calls, as those are among
+ * themselves.
  */
 #ifndef GRAFT_EXPERTS_ABI_H
 #define GRAFT_EXPERTS_ABI_H
@@ -209,8 +210,8 @@ typedef struct NormGateOption {
  * over each row, statistics in fp32, h from y before its rounding.  gate
  * [ceil(numRows / gateRows) x D].  Weights and biases fp32 [D]; a NULL weight is
  * 1, a NULL bias 0.  f NULL: y = alpha x (no gate, no post norm).  y or h may be
- * NULL, not both; x is read before y is written, so y may be x.  y, h, x and f
- * do not overlap otherwise. */
+ * NULL, not both; a row of x is read before that of y is written, so y may be x,
+ * with its stride.  y, h, x and f do not overlap otherwise. */
 void launchNormGateResidual(const NormGateOption* opt, const void* d_x, const void* d_f, const void* d_gate,
                             const float* d_postWeight, const float* d_postBias, const float* d_preWeight,
                             const float* d_preBias, void* d_y, void* d_h, int numRows, hipStream_t stream);
