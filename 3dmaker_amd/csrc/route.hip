@@ -101,7 +101,7 @@ __device__ __forceinline__ uint32_t load_logits(float (&z)[V], const RouteArgs& 
     return live;
 }
 
-// Scores of the lane's experts (0 where not live).  For the sigmoid q is 1 - s.
+// Scores of the lane's experts (0 where not live).
 template <int V, int LPT>
 __device__ __forceinline__ void scores_of(float (&s)[V], const float (&z)[V], uint32_t live, bool sigmoid)
 {
@@ -610,8 +610,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(PlanArgs a)
 }
 
 // A workgroup: each expert's segment from its slots in LDS (total, overwritten
-// with the segment's first row; ends with the row behind its last slot), by the
-// first wave.  Returns the rows of all.
+// with the segment's first row, total[experts] with the rows of all; ends with the
+// row behind its last slot), by the first wave.
 __device__ __forceinline__ void plan_offsets(const PlanArgs& a, int* total, int* ends, int lane, int wave)
 {
     if (wave == 0) {

@@ -102,9 +102,9 @@ class ExpertBlock:
         self.w1.quantize(p["w1"])
         self.w2.quantize(p["w2"])
         rows = Fp8(cap, D).quantize(self.h, self.order, k)
-        # rows outside all segments are not written by the products
-        self.hidden_rows = product(rows.q, rows.s, self.w1.q, self.w1.s, torch.zeros(cap, H, dtype=DT, device="cuda"), cap, H, D, E,
-                                   P.PRODUCT_ROWS, 128, self.offsets, relu=True)
+        # rows outside all segments are neither written by the products nor read by the next ones
+        self.hidden_rows = product(rows.q, rows.s, self.w1.q, self.w1.s, empty(cap, H), cap, H, D, E, P.PRODUCT_ROWS, 128,
+                                   self.offsets, relu=True)
         act = Fp8(cap, H).quantize(self.hidden_rows)
         self.rows = product(act.q, act.s, self.w2.q, self.w2.s, empty(cap, D), cap, D, H, E, P.PRODUCT_ROWS, 128, self.offsets)
         self.f = empty(T, D)
