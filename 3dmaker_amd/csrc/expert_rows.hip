@@ -7,7 +7,9 @@
 // The rows' type R is that of the tokens, T, or fp32 on request.  16-bit rows are
 // a rounding more, between the experts' products and this sum: half the bytes of
 // the largest tensor of the block, for errors of a result about sqrt(2) of those
-// of its own rounding (two experts, bf16: 0.0023 of its 2-norm, 0.0017 with fp32 rows).
+// of its own rounding (two experts, bf16: 0.0023 of its 2-norm, 0.0017 with fp32
+// rows, for which 32,768 x 2 rows of 2,048 take 121 us instead of 75, and the
+// product in front 327 instead of 213).
 #include "experts.h"
 #include "lanes.h"
 

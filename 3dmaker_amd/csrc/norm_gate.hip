@@ -7,7 +7,8 @@
 //   dn1 = du w1            df = r1 (dn1 - mean dn1 - n1 mean(dn1 n1))
 //   dw2 = sum dh n2, db2 = sum dh, dw1 = sum du n1, db1 = sum du over the rows
 // (the mean of dn only for layer norms).  Bound by memory: a row stays in
-// registers between its passes, statistics in fp32.
+// registers between its passes (but for gradients of rows above 4,096 elements),
+// statistics in fp32.
 #include "experts.h"
 #include "lanes.h"
 
@@ -279,7 +280,13 @@ __device__ __forceinline__ void norm_back(float (&d)[VEC * PER], const float (&n
 // next row is fetched while this one is worked on: without that a row waits for
 // four tensors one after the other (16,389 x 1,280 fp16, layer norms: 237 us;
 // 67 now, 3.8 TB/s).  Bound by about 600 instructions a thread and row, at three
-// waves a SIMD: 168 registers are the most for these.
+// waves a SIMD: 168 registers are the most for these, and aligned 16-bit rows of
+// 128 to 512 threads take 166.  16-bit rows of 64 threads take 169, fp32 and
+// unaligned ones 185 to 256: two waves (fp32 16,389 x 1,280: 122 us, 4.1 TB/s;
+// 8,195 x 4,096: 173 us, 4.7 TB/s; 16-bit 65,539 x 256: 86 us, 2.3 TB/s; 16,389 x
+// 1,281: 133 us, 1.9 TB/s).  Rows above 4,096 elements have 1,024 threads of 128
+// registers, and spill 176 bytes a lane (16 bits), 344 (fp32) or 480 to 524
+// (unaligned): 4,099 x 8,192 bf16 345 us, 1.2 TB/s, fp32 642.
 template <class T, int VEC, int THREADS, int PER, int WG>
 __global__ __launch_bounds__(WG) void norm_gate_backward_kernel(NormArgs a)
 {
@@ -549,8 +556,9 @@ void backward_launch(const NormArgs& a, hipStream_t s)
 }
 
 // Eight elements a thread: the five sums over rows, the row's own arrays and the
-// next row stay in registers.  Whole waves, as few as hold the row.  Twelve waves a CU are resident, which is how
-// many workgroups the rows are dealt to.
+// next row stay in registers, up to 512 threads.  Whole waves, as few as hold the
+// row.  The rows are dealt to twelve waves a CU, as many as are resident of aligned
+// 16-bit rows; of most others eight are, and a third of the workgroups wait.
 int backward_threads(int dim, int vec)
 {
     const int lanes = ((dim + vec - 1) / vec + 8 / vec - 1) / (8 / vec);

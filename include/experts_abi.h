@@ -101,8 +101,8 @@ void launchRoutePlan(const int* d_indices, int numTokens, int topK, int numExper
  */
 
 typedef struct Fp8QuantOption {
-    int rows, cols;            /* of one quantised matrix */
-    int batch;                 /* matrices; with order: 1 */
+    int rows, cols;            /* of one quantised matrix; cols 1..2^22 */
+    int batch;                 /* matrices, 1..65535; with order or gate: 1 */
     int blockRows;             /* rows that share a scale: 1, or 128 (then transposed blocks are the same blocks) */
     int srcType;               /* DATA_* */
     int slotsPerRow;           /* with order: source row = slot / slotsPerRow */
@@ -129,7 +129,7 @@ void launchFp8Quantize(const Fp8QuantOption* opt, const void* d_src, const int* 
 #define PRODUCT_SUM 2   /* out of expert e: A's and B's columns [offsets[e], offsets[e+1]) */
 
 typedef struct Fp8ProductOption {
-    int m, n, k;          /* A [m x k], B [n x k] (DENSE, SUM) or [numExperts x n x k] (ROWS) */
+    int m, n, k;          /* A [m x k], B [n x k] (DENSE, SUM) or [numExperts x n x k] (ROWS); n, k 1..2^22 (SUM: k from 0) */
     int numExperts;       /* 1..1024; DENSE: 1 */
     int grouping;         /* PRODUCT_* */
     int scaleRowsB;       /* rows of B that share a scale: 128 or 1 */
@@ -174,7 +174,7 @@ void launchFp8Product(const Fp8ProductOption* opt, const uint8_t* d_a, const uin
 /* out[t] = sum_j weights[t, j] * rows[position[t, j]] in fp32, rounded once
  * (weights NULL: 1 each; a position outside 0..numRows-1 adds nothing).
  * rows [numRows x dim], out [numTokens x dim], both of dataType (rows fp32 with
- * COMBINE_ROWS_F32). */
+ * COMBINE_ROWS_F32); dim 1..2^23, topK 1..32. */
 void launchExpertCombine(int dim, int dataType, const void* d_rows, int numRows, long long rowStride,
                          const int* d_position, const float* d_weights, void* d_out, long long outStride,
                          int numTokens, int topK, hipStream_t stream);
