@@ -40,7 +40,7 @@ void with_type(int type, F&& f)
 }
 
 // f(first, number) over `wgs` workgroups in launches of less than 2^32 threads,
-// which is what a grid can have.
+// which is what a grid can have: a larger one wraps without an error.
 template <class F>
 void in_launches(long long wgs, int threads, F&& f)
 {
