@@ -20,6 +20,9 @@ LIB_PATH = os.path.join(_HERE, "lib3dmaker_amd.so")
 __all__ = [
     "LIB_PATH", "lib", "launch", "MLPOption", "MLPGridOptions", "HashGrid", "Net",
     "OUT_ACT_NONE", "OUT_ACT_SIGMOID", "ptr", "check", "RouteOption", "Fp8QuantOption", "Fp8ProductOption", "NormGateOption",
+    "Fp4QuantOption", "Fp4ProductOption", "ExpertLayerOption", "GradTensor", "FP4_SCALE_FLOOR", "FP4_SCALE_COVER",
+    "EXPERT_FP8", "EXPERT_FP4", "EXPERT_LINEAR", "EXPERT_RELU", "EXPERT_SILU", "EXPERT_GELU", "EXPERT_LAYER_TOKENS",
+    "GRAD_NORM_2", "GRAD_NORM_MAX", "GRAD_NONFINITE_KEEP", "GRAD_NONFINITE_ZERO", "fp4_pitch", "fp4_scale_pitch",
     "DATA_F32", "DATA_F16", "DATA_BF16", "ROUTE_SOFTMAX", "ROUTE_SIGMOID", "PRODUCT_DENSE", "PRODUCT_ROWS", "PRODUCT_SUM", "PRODUCT_EXACT", "COMBINE_ROWS_F32",
     "NORM_NONE", "NORM_RMS", "NORM_LAYER", "fp8_pitch", "fp8_scale_pitch", "Float3", "Uint3", "NerfOptions", "Nerf", "NerfTrainer", "NtrConfig", "NtrStats",
 ]
@@ -34,6 +37,14 @@ PRODUCT_DENSE, PRODUCT_ROWS, PRODUCT_SUM = 0, 1, 2
 PRODUCT_EXACT = 0x100
 COMBINE_ROWS_F32 = 0x100
 NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+FP4_SCALE_FLOOR, FP4_SCALE_COVER = 0, 1
+EXPERT_FP8, EXPERT_FP4 = 0, 1
+EXPERT_LINEAR, EXPERT_RELU, EXPERT_SILU, EXPERT_GELU = 0, 1, 2, 3
+EXPERT_LAYER_TOKENS = 64
+
+# include/grad_abi.h
+GRAD_NORM_2, GRAD_NORM_MAX = 0, 1
+GRAD_NONFINITE_KEEP, GRAD_NONFINITE_ZERO = 0, 1
 
 
 class MLPOption(C.Structure):
@@ -133,6 +144,31 @@ class NormGateOption(C.Structure):
                 ("strideY", C.c_longlong), ("strideH", C.c_longlong)]
 
 
+class Fp4QuantOption(C.Structure):
+    """include/experts_abi.h Fp4QuantOption"""
+    _fields_ = [("rows", C.c_int), ("cols", C.c_int), ("batch", C.c_int), ("scaleRule", C.c_int), ("srcType", C.c_int),
+                ("slotsPerRow", C.c_int), ("srcRows", C.c_int), ("srcStride", C.c_longlong),
+                ("srcBatchStride", C.c_longlong)]
+
+
+class Fp4ProductOption(C.Structure):
+    """include/experts_abi.h Fp4ProductOption"""
+    _fields_ = [("m", C.c_int), ("n", C.c_int), ("k", C.c_int), ("numExperts", C.c_int), ("grouping", C.c_int),
+                ("activation", C.c_int), ("outType", C.c_int), ("outStride", C.c_longlong)]
+
+
+class ExpertLayerOption(C.Structure):
+    """include/experts_abi.h ExpertLayerOption"""
+    _fields_ = [("route", RouteOption), ("dim", C.c_int), ("hidden", C.c_int), ("activation", C.c_int), ("gated", C.c_int),
+                ("weightFormat", C.c_int), ("scaleRows", C.c_int), ("dataType", C.c_int), ("routerType", C.c_int),
+                ("strideX", C.c_longlong), ("strideOut", C.c_longlong)]
+
+
+class GradTensor(C.Structure):
+    """include/grad_abi.h GradTensor"""
+    _fields_ = [("data", C.c_void_p), ("out", C.c_void_p), ("n", C.c_longlong), ("dataType", C.c_int)]
+
+
 def fp8_pitch(cols: int) -> int:
     """Bytes between the rows of an 8-bit matrix of `cols` columns (include/experts_abi.h)."""
     return -(-cols // 128) * 128
@@ -141,6 +177,16 @@ def fp8_pitch(cols: int) -> int:
 def fp8_scale_pitch(cols: int) -> int:
     """Scale bytes between its rows of blocks."""
     return -(-fp8_pitch(cols) // 512) * 4
+
+
+def fp4_pitch(cols: int) -> int:
+    """Bytes between the rows of a 4-bit matrix of `cols` columns (include/experts_abi.h)."""
+    return -(-cols // 128) * 64
+
+
+def fp4_scale_pitch(cols: int) -> int:
+    """Scale bytes between its rows."""
+    return -(-cols // 128) * 4
 
 
 class StepBuffers(C.Structure):
@@ -185,10 +231,17 @@ SIGNATURES = {
     "launchRoutePlan": (None, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "launchFp8Quantize": (None, [_vp] * 10),
     "launchFp8Product": (None, [_vp] * 8),
+    "launchFp4Quantize": (None, [_vp] * 6),
+    "launchFp4Product": (None, [_vp] * 8),
+    "launchExpertLayer": (None, [_vp] * 9 + [_i, _vp]),
     "launchExpertCombine": (None, [_i, _i, _vp, _i, _ll, _vp, _vp, _vp, _ll, _i, _i, _vp]),
     "launchExpertCombineBackward": (None, [_i, _i, _vp, _i, _ll, _vp, _vp, _ll, _vp, _i, _i, _vp]),
     "launchNormGateResidual": (None, [_vp] * 10 + [_i, _vp]),
     "launchNormGateResidualBackward": (None, [_vp] * 17 + [_i, _vp]),
+    # include/grad_abi.h (the gradients' norm)
+    "launchGradNorm": (None, [_vp, _i, _i, _f, _vp, _vp]),
+    "launchGradClip": (None, [_vp, _i, _f, _i, _vp, _vp]),
+    "launchGradNormClip": (None, [_vp, _i, _i, _f, _f, _i, _vp, _vp]),
     "tinymlp_last_error": (_i, []),
     "tinymlp_last_error_message": (C.c_char_p, []),
     # include/tinymlp_capi.h (flat handle API)

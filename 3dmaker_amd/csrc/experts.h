@@ -1,6 +1,6 @@
 // Internal interface of the mixture-of-experts operators (route.hip,
-// fp8_quant.hip, fp8_product.hip, expert_rows.hip, norm_gate.hip); the options
-// are those of experts_abi.h.  Every function checks its arguments before its
+// fp8_quant.hip, fp8_product.hip, fp4_quant.hip, fp4_product.hip,
+// expert_rows.hip, expert_layer.hip, norm_gate.hip); the options are those of experts_abi.h.  Every function checks its arguments before its
 // first device call and throws std::runtime_error.
 #pragma once
 
@@ -63,6 +63,12 @@ constexpr I round_up(I n, I m)
 constexpr int fp8_pitch(int cols) { return round_up(cols, 128); }
 constexpr int fp8_scale_pitch(int cols) { return round_up(fp8_pitch(cols) / 128, 4); }
 
+// The same of a 4-bit matrix.
+constexpr int fp4_pitch(int cols) { return round_up(cols, 128) / 2; }
+constexpr int fp4_scale_pitch(int cols) { return round_up(cols, 128) / 32; }
+
+// What route_experts requires of its option.
+void check_route_option(const RouteOption& o);
 void route_experts(const RouteOption& o, const void* logits, long long stride, const float* bias, int* indices,
                    float* weights, int tokens, hipStream_t s);
 void route_experts_backward(const RouteOption& o, const void* logits, long long stride, const int* indices,
@@ -76,11 +82,22 @@ void fp8_quantize(const Fp8QuantOption& o, const void* src, const int* order, co
 void fp8_product(const Fp8ProductOption& o, const uint8_t* a, const uint8_t* a_scales, const uint8_t* b,
                  const uint8_t* b_scales, const int* offsets, void* out, hipStream_t s);
 
+void fp4_quantize(const Fp4QuantOption& o, const void* src, const int* order, uint8_t* q, uint8_t* scales, hipStream_t s);
+void fp4_product(const Fp4ProductOption& o, const uint8_t* a, const uint8_t* a_scales, const uint8_t* b,
+                 const uint8_t* b_scales, const int* offsets, void* out, hipStream_t s);
+
 void expert_combine(int dim, int type, const void* rows, int num_rows, long long row_stride, const int* position,
                     const float* weights, void* out, long long out_stride, int tokens, int topK, hipStream_t s);
 void expert_combine_backward(int dim, int type, const void* rows, int num_rows, long long row_stride, const int* position,
                              const void* dout, long long dout_stride, float* dweights, int tokens, int topK,
                              hipStream_t s);
+
+struct ExpertLayerTensors {
+    const void *x, *router;
+    const float* bias;
+    const uint8_t *w1, *w1_scales, *w2, *w2_scales;
+};
+void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void* out, int tokens, hipStream_t s);
 
 struct NormGateTensors {
     const void *x, *f, *gate;

@@ -62,6 +62,34 @@ void launchFp8Product(const Fp8ProductOption* opt, const uint8_t* d_a, const uin
     });
 }
 
+void launchFp4Quantize(const Fp4QuantOption* opt, const void* d_src, const int* d_order, uint8_t* d_q, uint8_t* d_scales,
+                       hipStream_t stream)
+{
+    guarded("launchFp4Quantize", [&] {
+        require(opt, "null option");
+        graft::fp4_quantize(*opt, d_src, d_order, d_q, d_scales, stream);
+    });
+}
+
+void launchFp4Product(const Fp4ProductOption* opt, const uint8_t* d_a, const uint8_t* d_aScales, const uint8_t* d_b,
+                      const uint8_t* d_bScales, const int* d_offsets, void* d_out, hipStream_t stream)
+{
+    guarded("launchFp4Product", [&] {
+        require(opt, "null option");
+        graft::fp4_product(*opt, d_a, d_aScales, d_b, d_bScales, d_offsets, d_out, stream);
+    });
+}
+
+void launchExpertLayer(const ExpertLayerOption* opt, const void* d_x, const void* d_router, const float* d_bias,
+                       const uint8_t* d_w1, const uint8_t* d_w1Scales, const uint8_t* d_w2, const uint8_t* d_w2Scales,
+                       void* d_out, int numTokens, hipStream_t stream)
+{
+    guarded("launchExpertLayer", [&] {
+        require(opt, "null option");
+        graft::expert_layer(*opt, {d_x, d_router, d_bias, d_w1, d_w1Scales, d_w2, d_w2Scales}, d_out, numTokens, stream);
+    });
+}
+
 void launchExpertCombine(int dim, int dataType, const void* d_rows, int numRows, long long rowStride,
                          const int* d_position, const float* d_weights, void* d_out, long long outStride, int numTokens,
                          int topK, hipStream_t stream)

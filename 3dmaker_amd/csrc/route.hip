@@ -424,15 +424,7 @@ void with_layout(int lanes, int per_lane, F&& f)
 
 void check_route(const RouteOption& o, const void* logits, long long stride, int tokens)
 {
-    require(o.numExperts >= 1 && o.numExperts <= kMaxExperts, "numExperts must be 1..1024");
-    require(o.topK >= 1 && o.topK <= 32 && o.topK <= o.numExperts, "topK must be 1..32 and at most numExperts");
-    require(o.scoreType == ROUTE_SOFTMAX || o.scoreType == ROUTE_SIGMOID, "unknown scoreType");
-    require(o.numGroups >= 1 && o.numGroups <= 64 && o.numExperts % o.numGroups == 0,
-            "numGroups must be 1..64 and divide numExperts");
-    require(o.topGroups >= 1 && o.topGroups <= o.numGroups, "topGroups must be 1..numGroups");
-    require(o.numGroups == 1 || o.groupScore == 1 || o.groupScore == 2, "groupScore must be 1 or 2");
-    require(std::isfinite(o.scale), "scale must be finite");
-    require_type(o.logitsType);
+    check_route_option(o);
     require(tokens >= 0 && tokens <= kMaxRows, "numTokens must be 0..2^30");
     require(stride >= o.numExperts, "logitsStride must be at least numExperts");
     require(tokens == 0 || logits, "null argument");
@@ -461,6 +453,19 @@ bool can_vec(const void* p, long long stride, int per_group, int V, int type)
 }
 
 }  // namespace
+
+void check_route_option(const RouteOption& o)
+{
+    require(o.numExperts >= 1 && o.numExperts <= kMaxExperts, "numExperts must be 1..1024");
+    require(o.topK >= 1 && o.topK <= 32 && o.topK <= o.numExperts, "topK must be 1..32 and at most numExperts");
+    require(o.scoreType == ROUTE_SOFTMAX || o.scoreType == ROUTE_SIGMOID, "unknown scoreType");
+    require(o.numGroups >= 1 && o.numGroups <= 64 && o.numExperts % o.numGroups == 0,
+            "numGroups must be 1..64 and divide numExperts");
+    require(o.topGroups >= 1 && o.topGroups <= o.numGroups, "topGroups must be 1..numGroups");
+    require(o.numGroups == 1 || o.groupScore == 1 || o.groupScore == 2, "groupScore must be 1 or 2");
+    require(std::isfinite(o.scale), "scale must be finite");
+    require_type(o.logitsType);
+}
 
 void route_experts(const RouteOption& o, const void* logits, long long stride, const float* bias, int* indices,
                    float* weights, int tokens, hipStream_t s)

@@ -3,7 +3,8 @@
  * (gfx950): routing of tokens (samples) to experts, products of 8-bit
  * matrices with a scale for each block of 128, the gather and combine of the
  * experts' rows, and the norms, gate and residual around a block; forward and
- * backward.  No counterpart exists in the reference, whose heads are single
+ * backward.  For serving, 4-bit matrices with a scale for each block of 32, and
+ * the whole layer of experts for few tokens in one call.  No counterpart exists in the reference, whose heads are single
  * MLPs of at most 128 (modules/TinyMLP).
  *
  * Conventions are those of tinymlp_abi.h: device pointers unless stated, a
@@ -164,6 +165,57 @@ typedef struct Fp8ProductOption {
 void launchFp8Product(const Fp8ProductOption* opt, const uint8_t* d_a, const uint8_t* d_aScales, const uint8_t* d_b,
                       const uint8_t* d_bScales, const int* d_offsets, void* d_out, hipStream_t stream);
 
+/* ---- 4-bit matrices ---------------------------------------------------------
+ *
+ * A 4-bit matrix [rows x cols] is held as OCP e2m1 values (0, 1/2, 1, 3/2, 2, 3,
+ * 4, 6 and their negatives), two a byte, the even column in the low four bits:
+ * bytes [rows x pitch], pitch = half of cols rounded up to a multiple of 128, zero
+ * behind cols; and one scale byte for each block of 32 columns of a row, the
+ * power of two 2^(byte - 127): [rows x scale pitch], scale pitch = blocks of the
+ * filled row, a multiple of 4.  Both start at a multiple of 16 (bytes) and 4
+ * (scales).  A scale is at least 2^-126; byte 255 is a block of NaN, which any
+ * infinity or NaN in it makes of a block.
+ */
+
+/* 2^(floor(log2 max) - 2) of the block's largest magnitude (the rule of the OCP
+ * microscaling formats): values beyond 6 of it become 6. */
+#define FP4_SCALE_FLOOR 0
+/* The smallest power of two that brings the block within 6. */
+#define FP4_SCALE_COVER 1
+
+typedef struct Fp4QuantOption {
+    int rows, cols;            /* of one quantised matrix; cols 1..2^22 */
+    int batch;                 /* matrices, 1..65535; with order: 1 */
+    int scaleRule;             /* FP4_SCALE_* */
+    int srcType;               /* DATA_* */
+    int slotsPerRow;           /* with order: source row = slot / slotsPerRow */
+    int srcRows;               /* rows of the source; slots beyond them read as zero */
+    long long srcStride;       /* between source rows */
+    long long srcBatchStride;  /* between source matrices */
+} Fp4QuantOption;
+
+/* Quantises x, or rows gathered from it: row r of the result is source row r, or
+ * with d_order (nullable) source row d_order[r] / slotsPerRow, and zero where
+ * d_order[r] is -1.  One rounding, to nearest, ties to even. */
+void launchFp4Quantize(const Fp4QuantOption* opt, const void* d_src, const int* d_order, uint8_t* d_q, uint8_t* d_scales,
+                       hipStream_t stream);
+
+typedef struct Fp4ProductOption {
+    int m, n, k;          /* A [m x k], B [n x k] (DENSE) or [numExperts x n x k] (ROWS); n, k 1..2^22 */
+    int numExperts;       /* 1..1024; DENSE: 1 */
+    int grouping;         /* PRODUCT_DENSE or PRODUCT_ROWS */
+    int activation;       /* 0: none, 1: ReLU on the result */
+    int outType;          /* DATA_* */
+    long long outStride;  /* between rows of out */
+} Fp4ProductOption;
+
+/* out [m x n] = A B^T from 4-bit matrices, groupings and d_offsets as for
+ * launchFp8Product.  Results of any type are sums of exact products in fp32,
+ * rounded once; products of 2^128 and more are infinite, and what is below
+ * 2^-149 is lost. */
+void launchFp4Product(const Fp4ProductOption* opt, const uint8_t* d_a, const uint8_t* d_aScales, const uint8_t* d_b,
+                      const uint8_t* d_bScales, const int* d_offsets, void* d_out, hipStream_t stream);
+
 /* ---- the experts' rows back to tokens --------------------------------------- */
 
 /* Or'ed to the dataType of the two launchers below: rows are fp32 whatever the
@@ -185,6 +237,45 @@ void launchExpertCombine(int dim, int dataType, const void* d_rows, int numRows,
 void launchExpertCombineBackward(int dim, int dataType, const void* d_rows, int numRows, long long rowStride,
                                  const int* d_position, const void* d_dout, long long doutStride, float* d_dweights,
                                  int numTokens, int topK, hipStream_t stream);
+
+/* ---- the whole layer for few tokens -------------------------------------------- */
+
+#define EXPERT_FP8 0 /* e4m3 with a scale for scaleRows rows by 128 columns */
+#define EXPERT_FP4 1 /* e2m1 with a scale for 32 columns of a row */
+
+#define EXPERT_LINEAR 0
+#define EXPERT_RELU 1
+#define EXPERT_SILU 2 /* v / (1 + exp(-v)) */
+#define EXPERT_GELU 3 /* v (1 + erf(v / sqrt 2)) / 2 */
+
+typedef struct ExpertLayerOption {
+    RouteOption route;    /* logitsType DATA_F32: the logits stay in the call */
+    int dim;              /* D, 1..16384 */
+    int hidden;           /* H, 1..16384 */
+    int activation;       /* EXPERT_* */
+    int gated;            /* nonzero: W1 has 2 H rows, the activation's and those that it is multiplied by */
+    int weightFormat;     /* EXPERT_FP8 or EXPERT_FP4 */
+    int scaleRows;        /* rows of a matrix that share a scale: EXPERT_FP8 1 or 128, EXPERT_FP4 1 */
+    int dataType;         /* DATA_*, of x and out */
+    int routerType;       /* DATA_*, of the router */
+    long long strideX, strideOut; /* between rows */
+} ExpertLayerOption;
+
+#define EXPERT_LAYER_TOKENS 64
+
+/* out[t] = sum_j w_j W2_e a(W1_e x[t]) over the experts e = e_j and weights w_j
+ * that launchRouteExperts gives for the logits x router^T (and d_bias, nullable):
+ *   a(h) = act(h), or gated act(h[0..H-1]) * h[H..2H-1]
+ * for 0..EXPERT_LAYER_TOKENS tokens.  router [E x D] without gaps; W1 [E x (H or
+ * 2 H) x D] and W2 [E x D x H] as the quantising launchers write them (scale
+ * bytes of EXPERT_FP8 17 to 246).  Neither x nor a is quantised: products of the
+ * weights' values and the tokens' are exact, a is held in 16 bits more than a
+ * 16-bit token (in all of fp32 for fp32 tokens), sums are fp32, and out is rounded
+ * once.  A token none of whose experts is available (NaN among its logits) gets
+ * zeros.  out and x do not overlap. */
+void launchExpertLayer(const ExpertLayerOption* opt, const void* d_x, const void* d_router, const float* d_bias,
+                       const uint8_t* d_w1, const uint8_t* d_w1Scales, const uint8_t* d_w2, const uint8_t* d_w2Scales,
+                       void* d_out, int numTokens, hipStream_t stream);
 
 /* ---- norms around a block, gate and residual --------------------------------- */
 
