@@ -30,8 +30,10 @@ __device__ __forceinline__ f4 mfma_fp4(i4v b, int sb, i4v a, int sa, f4 c)
 #endif
 }
 
-// Up to 16 MT rows by 16 rows of B a workgroup, its waves sharing out k, four
-// times 128 at a time, and their sums joined in LDS in wave order.
+// Few rows of A, or few tiles with a long k: up to 16 MT rows by 16 rows of B a
+// workgroup, its waves sharing out k, four times 128 at a time, straight from memory
+// to registers, and their sums joined in LDS in wave order.  With few rows B's bytes
+// and one round trip bound it: one row by 4096 x 4096 5.2 us, 9 MB at 1.7 TB/s.
 constexpr int kFewWaves = 8;
 template <class T, int MT>
 __global__ __launch_bounds__(kFewWaves * 64) void product4_few_kernel(ProductArgs a)
@@ -126,6 +128,13 @@ void few_launch(ProductArgs& a, hipStream_t s)
 // B's row of fragment i and lane column c is (i / 2) 32 + (c / 4) 8 + (i % 2) 4 +
 // c % 4: a lane ends with eight consecutive columns of two fragments, one 16-byte
 // store of 16-bit results.
+//
+// 256 x 256 by eight waves: 8192 cubed 255 us, 4.3 PFLOP/s (5.0 of zeros: power), its
+// matrix cores busy 55% of the time; four waves of 128 x 128 need more registers for
+// two halves of A than there are, and spill (750 us).  128 x 128, two workgroups a CU,
+// copies twice the bytes for the same work (342 us).  Rows of 64 bytes in four places
+// made twice the L2 requests (326 us), copies in a burst behind the barrier instead of
+// between the matrix instructions 261.
 template <class T, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64, 2) void product4_kernel(ProductArgs a)
 {
@@ -288,9 +297,11 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product4_kernel(ProductArgs a
                 const i8v q{fa[i][0], fa[i][1], fa[i][2], fa[i][3], 0, 0, 0, 0};
                 c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(p, q, c, 4, 4, j, sbx, i % 4, sax[i / 4]);
                 asm volatile("" : "+v"(c));
-                constexpr int n = 2 * (i - 1) + (j & 1), m = 3 * (i - 1) + j - 1;  // of the next half's B, and of the copies
+                constexpr int n = 2 * (i - 1) + (j & 1);  // of the next half's B
+                constexpr int slots = (MT - 1) * NT, at = (i - 1) * NT + j;
+                constexpr int m = (at * kCopies + slots - 1) / slots, m1 = ((at + 1) * kCopies + slots - 1) / slots;  // copies
                 if constexpr (i > 0 && j < 2 && n < NT) read_b(by[n], to, 1 - h, n);
-                if constexpr (h && i > 0 && j >= 1 && m < kCopies) copy(place, m);
+                if constexpr (h && i > 0 && m < m1) copy(place, m);
                 __builtin_amdgcn_sched_barrier(0);
             });
             if constexpr (h && i == 0) {
@@ -392,6 +403,37 @@ void product_launch(ProductArgs& a, hipStream_t s)
     GRAFT_LAUNCH_CHECK();
 }
 
+// The form by what it takes for 128 of k, in units of 10 ns: rows of a workgroup
+// that shares out k (16, 32, 64), or of a tile (128, 256).  Measured (dense, k =
+// 4096, us sharing 16, 32 or 64 rows and in tiles of 128 and 256): 16 x 8192 9.6,
+// 10.3, 11.7, 14.2, 25.7; 128 x 2048 17.0, 13.1, 11.6, 14.8, 27.3; 256 x 2048 31,
+// 24, 21, 14.9, 28.4; 4096 x 2048 446, 336, 281, 25.6, 35.8; 4096 x 8192 1775, 1332,
+// 1113, 93, 80.  Workgroups that share k take 5 and 6.1 for each 16 rows, as many at
+// a time as there are CUs; a CU's tiles of 128 37, or 44 the only one; a round of
+// tiles of 256 112, or 85 if there is one.  Of rows by expert, every segment may
+// end inside a large tile: they are counted with all such ends, the others without
+// (19,200 rows of 64 experts, 2048 x 1024: 44 us in tiles of 128, 52 of 256; 96,000
+// 223 and 188).  Experts are taken to be of equal length, without the empty ones
+// that a short plan is bound to have.
+int form_of(const Fp4ProductOption& o)
+{
+    const long long cus = num_cus(), experts = o.grouping == PRODUCT_DENSE ? 1 : std::min(o.numExperts, o.m);
+    const long long rows = (o.m + experts - 1) / experts;
+    auto up = [](long long n, long long d) { return (n + d - 1) / d; };
+    const long long small = experts * up(rows, 128) * up(o.n, 128);
+    const long long large = (o.grouping == PRODUCT_DENSE ? up(o.m, 256) : o.m / 256 + o.numExperts) * up(o.n, 256);
+    double best = small <= cus ? 44 : 37.0 * up(small, cus);
+    int form = 128;
+    const double in_large = large <= cus ? 85 : 112.0 * up(large, cus);
+    if (in_large < best) best = in_large, form = 256;
+    for (int mt = 1; mt <= 4; mt *= 2) {
+        const long long groups = experts * up(rows, 16 * mt) * up(o.n, 16);
+        const double cost = std::max(1.0, (double)groups / cus) * (5 + 6.1 * mt);
+        if (cost < best) best = cost, form = 16 * mt;
+    }
+    return form;
+}
+
 }  // namespace
 
 void fp4_product(const Fp4ProductOption& o, const uint8_t* a, const uint8_t* a_scales, const uint8_t* b,
@@ -431,13 +473,13 @@ void fp4_product(const Fp4ProductOption& o, const uint8_t* a, const uint8_t* a_s
     p.vec = aligned16(out) && o.outStride * data_bytes(o.outType) % 16 == 0;
     with_type(o.outType, [&](auto zero) {
         using T = decltype(zero);
-        const char* f = getenv("FORM");
-        const int form = f ? atoi(f) : o.m <= 16 ? 1 : 256;
-        if (form == 1) few_launch<T, 1>(p, s);
-        else if (form == 2) few_launch<T, 2>(p, s);
-        else if (form == 4) few_launch<T, 4>(p, s);
-        else if (form == 128) product_launch<T, 128, 128, 2, 2>(p, s);
-        else product_launch<T, 256, 256, 2, 4>(p, s);
+        switch (form_of(o)) {
+            case 16: return few_launch<T, 1>(p, s);
+            case 32: return few_launch<T, 2>(p, s);
+            case 64: return few_launch<T, 4>(p, s);
+            case 128: return product_launch<T, 128, 128, 2, 2>(p, s);
+            default: return product_launch<T, 256, 256, 2, 4>(p, s);
+        }
     });
 }
 
