@@ -62,52 +62,94 @@ struct Span {
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-// A thread's sum of squares, or its largest magnitude as bits (NaN above all).
+// A thread's sum of squares, or its largest magnitude as bits (NaN above all); four
+// of them, so that an addition does not wait for the one before.
+template <bool TOP>
 struct Sum {
-    double sq = 0.0;
+    double sq[4] = {};
     uint32_t top = 0;
-    __device__ __forceinline__ void add(float v, int kind)
+    __device__ __forceinline__ void add(float v, int i)
     {
-        if (kind == GRAD_NORM_2) sq = fma((double)v, (double)v, sq);
-        else top = max(top, magnitude(v));
+        if constexpr (TOP) top = max(top, magnitude(v));
+        else sq[i & 3] = fma((double)v, (double)v, sq[i & 3]);
     }
+    __device__ __forceinline__ double value() const { return TOP ? (double)top : (sq[0] + sq[1]) + (sq[2] + sq[3]); }
 };
 
-template <class T>
-__device__ __forceinline__ void add_piece(Sum& s, const Span<T>& t, long long first, int kind)
+// f(first element) of the thread's 16-byte parts of a piece: whole ones by f, the
+// tensor's first and last by g(element) for each element of it.
+template <class T, class F, class G>
+__device__ __forceinline__ void for_parts(const Span<T>& t, uint32_t piece, F&& f, G&& g)
 {
     constexpr int N = Span<T>::N, kPer = kPieceBytes / 16 / kGradThreads;
+    const long long first = (long long)piece * (kPieceBytes / (int)sizeof(T));
+    if (first >= t.lo && first + kPieceBytes / (int)sizeof(T) <= t.hi) {
+        Vec<T, N> v[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-        const long long at = first + (i * kGradThreads + (int)threadIdx.x) * N;
-        if (at >= t.lo && at + N <= t.hi) {
-            const Vec<T, N> v = *reinterpret_cast<const Vec<T, N>*>(t.base + at);
+        for (int i = 0; i < kPer; i++)
+            v[i] = *reinterpret_cast<const Vec<T, N>*>(t.base + first + (i * kGradThreads + (int)threadIdx.x) * N);
 #pragma unroll
-            for (int j = 0; j < N; j++) s.add((float)v[j], kind);
-        } else {
-            for (int j = 0; j < N; j++)
-                if (at + j >= t.lo && at + j < t.hi) s.add((float)t.base[at + j], kind);
+        for (int i = 0; i < kPer; i++) f(first + (i * kGradThreads + (int)threadIdx.x) * N, v[i]);
+    } else {
+        for (int i = 0; i < kPer; i++) {
+            const long long at = first + (i * kGradThreads + (int)threadIdx.x) * N;
+            if (at >= t.lo && at + N <= t.hi) f(at, *reinterpret_cast<const Vec<T, N>*>(t.base + at));
+            else
+                for (int j = 0; j < N; j++)
+                    if (at + j >= t.lo && at + j < t.hi) g(at + j);
         }
     }
 }
 
-// f(tensor, piece of it) over the workgroup's pieces.
-template <class F>
+template <class T, bool TOP>
+__device__ __forceinline__ void add_piece(Sum<TOP>& s, const Span<T>& t, uint32_t piece)
+{
+    for_parts(
+        t, piece,
+        [&](long long, Vec<T, Span<T>::N> v) {
+#pragma unroll
+            for (int j = 0; j < Span<T>::N; j++) s.add((float)v[j], j);
+        },
+        [&](long long at) { s.add((float)t.base[at], 0); });
+}
+
+// f(tensor, piece of it) over the workgroup's pieces, from the last to the first:
+// what the pass for the norm has read last may still be in the cache for the one
+// that clips, which runs the other way.
+template <bool BACK, class F>
 __device__ __forceinline__ void for_pieces(const GradTable& t, F&& f)
 {
     const uint32_t pieces = t.end[t.count - 1];
     const uint32_t p0 = (uint32_t)((uint64_t)pieces * blockIdx.x / gridDim.x);
     const uint32_t p1 = (uint32_t)((uint64_t)pieces * (blockIdx.x + 1) / gridDim.x);
-    int lo = 0, hi = t.count - 1;  // the first tensor that ends behind p0
+    if (p0 == p1) return;
+    const uint32_t start = BACK ? p1 - 1 : p0;
+    int lo = 0, hi = t.count - 1;  // the first tensor that ends behind it
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        if (t.end[mid] > p0) hi = mid;
+        if (t.end[mid] > start) hi = mid;
         else lo = mid + 1;
     }
-    for (uint32_t p = p0; p < p1; p++) {
-        while (p >= t.end[lo]) lo++;
-        f(lo, p - (lo ? t.end[lo - 1] : 0u));
+    if (BACK) {
+        for (uint32_t p = p1; p-- > p0;) {
+            while (lo > 0 && p < t.end[lo - 1]) lo--;
+            f(lo, p - (lo ? t.end[lo - 1] : 0u));
+        }
+    } else {
+        for (uint32_t p = p0; p < p1; p++) {
+            while (p >= t.end[lo]) lo++;
+            f(lo, p - (lo ? t.end[lo - 1] : 0u));
+        }
     }
+}
+
+// f(T{}) with the C++ type of a tensor.
+template <class F>
+__device__ __forceinline__ void with_type_of(int type, F&& f)
+{
+    if (type == DATA_F32) f(0.0f);
+    else if (type == DATA_F16) f((_Float16)0.0f);
+    else f((__bf16)0.0f);
 }
 
 __device__ __forceinline__ double wave_sum(double v)
@@ -136,19 +178,14 @@ __device__ __forceinline__ double join(double v, int kind)
 }
 
 // Largest magnitudes travel as their bits: whole numbers, so that NaN are the largest.
+template <bool TOP>
 __global__ __launch_bounds__(kGradThreads) void grad_sum_kernel(GradTable t, GradArgs a)
 {
-    Sum s;
-    for_pieces(t, [&](int i, uint32_t piece) {
-        auto add = [&](auto zero) {
-            using T = decltype(zero);
-            add_piece(s, Span<T>(t.data[i], t.n[i]), (long long)piece * (kPieceBytes / sizeof(T)), a.kind);
-        };
-        if (t.type[i] == DATA_F32) add(0.0f);
-        else if (t.type[i] == DATA_F16) add((_Float16)0.0f);
-        else add((__bf16)0.0f);
+    Sum<TOP> s;
+    for_pieces<false>(t, [&](int i, uint32_t piece) {
+        with_type_of(t.type[i], [&](auto zero) { add_piece(s, Span<decltype(zero)>(t.data[i], t.n[i]), piece); });
     });
-    const double v = join(a.kind == GRAD_NORM_2 ? s.sq : (double)s.top, a.kind);
+    const double v = join(s.value(), a.kind);
     if (threadIdx.x == 0) a.sums[blockIdx.x] = v;
 }
 
@@ -174,24 +211,29 @@ __global__ __launch_bounds__(kGradThreads) void grad_norm_kernel(GradArgs a)
 template <class T>
 __device__ __forceinline__ void clip_piece(const void* data, void* out, long long n, uint32_t piece, float factor, bool zero)
 {
-    constexpr int N = Span<T>::N, kPer = kPieceBytes / 16 / kGradThreads;
+    constexpr int N = Span<T>::N;
     const Span<T> t(data, n);
     T* const to = (T*)out - t.lo;
-    const bool vec = ((uintptr_t)to & 15) == 0;
-    const long long first = (long long)piece * (kPieceBytes / sizeof(T));
-    auto scaled = [&](T v) { return zero ? (T)0.0f : factor == 1.0f ? v : (T)((float)v * factor); };
+    auto scaled = [&](T v) { return zero ? (T)0.0f : (T)((float)v * factor); };
+    if (((uintptr_t)to & 15) == 0) {
+        for_parts(
+            t, piece,
+            [&](long long at, Vec<T, N> v) {
+                if (factor != 1.0f || zero) {
 #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-        const long long at = first + (i * kGradThreads + (int)threadIdx.x) * N;
-        if (vec && at >= t.lo && at + N <= t.hi) {
-            Vec<T, N> v = *reinterpret_cast<const Vec<T, N>*>(t.base + at);
+                    for (int j = 0; j < N; j++) v[j] = scaled(v[j]);
+                }
+                *reinterpret_cast<Vec<T, N>*>(to + at) = v;
+            },
+            [&](long long at) { to[at] = scaled(t.base[at]); });
+    } else {  // an output that starts elsewhere in 16 bytes than its input: element by element
+        for_parts(
+            t, piece,
+            [&](long long at, Vec<T, N> v) {
 #pragma unroll
-            for (int j = 0; j < N; j++) v[j] = scaled(v[j]);
-            *reinterpret_cast<Vec<T, N>*>(to + at) = v;
-        } else {
-            for (int j = 0; j < N; j++)
-                if (at + j >= t.lo && at + j < t.hi) to[at + j] = scaled(t.base[at + j]);
-        }
+                for (int j = 0; j < N; j++) to[at + j] = scaled(v[j]);
+            },
+            [&](long long at) { to[at] = scaled(t.base[at]); });
     }
 }
 
@@ -201,12 +243,10 @@ __global__ __launch_bounds__(kGradThreads) void grad_clip_kernel(GradTable t, Gr
     if (a.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *a.norm_out = n;
     const bool finite = magnitude(n) < 0x7f800000u, zero = !finite && a.zero;
     const float factor = finite && n > a.max_norm ? a.max_norm / n : 1.0f;
-    for_pieces(t, [&](int i, uint32_t piece) {
+    for_pieces<true>(t, [&](int i, uint32_t piece) {
         void* const out = t.out[i];
         if (out == t.data[i] && factor == 1.0f && !zero) return;
-        if (t.type[i] == DATA_F32) clip_piece<float>(t.data[i], out, t.n[i], piece, factor, zero);
-        else if (t.type[i] == DATA_F16) clip_piece<_Float16>(t.data[i], out, t.n[i], piece, factor, zero);
-        else clip_piece<__bf16>(t.data[i], out, t.n[i], piece, factor, zero);
+        with_type_of(t.type[i], [&](auto z) { clip_piece<decltype(z)>(t.data[i], out, t.n[i], piece, factor, zero); });
     });
 }
 
@@ -307,7 +347,8 @@ int sums(const GradTensor* tensors, int count, GradArgs& a, hipStream_t s)
     in_tables(tensors, count, [&](const GradTable& t, unsigned wgs) {
         GradArgs b = a;
         b.sums += n;
-        grad_sum_kernel<<<wgs, kGradThreads, 0, s>>>(t, b);
+        if (a.kind == GRAD_NORM_2) grad_sum_kernel<false><<<wgs, kGradThreads, 0, s>>>(t, b);
+        else grad_sum_kernel<true><<<wgs, kGradThreads, 0, s>>>(t, b);
         GRAFT_LAUNCH_CHECK();
         n += (int)wgs;
     });
