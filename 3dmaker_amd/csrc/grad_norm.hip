@@ -4,8 +4,9 @@
 // Bound by memory: one read for the norm, one read and one write for the clipping.
 //
 // The list of tensors goes to the kernels by value, kMostTensors to a launch, so
-// that nothing has to be kept for it.  It is worked through as pieces of 16 KiB; a
-// workgroup takes consecutive ones, so that it looks its first tensor up once.
+// that nothing has to be kept for it.  It is worked through in pieces of 64 bytes a
+// thread; a workgroup (of few gradients: a wave of the only one) takes consecutive
+// ones, so that it looks its first tensor up once.
 // Squares of fp32 numbers are exact in 64 bits, and neither overflow nor vanish:
 // the sum is off by 2^-53 an addition.  Sums of workgroups are joined in their
 // order.
@@ -20,8 +21,8 @@ namespace graft {
 
 namespace {
 
-constexpr int kGradThreads = 256, kGradWaves = kGradThreads / 64;
-constexpr int kPieceBytes = 16384;
+constexpr int kGradThreads = 256, kSmallThreads = 1024;
+constexpr int piece_bytes(int threads) { return threads * 64; }
 constexpr int kMostTensors = 128;  // kernel arguments of 4 KiB
 
 struct GradTable {
@@ -36,7 +37,7 @@ struct GradTable {
 struct GradArgs {
     double* sums;         // of the workgroups
     int num_sums;
-    int kind;
+    bool top;             // the largest magnitude
     float scale, max_norm;
     bool zero;            // where the norm is not finite
     const float* norm_in; // given, or from the sums
@@ -78,21 +79,21 @@ struct Sum {
 
 // f(first element) of the thread's 16-byte parts of a piece: whole ones by f, the
 // tensor's first and last by g(element) for each element of it.
-template <class T, class F, class G>
+template <int THREADS, class T, class F, class G>
 __device__ __forceinline__ void for_parts(const Span<T>& t, uint32_t piece, F&& f, G&& g)
 {
-    constexpr int N = Span<T>::N, kPer = kPieceBytes / 16 / kGradThreads;
-    const long long first = (long long)piece * (kPieceBytes / (int)sizeof(T));
-    if (first >= t.lo && first + kPieceBytes / (int)sizeof(T) <= t.hi) {
+    constexpr int N = Span<T>::N, kPer = 4, kElements = piece_bytes(THREADS) / (int)sizeof(T);
+    const int thread = threadIdx.x & (THREADS - 1);
+    const long long first = (long long)piece * kElements;
+    if (first >= t.lo && first + kElements <= t.hi) {
         Vec<T, N> v[kPer];
 #pragma unroll
-        for (int i = 0; i < kPer; i++)
-            v[i] = *reinterpret_cast<const Vec<T, N>*>(t.base + first + (i * kGradThreads + (int)threadIdx.x) * N);
+        for (int i = 0; i < kPer; i++) v[i] = *reinterpret_cast<const Vec<T, N>*>(t.base + first + (i * THREADS + thread) * N);
 #pragma unroll
-        for (int i = 0; i < kPer; i++) f(first + (i * kGradThreads + (int)threadIdx.x) * N, v[i]);
+        for (int i = 0; i < kPer; i++) f(first + (i * THREADS + thread) * N, v[i]);
     } else {
         for (int i = 0; i < kPer; i++) {
-            const long long at = first + (i * kGradThreads + (int)threadIdx.x) * N;
+            const long long at = first + (i * THREADS + thread) * N;
             if (at >= t.lo && at + N <= t.hi) f(at, *reinterpret_cast<const Vec<T, N>*>(t.base + at));
             else
                 for (int j = 0; j < N; j++)
@@ -101,10 +102,10 @@ __device__ __forceinline__ void for_parts(const Span<T>& t, uint32_t piece, F&& 
     }
 }
 
-template <class T, bool TOP>
+template <int THREADS, class T, bool TOP>
 __device__ __forceinline__ void add_piece(Sum<TOP>& s, const Span<T>& t, uint32_t piece)
 {
-    for_parts(
+    for_parts<THREADS>(
         t, piece,
         [&](long long, Vec<T, Span<T>::N> v) {
 #pragma unroll
@@ -113,15 +114,15 @@ __device__ __forceinline__ void add_piece(Sum<TOP>& s, const Span<T>& t, uint32_
         [&](long long at) { s.add((float)t.base[at], 0); });
 }
 
-// f(tensor, piece of it) over the workgroup's pieces, from the last to the first:
-// what the pass for the norm has read last may still be in the cache for the one
-// that clips, which runs the other way.
+// f(tensor, piece of it) over the pieces of one of `workers`; BACK: from the last to
+// the first, as what the pass for the norm has read last may still be in the cache
+// for the one that clips.
 template <bool BACK, class F>
-__device__ __forceinline__ void for_pieces(const GradTable& t, F&& f)
+__device__ __forceinline__ void for_pieces(const GradTable& t, uint32_t worker, uint32_t workers, F&& f)
 {
     const uint32_t pieces = t.end[t.count - 1];
-    const uint32_t p0 = (uint32_t)((uint64_t)pieces * blockIdx.x / gridDim.x);
-    const uint32_t p1 = (uint32_t)((uint64_t)pieces * (blockIdx.x + 1) / gridDim.x);
+    const uint32_t p0 = (uint32_t)((uint64_t)pieces * worker / workers);
+    const uint32_t p1 = (uint32_t)((uint64_t)pieces * (worker + 1) / workers);
     if (p0 == p1) return;
     const uint32_t start = BACK ? p1 - 1 : p0;
     int lo = 0, hi = t.count - 1;  // the first tensor that ends behind it
@@ -159,10 +160,12 @@ __device__ __forceinline__ double wave_sum(double v)
 }
 
 // Of a workgroup, in every thread: the sum or the largest.
-__device__ __forceinline__ double join(double v, int kind)
+template <int THREADS>
+__device__ __forceinline__ double join(double v, bool top)
 {
-    __shared__ double part[kGradWaves];
-    if (kind == GRAD_NORM_2) v = wave_sum(v);
+    constexpr int kWaves = THREADS / 64;
+    __shared__ double part[kWaves];
+    if (!top) v = wave_sum(v);
     else
         for (int o = 32; o > 0; o >>= 1) {
             const double u = __shfl_xor(v, o, 64);
@@ -172,51 +175,61 @@ __device__ __forceinline__ double join(double v, int kind)
     __syncthreads();
     v = part[0];
 #pragma unroll
-    for (int w = 1; w < kGradWaves; w++) v = kind == GRAD_NORM_2 ? v + part[w] : (part[w] > v ? part[w] : v);
-    __syncthreads();
+    for (int w = 1; w < kWaves; w++) v = !top ? v + part[w] : (part[w] > v ? part[w] : v);
     return v;
 }
 
 // Largest magnitudes travel as their bits: whole numbers, so that NaN are the largest.
+template <int THREADS, bool TOP>
+__device__ __forceinline__ double sum_of(const GradTable& t, uint32_t worker, uint32_t workers)
+{
+    Sum<TOP> s;
+    for_pieces<false>(t, worker, workers, [&](int i, uint32_t piece) {
+        with_type_of(t.type[i], [&](auto zero) { add_piece<THREADS>(s, Span<decltype(zero)>(t.data[i], t.n[i]), piece); });
+    });
+    return s.value();
+}
+
+__device__ __forceinline__ float norm_of_sum(const GradArgs& a, double v)
+{
+    const double n = a.top ? (double)__builtin_bit_cast(float, (uint32_t)v) : sqrt(v);
+    return (float)(n / (double)a.scale);
+}
+
 template <bool TOP>
 __global__ __launch_bounds__(kGradThreads) void grad_sum_kernel(GradTable t, GradArgs a)
 {
-    Sum<TOP> s;
-    for_pieces<false>(t, [&](int i, uint32_t piece) {
-        with_type_of(t.type[i], [&](auto zero) { add_piece(s, Span<decltype(zero)>(t.data[i], t.n[i]), piece); });
-    });
-    const double v = join(s.value(), a.kind);
+    const double v = join<kGradThreads>(sum_of<kGradThreads, TOP>(t, blockIdx.x, gridDim.x), TOP);
     if (threadIdx.x == 0) a.sums[blockIdx.x] = v;
 }
 
 // The norm from the workgroups' sums, in every thread of a workgroup.
-__device__ __forceinline__ float norm_of(const GradArgs& a)
+__device__ __forceinline__ float norm_of_sums(const GradArgs& a)
 {
     double v = 0.0;
     for (int i = threadIdx.x; i < a.num_sums; i += kGradThreads) {
         const double u = a.sums[i];
-        v = a.kind == GRAD_NORM_2 ? v + u : (u > v ? u : v);
+        v = !a.top ? v + u : (u > v ? u : v);
     }
-    v = join(v, a.kind);
-    const double n = a.kind == GRAD_NORM_2 ? sqrt(v) : (double)__builtin_bit_cast(float, (uint32_t)v);
-    return (float)(n / (double)a.scale);
+    return norm_of_sum(a, join<kGradThreads>(v, a.top));
 }
 
 __global__ __launch_bounds__(kGradThreads) void grad_norm_kernel(GradArgs a)
 {
-    const float n = norm_of(a);
+    const float n = norm_of_sums(a);
     if (threadIdx.x == 0) *a.norm_out = n;
 }
 
-template <class T>
+template <int THREADS, class T>
 __device__ __forceinline__ void clip_piece(const void* data, void* out, long long n, uint32_t piece, float factor, bool zero)
 {
     constexpr int N = Span<T>::N;
     const Span<T> t(data, n);
     T* const to = (T*)out - t.lo;
     auto scaled = [&](T v) { return zero ? (T)0.0f : (T)((float)v * factor); };
+    auto one = [&](long long at) { to[at] = scaled(t.base[at]); };
     if (((uintptr_t)to & 15) == 0) {
-        for_parts(
+        for_parts<THREADS>(
             t, piece,
             [&](long long at, Vec<T, N> v) {
                 if (factor != 1.0f || zero) {
@@ -225,35 +238,52 @@ __device__ __forceinline__ void clip_piece(const void* data, void* out, long lon
                 }
                 *reinterpret_cast<Vec<T, N>*>(to + at) = v;
             },
-            [&](long long at) { to[at] = scaled(t.base[at]); });
+            one);
     } else {  // an output that starts elsewhere in 16 bytes than its input: element by element
-        for_parts(
+        for_parts<THREADS>(
             t, piece,
             [&](long long at, Vec<T, N> v) {
 #pragma unroll
                 for (int j = 0; j < N; j++) to[at + j] = scaled(v[j]);
             },
-            [&](long long at) { to[at] = scaled(t.base[at]); });
+            one);
     }
+}
+
+template <int THREADS>
+__device__ __forceinline__ void clip_all(const GradTable& t, const GradArgs& a, float n, uint32_t worker, uint32_t workers)
+{
+    const bool finite = magnitude(n) < 0x7f800000u, zero = !finite && a.zero;
+    const float factor = finite && n > a.max_norm ? a.max_norm / n : 1.0f;
+    for_pieces<true>(t, worker, workers, [&](int i, uint32_t piece) {
+        void* const out = t.out[i];
+        if (out == t.data[i] && factor == 1.0f && !zero) return;
+        with_type_of(t.type[i], [&](auto z) { clip_piece<THREADS, decltype(z)>(t.data[i], out, t.n[i], piece, factor, zero); });
+    });
 }
 
 __global__ __launch_bounds__(kGradThreads) void grad_clip_kernel(GradTable t, GradArgs a)
 {
-    const float n = a.norm_in ? *a.norm_in : norm_of(a);
+    const float n = a.norm_in ? *a.norm_in : norm_of_sums(a);
     if (a.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *a.norm_out = n;
-    const bool finite = magnitude(n) < 0x7f800000u, zero = !finite && a.zero;
-    const float factor = finite && n > a.max_norm ? a.max_norm / n : 1.0f;
-    for_pieces<true>(t, [&](int i, uint32_t piece) {
-        void* const out = t.out[i];
-        if (out == t.data[i] && factor == 1.0f && !zero) return;
-        with_type_of(t.type[i], [&](auto z) { clip_piece<decltype(z)>(t.data[i], out, t.n[i], piece, factor, zero); });
-    });
+    clip_all<kGradThreads>(t, a, n, blockIdx.x, gridDim.x);
 }
 
-long long pieces_of(const GradTensor& t)
+// Few gradients: one workgroup does all of it, its waves with pieces of their own.
+template <bool TOP, bool CLIP>
+__global__ __launch_bounds__(kSmallThreads) void grad_small_kernel(GradTable t, GradArgs a)
+{
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = kSmallThreads / 64;
+    const double v = t.count ? sum_of<64, TOP>(t, wave, waves) : 0.0;
+    const float n = norm_of_sum(a, join<kSmallThreads>(v, TOP));
+    if (threadIdx.x == 0) *a.norm_out = n;
+    if (CLIP && t.count) clip_all<64>(t, a, n, wave, waves);
+}
+
+long long pieces_of(const GradTensor& t, int threads)
 {
     const long long bytes = ((uintptr_t)t.data & 15) + t.n * data_bytes(t.dataType);
-    return t.n ? (bytes + kPieceBytes - 1) / kPieceBytes : 0;
+    return t.n ? (bytes + piece_bytes(threads) - 1) / piece_bytes(threads) : 0;
 }
 
 void check_list(const GradTensor* tensors, int count)
@@ -307,55 +337,82 @@ void check_clip(const GradTensor* tensors, int count, float max_norm, int non_fi
 
 constexpr int kMostSums = 1024;
 
+void add_to(GradTable& t, const GradTensor& g, long long pieces)
+{
+    t.data[t.count] = g.data;
+    t.out[t.count] = g.out ? g.out : const_cast<void*>(g.data);
+    t.n[t.count] = g.n;
+    t.type[t.count] = (uint8_t)g.dataType;
+    t.end[t.count] = (uint32_t)pieces + (t.count ? t.end[t.count - 1] : 0u);
+    t.count++;
+}
+
 // f(table, workgroups) for the list in launches; all of them have kMostSums
-// workgroups at most but for one more a launch.
+// workgroups at most but for one more a launch.  The number of launches.
 template <class F>
-void in_tables(const GradTensor* tensors, int count, F&& f)
+int in_tables(const GradTensor* tensors, int count, F&& f)
 {
     long long all = 0;
-    for (int i = 0; i < count; i++) all += pieces_of(tensors[i]);
+    for (int i = 0; i < count; i++) all += pieces_of(tensors[i], kGradThreads);
     GradTable t;
     t.count = 0;
     long long pieces = 0;
+    int launches = 0;
     auto flush = [&] {
-        if (t.count) f(t, (unsigned)std::max(1ll, std::min(pieces, kMostSums * pieces / all)));
+        if (t.count) f(t, (unsigned)std::max(1ll, std::min(pieces, kMostSums * pieces / all))), launches++;
         t.count = 0;
         pieces = 0;
     };
     for (int i = 0; i < count; i++) {
-        const GradTensor& g = tensors[i];
-        const long long own = pieces_of(g);
+        const long long own = pieces_of(tensors[i], kGradThreads);
         if (own == 0) continue;
         if (t.count == kMostTensors || pieces + own >= 1ll << 31) flush();
-        t.data[t.count] = g.data;
-        t.out[t.count] = g.out ? g.out : const_cast<void*>(g.data);
-        t.n[t.count] = g.n;
-        t.type[t.count] = (uint8_t)g.dataType;
+        add_to(t, tensors[i], own);
         pieces += own;
-        t.end[t.count] = (uint32_t)pieces;
-        t.count++;
     }
     flush();
+    return launches;
 }
 
-// The workgroups' sums; their number.
+// The whole list in one workgroup's hands where it is short: up to kSmallPieces of a
+// wave.
+constexpr int kSmallPieces = 128;
+bool small_table(const GradTensor* tensors, int count, GradTable& t)
+{
+    t.count = 0;
+    long long pieces = 0;
+    for (int i = 0; i < count; i++) {
+        const long long own = pieces_of(tensors[i], 64);
+        if (own == 0) continue;
+        pieces += own;
+        if (pieces > kSmallPieces || t.count == kMostTensors) return false;
+        add_to(t, tensors[i], own);
+    }
+    return true;
+}
+
+// The workgroups' sums, in how many launches.
 int sums(const GradTensor* tensors, int count, GradArgs& a, hipStream_t s)
 {
     const size_t most = kMostSums + (size_t)count + 1;
     a.sums = (double*)stream_workspace(s).get(most * sizeof(double));
-    int n = 0;
-    in_tables(tensors, count, [&](const GradTable& t, unsigned wgs) {
+    return in_tables(tensors, count, [&](const GradTable& t, unsigned wgs) {
         GradArgs b = a;
-        b.sums += n;
-        if (a.kind == GRAD_NORM_2) grad_sum_kernel<false><<<wgs, kGradThreads, 0, s>>>(t, b);
-        else grad_sum_kernel<true><<<wgs, kGradThreads, 0, s>>>(t, b);
+        b.sums += a.num_sums;
+        if (a.top) grad_sum_kernel<true><<<wgs, kGradThreads, 0, s>>>(t, b);
+        else grad_sum_kernel<false><<<wgs, kGradThreads, 0, s>>>(t, b);
         GRAFT_LAUNCH_CHECK();
-        n += (int)wgs;
+        a.num_sums += (int)wgs;
     });
-    return n;
 }
 
-void clip(const GradTensor* tensors, int count, GradArgs a, hipStream_t s)
+void norm(const GradArgs& a, hipStream_t s)
+{
+    grad_norm_kernel<<<1, kGradThreads, 0, s>>>(a);
+    GRAFT_LAUNCH_CHECK();
+}
+
+void clip(const GradTensor* tensors, int count, const GradArgs& a, hipStream_t s)
 {
     in_tables(tensors, count, [&](const GradTable& t, unsigned wgs) {
         grad_clip_kernel<<<wgs, kGradThreads, 0, s>>>(t, a);
@@ -365,17 +422,23 @@ void clip(const GradTensor* tensors, int count, GradArgs a, hipStream_t s)
 
 }  // namespace
 
-void grad_norm(const GradTensor* tensors, int count, int norm, float scale, float* d_norm, hipStream_t s)
+void grad_norm(const GradTensor* tensors, int count, int norm_kind, float scale, float* d_norm, hipStream_t s)
 {
     check_list(tensors, count);
-    check_norm(norm, scale, d_norm);
+    check_norm(norm_kind, scale, d_norm);
     GradArgs a{};
-    a.kind = norm;
+    a.top = norm_kind == GRAD_NORM_MAX;
     a.scale = scale;
     a.norm_out = d_norm;
-    a.num_sums = sums(tensors, count, a, s);
-    grad_norm_kernel<<<1, kGradThreads, 0, s>>>(a);
-    GRAFT_LAUNCH_CHECK();
+    GradTable t;
+    if (small_table(tensors, count, t)) {
+        if (a.top) grad_small_kernel<true, false><<<1, kSmallThreads, 0, s>>>(t, a);
+        else grad_small_kernel<false, false><<<1, kSmallThreads, 0, s>>>(t, a);
+        GRAFT_LAUNCH_CHECK();
+        return;
+    }
+    sums(tensors, count, a, s);
+    norm(a, s);
 }
 
 void grad_clip(const GradTensor* tensors, int count, float max_norm, int non_finite, const float* d_norm, hipStream_t s)
@@ -390,14 +453,33 @@ void grad_clip(const GradTensor* tensors, int count, float max_norm, int non_fin
     clip(tensors, count, a, s);
 }
 
-void grad_norm_clip(const GradTensor* tensors, int count, int norm, float scale, float max_norm, int non_finite, float* d_norm,
-                    hipStream_t s)
+void grad_norm_clip(const GradTensor* tensors, int count, int norm_kind, float scale, float max_norm, int non_finite,
+                    float* d_norm, hipStream_t s)
 {
     check_list(tensors, count);
-    check_norm(norm, scale, d_norm);
+    check_norm(norm_kind, scale, d_norm);
     check_clip(tensors, count, max_norm, non_finite);
-    grad_norm(tensors, count, norm, scale, d_norm, s);
-    grad_clip(tensors, count, max_norm, non_finite, d_norm, s);
+    GradArgs a{};
+    a.top = norm_kind == GRAD_NORM_MAX;
+    a.scale = scale;
+    a.max_norm = max_norm;
+    a.zero = non_finite == GRAD_NONFINITE_ZERO;
+    a.norm_out = d_norm;
+    GradTable t;
+    if (small_table(tensors, count, t)) {
+        if (a.top) grad_small_kernel<true, true><<<1, kSmallThreads, 0, s>>>(t, a);
+        else grad_small_kernel<false, true><<<1, kSmallThreads, 0, s>>>(t, a);
+        GRAFT_LAUNCH_CHECK();
+        return;
+    }
+    // One launch's workgroups each form the norm from the sums; of several, a kernel
+    // of its own does.
+    if (sums(tensors, count, a, s) > 1) {
+        norm(a, s);
+        a.norm_in = d_norm;
+        a.norm_out = nullptr;
+    }
+    clip(tensors, count, a, s);
 }
 
 }  // namespace graft
