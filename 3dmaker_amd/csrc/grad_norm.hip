@@ -77,27 +77,39 @@ struct Sum {
     __device__ __forceinline__ double value() const { return TOP ? (double)top : (sq[0] + sq[1]) + (sq[2] + sq[3]); }
 };
 
-// f(first element) of the thread's 16-byte parts of a piece: whole ones by f, the
-// tensor's first and last by g(element) for each element of it.
+// f(first element, elements) of the thread's whole 16-byte parts of a piece, and
+// g(element, its place in the part, value) for the elements of the tensor's first and
+// last part, which are another's for the rest.  A part's loads are under way together.
 template <int THREADS, class T, class F, class G>
 __device__ __forceinline__ void for_parts(const Span<T>& t, uint32_t piece, F&& f, G&& g)
 {
     constexpr int N = Span<T>::N, kPer = 4, kElements = piece_bytes(THREADS) / (int)sizeof(T);
     const int thread = threadIdx.x & (THREADS - 1);
     const long long first = (long long)piece * kElements;
+    Vec<T, N> v[kPer];
     if (first >= t.lo && first + kElements <= t.hi) {
-        Vec<T, N> v[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; i++) v[i] = *reinterpret_cast<const Vec<T, N>*>(t.base + first + (i * THREADS + thread) * N);
 #pragma unroll
         for (int i = 0; i < kPer; i++) f(first + (i * THREADS + thread) * N, v[i]);
     } else {
+#pragma unroll
         for (int i = 0; i < kPer; i++) {
             const long long at = first + (i * THREADS + thread) * N;
-            if (at >= t.lo && at + N <= t.hi) f(at, *reinterpret_cast<const Vec<T, N>*>(t.base + at));
-            else
+            if (at >= t.lo && at + N <= t.hi) v[i] = *reinterpret_cast<const Vec<T, N>*>(t.base + at);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const long long at = first + (i * THREADS + thread) * N;
+            if (at >= t.lo && at + N <= t.hi) f(at, v[i]);
+            else if (at + N > t.lo && at < t.hi) {
+                T e[N];
+#pragma unroll
+                for (int j = 0; j < N; j++) e[j] = t.base[min(max(at + j, t.lo), t.hi - 1)];
+#pragma unroll
                 for (int j = 0; j < N; j++)
-                    if (at + j >= t.lo && at + j < t.hi) g(at + j);
+                    if (at + j >= t.lo && at + j < t.hi) g(at + j, j, e[j]);
+            }
         }
     }
 }
@@ -111,7 +123,7 @@ __device__ __forceinline__ void add_piece(Sum<TOP>& s, const Span<T>& t, uint32_
 #pragma unroll
             for (int j = 0; j < Span<T>::N; j++) s.add((float)v[j], j);
         },
-        [&](long long at) { s.add((float)t.base[at], 0); });
+        [&](long long, int j, T v) { s.add((float)v, j); });
 }
 
 // f(tensor, piece of it) over the pieces of one of `workers`; BACK: from the last to
@@ -125,12 +137,12 @@ __device__ __forceinline__ void for_pieces(const GradTable& t, uint32_t worker, 
     const uint32_t p1 = (uint32_t)((uint64_t)pieces * (worker + 1) / workers);
     if (p0 == p1) return;
     const uint32_t start = BACK ? p1 - 1 : p0;
-    int lo = 0, hi = t.count - 1;  // the first tensor that ends behind it
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (t.end[mid] > start) hi = mid;
-        else lo = mid + 1;
-    }
+    // The first tensor that ends behind it, found by all lanes at once: a search in
+    // steps waits for the kernel's arguments at each of them.
+    static_assert(kMostTensors <= 128, "two a lane");
+    const int lane = threadIdx.x & 63;
+    int lo = __popcll(__ballot(lane < t.count && t.end[lane] <= start));
+    lo += __popcll(__ballot(64 + lane < t.count && t.end[64 + lane] <= start));
     if (BACK) {
         for (uint32_t p = p1; p-- > p0;) {
             while (lo > 0 && p < t.end[lo - 1]) lo--;
@@ -227,7 +239,7 @@ __device__ __forceinline__ void clip_piece(const void* data, void* out, long lon
     const Span<T> t(data, n);
     T* const to = (T*)out - t.lo;
     auto scaled = [&](T v) { return zero ? (T)0.0f : (T)((float)v * factor); };
-    auto one = [&](long long at) { to[at] = scaled(t.base[at]); };
+    auto one = [&](long long at, int, T v) { to[at] = scaled(v); };
     if (((uintptr_t)to & 15) == 0) {
         for_parts<THREADS>(
             t, piece,
@@ -335,7 +347,7 @@ void check_clip(const GradTensor* tensors, int count, float max_norm, int non_fi
     }
 }
 
-constexpr int kMostSums = 1024;
+constexpr int kMostWorkgroups = 1024;  // of a launch
 
 void add_to(GradTable& t, const GradTensor& g, long long pieces)
 {
@@ -347,19 +359,16 @@ void add_to(GradTable& t, const GradTensor& g, long long pieces)
     t.count++;
 }
 
-// f(table, workgroups) for the list in launches; all of them have kMostSums
-// workgroups at most but for one more a launch.  The number of launches.
+// f(table, workgroups) for the list in launches.  Their number.
 template <class F>
 int in_tables(const GradTensor* tensors, int count, F&& f)
 {
-    long long all = 0;
-    for (int i = 0; i < count; i++) all += pieces_of(tensors[i], kGradThreads);
     GradTable t;
     t.count = 0;
     long long pieces = 0;
     int launches = 0;
     auto flush = [&] {
-        if (t.count) f(t, (unsigned)std::max(1ll, std::min(pieces, kMostSums * pieces / all))), launches++;
+        if (t.count) f(t, (unsigned)std::min<long long>(pieces, kMostWorkgroups)), launches++;
         t.count = 0;
         pieces = 0;
     };
@@ -376,7 +385,7 @@ int in_tables(const GradTensor* tensors, int count, F&& f)
 
 // The whole list in one workgroup's hands where it is short: up to kSmallPieces of a
 // wave.
-constexpr int kSmallPieces = 128;
+constexpr int kSmallPieces = 32;
 bool small_table(const GradTensor* tensors, int count, GradTable& t)
 {
     t.count = 0;
@@ -394,7 +403,8 @@ bool small_table(const GradTensor* tensors, int count, GradTable& t)
 // The workgroups' sums, in how many launches.
 int sums(const GradTensor* tensors, int count, GradArgs& a, hipStream_t s)
 {
-    const size_t most = kMostSums + (size_t)count + 1;
+    size_t most = 0;
+    in_tables(tensors, count, [&](const GradTable&, unsigned wgs) { most += wgs; });
     a.sums = (double*)stream_workspace(s).get(most * sizeof(double));
     return in_tables(tensors, count, [&](const GradTable& t, unsigned wgs) {
         GradArgs b = a;
