@@ -3,12 +3,16 @@
 //   y = sum_j w_j W2_{e_j} a_j
 // Bound by the weights' bytes: each selected expert's matrices are read once, for
 // all tokens that take it.  Weights are widened to bf16 with their scales, which is
-// exact, and go to v_mfma_f32_16x16x32_bf16 as 16 rows by 32 of k; tokens are its
-// 16 columns, few or many, at the same cost.  Tokens and a_j are split into as many
-// bf16 terms as they need (16-bit tokens are exact in one or two, fp32 ones in
-// three; a_j has two, 16 bits, or three under fp32 tokens), so that nothing is
-// rounded to 8 bits on the way.
+// exact, and go to v_mfma_f32_16x16x32_bf16 as 16 rows by 32 of k; an expert's slots
+// (a token's place for it) are its 16 columns, few or many, at the same cost.  Tokens
+// and a_j are split into as many bf16 terms as they need (16-bit tokens are exact in
+// one or two, fp32 ones in three; a_j has two, 16 bits, or three under fp32 tokens),
+// so that nothing is rounded to 8 bits on the way.
+//
+// Three launches: routing (the last workgroup to have its logits ready routes all
+// tokens), the hidden activations, the outputs.
 #include "product.h"
+#include "route_math.h"
 
 #include <algorithm>
 
@@ -17,6 +21,7 @@ namespace graft {
 namespace {
 
 constexpr int kLayerThreads = 512, kLayerWaves = kLayerThreads / 64;
+constexpr int kRouteThreads = 1024, kRouteWaves = kRouteThreads / 64;
 constexpr int kMaxTokens = EXPERT_LAYER_TOKENS;
 
 struct LayerArgs {
@@ -26,21 +31,23 @@ struct LayerArgs {
     void* out;
     long long stride_x, stride_out;
     int tokens, experts, topk, dim, hidden, activation;
-    bool gated, vec_x, vec_router, vec_out;
-    int scale_shift;  // rows of a scale, as a shift
+    int groups, kept, group_best;
+    float scale;
+    bool sigmoid, renorm, gated, vec_x, vec_router, vec_out;
+    int scale_shift;          // rows of a scale, as a shift
     int dim_pad, hidden_pad;  // filled up to whole blocks of 128
     // scratch
-    float *logits, *weights;  // [tokens][experts], [tokens][topk]
-    int *indices, *active;    // [tokens][topk]; number of experts that a token takes, and which
-    uint8_t* place;           // [active][kMaxTokens]: the token's place for that expert, or kNone
-    __bf16* acts;             // [tokens * topk][terms][hidden_pad]
+    float *logits, *weights;  // [tokens][experts], [slots]
+    int* active;              // number of experts that some token takes, and which
+    int *first, *slots;       // where their slots begin in the list of slots, and its end
+    __bf16 *xs, *acts;        // [tokens][terms][dim_pad], [slots][terms][hidden_pad]
+    float* parts;             // [parts][tokens][dim], of more than one part
+    uint32_t *route_ticket, *out_tickets;
 };
-
-constexpr int kNone = 255;
 
 template <class T>
 struct Terms {
-    static constexpr int kX = sizeof(T) == 4 ? 3 : std::is_same_v<T, __bf16> ? 1 : 2;  // of a token
+    static constexpr int kX = sizeof(T) == 4 ? 3 : std::is_same_v<T, __bf16> ? 1 : 2;  // of a token or a router's row
     static constexpr int kA = sizeof(T) == 4 ? 3 : 2;                                  // of a hidden activation
 };
 
@@ -82,67 +89,241 @@ __device__ __forceinline__ void load8(T (&v)[8], const T* p, int n, bool vec)
     }
 }
 
-// Logits of eight tokens and a wave's expert.
-constexpr int kRouterTokens = 8;
-template <class T, class R>
-__global__ __launch_bounds__(256) void layer_logits_kernel(LayerArgs a)
+template <class T, int N = Terms<T>::kX>
+__device__ __forceinline__ void split8(const T (&v)[8], bf16x8 (&t)[N])
 {
-    const int e = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, t0 = blockIdx.y * kRouterTokens;
-    if (e >= a.experts) return;
-    float acc[kRouterTokens];
 #pragma unroll
-    for (int t = 0; t < kRouterTokens; t++) acc[t] = 0.0f;
-    const R* r = (const R*)a.router + (long long)e * a.dim;
-    for (int d = lane * 8; d < a.dim; d += 512) {
-        R w[8];
-        load8(w, r + d, a.dim - d, a.vec_router);
+    for (int i = 0; i < 8; i++) {
+        __bf16 s[N];
+        if constexpr (N == 1) s[0] = v[i];
+        else split((float)v[i], s);
 #pragma unroll
-        for (int t = 0; t < kRouterTokens; t++) {
-            if (t0 + t >= a.tokens) break;
-            T x[8];
-            load8(x, (const T*)a.x + (t0 + t) * a.stride_x + d, a.dim - d, a.vec_x);
-#pragma unroll
-            for (int j = 0; j < 8; j++) acc[t] = fmaf((float)x[j], (float)w[j], acc[t]);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < kRouterTokens; t++) {
-        const float z = lanes_sum<64>(acc[t]);
-        if (lane == 0 && t0 + t < a.tokens) a.logits[(long long)(t0 + t) * a.experts + e] = z;
+        for (int u = 0; u < N; u++) t[u][i] = s[u];
     }
 }
 
-// The experts that some token takes, in their order, and the tokens' places for
-// them.  One workgroup.
-__global__ __launch_bounds__(256) void layer_plan_kernel(LayerArgs a)
+// ---------------------------------------------------------------------------
+// routing
+// ---------------------------------------------------------------------------
+
+// A token by a wave: lane l has experts PER l .. PER l + PER - 1, so that lane order
+// is index order.  scores, and keys with groups: LDS of the wave, one an expert.
+template <int PER>
+__device__ __forceinline__ void route_token(const LayerArgs& a, int t, float* scores, uint32_t* keys)
 {
-    __shared__ uint32_t taken[32];
-    __shared__ int before[32];
-    if (threadIdx.x < 32) taken[threadIdx.x] = 0;
-    __syncthreads();
+    const int lane = threadIdx.x & 63, first = lane * PER, n = a.experts - first;
+    float s[PER];
+    uint32_t key[PER];
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const float z = i < n ? a.logits[(long long)t * a.experts + first + i] : -INFINITY;
+        s[i] = z > -INFINITY ? fminf(z, 3.402823466e38f) : -INFINITY;  // NaN: none
+        top = fmaxf(top, s[i]);
+    }
+    float sum = 0.0f;
+    top = lanes_max<64>(top);
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        key[i] = s[i] > -INFINITY;
+        if (a.sigmoid) {
+            const float e = exp_neg(-fabsf(s[i])), r = __builtin_amdgcn_rcpf(1.0f + e);
+            s[i] = key[i] ? (s[i] >= 0.0f ? r : e * r) : 0.0f;
+        } else {
+            s[i] = key[i] ? exp_neg(s[i] - top) : 0.0f;
+            sum += s[i];
+        }
+    }
+    if (!a.sigmoid) {
+        sum = lanes_sum<64>(sum);
+        sum = sum > 0.0f ? 1.0f / sum : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        if (!a.sigmoid) s[i] *= sum;
+        const float c = s[i] + (a.bias && i < n ? a.bias[first + i] : 0.0f);
+        key[i] = key[i] && c > -INFINITY ? key_of(c) : 0u;
+        if (i < n) scores[first + i] = s[i];
+    }
+    if (a.groups > 1) {
+        const int size = a.experts / a.groups;
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (i < n) keys[first + i] = key[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        uint32_t b1 = 0, b2 = 0;  // lane g: the best two of group g
+        if (lane < a.groups)
+            for (int i = 0; i < size; i++) {
+                const uint32_t k = keys[lane * size + i];
+                b2 = max(b2, min(b1, k));
+                b1 = max(b1, k);
+            }
+        uint32_t g = b1;
+        if (a.group_best == 2 && b2 != 0) g = key_of(of_key(b1) + of_key(b2));
+        int ahead = 0;
+        for (int o = 0; o < a.groups; o++) {
+            const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)g, o);
+            ahead += k > g || (k == g && o < lane);
+        }
+        const uint64_t kept = __ballot(lane < a.groups && ahead < a.kept);
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (i < n && !(kept >> ((first + i) / size) & 1)) key[i] = 0;
+        __builtin_amdgcn_wave_barrier();
+    }
+    int mine = -1;  // lane j: the j-th pick
+#pragma unroll 1
+    for (int j = 0; j < a.topk; j++) {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < PER; i++) best = max(best, key[i]);
+        const uint32_t all = lanes_umax<64>(best);
+        if (all == 0) break;
+        const int l = __ffsll((unsigned long long)__ballot(best == all)) - 1;
+        int at = 0;
+#pragma unroll
+        for (int i = PER - 1; i >= 0; i--) at = key[i] == all ? i : at;
+#pragma unroll
+        for (int i = 0; i < PER; i++) key[i] = lane == l && i == at ? 0u : key[i];
+        const int e = __builtin_amdgcn_readlane(first + at, l);
+        mine = lane == j ? e : mine;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float score = mine >= 0 ? scores[mine] : 0.0f;
+    __builtin_amdgcn_wave_barrier();
+    if (a.renorm) {
+        const float total = lanes_sum<64>(score);
+        score *= a.scale / (total + 1e-20f);
+    } else score *= a.scale;
+    if (lane < a.topk) {
+        a.weights[t * a.topk + lane] = score;
+        a.slots[t * a.topk + lane] = mine;  // for now the slot's expert
+    }
+}
+
+// The experts that some token takes, in their order, and the list of their slots.
+__device__ __forceinline__ void plan(const LayerArgs& a, int* lds)
+{
+    int* const count = lds;              // [experts]: slots; then where the expert's next goes
+    int* const expert = lds + a.experts; // [slots]
     const int slots = a.tokens * a.topk;
-    for (int i = threadIdx.x; i < slots; i += 256) {
-        const int e = a.indices[i];
-        if ((unsigned)e < (unsigned)a.experts) atomicOr(&taken[e >> 5], 1u << (e & 31));
+    for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) count[e] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < slots; i += kRouteThreads) {
+        expert[i] = a.slots[i];
+        if (expert[i] >= 0) atomicAdd(&count[expert[i]], 1);
     }
     __syncthreads();
     if (threadIdx.x < 64) {
-        const int n = threadIdx.x < 32 ? __popc(taken[threadIdx.x]) : 0, up = lanes_scan(n);
-        if (threadIdx.x < 32) before[threadIdx.x] = up - n;
-        if (threadIdx.x == 63) a.active[0] = up;
+        int number = 0, begin = 0;
+        for (int e0 = 0; e0 < a.experts; e0 += 64) {
+            const int e = e0 + threadIdx.x, n = e < a.experts ? count[e] : 0;
+            const int upn = lanes_scan(n > 0), ups = lanes_scan(n);
+            if (n > 0) {
+                a.active[1 + number + upn - 1] = e;
+                a.first[number + upn - 1] = begin + ups - n;
+                count[e] = begin + ups - n;
+            }
+            number += __shfl(upn, 63);
+            begin += __shfl(ups, 63);
+        }
+        if (threadIdx.x == 0) a.active[0] = number, a.first[number] = begin;
     }
     __syncthreads();
-    auto number = [&](int e) { return before[e >> 5] + __popc(taken[e >> 5] & ((1u << (e & 31)) - 1)); };
-    const int count = before[31] + __popc(taken[31]);
-    for (int e = threadIdx.x; e < a.experts; e += 256)
-        if (taken[e >> 5] >> (e & 31) & 1) a.active[1 + number(e)] = e;
-    for (int i = threadIdx.x; i < count * (kMaxTokens / 4); i += 256) reinterpret_cast<uint32_t*>(a.place)[i] = 0xffffffffu;
-    __syncthreads();
-    for (int i = threadIdx.x; i < slots; i += 256) {
-        const int e = a.indices[i];
-        if ((unsigned)e < (unsigned)a.experts) a.place[number(e) * kMaxTokens + i / a.topk] = (uint8_t)(i % a.topk);
-    }
+    // an expert's slots in any order: each has a column of its own
+    for (int i = threadIdx.x; i < slots; i += kRouteThreads)
+        if (expert[i] >= 0) a.slots[atomicAdd(&count[expert[i]], 1)] = i;
 }
+
+// Logits of 16 experts, waves sharing out k; the tokens' terms on the way; routing
+// and plan by the workgroup that is last.  Products of terms are exact; those of
+// 2^-24 of a product and less are left out.
+template <class T, class R, int MT>
+__global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
+{
+    constexpr int X = Terms<T>::kX, Y = Terms<R>::kX;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ bool last;
+    f4* const sums = reinterpret_cast<f4*>(lds);  // [waves][MT][64]
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int col = lane & 15, quad = lane >> 4, e0 = blockIdx.x * 16;
+    const int blocks = a.dim_pad / 128;
+    f4 acc[MT];
+#pragma unroll
+    for (int j = 0; j < MT; j++) acc[j] = f4zero();
+    const R* r = (const R*)a.router + (long long)min(e0 + col, a.experts - 1) * a.dim;
+    for (int kb = wave; kb < blocks; kb += kRouteWaves) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int k = kb * 128 + quad * 32 + q * 8;
+            R v[8];
+            bf16x8 y[Y];
+            load8(v, r + k, a.dim - k, a.vec_router);
+            split8(v, y);
+#pragma unroll
+            for (int j = 0; j < MT; j++) {
+                const int t = j * 16 + col;
+                T u[8];
+                bf16x8 x[X];
+                load8(u, (const T*)a.x + min(t, a.tokens - 1) * a.stride_x + k, a.dim - k, a.vec_x);
+                split8(u, x);
+#pragma unroll
+                for (int m = 0; m < X; m++)
+#pragma unroll
+                    for (int n = 0; n < Y; n++)
+                        if (m + n < 3) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[n], x[m], acc[j], 0, 0, 0);
+                // each workgroup stores some blocks of the terms
+                if (kb % gridDim.x == blockIdx.x && t < a.tokens) {
+#pragma unroll
+                    for (int m = 0; m < X; m++)
+                        *reinterpret_cast<bf16x8*>(a.xs + ((long long)t * X + m) * a.dim_pad + k) = x[m];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < MT; j++) sums[(wave * MT + j) * 64 + lane] = acc[j];
+    __syncthreads();
+    if (wave < MT) {
+        f4 v = sums[wave * 64 + lane];
+        for (int w = 1; w < kRouteWaves; w++) v += sums[(w * MT + wave) * 64 + lane];
+        const int t = wave * 16 + col;
+        if (t < a.tokens) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (e0 + quad * 4 + i < a.experts) a.logits[(long long)t * a.experts + e0 + quad * 4 + i] = v[i];
+        }
+    }
+    __syncthreads();
+    if (gridDim.x > 1) {
+        if (threadIdx.x == 0) {
+            __threadfence();
+            last = atomicAdd(a.route_ticket, 1u) == gridDim.x - 1;
+        }
+        __syncthreads();
+        if (!last) return;
+        if (threadIdx.x == 0) *a.route_ticket = 0;
+        __threadfence();
+    }
+    if (a.out_tickets)
+        for (int i = threadIdx.x; i < (a.dim + 15) / 16; i += kRouteThreads) a.out_tickets[i] = 0;
+    float* const scores = reinterpret_cast<float*>(lds) + wave * a.experts;
+    uint32_t* const keys = reinterpret_cast<uint32_t*>(lds) + (kRouteWaves + wave) * a.experts;
+    for (int t = wave; t < a.tokens; t += kRouteWaves) {
+        if (a.experts <= 64) route_token<1>(a, t, scores, keys);
+        else if (a.experts <= 128) route_token<2>(a, t, scores, keys);
+        else if (a.experts <= 256) route_token<4>(a, t, scores, keys);
+        else route_token<16>(a, t, scores, keys);
+    }
+    __syncthreads();
+    plan(a, reinterpret_cast<int*>(lds));
+}
+
+// ---------------------------------------------------------------------------
+// the experts' products
+// ---------------------------------------------------------------------------
 
 // A lane's 32 of the 128 k of a row: those from 32 quad on, eight to a matrix
 // instruction.
@@ -211,161 +392,231 @@ __device__ __forceinline__ float activate(int kind, float v)
     }
 }
 
-// The hidden activations of 16 rows for all tokens of an active expert: waves share
-// out k.
-template <int FORMAT, class T, int MT>
+// The hidden activations of 16 NT rows for the slots of an active expert, 16 CT at a
+// time: waves share out k, and their sums are joined in LDS in wave order.  A lane
+// whose column has no slot works on the first one's for nothing.
+template <int FORMAT, class T, int G, int NT, int CT>
 __global__ __launch_bounds__(kLayerThreads) void layer_hidden_kernel(LayerArgs a)
 {
-    constexpr int X = Terms<T>::kX, A = Terms<T>::kA;
-    __shared__ f4 sums[kLayerWaves][2][MT][64];
-    __shared__ int slots[kMaxTokens];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int col = lane & 15, quad = lane >> 4, n0 = blockIdx.x * 16;
-    if ((int)blockIdx.y >= a.active[0]) return;
-    const int e = a.active[1 + blockIdx.y];
-    const int place = lane < a.tokens ? a.place[blockIdx.y * kMaxTokens + lane] : kNone;
-    const uint64_t mask = __ballot(place != kNone);
-    const int count = __popcll(mask);
-    if (wave == 0 && place != kNone) slots[__popcll(mask & ((1ull << lane) - 1))] = lane * a.topk + place;
-    __syncthreads();
-    const T* x[MT];
+    constexpr int X = Terms<T>::kX, A = Terms<T>::kA, F = G * NT;
+    __shared__ f4 sums[kLayerWaves][F][CT][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int col = lane & 15, quad = lane >> 4, n0 = blockIdx.x * 16 * NT, n = blockIdx.y;
+    if (n >= a.active[0]) return;
+    const int e = a.active[1 + n], first = a.first[n], count = a.first[n + 1] - first;
+    const uint8_t *W[F], *S[F];
 #pragma unroll
-    for (int j = 0; j < MT; j++)
-        x[j] = j * 16 + col < count ? (const T*)a.x + slots[j * 16 + col] / a.topk * a.stride_x + quad * 32 : nullptr;
-    const int rows = a.gated ? 2 * a.hidden : a.hidden, row = min(n0 + col, a.hidden - 1);
-    const uint8_t *W[2], *S[2];
-#pragma unroll
-    for (int g = 0; g < 2; g++) {
-        const int r = g && a.gated ? a.hidden + row : row;
-        W[g] = row_of<FORMAT>(a.w1, e, rows, a.dim_pad, r);
-        S[g] = scales_of<FORMAT>(a.s1, e, rows, a.dim_pad, r, a.scale_shift);
+    for (int f = 0; f < F; f++) {
+        const int row = min(n0 + f % NT * 16 + col, a.hidden - 1) + f / NT * a.hidden;
+        W[f] = row_of<FORMAT>(a.w1, e, G * a.hidden, a.dim_pad, row);
+        S[f] = scales_of<FORMAT>(a.s1, e, G * a.hidden, a.dim_pad, row, a.scale_shift);
     }
-    f4 acc[2][MT];
+    const int blocks = a.dim_pad / 128;
+    for (int s0 = 0; s0 < count; s0 += 16 * CT) {
+        int slot[CT];
+        const __bf16* x[CT];
+        f4 acc[F][CT];
 #pragma unroll
-    for (int j = 0; j < MT; j++) acc[0][j] = acc[1][j] = f4zero();
-    for (int kb = wave; kb < a.dim_pad / 128; kb += kLayerWaves) {
-        Piece<FORMAT> w[2];
-        w[0].load(W[0], S[0], kb, quad);
-        if (a.gated) w[1].load(W[1], S[1], kb, quad);
+        for (int j = 0; j < CT; j++) {
+            const int c = s0 + j * 16 + col;
+            slot[j] = c < count ? a.slots[first + c] : -1;
+            x[j] = a.xs + (long long)(max(slot[j], 0) / a.topk) * X * a.dim_pad + quad * 32;
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            bf16x8 t[MT][X];
+            for (int f = 0; f < F; f++) acc[f][j] = f4zero();
+        }
+        auto load = [&](Piece<FORMAT>(&w)[F], int kb) {
 #pragma unroll
-            for (int j = 0; j < MT; j++) {
-                T v[8];
-                if (x[j]) load8(v, x[j] + kb * 128 + q * 8, a.dim - (kb * 128 + quad * 32 + q * 8), a.vec_x);
-                else {
+            for (int f = 0; f < F; f++) w[f].load(W[f], S[f], kb, quad);
+        };
+        auto work = [&](const Piece<FORMAT>(&w)[F], int kb) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = (T)0.0f;
-                }
+            for (int q = 0; q < 4; q++) {
+                bf16x8 t[CT][X];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    __bf16 s[X];
-                    if constexpr (X == 1) s[0] = v[i];
-                    else split((float)v[i], s);
+                for (int j = 0; j < CT; j++)
 #pragma unroll
-                    for (int u = 0; u < X; u++) t[j][u][i] = s[u];
+                    for (int u = 0; u < X; u++)
+                        t[j][u] = *reinterpret_cast<const bf16x8*>(x[j] + (long long)u * a.dim_pad + kb * 128 + q * 8);
+#pragma unroll
+                for (int f = 0; f < F; f++) {
+                    const bf16x8 b = w[f](q);
+#pragma unroll
+                    for (int j = 0; j < CT; j++)
+#pragma unroll
+                        for (int u = 0; u < X; u++)
+                            acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, t[j][u], acc[f][j], 0, 0, 0);
                 }
             }
+        };
+        Piece<FORMAT> w0[F], w1[F];
+        int kb = wave;
+        if (kb < blocks) load(w0, kb);
+        while (kb < blocks) {
+            if (kb + waves < blocks) load(w1, kb + waves);
+            work(w0, kb);
+            kb += waves;
+            if (kb >= blocks) break;
+            if (kb + waves < blocks) load(w0, kb + waves);
+            work(w1, kb);
+            kb += waves;
+        }
+        if (s0 > 0) __syncthreads();
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
-                if (g && !a.gated) break;
-                const bf16x8 b = w[g](q);
+        for (int f = 0; f < F; f++)
 #pragma unroll
-                for (int j = 0; j < MT; j++) {
-                    if (j * 16 >= count) break;
+            for (int j = 0; j < CT; j++) sums[wave][f][j][lane] = acc[f][j];
+        __syncthreads();
 #pragma unroll
-                    for (int u = 0; u < X; u++) acc[g][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, t[j][u], acc[g][j], 0, 0, 0);
+        for (int f = 0; f < NT; f++)
+#pragma unroll
+            for (int j = 0; j < CT; j++) {
+                if ((f * CT + j) % waves != wave || slot[j] < 0) continue;
+                f4 v = sums[0][f][j][lane], u = f4zero();
+                for (int w = 1; w < waves; w++) v += sums[w][f][j][lane];
+                if (G == 2)
+                    for (int w = 0; w < waves; w++) u += sums[w][F - NT + f][j][lane];
+                const int row = n0 + f * 16 + quad * 4;
+                Vec<__bf16, 4> o[A];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float h = activate(a.activation, v[i]);
+                    if (G == 2) h *= u[i];
+                    if (row + i >= a.hidden) h = 0.0f;
+                    __bf16 s[A];
+                    split(h, s);
+#pragma unroll
+                    for (int t = 0; t < A; t++) o[t][i] = s[t];
                 }
+                __bf16* to = a.acts + (long long)slot[j] * A * a.hidden_pad + row;
+#pragma unroll
+                for (int t = 0; t < A; t++) *reinterpret_cast<Vec<__bf16, 4>*>(to + (long long)t * a.hidden_pad) = o[t];
             }
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < MT; j++) sums[wave][0][j][lane] = acc[0][j], sums[wave][1][j][lane] = acc[1][j];
-    __syncthreads();
-    for (int j = wave; j < MT; j += kLayerWaves) {
-        if (j * 16 + col >= count) continue;
-        f4 v = sums[0][0][j][lane], u = sums[0][1][j][lane];
-        for (int w = 1; w < kLayerWaves; w++) v += sums[w][0][j][lane], u += sums[w][1][j][lane];
-        Vec<__bf16, 4> o[A];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float h = activate(a.activation, v[i]);
-            if (a.gated) h *= u[i];
-            if (n0 + quad * 4 + i >= a.hidden) h = 0.0f;
-            __bf16 s[A];
-            split(h, s);
-#pragma unroll
-            for (int t = 0; t < A; t++) o[t][i] = s[t];
-        }
-        __bf16* to = a.acts + (long long)slots[j * 16 + col] * A * a.hidden_pad + n0 + quad * 4;
-#pragma unroll
-        for (int t = 0; t < A; t++) *reinterpret_cast<Vec<__bf16, 4>*>(to + (long long)t * a.hidden_pad) = o[t];
     }
 }
 
-// 16 columns of the outputs for all tokens: waves share out the active experts' k.
-// An expert's sums are kept apart, so that its NaN reach its own tokens alone.
-template <int FORMAT, class T, int MT>
+// 16 NT columns of the outputs for all tokens, and a part of the active experts' k:
+// its waves share that out in runs of one expert's, whose sums go, weighted, to the
+// tokens' in LDS.  Where k is in more than one part, the last workgroup of a tile
+// joins them in their order.
+template <int FORMAT, class T, int NT, int CT>
 __global__ __launch_bounds__(kLayerThreads) void layer_out_kernel(LayerArgs a)
 {
     constexpr int A = Terms<T>::kA;
-    __shared__ f4 sums[kLayerWaves][MT][64];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int col = lane & 15, quad = lane >> 4, d0 = blockIdx.x * 16;
-    const int blocks = a.hidden_pad / 128, items = a.active[0] * blocks;  // at most 2^10 * 2^7
-    const int first = items * wave / kLayerWaves, last = items * (wave + 1) / kLayerWaves;
-    const int row = min(d0 + col, a.dim - 1);
-    f4 acc[MT], own[MT];
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ bool last;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int col = lane & 15, quad = lane >> 4, d0 = blockIdx.x * 16 * NT;
+    const int slots = a.tokens * a.topk, most = min(a.experts, slots);
+    f4* const sums = reinterpret_cast<f4*>(lds);  // [waves][tokens][4 NT]
+    int* const active = reinterpret_cast<int*>(sums + waves * a.tokens * 4 * NT);
+    int *const first = active + most, *const list = first + most + 1;
+    const int number = a.active[0];
+    for (int i = threadIdx.x; i < number; i += blockDim.x) active[i] = a.active[1 + i];
+    for (int i = threadIdx.x; i <= number; i += blockDim.x) first[i] = a.first[i];
+    for (int i = threadIdx.x; i < slots; i += blockDim.x) list[i] = a.slots[i];
+    for (int i = threadIdx.x; i < waves * a.tokens * 4 * NT; i += blockDim.x) sums[i] = f4zero();
+    __syncthreads();
+    const int blocks = a.hidden_pad / 128, items = number * blocks;  // at most 2^10 * 2^7
+    const int workers = waves * gridDim.y, worker = blockIdx.y * waves + wave;
+    const int begin = (int)((long long)items * worker / workers), end = (int)((long long)items * (worker + 1) / workers);
+    int row[NT];
 #pragma unroll
-    for (int j = 0; j < MT; j++) acc[j] = f4zero();
-    for (int n = first / blocks; n * blocks < last; n++) {
-        const int e = a.active[1 + n];
-        const __bf16* act[MT];
-        float weight[MT];
-        bool some[MT];
+    for (int f = 0; f < NT; f++) row[f] = min(d0 + f * 16 + col, a.dim - 1);
+
+    // Where the wave is: block kb of up to `to` of expert `at`, for its slots from s0 on.
+    struct Cursor {
+        int at, kb, from, to, s0;
+    };
+    auto enter = [&](int n) {
+        Cursor c{n, 0, max(begin - n * blocks, 0), min(end - n * blocks, blocks), 0};
+        c.kb = c.from;
+        return c;
+    };
+    auto after = [&](Cursor c) {  // past the end: to <= from
+        if (c.kb + 1 < c.to) c.kb++;
+        else if (c.s0 + 16 * CT < __builtin_amdgcn_readfirstlane(first[c.at + 1] - first[c.at])) c.s0 += 16 * CT, c.kb = c.from;
+        else if ((c.at + 1) * blocks < end) c = enter(c.at + 1);
+        else c.to = c.from;
+        return c;
+    };
+    auto load = [&](Piece<FORMAT>(&w)[NT], const Cursor& c) {
+        const int e = __builtin_amdgcn_readfirstlane(active[c.at]);
 #pragma unroll
-        for (int j = 0; j < MT; j++) {
-            const int t = j * 16 + col, place = t < a.tokens ? a.place[n * kMaxTokens + t] : kNone;
-            const int slot = t * a.topk + place;
-            act[j] = place != kNone ? a.acts + (long long)slot * A * a.hidden_pad + quad * 32 : nullptr;
-            weight[j] = place != kNone ? a.weights[slot] : 0.0f;
-            some[j] = __ballot(place != kNone) != 0;
-            own[j] = f4zero();
+        for (int f = 0; f < NT; f++)
+            w[f].load(row_of<FORMAT>(a.w2, e, a.dim, a.hidden_pad, row[f]),
+                      scales_of<FORMAT>(a.s2, e, a.dim, a.hidden_pad, row[f], a.scale_shift), c.kb, quad);
+    };
+    f4 own[NT][CT];
+    int slot[CT];
+    const __bf16* act[CT];
+    auto start = [&](const Cursor& c) {
+        const int f0 = first[c.at], count = first[c.at + 1] - f0;
+#pragma unroll
+        for (int j = 0; j < CT; j++) {
+            const int i = c.s0 + j * 16 + col;
+            slot[j] = i < count ? list[f0 + i] : -1;
+            act[j] = a.acts + (long long)(slot[j] >= 0 ? slot[j] : list[f0]) * A * a.hidden_pad + quad * 32;
+#pragma unroll
+            for (int f = 0; f < NT; f++) own[f][j] = f4zero();
         }
-        const uint8_t* W = row_of<FORMAT>(a.w2, e, a.dim, a.hidden_pad, row);
-        const uint8_t* S = scales_of<FORMAT>(a.s2, e, a.dim, a.hidden_pad, row, a.scale_shift);
-        for (int kb = max(first - n * blocks, 0); kb < min(last - n * blocks, blocks); kb++) {
-            Piece<FORMAT> w;
-            w.load(W, S, kb, quad);
+    };
+    auto finish_run = [&] {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const bf16x8 b = w(q);
+        for (int j = 0; j < CT; j++) {
+            if (slot[j] < 0) continue;
+            const float w = a.weights[slot[j]];
+            f4* to = sums + (wave * a.tokens + slot[j] / a.topk) * 4 * NT + quad;
 #pragma unroll
-                for (int j = 0; j < MT; j++) {
-                    if (!some[j]) continue;
+            for (int f = 0; f < NT; f++) {
+                f4 v = to[f * 4];
 #pragma unroll
-                    for (int u = 0; u < A; u++) {
-                        bf16x8 t{};
-                        if (act[j]) t = *reinterpret_cast<const bf16x8*>(act[j] + (long long)u * a.hidden_pad + kb * 128 + q * 8);
-                        own[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, t, own[j], 0, 0, 0);
-                    }
-                }
+                for (int i = 0; i < 4; i++) v[i] = fmaf(w, own[f][j][i], v[i]);
+                to[f * 4] = v;
             }
         }
+    };
+    auto work = [&](const Piece<FORMAT>(&w)[NT], int kb) {
 #pragma unroll
-        for (int j = 0; j < MT; j++)
+        for (int q = 0; q < 4; q++) {
+            bf16x8 t[CT][A];
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[j][i] = act[j] ? fmaf(weight[j], own[j][i], acc[j][i]) : acc[j][i];
+            for (int j = 0; j < CT; j++)
+#pragma unroll
+                for (int u = 0; u < A; u++)
+                    t[j][u] = *reinterpret_cast<const bf16x8*>(act[j] + (long long)u * a.hidden_pad + kb * 128 + q * 8);
+#pragma unroll
+            for (int f = 0; f < NT; f++) {
+                const bf16x8 b = w[f](q);
+#pragma unroll
+                for (int j = 0; j < CT; j++)
+#pragma unroll
+                    for (int u = 0; u < A; u++)
+                        own[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, t[j][u], own[f][j], 0, 0, 0);
+            }
+        }
+    };
+    if (begin < end) {
+        Cursor c = enter(begin / blocks);
+        Piece<FORMAT> w0[NT], w1[NT];
+        load(w0, c);
+        start(c);
+        auto step = [&](Piece<FORMAT>(&w)[NT], Piece<FORMAT>(&ahead)[NT]) {
+            const Cursor d = after(c);
+            const bool more = d.to > d.from;
+            if (more) load(ahead, d);
+            work(w, c.kb);
+            if (!more || d.at != c.at || d.s0 != c.s0) {
+                finish_run();
+                if (more) start(d);
+            }
+            c = d;
+            return more;
+        };
+        while (step(w0, w1) && step(w1, w0)) {}
     }
-#pragma unroll
-    for (int j = 0; j < MT; j++) sums[wave][j][lane] = acc[j];
     __syncthreads();
-    for (int j = wave; j < MT; j += kLayerWaves) {
-        f4 v = sums[0][j][lane];
-        for (int w = 1; w < kLayerWaves; w++) v += sums[w][j][lane];
-        const int t = j * 16 + col, d = d0 + quad * 4;
-        if (t >= a.tokens) continue;
+    // Of token t, columns d .. d + 3.
+    auto store = [&](int t, int d, f4 v) {
         T* to = (T*)a.out + t * a.stride_out + d;
         if (a.vec_out && d + 4 <= a.dim) {
             Vec<T, 4> o;
@@ -377,17 +628,97 @@ __global__ __launch_bounds__(kLayerThreads) void layer_out_kernel(LayerArgs a)
             for (int i = 0; i < 4; i++)
                 if (d + i < a.dim) to[i] = (T)v[i];
         }
+    };
+    const int pieces = a.tokens * 4 * NT;
+    const long long plane = (long long)gridDim.x * pieces;
+    f4* const parts = reinterpret_cast<f4*>(a.parts) + (long long)blockIdx.x * pieces;
+    for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+        f4 v = sums[i];
+        for (int w = 1; w < waves; w++) v += sums[w * pieces + i];
+        if (gridDim.y == 1) store(i / (4 * NT), d0 + i % (4 * NT) * 4, v);
+        else parts[blockIdx.y * plane + i] = v;
+    }
+    if (gridDim.y == 1) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(a.out_tickets + blockIdx.x, 1u) == gridDim.y - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
+        f4 v = parts[i];
+        for (unsigned p = 1; p < gridDim.y; p++) v += parts[p * plane + i];
+        store(i / (4 * NT), d0 + i % (4 * NT) * 4, v);
     }
 }
 
-template <int FORMAT, class T, int MT>
-void layer_launch(const LayerArgs& a, hipStream_t s)
+// What a call launches, by its sizes.
+struct LayerPlan {
+    bool many;       // several slots an expert
+    int hidden_waves, out_tiles, out_parts, out_waves;
+};
+
+LayerPlan layer_plan(const LayerArgs& a)
+{
+    LayerPlan p{};
+    const int slots = a.tokens * a.topk, experts = std::min(a.experts, slots);
+    p.many = slots >= 4 * experts;
+    p.hidden_waves = std::min(kLayerWaves, a.dim_pad / 128);
+    const int nt = p.many ? 2 : 1, items = experts * (a.hidden_pad / 128);
+    p.out_tiles = (a.dim + 16 * nt - 1) / (16 * nt);
+    p.out_waves = std::min(kLayerWaves, items);
+    p.out_parts = std::max(1, std::min((2 * num_cus() + p.out_tiles - 1) / p.out_tiles, items / (4 * kLayerWaves)));
+    return p;
+}
+
+// More dynamic LDS than any kernel may have has to be asked for.
+void allow_lds(const void* kernel, size_t lds)
+{
+    if (lds > 64 * 1024) GRAFT_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+}
+
+template <int FORMAT, class T, int G, int NT, int CT>
+void hidden_launch(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
     const unsigned most = (unsigned)std::min(a.experts, a.tokens * a.topk);
-    layer_hidden_kernel<FORMAT, T, MT><<<dim3(a.hidden_pad / 16, most), kLayerThreads, 0, s>>>(a);
+    layer_hidden_kernel<FORMAT, T, G, NT, CT><<<dim3(a.hidden_pad / (16 * NT), most), p.hidden_waves * 64, 0, s>>>(a);
     GRAFT_LAUNCH_CHECK();
-    layer_out_kernel<FORMAT, T, MT><<<(a.dim + 15) / 16, kLayerThreads, 0, s>>>(a);
+}
+
+template <int FORMAT, class T, int NT, int CT>
+void out_launch(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
+{
+    const int slots = a.tokens * a.topk, most = std::min(a.experts, slots);
+    const size_t lds = (size_t)p.out_waves * a.tokens * 64 * NT + (size_t)(2 * most + 1 + slots) * 4;
+    allow_lds((const void*)layer_out_kernel<FORMAT, T, NT, CT>, lds);
+    layer_out_kernel<FORMAT, T, NT, CT><<<dim3(p.out_tiles, p.out_parts), p.out_waves * 64, lds, s>>>(a);
     GRAFT_LAUNCH_CHECK();
+}
+
+template <class T, class R, int MT>
+void route_launch(const LayerArgs& a, hipStream_t s)
+{
+    const size_t scores = (size_t)kRouteWaves * a.experts * 4 * (a.groups > 1 ? 2 : 1);
+    const size_t lds = std::max({(size_t)kRouteWaves * MT * 1024, scores, (size_t)(a.experts + a.tokens * a.topk) * 4});
+    allow_lds((const void*)layer_route_kernel<T, R, MT>, lds);
+    layer_route_kernel<T, R, MT><<<(a.experts + 15) / 16, kRouteThreads, lds, s>>>(a);
+    GRAFT_LAUNCH_CHECK();
+}
+
+template <int FORMAT, class T>
+void products(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
+{
+    if (p.many) {
+        if (a.gated) hidden_launch<FORMAT, T, 2, 2, 2>(a, p, s);
+        else hidden_launch<FORMAT, T, 1, 4, 2>(a, p, s);
+        out_launch<FORMAT, T, 2, 2>(a, p, s);
+    } else {
+        if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1>(a, p, s);
+        else hidden_launch<FORMAT, T, 1, 1, 1>(a, p, s);
+        out_launch<FORMAT, T, 1, 1>(a, p, s);
+    }
 }
 
 }  // namespace
@@ -426,6 +757,12 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     a.dim = o.dim;
     a.hidden = o.hidden;
     a.activation = o.activation;
+    a.groups = o.route.numGroups;
+    a.kept = o.route.topGroups;
+    a.group_best = o.route.groupScore;
+    a.scale = o.route.scale;
+    a.sigmoid = o.route.scoreType == ROUTE_SIGMOID;
+    a.renorm = o.route.renormalize != 0;
     a.gated = o.gated != 0;
     const int bytes = data_bytes(o.dataType);
     a.vec_x = aligned16(t.x) && o.strideX * bytes % 16 == 0;
@@ -434,6 +771,7 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     a.scale_shift = o.scaleRows == 128 ? 7 : 0;
     a.dim_pad = round_up(o.dim, 128);
     a.hidden_pad = round_up(o.hidden, 128);
+    const LayerPlan p = layer_plan(a);
     const int slots = tokens * a.topk, most = std::min(a.experts, slots);
     size_t size = 0;
     auto take = [&](size_t n) {
@@ -441,35 +779,34 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
         size += round_up<size_t>(n, 256);
         return at;
     };
+    const size_t x_terms = o.dataType == DATA_F32 ? 3 : o.dataType == DATA_BF16 ? 1 : 2, a_terms = o.dataType == DATA_F32 ? 3 : 2;
     const size_t at_logits = take((size_t)tokens * a.experts * 4), at_weights = take((size_t)slots * 4);
-    const size_t at_indices = take((size_t)slots * 4), at_active = take((size_t)(most + 1) * 4);
-    const size_t at_place = take((size_t)most * kMaxTokens);
-    const size_t at_acts = take((size_t)slots * (o.dataType == DATA_F32 ? 3 : 2) * a.hidden_pad * 2);
+    const size_t at_active = take((size_t)(most + 1) * 4), at_first = take((size_t)(most + 1) * 4), at_slots = take((size_t)slots * 4);
+    const size_t at_xs = take((size_t)tokens * x_terms * a.dim_pad * 2), at_acts = take((size_t)slots * a_terms * a.hidden_pad * 2);
+    const bool split = p.out_parts > 1;
+    const size_t at_parts = take(split ? (size_t)p.out_parts * p.out_tiles * tokens * (p.many ? 32 : 16) * 4 : 0);
+    const size_t at_tickets = take(split ? (size_t)(o.dim + 15) / 16 * 4 : 0);
+    a.route_ticket = stream_tickets(s);
     char* ws = (char*)stream_workspace(s).get(size);
     a.logits = (float*)(ws + at_logits);
     a.weights = (float*)(ws + at_weights);
-    a.indices = (int*)(ws + at_indices);
     a.active = (int*)(ws + at_active);
-    a.place = (uint8_t*)(ws + at_place);
+    a.first = (int*)(ws + at_first);
+    a.slots = (int*)(ws + at_slots);
+    a.xs = (__bf16*)(ws + at_xs);
     a.acts = (__bf16*)(ws + at_acts);
+    if (split) {
+        a.parts = (float*)(ws + at_parts);
+        a.out_tickets = (uint32_t*)(ws + at_tickets);
+    }
     with_type(o.dataType, [&](auto x) {
         using T = decltype(x);
         with_type(o.routerType, [&](auto r) {
-            layer_logits_kernel<T, decltype(r)>
-                <<<dim3((a.experts + 3) / 4, (tokens + kRouterTokens - 1) / kRouterTokens), 256, 0, s>>>(a);
+            if (tokens <= 16) route_launch<T, decltype(r), 1>(a, s);
+            else route_launch<T, decltype(r), 4>(a, s);
         });
-        GRAFT_LAUNCH_CHECK();
-        route_experts(o.route, a.logits, a.experts, a.bias, a.indices, a.weights, tokens, s);
-        layer_plan_kernel<<<1, 256, 0, s>>>(a);
-        GRAFT_LAUNCH_CHECK();
-        auto with_tiles = [&](auto F) {
-            constexpr int format = decltype(F)::value;
-            if (tokens <= 16) layer_launch<format, T, 1>(a, s);
-            else if (tokens <= 32) layer_launch<format, T, 2>(a, s);
-            else layer_launch<format, T, 4>(a, s);
-        };
-        if (o.weightFormat == EXPERT_FP8) with_tiles(std::integral_constant<int, EXPERT_FP8>{});
-        else with_tiles(std::integral_constant<int, EXPERT_FP4>{});
+        if (o.weightFormat == EXPERT_FP8) products<EXPERT_FP8, T>(a, p, s);
+        else products<EXPERT_FP4, T>(a, p, s);
     });
 }
 

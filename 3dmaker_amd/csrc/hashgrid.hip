@@ -435,6 +435,52 @@ Workspace& stream_workspace(hipStream_t s)
     return *w;
 }
 
+namespace {
+
+__global__ void zero_tickets_kernel(uint32_t* t) { t[threadIdx.x] = 0; }
+
+struct Tickets {
+    uint32_t* p = nullptr;
+    Tickets() = default;
+    Tickets(const Tickets&) = delete;
+    Tickets& operator=(const Tickets&) = delete;
+    ~Tickets()
+    {
+        if (p) (void)hipFree(p);
+    }
+    uint32_t* get(hipStream_t s)
+    {
+        if (!p) {
+            hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+            if (hipStreamIsCapturing(s, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
+                (void)hipGetLastError();
+                throw std::runtime_error("the first call of this kind on a stream cannot be captured: make one before");
+            }
+            uint32_t* fresh = nullptr;
+            GRAFT_HIP_CHECK(hipMalloc(&fresh, kStreamTickets * sizeof(uint32_t)));
+            p = fresh;
+            hipLaunchKernelGGL(zero_tickets_kernel, dim3(1), dim3(kStreamTickets), 0, s, p);
+            GRAFT_LAUNCH_CHECK();
+        }
+        return p;
+    }
+};
+
+}  // namespace
+
+uint32_t* stream_tickets(hipStream_t s)
+{
+    int dev = 0;
+    GRAFT_HIP_CHECK(hipGetDevice(&dev));
+    if (s == hipStreamPerThread) {
+        thread_local std::map<int, Tickets> own;
+        return own[dev].get(s);
+    }
+    std::lock_guard<std::mutex> lk(g_ws_mu);
+    static auto* all = new std::map<std::pair<int, hipStream_t>, Tickets>();  // outlives static destructors
+    return (*all)[{dev, s}].get(s);
+}
+
 int num_cus()
 {
     if (g_cus == 0) {
