@@ -20,7 +20,6 @@ namespace graft {
 
 namespace {
 
-constexpr int kLayerThreads = 512, kLayerWaves = kLayerThreads / 64;
 constexpr int kRouteThreads = 1024, kRouteWaves = kRouteThreads / 64;
 constexpr int kMaxTokens = EXPERT_LAYER_TOKENS;
 
@@ -37,12 +36,11 @@ struct LayerArgs {
     int scale_shift;          // rows of a scale, as a shift
     int dim_pad, hidden_pad;  // filled up to whole blocks of 128
     // scratch
-    float *logits, *weights;  // [tokens][experts], [slots]
+    float *logits, *weights;  // [parts][tokens][experts], [slots]
     int* active;              // number of experts that some token takes, and which
     int *first, *slots;       // where their slots begin in the list of slots, and its end
     __bf16 *xs, *acts;        // [tokens][terms][dim_pad], [slots][terms][hidden_pad]
-    float* parts;             // [parts][tokens][dim], of more than one part
-    uint32_t *route_ticket, *out_tickets;
+    uint32_t* route_ticket;
 };
 
 template <class T>
@@ -52,21 +50,15 @@ struct Terms {
 };
 
 // v as N bf16 numbers: the first N - 1 cut, so that what is left over is exact, the
-// last rounded.  Infinities and NaN are the first alone.
+// last rounded.  An infinity is the first alone, a NaN also the last.
 template <int N>
 __device__ __forceinline__ void split(float v, __bf16 (&t)[N])
 {
 #pragma unroll
     for (int i = 0; i < N - 1; i++) {
-        const uint32_t bits = __builtin_bit_cast(uint32_t, v);
-        if ((bits & 0x7f800000u) == 0x7f800000u) {
-            t[i] = (__bf16)v;
-            v = 0.0f;
-        } else {
-            const float cut = __builtin_bit_cast(float, bits & 0xffff0000u);
-            t[i] = (__bf16)cut;
-            v -= cut;
-        }
+        const float cut = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);
+        t[i] = (__bf16)cut;
+        v = __builtin_isinf(v) ? 0.0f : v - cut;
     }
     t[N - 1] = (__bf16)v;
 }
@@ -106,117 +98,149 @@ __device__ __forceinline__ void split8(const T (&v)[8], bf16x8 (&t)[N])
 // routing
 // ---------------------------------------------------------------------------
 
-// A token by a wave: lane l has experts PER l .. PER l + PER - 1, so that lane order
-// is index order.  scores, and keys with groups: LDS of the wave, one an expert.
-template <int PER>
-__device__ __forceinline__ void route_token(const LayerArgs& a, int t, float* scores, uint32_t* keys)
+// Tokens by LANES lanes of a wave, lane l of them with experts PER l .. PER l + PER - 1,
+// so that lane order is index order.  Logits are in LDS or the sum of `parts` in
+// memory; scores, and with groups keys, are LDS for PER experts of each thread, and
+// group_keys of one.  Bound by instructions: some 400 a wave and round, on one CU.
+template <int LANES, int PER>
+__device__ __forceinline__ void route_tokens(const LayerArgs& a, const float* logits, int parts, float* lds, int* expert)
 {
-    const int lane = threadIdx.x & 63, first = lane * PER, n = a.experts - first;
-    float s[PER];
-    uint32_t key[PER];
-    float top = -INFINITY;
+    const int threads = blockDim.x, lane = threadIdx.x & 63, sub = lane & (LANES - 1), local = threadIdx.x / LANES;
+    const int first = sub * PER, n = a.experts - first, size = a.experts / a.groups;
+    const uint64_t lanes = (LANES == 64 ? ~0ull : ((1ull << (LANES & 63)) - 1)) << (lane - sub);  // the token's
+    float* const scores = lds + local * (LANES * PER);
+    uint32_t* const keys = reinterpret_cast<uint32_t*>(lds) + (threads + local * LANES) * PER;
+    uint32_t* const group_keys = reinterpret_cast<uint32_t*>(lds) + 2 * threads * PER + local * LANES;
+    float bias[PER];
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const float z = i < n ? a.logits[(long long)t * a.experts + first + i] : -INFINITY;
-        s[i] = z > -INFINITY ? fminf(z, 3.402823466e38f) : -INFINITY;  // NaN: none
-        top = fmaxf(top, s[i]);
-    }
-    float sum = 0.0f;
-    top = lanes_max<64>(top);
+    for (int i = 0; i < PER; i++) bias[i] = a.bias && i < n ? a.bias[first + i] : 0.0f;
+    for (int t0 = 0; t0 < a.tokens; t0 += threads / LANES) {
+        const int t = min(t0 + local, a.tokens - 1);  // behind the last token: that once more
+        float s[PER];
+        uint32_t key[PER];
+        if (logits) {
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        key[i] = s[i] > -INFINITY;
-        if (a.sigmoid) {
-            const float e = exp_neg(-fabsf(s[i])), r = __builtin_amdgcn_rcpf(1.0f + e);
-            s[i] = key[i] ? (s[i] >= 0.0f ? r : e * r) : 0.0f;
+            for (int i = 0; i < PER; i++) s[i] = i < n ? logits[t * a.experts + first + i] : -INFINITY;
         } else {
-            s[i] = key[i] ? exp_neg(s[i] - top) : 0.0f;
+            const float* z = a.logits + (long long)t * a.experts + first;
+#pragma unroll
+            for (int i = 0; i < PER; i++) s[i] = i < n ? z[i] : -INFINITY;
+            for (int p = 1; p < parts; p++) {
+                z += (long long)a.tokens * a.experts;
+#pragma unroll
+                for (int i = 0; i < PER; i++) s[i] += i < n ? z[i] : 0.0f;
+            }
+        }
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            s[i] = s[i] > -INFINITY ? fminf(s[i], 3.402823466e38f) : -INFINITY;  // NaN: none
+            top = fmaxf(top, s[i]);
+        }
+        if (!a.sigmoid) top = lanes_max<LANES>(top);
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const bool live = s[i] > -INFINITY;
+            const float e = exp_neg(a.sigmoid ? -fabsf(s[i]) : s[i] - top), r = __builtin_amdgcn_rcpf(1.0f + e);
+            key[i] = live;
+            s[i] = !live ? 0.0f : !a.sigmoid ? e : s[i] >= 0.0f ? r : e * r;
             sum += s[i];
         }
-    }
-    if (!a.sigmoid) {
-        sum = lanes_sum<64>(sum);
-        sum = sum > 0.0f ? 1.0f / sum : 0.0f;
-    }
+        if (!a.sigmoid) {
+            sum = lanes_sum<LANES>(sum);
+            const float r = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        if (!a.sigmoid) s[i] *= sum;
-        const float c = s[i] + (a.bias && i < n ? a.bias[first + i] : 0.0f);
-        key[i] = key[i] && c > -INFINITY ? key_of(c) : 0u;
-        if (i < n) scores[first + i] = s[i];
-    }
-    if (a.groups > 1) {
-        const int size = a.experts / a.groups;
+            for (int i = 0; i < PER; i++) s[i] *= r;
+        }
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (i < n) keys[first + i] = key[i];
+        for (int i = 0; i < PER; i++) {
+            const float c = s[i] + bias[i];
+            key[i] = key[i] && c > -INFINITY ? key_of(c) : 0u;
+            if (i < n) scores[first + i] = s[i];
+        }
+        if (a.groups > 1) {
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (i < n) keys[first + i] = key[i];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            uint32_t g = 0;  // lane l: group l, by the best one or two of it
+            if (sub < a.groups) {
+                uint32_t b2 = 0;
+#pragma unroll 8
+                for (int i = 0; i < size; i++) {
+                    const uint32_t k = keys[sub * size + i];
+                    b2 = max(b2, min(g, k));
+                    g = max(g, k);
+                }
+                if (a.group_best == 2 && b2 != 0) g = key_of(of_key(g) + of_key(b2));
+                group_keys[sub] = g;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            int ahead = 0;
+#pragma unroll 4
+            for (int o = 0; o < a.groups; o++) {
+                const uint32_t k = group_keys[o];
+                ahead += k > g || (k == g && o < sub);
+            }
+            const uint64_t kept = __ballot(sub < a.groups && ahead < a.kept) >> (lane - sub);
+            const float r = 1.0f / (float)size;
+#pragma unroll
+            for (int i = 0; i < PER; i++)  // of at most 1,024 experts: the quotient's error is far below 1 / 2 size
+                if (i < n && !(kept >> (int)(((float)(first + i) + 0.5f) * r) & 1)) key[i] = 0;
+        }
+#pragma unroll 1
+        for (int j = 0; j < a.topk; j++) {
+            uint32_t best = key[0];
+#pragma unroll
+            for (int i = 1; i < PER; i++) best = max(best, key[i]);
+            const uint32_t all = lanes_umax<LANES>(best);
+            const uint64_t have = __ballot(best == all) & lanes;
+            const bool mine = lane == __ffsll((unsigned long long)have) - 1;  // the lowest
+            int at = 0;
+#pragma unroll
+            for (int i = PER - 1; i >= 0; i--) at = key[i] == all ? i : at;
+#pragma unroll
+            for (int i = 0; i < PER; i++) key[i] = mine && i == at ? 0u : key[i];
+            if (mine) expert[t * a.topk + j] = all ? first + at : -1;
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        uint32_t b1 = 0, b2 = 0;  // lane g: the best two of group g
-        if (lane < a.groups)
-            for (int i = 0; i < size; i++) {
-                const uint32_t k = keys[lane * size + i];
-                b2 = max(b2, min(b1, k));
-                b1 = max(b1, k);
-            }
-        uint32_t g = b1;
-        if (a.group_best == 2 && b2 != 0) g = key_of(of_key(b1) + of_key(b2));
-        int ahead = 0;
-        for (int o = 0; o < a.groups; o++) {
-            const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)g, o);
-            ahead += k > g || (k == g && o < lane);
-        }
-        const uint64_t kept = __ballot(lane < a.groups && ahead < a.kept);
-#pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (i < n && !(kept >> ((first + i) / size) & 1)) key[i] = 0;
+        const int e = sub < a.topk ? expert[t * a.topk + sub] : -1;  // topk is at most LANES
+        float score = e >= 0 ? scores[e] : 0.0f, factor = a.scale;
+        if (a.renorm) factor /= lanes_sum<LANES>(score) + 1e-20f;
+        if (sub < a.topk) a.weights[t * a.topk + sub] = score * factor;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-    }
-    int mine = -1;  // lane j: the j-th pick
-#pragma unroll 1
-    for (int j = 0; j < a.topk; j++) {
-        uint32_t best = key[0];
-#pragma unroll
-        for (int i = 1; i < PER; i++) best = max(best, key[i]);
-        const uint32_t all = lanes_umax<64>(best);
-        if (all == 0) break;
-        const int l = __ffsll((unsigned long long)__ballot(best == all)) - 1;
-        int at = 0;
-#pragma unroll
-        for (int i = PER - 1; i >= 0; i--) at = key[i] == all ? i : at;
-#pragma unroll
-        for (int i = 0; i < PER; i++) key[i] = lane == l && i == at ? 0u : key[i];
-        const int e = __builtin_amdgcn_readlane(first + at, l);
-        mine = lane == j ? e : mine;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    float score = mine >= 0 ? scores[mine] : 0.0f;
-    __builtin_amdgcn_wave_barrier();
-    if (a.renorm) {
-        const float total = lanes_sum<64>(score);
-        score *= a.scale / (total + 1e-20f);
-    } else score *= a.scale;
-    if (lane < a.topk) {
-        a.weights[t * a.topk + lane] = score;
-        a.slots[t * a.topk + lane] = mine;  // for now the slot's expert
     }
 }
 
-// The experts that some token takes, in their order, and the list of their slots.
-__device__ __forceinline__ void plan(const LayerArgs& a, int* lds)
+// f(lanes of a token, experts of a lane): as many tokens a wave as leave a lane at most
+// four experts (or 16, of more than 256) and a lane for each group and pick.
+template <class F>
+__host__ __device__ inline void with_lanes(const LayerArgs& a, F&& f)
 {
-    int* const count = lds;              // [experts]: slots; then where the expert's next goes
-    int* const expert = lds + a.experts; // [slots]
+    using std::integral_constant;
+    const int per_group_or_pick = a.groups > a.topk ? a.groups : a.topk;
+    if (a.experts <= 8) f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+    else if (a.experts <= 64 && per_group_or_pick <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    else if (a.experts <= 128 && per_group_or_pick <= 32) f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+    else if (a.experts <= 256) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    else f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+}
+
+// The experts that some token takes, in their order, and the list of their slots,
+// from the slots' experts and count [experts] in LDS.
+__device__ __forceinline__ void plan(const LayerArgs& a, const int* expert, int* count)
+{
     const int slots = a.tokens * a.topk;
-    for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) count[e] = 0;
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) count[e] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < slots; i += kRouteThreads) {
-        expert[i] = a.slots[i];
+    for (int i = threadIdx.x; i < slots; i += blockDim.x)
         if (expert[i] >= 0) atomicAdd(&count[expert[i]], 1);
-    }
     __syncthreads();
-    if (threadIdx.x < 64) {
+    if (threadIdx.x < 64) {  // count: where the expert's next slot goes
         int number = 0, begin = 0;
         for (int e0 = 0; e0 < a.experts; e0 += 64) {
             const int e = e0 + threadIdx.x, n = e < a.experts ? count[e] : 0;
@@ -233,13 +257,35 @@ __device__ __forceinline__ void plan(const LayerArgs& a, int* lds)
     }
     __syncthreads();
     // an expert's slots in any order: each has a column of its own
-    for (int i = threadIdx.x; i < slots; i += kRouteThreads)
+    for (int i = threadIdx.x; i < slots; i += blockDim.x)
         if (expert[i] >= 0) a.slots[atomicAdd(&count[expert[i]], 1)] = i;
 }
 
-// Logits of 16 experts, waves sharing out k; the tokens' terms on the way; routing
-// and plan by the workgroup that is last.  Products of terms are exact; those of
-// 2^-24 of a product and less are left out.
+// LDS of the routing kernel: sums of its waves, then scores and keys, then the plan's
+// counts, in one place; the slots' experts; the logits.
+struct RouteLds {
+    int experts_at, logits_at, size;
+};
+__host__ __device__ inline RouteLds route_lds(const LayerArgs& a, int waves, int tiles, int logits)
+{
+    int scores = 0;
+    with_lanes(a, [&](auto, auto P) { scores = waves * 64 * 4 * (a.groups > 1 ? 2 * decltype(P)::value + 1 : decltype(P)::value); });
+    const int sums = waves * tiles * 1024, counts = a.experts * 4;
+    RouteLds l;
+    l.experts_at = sums > scores ? sums : scores;
+    if (counts > l.experts_at) l.experts_at = counts;
+    l.logits_at = l.experts_at + a.tokens * a.topk * 4;
+    l.size = l.logits_at + logits * 4;
+    return l;
+}
+constexpr int kLogitsInLds = 16384;  // more of them are read token by token
+constexpr int kRouteParts = 8;
+
+// Logits of 16 experts over a part of k that the waves share out; the tokens' terms on
+// the way; routing and plan by the workgroup that is last.  Products of terms are
+// exact; those of 2^-24 of a product and less are left out.  A part is four blocks of
+// k, a quarter of one for each of 16 waves, while that makes no more than 128
+// workgroups: one round trip, and the splitting of fp32 numbers spread.
 template <class T, class R, int MT>
 __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
 {
@@ -247,78 +293,97 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ bool last;
     f4* const sums = reinterpret_cast<f4*>(lds);  // [waves][MT][64]
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const int col = lane & 15, quad = lane >> 4, e0 = blockIdx.x * 16;
-    const int blocks = a.dim_pad / 128;
+    const int blocks = a.dim_pad / 128, parts = gridDim.y;
+    const int kb0 = blocks * blockIdx.y / parts, kb1 = blocks * (blockIdx.y + 1) / parts;
+    const bool alone = gridDim.x * parts == 1;
+    const RouteLds at = route_lds(a, waves, MT, 0);
+    int* const expert = reinterpret_cast<int*>(lds + at.experts_at);
+    const int all = a.tokens * a.experts;
+    float* const logits = all <= kLogitsInLds ? reinterpret_cast<float*>(lds + at.logits_at) : nullptr;
     f4 acc[MT];
 #pragma unroll
     for (int j = 0; j < MT; j++) acc[j] = f4zero();
     const R* r = (const R*)a.router + (long long)min(e0 + col, a.experts - 1) * a.dim;
-    for (int kb = wave; kb < blocks; kb += kRouteWaves) {
+    for (int u = 4 * kb0 + wave; u < 4 * kb1; u += waves) {  // a quarter of a block at a time
+        const int kb = u / 4, k = kb * 128 + quad * 32 + u % 4 * 8;
+        R v[8];
+        bf16x8 y[Y];
+        load8(v, r + k, a.dim - k, a.vec_router);
+        T w[MT][8];
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const int k = kb * 128 + quad * 32 + q * 8;
-            R v[8];
-            bf16x8 y[Y];
-            load8(v, r + k, a.dim - k, a.vec_router);
-            split8(v, y);
+        for (int j = 0; j < MT; j++)
+            if (j * 16 < a.tokens)
+                load8(w[j], (const T*)a.x + min(j * 16 + col, a.tokens - 1) * a.stride_x + k, a.dim - k, a.vec_x);
+        split8(v, y);
 #pragma unroll
-            for (int j = 0; j < MT; j++) {
-                const int t = j * 16 + col;
-                T u[8];
-                bf16x8 x[X];
-                load8(u, (const T*)a.x + min(t, a.tokens - 1) * a.stride_x + k, a.dim - k, a.vec_x);
-                split8(u, x);
+        for (int j = 0; j < MT; j++) {
+            if (j * 16 >= a.tokens) break;
+            const int t = j * 16 + col;
+            bf16x8 x[X];
+            split8(w[j], x);
+#pragma unroll
+            for (int m = 0; m < X; m++)
+#pragma unroll
+                for (int n = 0; n < Y; n++)
+                    if (m + n < 3) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[n], x[m], acc[j], 0, 0, 0);
+            // each workgroup of a part stores some blocks of the terms
+            if (kb % gridDim.x == blockIdx.x && t < a.tokens) {
 #pragma unroll
                 for (int m = 0; m < X; m++)
-#pragma unroll
-                    for (int n = 0; n < Y; n++)
-                        if (m + n < 3) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[n], x[m], acc[j], 0, 0, 0);
-                // each workgroup stores some blocks of the terms
-                if (kb % gridDim.x == blockIdx.x && t < a.tokens) {
-#pragma unroll
-                    for (int m = 0; m < X; m++)
-                        *reinterpret_cast<bf16x8*>(a.xs + ((long long)t * X + m) * a.dim_pad + k) = x[m];
-                }
+                    *reinterpret_cast<bf16x8*>(a.xs + ((long long)t * X + m) * a.dim_pad + k) = x[m];
             }
         }
     }
 #pragma unroll
     for (int j = 0; j < MT; j++) sums[(wave * MT + j) * 64 + lane] = acc[j];
     __syncthreads();
-    if (wave < MT) {
-        f4 v = sums[wave * 64 + lane];
-        for (int w = 1; w < kRouteWaves; w++) v += sums[(w * MT + wave) * 64 + lane];
-        const int t = wave * 16 + col;
+    for (int j = wave; j * 16 < a.tokens; j += waves) {
+        f4 v = sums[j * 64 + lane];
+        for (int w = 1; w < min(waves, 4 * (kb1 - kb0)); w++) v += sums[(w * MT + j) * 64 + lane];
+        const int t = j * 16 + col;
         if (t < a.tokens) {
+            float* to = alone ? logits : a.logits + (long long)blockIdx.y * all;
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if (e0 + quad * 4 + i < a.experts) a.logits[(long long)t * a.experts + e0 + quad * 4 + i] = v[i];
+                if (e0 + quad * 4 + i < a.experts) to[t * a.experts + e0 + quad * 4 + i] = v[i];
         }
     }
     __syncthreads();
-    if (gridDim.x > 1) {
+    if (!alone) {
         if (threadIdx.x == 0) {
-            __threadfence();
-            last = atomicAdd(a.route_ticket, 1u) == gridDim.x - 1;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");  // what the workgroup has stored
+            last = atomicAdd(a.route_ticket, 1u) == gridDim.x * parts - 1;
         }
         __syncthreads();
         if (!last) return;
         if (threadIdx.x == 0) *a.route_ticket = 0;
-        __threadfence();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+        if (logits) {  // all parts' loads together
+            for (int i0 = threadIdx.x; i0 < all; i0 += 4 * blockDim.x) {
+                float z[4][kRouteParts];
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int p = 0; p < kRouteParts; p++)
+                        z[u][p] = a.logits[min(p, parts - 1) * all + min(i0 + u * (int)blockDim.x, all - 1)];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    float v = z[u][0];
+#pragma unroll
+                    for (int p = 1; p < kRouteParts; p++) v += p < parts ? z[u][p] : 0.0f;
+                    if (i0 + u * (int)blockDim.x < all) logits[i0 + u * blockDim.x] = v;
+                }
+            }
+            __syncthreads();
+        }
     }
-    if (a.out_tickets)
-        for (int i = threadIdx.x; i < (a.dim + 15) / 16; i += kRouteThreads) a.out_tickets[i] = 0;
-    float* const scores = reinterpret_cast<float*>(lds) + wave * a.experts;
-    uint32_t* const keys = reinterpret_cast<uint32_t*>(lds) + (kRouteWaves + wave) * a.experts;
-    for (int t = wave; t < a.tokens; t += kRouteWaves) {
-        if (a.experts <= 64) route_token<1>(a, t, scores, keys);
-        else if (a.experts <= 128) route_token<2>(a, t, scores, keys);
-        else if (a.experts <= 256) route_token<4>(a, t, scores, keys);
-        else route_token<16>(a, t, scores, keys);
-    }
+    with_lanes(a, [&](auto L, auto P) {
+        route_tokens<decltype(L)::value, decltype(P)::value>(a, logits, parts, reinterpret_cast<float*>(lds), expert);
+    });
     __syncthreads();
-    plan(a, reinterpret_cast<int*>(lds));
+    plan(a, expert, reinterpret_cast<int*>(lds));
 }
 
 // ---------------------------------------------------------------------------
@@ -392,18 +457,61 @@ __device__ __forceinline__ float activate(int kind, float v)
     }
 }
 
-// The hidden activations of 16 NT rows for the slots of an active expert, 16 CT at a
-// time: waves share out k, and their sums are joined in LDS in wave order.  A lane
-// whose column has no slot works on the first one's for nothing.
-template <int FORMAT, class T, int G, int NT, int CT>
-__global__ __launch_bounds__(kLayerThreads) void layer_hidden_kernel(LayerArgs a)
+// The 16 columns of a matrix instruction are SLOTS slots by TERMS terms, one term of
+// all slots behind the other: a value's terms are products of their own, added up at
+// the end.
+template <int TERMS>
+struct Columns {
+    static constexpr int kSlots = 16 / TERMS;
+    int slot, term;
+    __device__ __forceinline__ explicit Columns(int col)
+    {
+        term = col / kSlots;
+        slot = term < TERMS ? col - term * kSlots : kSlots;  // none behind the last term's
+    }
+};
+
+// What a wave has under way of 128 of k: F fragments of weights, CT of tokens or
+// hidden activations.
+template <int FORMAT, int F, int CT>
+struct Bundle {
+    Piece<FORMAT> w[F];
+    bf16x8 t[CT][4];
+
+    __device__ __forceinline__ void load_columns(const __bf16* const (&from)[CT], int kb)
+    {
+#pragma unroll
+        for (int j = 0; j < CT; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) t[j][q] = *reinterpret_cast<const bf16x8*>(from[j] + kb * 128 + q * 8);
+    }
+    __device__ __forceinline__ void multiply(f4 (&acc)[F][CT]) const
+    {
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+#pragma unroll
+            for (int f = 0; f < F; f++) {
+                const bf16x8 b = w[f](q);
+#pragma unroll
+                for (int j = 0; j < CT; j++) acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, t[j][q], acc[f][j], 0, 0, 0);
+            }
+    }
+};
+
+// The hidden activations of 16 NT rows (with their gate's: G 2) for the slots of an
+// active expert, as many at a time as CT fragments have: waves share out k, and their
+// sums are joined in LDS in wave order.  A lane whose column has no slot works on the
+// first one's for nothing.
+template <int FORMAT, class T, int G, int NT, int CT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void layer_hidden_kernel(LayerArgs a)
 {
-    constexpr int X = Terms<T>::kX, A = Terms<T>::kA, F = G * NT;
-    __shared__ f4 sums[kLayerWaves][F][CT][64];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    constexpr int X = Terms<T>::kX, A = Terms<T>::kA, F = G * NT, kSlots = Columns<X>::kSlots;
+    __shared__ f4 sums[WAVES][F][CT][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int col = lane & 15, quad = lane >> 4, n0 = blockIdx.x * 16 * NT, n = blockIdx.y;
-    if (n >= a.active[0]) return;
-    const int e = a.active[1 + n], first = a.first[n], count = a.first[n + 1] - first;
+    // one round trip for all four; behind the active experts they are of no use
+    const int number = a.active[0], e = a.active[1 + n], first = a.first[n], count = a.first[n + 1] - first;
+    if (n >= number) return;
     const uint8_t *W[F], *S[F];
 #pragma unroll
     for (int f = 0; f < F; f++) {
@@ -412,53 +520,50 @@ __global__ __launch_bounds__(kLayerThreads) void layer_hidden_kernel(LayerArgs a
         S[f] = scales_of<FORMAT>(a.s1, e, G * a.hidden, a.dim_pad, row, a.scale_shift);
     }
     const int blocks = a.dim_pad / 128;
-    for (int s0 = 0; s0 < count; s0 += 16 * CT) {
+    const Columns<X> mine(col);
+    for (int s0 = 0; s0 < count; s0 += kSlots * CT) {
         int slot[CT];
         const __bf16* x[CT];
         f4 acc[F][CT];
 #pragma unroll
         for (int j = 0; j < CT; j++) {
-            const int c = s0 + j * 16 + col;
-            slot[j] = c < count ? a.slots[first + c] : -1;
-            x[j] = a.xs + (long long)(max(slot[j], 0) / a.topk) * X * a.dim_pad + quad * 32;
+            const int i = s0 + j * kSlots + mine.slot;
+            slot[j] = mine.slot < kSlots && i < count ? a.slots[first + i] : -1;
 #pragma unroll
             for (int f = 0; f < F; f++) acc[f][j] = f4zero();
         }
-        auto load = [&](Piece<FORMAT>(&w)[F], int kb) {
+        using Part = Bundle<FORMAT, F, CT>;
+        // Columns of several fragments are read when their turn comes, from the L2: ahead
+        // they would not fit the registers.
+        auto load = [&](Part& b, int kb) {
 #pragma unroll
-            for (int f = 0; f < F; f++) w[f].load(W[f], S[f], kb, quad);
+            for (int f = 0; f < F; f++) b.w[f].load(W[f], S[f], kb, quad);
+            if (CT == 1) b.load_columns(x, kb);
         };
-        auto work = [&](const Piece<FORMAT>(&w)[F], int kb) {
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                bf16x8 t[CT][X];
-#pragma unroll
-                for (int j = 0; j < CT; j++)
-#pragma unroll
-                    for (int u = 0; u < X; u++)
-                        t[j][u] = *reinterpret_cast<const bf16x8*>(x[j] + (long long)u * a.dim_pad + kb * 128 + q * 8);
-#pragma unroll
-                for (int f = 0; f < F; f++) {
-                    const bf16x8 b = w[f](q);
-#pragma unroll
-                    for (int j = 0; j < CT; j++)
-#pragma unroll
-                        for (int u = 0; u < X; u++)
-                            acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, t[j][u], acc[f][j], 0, 0, 0);
-                }
-            }
+        auto multiply = [&](Part& b, int kb) {
+            if (CT > 1) b.load_columns(x, kb);
+            b.multiply(acc);
         };
-        Piece<FORMAT> w0[F], w1[F];
+        Part b0, b1;
         int kb = wave;
-        if (kb < blocks) load(w0, kb);
+        if (kb < blocks) {
+#pragma unroll
+            for (int f = 0; f < F; f++) b0.w[f].load(W[f], S[f], kb, quad);  // they need no slots
+        }
+#pragma unroll
+        for (int j = 0; j < CT; j++) {
+            const int token = (slot[j] >= 0 ? slot[j] : a.slots[first]) / a.topk;
+            x[j] = a.xs + ((long long)token * X + (slot[j] >= 0 ? mine.term : 0)) * a.dim_pad + quad * 32;
+        }
+        if (CT == 1 && kb < blocks) b0.load_columns(x, kb);
         while (kb < blocks) {
-            if (kb + waves < blocks) load(w1, kb + waves);
-            work(w0, kb);
-            kb += waves;
+            if (kb + WAVES < blocks) load(b1, kb + WAVES);
+            multiply(b0, kb);
+            kb += WAVES;
             if (kb >= blocks) break;
-            if (kb + waves < blocks) load(w0, kb + waves);
-            work(w1, kb);
-            kb += waves;
+            if (kb + WAVES < blocks) load(b0, kb + WAVES);
+            multiply(b1, kb);
+            kb += WAVES;
         }
         if (s0 > 0) __syncthreads();
 #pragma unroll
@@ -466,24 +571,28 @@ __global__ __launch_bounds__(kLayerThreads) void layer_hidden_kernel(LayerArgs a
 #pragma unroll
             for (int j = 0; j < CT; j++) sums[wave][f][j][lane] = acc[f][j];
         __syncthreads();
+        const int used = min(WAVES, blocks);
 #pragma unroll
         for (int f = 0; f < NT; f++)
 #pragma unroll
             for (int j = 0; j < CT; j++) {
-                if ((f * CT + j) % waves != wave || slot[j] < 0) continue;
-                f4 v = sums[0][f][j][lane], u = f4zero();
-                for (int w = 1; w < waves; w++) v += sums[w][f][j][lane];
-                if (G == 2)
-                    for (int w = 0; w < waves; w++) u += sums[w][F - NT + f][j][lane];
+                if ((f * CT + j) % WAVES != wave || slot[j] < 0 || mine.term > 0) continue;
+                f4 h[G];
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    h[g] = f4zero();
+                    for (int u = 0; u < X; u++)
+                        for (int w = 0; w < used; w++) h[g] += sums[w][g * NT + f][j][lane + u * kSlots];
+                }
                 const int row = n0 + f * 16 + quad * 4;
                 Vec<__bf16, 4> o[A];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float h = activate(a.activation, v[i]);
-                    if (G == 2) h *= u[i];
-                    if (row + i >= a.hidden) h = 0.0f;
+                    float v = activate(a.activation, h[0][i]);
+                    if (G == 2) v *= h[G - 1][i];
+                    if (row + i >= a.hidden) v = 0.0f;
                     __bf16 s[A];
-                    split(h, s);
+                    split(v, s);
 #pragma unroll
                     for (int t = 0; t < A; t++) o[t][i] = s[t];
                 }
@@ -494,182 +603,170 @@ __global__ __launch_bounds__(kLayerThreads) void layer_hidden_kernel(LayerArgs a
     }
 }
 
-// 16 NT columns of the outputs for all tokens, and a part of the active experts' k:
-// its waves share that out in runs of one expert's, whose sums go, weighted, to the
-// tokens' in LDS.  Where k is in more than one part, the last workgroup of a tile
-// joins them in their order.
-template <int FORMAT, class T, int NT, int CT>
-__global__ __launch_bounds__(kLayerThreads) void layer_out_kernel(LayerArgs a)
+// 16 NT columns of the outputs for all tokens: the waves share out the active experts'
+// k in runs of one expert's, whose sums go, weighted, to the tokens' in the wave's part
+// of LDS; those are joined in wave order.
+template <int FORMAT, class T, int NT, int CT, int WAVES, int DEPTH>
+__global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
 {
-    constexpr int A = Terms<T>::kA;
+    constexpr int A = Terms<T>::kA, kSlots = Columns<A>::kSlots;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    __shared__ bool last;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int col = lane & 15, quad = lane >> 4, d0 = blockIdx.x * 16 * NT;
     const int slots = a.tokens * a.topk, most = min(a.experts, slots);
     f4* const sums = reinterpret_cast<f4*>(lds);  // [waves][tokens][4 NT]
-    int* const active = reinterpret_cast<int*>(sums + waves * a.tokens * 4 * NT);
+    int* const active = reinterpret_cast<int*>(sums + WAVES * a.tokens * 4 * NT);
     int *const first = active + most, *const list = first + most + 1;
+    float* const weights = reinterpret_cast<float*>(list + slots);  // in LDS as well: a load would wait for all that are ahead
     const int number = a.active[0];
-    for (int i = threadIdx.x; i < number; i += blockDim.x) active[i] = a.active[1 + i];
-    for (int i = threadIdx.x; i <= number; i += blockDim.x) first[i] = a.first[i];
-    for (int i = threadIdx.x; i < slots; i += blockDim.x) list[i] = a.slots[i];
-    for (int i = threadIdx.x; i < waves * a.tokens * 4 * NT; i += blockDim.x) sums[i] = f4zero();
+    for (int i = threadIdx.x; i < most; i += WAVES * 64) active[i] = a.active[1 + i];
+    for (int i = threadIdx.x; i <= most; i += WAVES * 64) first[i] = a.first[i];
+    for (int i = threadIdx.x; i < slots; i += WAVES * 64) list[i] = a.slots[i], weights[i] = a.weights[i];
+    for (int i = threadIdx.x; i < WAVES * a.tokens * 4 * NT; i += WAVES * 64) sums[i] = f4zero();
     __syncthreads();
     const int blocks = a.hidden_pad / 128, items = number * blocks;  // at most 2^10 * 2^7
-    const int workers = waves * gridDim.y, worker = blockIdx.y * waves + wave;
-    const int begin = (int)((long long)items * worker / workers), end = (int)((long long)items * (worker + 1) / workers);
+    const int begin = items * wave / WAVES, end = items * (wave + 1) / WAVES;
     int row[NT];
 #pragma unroll
     for (int f = 0; f < NT; f++) row[f] = min(d0 + f * 16 + col, a.dim - 1);
+    const Columns<A> mine(col);
 
-    // Where the wave is: block kb of up to `to` of expert `at`, for its slots from s0 on.
+    // Block kb, from .. to - 1, of expert `at`, for its slots from s0 on.
     struct Cursor {
         int at, kb, from, to, s0;
+        __device__ __forceinline__ bool valid() const { return kb < to; }
+        __device__ __forceinline__ bool first_of_run() const { return kb == from; }
+        __device__ __forceinline__ bool last_of_run() const { return kb + 1 == to; }
     };
     auto enter = [&](int n) {
-        Cursor c{n, 0, max(begin - n * blocks, 0), min(end - n * blocks, blocks), 0};
-        c.kb = c.from;
-        return c;
+        const int from = max(begin - n * blocks, 0);
+        return Cursor{n, from, from, min(end - n * blocks, blocks), 0};
     };
-    auto after = [&](Cursor c) {  // past the end: to <= from
-        if (c.kb + 1 < c.to) c.kb++;
-        else if (c.s0 + 16 * CT < __builtin_amdgcn_readfirstlane(first[c.at + 1] - first[c.at])) c.s0 += 16 * CT, c.kb = c.from;
-        else if ((c.at + 1) * blocks < end) c = enter(c.at + 1);
-        else c.to = c.from;
-        return c;
+    auto advance = [&](Cursor& c) {
+        if (++c.kb < c.to) return;
+        if (c.s0 + kSlots * CT < __builtin_amdgcn_readfirstlane(first[c.at + 1] - first[c.at])) {
+            c.s0 += kSlots * CT;
+            c.kb = c.from;
+        } else if ((c.at + 1) * blocks < end) c = enter(c.at + 1);
     };
-    auto load = [&](Piece<FORMAT>(&w)[NT], const Cursor& c) {
-        const int e = __builtin_amdgcn_readfirstlane(active[c.at]);
-#pragma unroll
-        for (int f = 0; f < NT; f++)
-            w[f].load(row_of<FORMAT>(a.w2, e, a.dim, a.hidden_pad, row[f]),
-                      scales_of<FORMAT>(a.s2, e, a.dim, a.hidden_pad, row[f], a.scale_shift), c.kb, quad);
+    auto slot_of = [&](const Cursor& c, int j) {  // of the lane's column, -1: none
+        const int f0 = first[c.at], i = c.s0 + j * kSlots + mine.slot;
+        return mine.slot < kSlots && i < first[c.at + 1] - f0 ? list[f0 + i] : -1;
     };
-    f4 own[NT][CT];
-    int slot[CT];
+    using Part = Bundle<FORMAT, NT, CT>;
+    const uint8_t *W[NT], *S[NT];
     const __bf16* act[CT];
-    auto start = [&](const Cursor& c) {
-        const int f0 = first[c.at], count = first[c.at + 1] - f0;
-#pragma unroll
-        for (int j = 0; j < CT; j++) {
-            const int i = c.s0 + j * 16 + col;
-            slot[j] = i < count ? list[f0 + i] : -1;
-            act[j] = a.acts + (long long)(slot[j] >= 0 ? slot[j] : list[f0]) * A * a.hidden_pad + quad * 32;
-#pragma unroll
-            for (int f = 0; f < NT; f++) own[f][j] = f4zero();
-        }
-    };
-    auto finish_run = [&] {
-#pragma unroll
-        for (int j = 0; j < CT; j++) {
-            if (slot[j] < 0) continue;
-            const float w = a.weights[slot[j]];
-            f4* to = sums + (wave * a.tokens + slot[j] / a.topk) * 4 * NT + quad;
+    auto load = [&](Part& b, const Cursor& c) {
+        if (c.first_of_run()) {
+            const int e = __builtin_amdgcn_readfirstlane(active[c.at]);
 #pragma unroll
             for (int f = 0; f < NT; f++) {
-                f4 v = to[f * 4];
+                W[f] = row_of<FORMAT>(a.w2, e, a.dim, a.hidden_pad, row[f]);
+                S[f] = scales_of<FORMAT>(a.s2, e, a.dim, a.hidden_pad, row[f], a.scale_shift);
+            }
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = fmaf(w, own[f][j][i], v[i]);
-                to[f * 4] = v;
+            for (int j = 0; j < CT; j++) {
+                const int slot = slot_of(c, j);
+                act[j] = a.acts + ((long long)(slot >= 0 ? slot : list[first[c.at]]) * A + (slot >= 0 ? mine.term : 0)) * a.hidden_pad +
+                         quad * 32;
             }
         }
+#pragma unroll
+        for (int f = 0; f < NT; f++) b.w[f].load(W[f], S[f], c.kb, quad);
+        b.load_columns(act, c.kb);
     };
-    auto work = [&](const Piece<FORMAT>(&w)[NT], int kb) {
+    f4 own[NT][CT];
+    auto finish_run = [&](const Cursor& c) {
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            bf16x8 t[CT][A];
-#pragma unroll
-            for (int j = 0; j < CT; j++)
-#pragma unroll
-                for (int u = 0; u < A; u++)
-                    t[j][u] = *reinterpret_cast<const bf16x8*>(act[j] + (long long)u * a.hidden_pad + kb * 128 + q * 8);
+        for (int j = 0; j < CT; j++) {
+            const int slot = slot_of(c, j);
+            const bool takes = slot >= 0 && mine.term == 0;
+            const float w = weights[max(slot, 0)];
+            f4* to = sums + (wave * a.tokens + max(slot, 0) / a.topk) * 4 * NT + quad;
 #pragma unroll
             for (int f = 0; f < NT; f++) {
-                const bf16x8 b = w[f](q);
+                f4 v = own[f][j];
 #pragma unroll
-                for (int j = 0; j < CT; j++)
+                for (int i = 0; i < 4; i++) {  // the other terms, kSlots lanes on
+                    const float x = own[f][j][i];
+                    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+                    if constexpr (A == 2) v[i] += __builtin_bit_cast(float, dpp_mov<0x108>(u));
+                    if constexpr (A == 3)
+                        v[i] += __builtin_bit_cast(float, dpp_mov<0x105>(u)) + __builtin_bit_cast(float, dpp_mov<0x10a>(u));
+                }
+                if (!takes) continue;
+                f4 sum = to[f * 4];
 #pragma unroll
-                    for (int u = 0; u < A; u++)
-                        own[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, t[j][u], own[f][j], 0, 0, 0);
+                for (int i = 0; i < 4; i++) sum[i] = fmaf(w, v[i], sum[i]);
+                to[f * 4] = sum;
             }
         }
     };
     if (begin < end) {
-        Cursor c = enter(begin / blocks);
-        Piece<FORMAT> w0[NT], w1[NT];
-        load(w0, c);
-        start(c);
-        auto step = [&](Piece<FORMAT>(&w)[NT], Piece<FORMAT>(&ahead)[NT]) {
-            const Cursor d = after(c);
-            const bool more = d.to > d.from;
-            if (more) load(ahead, d);
-            work(w, c.kb);
-            if (!more || d.at != c.at || d.s0 != c.s0) {
-                finish_run();
-                if (more) start(d);
+        Part b[DEPTH];
+        Cursor ahead = enter(begin / blocks), now = ahead;
+#pragma unroll
+        for (int d = 0; d + 1 < DEPTH; d++)
+            if (ahead.valid()) {
+                load(b[d], ahead);
+                advance(ahead);
             }
-            c = d;
-            return more;
-        };
-        while (step(w0, w1) && step(w1, w0)) {}
+        bool more = true;
+        while (more) {
+            each<DEPTH>([&](auto D) {
+                constexpr int d = decltype(D)::value;
+                if (!more) return;
+                if (ahead.valid()) {
+                    load(b[(d + DEPTH - 1) % DEPTH], ahead);
+                    advance(ahead);
+                }
+                if (now.first_of_run()) {
+#pragma unroll
+                    for (int j = 0; j < CT; j++)
+#pragma unroll
+                        for (int f = 0; f < NT; f++) own[f][j] = f4zero();
+                }
+                b[d].multiply(own);
+                if (now.last_of_run()) finish_run(now);
+                advance(now);
+                more = now.valid();
+            });
+        }
     }
     __syncthreads();
-    // Of token t, columns d .. d + 3.
-    auto store = [&](int t, int d, f4 v) {
+    const int pieces = a.tokens * 4 * NT;
+    for (int i = threadIdx.x; i < pieces; i += WAVES * 64) {
+        f4 v = sums[i];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) v += sums[w * pieces + i];
+        const int t = i / (4 * NT), d = d0 + i % (4 * NT) * 4;
         T* to = (T*)a.out + t * a.stride_out + d;
         if (a.vec_out && d + 4 <= a.dim) {
             Vec<T, 4> o;
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = (T)v[i];
+            for (int j = 0; j < 4; j++) o[j] = (T)v[j];
             *reinterpret_cast<Vec<T, 4>*>(to) = o;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (d + i < a.dim) to[i] = (T)v[i];
+            for (int j = 0; j < 4; j++)
+                if (d + j < a.dim) to[j] = (T)v[j];
         }
-    };
-    const int pieces = a.tokens * 4 * NT;
-    const long long plane = (long long)gridDim.x * pieces;
-    f4* const parts = reinterpret_cast<f4*>(a.parts) + (long long)blockIdx.x * pieces;
-    for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
-        f4 v = sums[i];
-        for (int w = 1; w < waves; w++) v += sums[w * pieces + i];
-        if (gridDim.y == 1) store(i / (4 * NT), d0 + i % (4 * NT) * 4, v);
-        else parts[blockIdx.y * plane + i] = v;
-    }
-    if (gridDim.y == 1) return;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        last = atomicAdd(a.out_tickets + blockIdx.x, 1u) == gridDim.y - 1;
-    }
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
-        f4 v = parts[i];
-        for (unsigned p = 1; p < gridDim.y; p++) v += parts[p * plane + i];
-        store(i / (4 * NT), d0 + i % (4 * NT) * 4, v);
     }
 }
 
 // What a call launches, by its sizes.
 struct LayerPlan {
-    bool many;       // several slots an expert
-    int hidden_waves, out_tiles, out_parts, out_waves;
+    int route_parts, route_waves;
+    bool many;  // several slots an expert
 };
 
 LayerPlan layer_plan(const LayerArgs& a)
 {
     LayerPlan p{};
-    const int slots = a.tokens * a.topk, experts = std::min(a.experts, slots);
-    p.many = slots >= 4 * experts;
-    p.hidden_waves = std::min(kLayerWaves, a.dim_pad / 128);
-    const int nt = p.many ? 2 : 1, items = experts * (a.hidden_pad / 128);
-    p.out_tiles = (a.dim + 16 * nt - 1) / (16 * nt);
-    p.out_waves = std::min(kLayerWaves, items);
-    p.out_parts = std::max(1, std::min((2 * num_cus() + p.out_tiles - 1) / p.out_tiles, items / (4 * kLayerWaves)));
+    const int slots = a.tokens * a.topk, blocks = a.dim_pad / 128, groups = (a.experts + 15) / 16;
+    p.route_parts = std::max(1, std::min({blocks / 4, 128 / groups, kRouteParts}));
+    p.route_waves = std::min(kRouteWaves, std::max(4 * ((blocks + p.route_parts - 1) / p.route_parts), a.tokens));
+    p.many = slots >= 4 * std::min(a.experts, slots);
     return p;
 }
 
@@ -679,45 +776,63 @@ void allow_lds(const void* kernel, size_t lds)
     if (lds > 64 * 1024) GRAFT_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
 }
 
-template <int FORMAT, class T, int G, int NT, int CT>
-void hidden_launch(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
+template <int FORMAT, class T, int G, int NT, int CT, int WAVES>
+void hidden_launch(const LayerArgs& a, hipStream_t s)
 {
     const unsigned most = (unsigned)std::min(a.experts, a.tokens * a.topk);
-    layer_hidden_kernel<FORMAT, T, G, NT, CT><<<dim3(a.hidden_pad / (16 * NT), most), p.hidden_waves * 64, 0, s>>>(a);
+    layer_hidden_kernel<FORMAT, T, G, NT, CT, WAVES><<<dim3(a.hidden_pad / (16 * NT), most), WAVES * 64, 0, s>>>(a);
     GRAFT_LAUNCH_CHECK();
 }
 
-template <int FORMAT, class T, int NT, int CT>
-void out_launch(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
+template <int FORMAT, class T, int NT, int CT, int WAVES, int DEPTH>
+void out_launch(const LayerArgs& a, hipStream_t s)
 {
     const int slots = a.tokens * a.topk, most = std::min(a.experts, slots);
-    const size_t lds = (size_t)p.out_waves * a.tokens * 64 * NT + (size_t)(2 * most + 1 + slots) * 4;
-    allow_lds((const void*)layer_out_kernel<FORMAT, T, NT, CT>, lds);
-    layer_out_kernel<FORMAT, T, NT, CT><<<dim3(p.out_tiles, p.out_parts), p.out_waves * 64, lds, s>>>(a);
+    const size_t lds = (size_t)WAVES * a.tokens * 64 * NT + (size_t)(2 * most + 1 + 2 * slots) * 4;
+    allow_lds((const void*)layer_out_kernel<FORMAT, T, NT, CT, WAVES, DEPTH>, lds);
+    layer_out_kernel<FORMAT, T, NT, CT, WAVES, DEPTH><<<(a.dim + 16 * NT - 1) / (16 * NT), WAVES * 64, lds, s>>>(a);
     GRAFT_LAUNCH_CHECK();
 }
 
 template <class T, class R, int MT>
-void route_launch(const LayerArgs& a, hipStream_t s)
+void route_launch(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
-    const size_t scores = (size_t)kRouteWaves * a.experts * 4 * (a.groups > 1 ? 2 : 1);
-    const size_t lds = std::max({(size_t)kRouteWaves * MT * 1024, scores, (size_t)(a.experts + a.tokens * a.topk) * 4});
+    const unsigned groups = (a.experts + 15) / 16;
+    const int logits = a.tokens * a.experts;
+    const size_t lds = route_lds(a, p.route_waves, MT, logits <= kLogitsInLds ? logits : 0).size;
     allow_lds((const void*)layer_route_kernel<T, R, MT>, lds);
-    layer_route_kernel<T, R, MT><<<(a.experts + 15) / 16, kRouteThreads, lds, s>>>(a);
+    layer_route_kernel<T, R, MT><<<dim3(groups, p.route_parts), p.route_waves * 64, lds, s>>>(a);
     GRAFT_LAUNCH_CHECK();
 }
 
 template <int FORMAT, class T>
 void products(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
+    constexpr int CT = sizeof(T) == 4 ? 4 : 2;
+    const char* v = getenv("HV");
+    const int hv = v ? atoi(v) : 0;
     if (p.many) {
-        if (a.gated) hidden_launch<FORMAT, T, 2, 2, 2>(a, p, s);
-        else hidden_launch<FORMAT, T, 1, 4, 2>(a, p, s);
-        out_launch<FORMAT, T, 2, 2>(a, p, s);
+        if (a.gated) hidden_launch<FORMAT, T, 2, 2, CT, 8>(a, s);
+        else hidden_launch<FORMAT, T, 1, 4, CT, 8>(a, s);
+        out_launch<FORMAT, T, 2, CT, 8, 2>(a, s);
     } else {
-        if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1>(a, p, s);
-        else hidden_launch<FORMAT, T, 1, 1, 1>(a, p, s);
-        out_launch<FORMAT, T, 1, 1>(a, p, s);
+        if (hv & 1) {
+            if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1, 4>(a, s);
+            else hidden_launch<FORMAT, T, 1, 1, 1, 4>(a, s);
+        } else if (hv & 2) {
+            if (a.gated) hidden_launch<FORMAT, T, 2, 2, 1, 8>(a, s);
+            else hidden_launch<FORMAT, T, 1, 2, 1, 8>(a, s);
+        } else if (hv & 4) {
+            if (a.gated) hidden_launch<FORMAT, T, 2, 2, 1, 4>(a, s);
+            else hidden_launch<FORMAT, T, 1, 2, 1, 4>(a, s);
+        } else {
+            if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1, 8>(a, s);
+            else hidden_launch<FORMAT, T, 1, 1, 1, 8>(a, s);
+        }
+        if (hv & 16) out_launch<FORMAT, T, 1, 1, 16, 2>(a, s);
+        else if (hv & 32) out_launch<FORMAT, T, 1, 1, 16, 4>(a, s);
+        else if (hv & 64) out_launch<FORMAT, T, 1, 1, 8, 3>(a, s);
+        else out_launch<FORMAT, T, 1, 1, 16, 3>(a, s);
     }
 }
 
@@ -780,12 +895,9 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
         return at;
     };
     const size_t x_terms = o.dataType == DATA_F32 ? 3 : o.dataType == DATA_BF16 ? 1 : 2, a_terms = o.dataType == DATA_F32 ? 3 : 2;
-    const size_t at_logits = take((size_t)tokens * a.experts * 4), at_weights = take((size_t)slots * 4);
+    const size_t at_logits = take((size_t)p.route_parts * tokens * a.experts * 4), at_weights = take((size_t)slots * 4);
     const size_t at_active = take((size_t)(most + 1) * 4), at_first = take((size_t)(most + 1) * 4), at_slots = take((size_t)slots * 4);
     const size_t at_xs = take((size_t)tokens * x_terms * a.dim_pad * 2), at_acts = take((size_t)slots * a_terms * a.hidden_pad * 2);
-    const bool split = p.out_parts > 1;
-    const size_t at_parts = take(split ? (size_t)p.out_parts * p.out_tiles * tokens * (p.many ? 32 : 16) * 4 : 0);
-    const size_t at_tickets = take(split ? (size_t)(o.dim + 15) / 16 * 4 : 0);
     a.route_ticket = stream_tickets(s);
     char* ws = (char*)stream_workspace(s).get(size);
     a.logits = (float*)(ws + at_logits);
@@ -795,15 +907,11 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     a.slots = (int*)(ws + at_slots);
     a.xs = (__bf16*)(ws + at_xs);
     a.acts = (__bf16*)(ws + at_acts);
-    if (split) {
-        a.parts = (float*)(ws + at_parts);
-        a.out_tickets = (uint32_t*)(ws + at_tickets);
-    }
     with_type(o.dataType, [&](auto x) {
         using T = decltype(x);
         with_type(o.routerType, [&](auto r) {
-            if (tokens <= 16) route_launch<T, decltype(r), 1>(a, s);
-            else route_launch<T, decltype(r), 4>(a, s);
+            if (tokens <= 16) route_launch<T, decltype(r), 1>(a, p, s);
+            else route_launch<T, decltype(r), 4>(a, p, s);
         });
         if (o.weightFormat == EXPERT_FP8) products<EXPERT_FP8, T>(a, p, s);
         else products<EXPERT_FP4, T>(a, p, s);
