@@ -40,7 +40,9 @@ struct LayerArgs {
     int* active;              // number of experts that some token takes, and which
     int *first, *slots;       // where their slots begin in the list of slots, and its end
     __bf16 *xs, *acts;        // [tokens][terms][dim_pad], [slots][terms][hidden_pad]
-    uint32_t* route_ticket;
+    float* sums;              // [parts][tiles][tokens][columns of a tile], of more than one part
+    uint32_t *route_ticket, *out_tickets;
+    int out_tiles;
 };
 
 template <class T>
@@ -379,6 +381,8 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
             __syncthreads();
         }
     }
+    if (a.out_tickets)
+        for (int i = threadIdx.x; i < a.out_tiles; i += blockDim.x) a.out_tickets[i] = 0;
     with_lanes(a, [&](auto L, auto P) {
         route_tokens<decltype(L)::value, decltype(P)::value>(a, logits, parts, reinterpret_cast<float*>(lds), expert);
     });
@@ -603,14 +607,16 @@ __global__ __launch_bounds__(WAVES * 64) void layer_hidden_kernel(LayerArgs a)
     }
 }
 
-// 16 NT columns of the outputs for all tokens: the waves share out the active experts'
-// k in runs of one expert's, whose sums go, weighted, to the tokens' in the wave's part
-// of LDS; those are joined in wave order.
+// 16 NT columns of the outputs for all tokens and a part of the active experts' k, which
+// its waves share out in runs of one expert's.  Their sums go, weighted, to the
+// tokens' in the wave's part of LDS; those are joined in wave order, and the parts in
+// their order by the workgroup of a tile that is last.
 template <int FORMAT, class T, int NT, int CT, int WAVES, int DEPTH>
 __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
 {
     constexpr int A = Terms<T>::kA, kSlots = Columns<A>::kSlots;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ bool last;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int col = lane & 15, quad = lane >> 4, d0 = blockIdx.x * 16 * NT;
     const int slots = a.tokens * a.topk, most = min(a.experts, slots);
@@ -625,7 +631,8 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
     for (int i = threadIdx.x; i < WAVES * a.tokens * 4 * NT; i += WAVES * 64) sums[i] = f4zero();
     __syncthreads();
     const int blocks = a.hidden_pad / 128, items = number * blocks;  // at most 2^10 * 2^7
-    const int begin = items * wave / WAVES, end = items * (wave + 1) / WAVES;
+    const int workers = WAVES * gridDim.y, worker = blockIdx.y * WAVES + wave;
+    const int begin = (int)((long long)items * worker / workers), end = (int)((long long)items * (worker + 1) / workers);
     int row[NT];
 #pragma unroll
     for (int f = 0; f < NT; f++) row[f] = min(d0 + f * 16 + col, a.dim - 1);
@@ -735,10 +742,7 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
     }
     __syncthreads();
     const int pieces = a.tokens * 4 * NT;
-    for (int i = threadIdx.x; i < pieces; i += WAVES * 64) {
-        f4 v = sums[i];
-#pragma unroll
-        for (int w = 1; w < WAVES; w++) v += sums[w * pieces + i];
+    auto store = [&](int i, f4 v) {
         const int t = i / (4 * NT), d = d0 + i % (4 * NT) * 4;
         T* to = (T*)a.out + t * a.stride_out + d;
         if (a.vec_out && d + 4 <= a.dim) {
@@ -751,6 +755,37 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
             for (int j = 0; j < 4; j++)
                 if (d + j < a.dim) to[j] = (T)v[j];
         }
+    };
+    // Parts are written and read past the L2, which the XCDs do not share, word by word
+    // as atomics of the device's scope: a release fence, which writes back all of the
+    // L2, took 256 workgroups 11 us and 512 of them 21.
+    const long long plane = (long long)gridDim.x * pieces * 4;
+    float* const parts = a.sums + (long long)blockIdx.x * pieces * 4;
+    for (int i = threadIdx.x; i < pieces; i += WAVES * 64) {
+        f4 v = sums[i];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) v += sums[w * pieces + i];
+        if (gridDim.y == 1) store(i, v);
+        else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                __hip_atomic_store(parts + blockIdx.y * plane + i * 4 + j, v[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    if (gridDim.y == 1) return;
+    __builtin_amdgcn_s_waitcnt(kCopiesDone);  // written when the counter says so
+    __syncthreads();
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(a.out_tickets + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.y - 1;
+    __syncthreads();
+    if (!last) return;
+    for (int i = threadIdx.x; i < pieces; i += WAVES * 64) {
+        f4 v = f4zero();
+        for (unsigned p = 0; p < gridDim.y; p++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                v[j] += __hip_atomic_load(parts + p * plane + i * 4 + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        store(i, v);
     }
 }
 
@@ -758,6 +793,7 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
 struct LayerPlan {
     int route_parts, route_waves;
     bool many;  // several slots an expert
+    int out_tiles, out_parts;
 };
 
 LayerPlan layer_plan(const LayerArgs& a)
@@ -766,7 +802,12 @@ LayerPlan layer_plan(const LayerArgs& a)
     const int slots = a.tokens * a.topk, blocks = a.dim_pad / 128, groups = (a.experts + 15) / 16;
     p.route_parts = std::max(1, std::min({blocks / 4, 128 / groups, kRouteParts}));
     p.route_waves = std::min(kRouteWaves, std::max(4 * ((blocks + p.route_parts - 1) / p.route_parts), a.tokens));
-    p.many = slots >= 4 * std::min(a.experts, slots);
+    const int most = std::min(a.experts, slots);
+    p.many = slots >= 4 * most;
+    p.out_tiles = (a.dim + (p.many ? 31 : 15)) / (p.many ? 32 : 16);
+    const char* v = getenv("SP");
+    const int sp = v ? atoi(v) : 2;
+    p.out_parts = std::max(1, std::min((sp * num_cus() + p.out_tiles - 1) / p.out_tiles, most * (a.hidden_pad / 128) / 32));
     return p;
 }
 
@@ -785,12 +826,12 @@ void hidden_launch(const LayerArgs& a, hipStream_t s)
 }
 
 template <int FORMAT, class T, int NT, int CT, int WAVES, int DEPTH>
-void out_launch(const LayerArgs& a, hipStream_t s)
+void out_launch(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
     const int slots = a.tokens * a.topk, most = std::min(a.experts, slots);
     const size_t lds = (size_t)WAVES * a.tokens * 64 * NT + (size_t)(2 * most + 1 + 2 * slots) * 4;
     allow_lds((const void*)layer_out_kernel<FORMAT, T, NT, CT, WAVES, DEPTH>, lds);
-    layer_out_kernel<FORMAT, T, NT, CT, WAVES, DEPTH><<<(a.dim + 16 * NT - 1) / (16 * NT), WAVES * 64, lds, s>>>(a);
+    layer_out_kernel<FORMAT, T, NT, CT, WAVES, DEPTH><<<dim3(p.out_tiles, p.out_parts), WAVES * 64, lds, s>>>(a);
     GRAFT_LAUNCH_CHECK();
 }
 
@@ -809,30 +850,14 @@ template <int FORMAT, class T>
 void products(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
     constexpr int CT = sizeof(T) == 4 ? 4 : 2;
-    const char* v = getenv("HV");
-    const int hv = v ? atoi(v) : 0;
     if (p.many) {
         if (a.gated) hidden_launch<FORMAT, T, 2, 2, CT, 8>(a, s);
         else hidden_launch<FORMAT, T, 1, 4, CT, 8>(a, s);
-        out_launch<FORMAT, T, 2, CT, 8, 2>(a, s);
+        out_launch<FORMAT, T, 2, CT, 8, 2>(a, p, s);
     } else {
-        if (hv & 1) {
-            if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1, 4>(a, s);
-            else hidden_launch<FORMAT, T, 1, 1, 1, 4>(a, s);
-        } else if (hv & 2) {
-            if (a.gated) hidden_launch<FORMAT, T, 2, 2, 1, 8>(a, s);
-            else hidden_launch<FORMAT, T, 1, 2, 1, 8>(a, s);
-        } else if (hv & 4) {
-            if (a.gated) hidden_launch<FORMAT, T, 2, 2, 1, 4>(a, s);
-            else hidden_launch<FORMAT, T, 1, 2, 1, 4>(a, s);
-        } else {
-            if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1, 8>(a, s);
-            else hidden_launch<FORMAT, T, 1, 1, 1, 8>(a, s);
-        }
-        if (hv & 16) out_launch<FORMAT, T, 1, 1, 16, 2>(a, s);
-        else if (hv & 32) out_launch<FORMAT, T, 1, 1, 16, 4>(a, s);
-        else if (hv & 64) out_launch<FORMAT, T, 1, 1, 8, 3>(a, s);
-        else out_launch<FORMAT, T, 1, 1, 16, 3>(a, s);
+        if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1, 4>(a, s);
+        else hidden_launch<FORMAT, T, 1, 1, 1, 4>(a, s);
+        out_launch<FORMAT, T, 1, 1, 8, 3>(a, p, s);
     }
 }
 
@@ -898,6 +923,9 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     const size_t at_logits = take((size_t)p.route_parts * tokens * a.experts * 4), at_weights = take((size_t)slots * 4);
     const size_t at_active = take((size_t)(most + 1) * 4), at_first = take((size_t)(most + 1) * 4), at_slots = take((size_t)slots * 4);
     const size_t at_xs = take((size_t)tokens * x_terms * a.dim_pad * 2), at_acts = take((size_t)slots * a_terms * a.hidden_pad * 2);
+    const bool split = p.out_parts > 1;
+    const size_t at_sums = take(split ? (size_t)p.out_parts * p.out_tiles * tokens * (p.many ? 32 : 16) * 4 : 0);
+    const size_t at_tickets = take(split ? (size_t)p.out_tiles * 4 : 0);
     a.route_ticket = stream_tickets(s);
     char* ws = (char*)stream_workspace(s).get(size);
     a.logits = (float*)(ws + at_logits);
@@ -907,6 +935,11 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     a.slots = (int*)(ws + at_slots);
     a.xs = (__bf16*)(ws + at_xs);
     a.acts = (__bf16*)(ws + at_acts);
+    if (split) {
+        a.sums = (float*)(ws + at_sums);
+        a.out_tickets = (uint32_t*)(ws + at_tickets);
+        a.out_tiles = p.out_tiles;
+    }
     with_type(o.dataType, [&](auto x) {
         using T = decltype(x);
         with_type(o.routerType, [&](auto r) {
