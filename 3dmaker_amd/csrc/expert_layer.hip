@@ -96,6 +96,23 @@ __device__ __forceinline__ void split8(const T (&v)[8], bf16x8 (&t)[N])
     }
 }
 
+// What workgroups of a launch leave for the last of them goes past the L2, which the
+// XCDs do not share, word by word as atomics of the device's scope.  A release fence,
+// which writes back all of an L2, took 256 workgroups 11 us and 512 of them 21.
+__device__ __forceinline__ void store_past(float* p, float v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float load_past(const float* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Whether the workgroup is the last of `number` to come here.  Its stores have been
+// made by then: the memory counter says when they are.
+__device__ __forceinline__ bool is_last(uint32_t* ticket, uint32_t number, bool* shared)
+{
+    __builtin_amdgcn_s_waitcnt(kCopiesDone);
+    __syncthreads();
+    if (threadIdx.x == 0) *shared = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == number - 1;
+    __syncthreads();
+    return *shared;
+}
+
 // ---------------------------------------------------------------------------
 // routing
 // ---------------------------------------------------------------------------
@@ -126,11 +143,11 @@ __device__ __forceinline__ void route_tokens(const LayerArgs& a, const float* lo
         } else {
             const float* z = a.logits + (long long)t * a.experts + first;
 #pragma unroll
-            for (int i = 0; i < PER; i++) s[i] = i < n ? z[i] : -INFINITY;
+            for (int i = 0; i < PER; i++) s[i] = i < n ? load_past(z + i) : -INFINITY;
             for (int p = 1; p < parts; p++) {
                 z += (long long)a.tokens * a.experts;
 #pragma unroll
-                for (int i = 0; i < PER; i++) s[i] += i < n ? z[i] : 0.0f;
+                for (int i = 0; i < PER; i++) s[i] += i < n ? load_past(z + i) : 0.0f;
             }
         }
         float top = -INFINITY, sum = 0.0f;
@@ -348,20 +365,18 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
         if (t < a.tokens) {
             float* to = alone ? logits : a.logits + (long long)blockIdx.y * all;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (e0 + quad * 4 + i < a.experts) to[t * a.experts + e0 + quad * 4 + i] = v[i];
+            for (int i = 0; i < 4; i++) {
+                const int e = e0 + quad * 4 + i;
+                if (e >= a.experts) continue;
+                if (alone) to[t * a.experts + e] = v[i];
+                else store_past(to + t * a.experts + e, v[i]);
+            }
         }
     }
-    __syncthreads();
-    if (!alone) {
-        if (threadIdx.x == 0) {
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");  // what the workgroup has stored
-            last = atomicAdd(a.route_ticket, 1u) == gridDim.x * parts - 1;
-        }
-        __syncthreads();
-        if (!last) return;
+    if (alone) __syncthreads();
+    else {
+        if (!is_last(a.route_ticket, gridDim.x * parts, &last)) return;
         if (threadIdx.x == 0) *a.route_ticket = 0;
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
         if (logits) {  // all parts' loads together
             for (int i0 = threadIdx.x; i0 < all; i0 += 4 * blockDim.x) {
                 float z[4][kRouteParts];
@@ -369,7 +384,7 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
                 for (int u = 0; u < 4; u++)
 #pragma unroll
                     for (int p = 0; p < kRouteParts; p++)
-                        z[u][p] = a.logits[min(p, parts - 1) * all + min(i0 + u * (int)blockDim.x, all - 1)];
+                        z[u][p] = load_past(a.logits + min(p, parts - 1) * all + min(i0 + u * (int)blockDim.x, all - 1));
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     float v = z[u][0];
@@ -475,40 +490,52 @@ struct Columns {
     }
 };
 
-// What a wave has under way of 128 of k: F fragments of weights, CT of tokens or
-// hidden activations.
-template <int FORMAT, int F, int CT>
-struct Bundle {
+// 128 of k: a wave's F fragments of weights, and its CT of tokens or hidden
+// activations.
+template <int FORMAT, int F>
+struct Weights {
     Piece<FORMAT> w[F];
-    bf16x8 t[CT][4];
+};
 
-    __device__ __forceinline__ void load_columns(const __bf16* const (&from)[CT], int kb)
+template <int CT>
+struct Values {
+    bf16x8 t[CT][4];
+    __device__ __forceinline__ void load(const __bf16* const (&from)[CT], int kb)
     {
 #pragma unroll
         for (int j = 0; j < CT; j++)
 #pragma unroll
             for (int q = 0; q < 4; q++) t[j][q] = *reinterpret_cast<const bf16x8*>(from[j] + kb * 128 + q * 8);
     }
-    __device__ __forceinline__ void multiply(f4 (&acc)[F][CT]) const
-    {
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-#pragma unroll
-            for (int f = 0; f < F; f++) {
-                const bf16x8 b = w[f](q);
-#pragma unroll
-                for (int j = 0; j < CT; j++) acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, t[j][q], acc[f][j], 0, 0, 0);
-            }
-    }
 };
+
+template <int FORMAT, int F, int CT>
+__device__ __forceinline__ void multiply(f4 (&acc)[F][CT], const Weights<FORMAT, F>& w, const Values<CT>& v)
+{
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+        for (int f = 0; f < F; f++) {
+            const bf16x8 b = w.w[f](q);
+#pragma unroll
+            for (int j = 0; j < CT; j++) acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, v.t[j][q], acc[f][j], 0, 0, 0);
+        }
+}
 
 // The hidden activations of 16 NT rows (with their gate's: G 2) for the slots of an
 // active expert, as many at a time as CT fragments have: waves share out k, and their
 // sums are joined in LDS in wave order.  A lane whose column has no slot works on the
-// first one's for nothing.
-template <int FORMAT, class T, int G, int NT, int CT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void layer_hidden_kernel(LayerArgs a)
+// first one's for nothing.  Bound by the weights' trips from memory, of which many
+// waves a CU have more under way than few that look far ahead: four waves of two blocks
+// in registers took 53.7 us where four of four took 61.1 and eight of two 67.1 (27
+// tokens, top 4 of 128, 1024 x 1536 fp8), and 25.7, 27.9 and 29.3 (7 tokens, top 6 of
+// 64, 2048 x 1024 fp4).
+constexpr int kHiddenWaves = 4;
+
+template <int FORMAT, class T, int G, int NT, int CT>
+__global__ __launch_bounds__(kHiddenWaves * 64) void layer_hidden_kernel(LayerArgs a)
 {
+    constexpr int WAVES = kHiddenWaves;
     constexpr int X = Terms<T>::kX, A = Terms<T>::kA, F = G * NT, kSlots = Columns<X>::kSlots;
     __shared__ f4 sums[WAVES][F][CT][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -536,38 +563,33 @@ __global__ __launch_bounds__(WAVES * 64) void layer_hidden_kernel(LayerArgs a)
 #pragma unroll
             for (int f = 0; f < F; f++) acc[f][j] = f4zero();
         }
-        using Part = Bundle<FORMAT, F, CT>;
-        // Columns of several fragments are read when their turn comes, from the L2: ahead
-        // they would not fit the registers.
-        auto load = [&](Part& b, int kb) {
+        // Weights of the next block are under way, and values, which are in the L2, where
+        // they cost no wave its place.
+        constexpr int VALUES = CT == 1 ? 2 : 1;
+        Weights<FORMAT, F> b[2];
+        Values<CT> v[VALUES];
+        auto load_weights = [&](Weights<FORMAT, F>& to, int kb) {
 #pragma unroll
-            for (int f = 0; f < F; f++) b.w[f].load(W[f], S[f], kb, quad);
-            if (CT == 1) b.load_columns(x, kb);
+            for (int f = 0; f < F; f++) to.w[f].load(W[f], S[f], kb, quad);
         };
-        auto multiply = [&](Part& b, int kb) {
-            if (CT > 1) b.load_columns(x, kb);
-            b.multiply(acc);
-        };
-        Part b0, b1;
-        int kb = wave;
-        if (kb < blocks) {
-#pragma unroll
-            for (int f = 0; f < F; f++) b0.w[f].load(W[f], S[f], kb, quad);  // they need no slots
-        }
+        if (wave < blocks) load_weights(b[0], wave);  // they need no slots
 #pragma unroll
         for (int j = 0; j < CT; j++) {
             const int token = (slot[j] >= 0 ? slot[j] : a.slots[first]) / a.topk;
             x[j] = a.xs + ((long long)token * X + (slot[j] >= 0 ? mine.term : 0)) * a.dim_pad + quad * 32;
         }
-        if (CT == 1 && kb < blocks) b0.load_columns(x, kb);
-        while (kb < blocks) {
-            if (kb + WAVES < blocks) load(b1, kb + WAVES);
-            multiply(b0, kb);
-            kb += WAVES;
-            if (kb >= blocks) break;
-            if (kb + WAVES < blocks) load(b0, kb + WAVES);
-            multiply(b1, kb);
-            kb += WAVES;
+        if (VALUES > 1 && wave < blocks) v[0].load(x, wave);
+        for (int kb = wave; kb < blocks;) {
+            each<2>([&](auto D) {
+                constexpr int d = decltype(D)::value;
+                if (kb >= blocks) return;
+                const bool more = kb + WAVES < blocks;
+                if (VALUES == 1) v[0].load(x, kb);
+                else if (more) v[(d + 1) % VALUES].load(x, kb + WAVES);
+                if (more) load_weights(b[1 - d], kb + WAVES);
+                multiply(acc, b[d], v[d % VALUES]);
+                kb += WAVES;
+            });
         }
         if (s0 > 0) __syncthreads();
 #pragma unroll
@@ -660,7 +682,10 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
         const int f0 = first[c.at], i = c.s0 + j * kSlots + mine.slot;
         return mine.slot < kSlots && i < first[c.at + 1] - f0 ? list[f0 + i] : -1;
     };
-    using Part = Bundle<FORMAT, NT, CT>;
+    struct Part {
+        Weights<FORMAT, NT> w;
+        Values<CT> v;
+    };
     const uint8_t *W[NT], *S[NT];
     const __bf16* act[CT];
     auto load = [&](Part& b, const Cursor& c) {
@@ -679,8 +704,8 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
             }
         }
 #pragma unroll
-        for (int f = 0; f < NT; f++) b.w[f].load(W[f], S[f], c.kb, quad);
-        b.load_columns(act, c.kb);
+        for (int f = 0; f < NT; f++) b.w.w[f].load(W[f], S[f], c.kb, quad);
+        b.v.load(act, c.kb);
     };
     f4 own[NT][CT];
     auto finish_run = [&](const Cursor& c) {
@@ -733,7 +758,7 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
 #pragma unroll
                         for (int f = 0; f < NT; f++) own[f][j] = f4zero();
                 }
-                b[d].multiply(own);
+                multiply(own, b[d].w, b[d].v);
                 if (now.last_of_run()) finish_run(now);
                 advance(now);
                 more = now.valid();
@@ -756,9 +781,6 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
                 if (d + j < a.dim) to[j] = (T)v[j];
         }
     };
-    // Parts are written and read past the L2, which the XCDs do not share, word by word
-    // as atomics of the device's scope: a release fence, which writes back all of the
-    // L2, took 256 workgroups 11 us and 512 of them 21.
     const long long plane = (long long)gridDim.x * pieces * 4;
     float* const parts = a.sums + (long long)blockIdx.x * pieces * 4;
     for (int i = threadIdx.x; i < pieces; i += WAVES * 64) {
@@ -769,22 +791,16 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
         else {
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                __hip_atomic_store(parts + blockIdx.y * plane + i * 4 + j, v[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                store_past(parts + blockIdx.y * plane + i * 4 + j, v[j]);
         }
     }
-    if (gridDim.y == 1) return;
-    __builtin_amdgcn_s_waitcnt(kCopiesDone);  // written when the counter says so
-    __syncthreads();
-    if (threadIdx.x == 0)
-        last = __hip_atomic_fetch_add(a.out_tickets + blockIdx.x, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.y - 1;
-    __syncthreads();
-    if (!last) return;
+    if (gridDim.y == 1 || !is_last(a.out_tickets + blockIdx.x, gridDim.y, &last)) return;
     for (int i = threadIdx.x; i < pieces; i += WAVES * 64) {
         f4 v = f4zero();
         for (unsigned p = 0; p < gridDim.y; p++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                v[j] += __hip_atomic_load(parts + p * plane + i * 4 + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                v[j] += load_past(parts + p * plane + i * 4 + j);
         store(i, v);
     }
 }
@@ -805,9 +821,10 @@ LayerPlan layer_plan(const LayerArgs& a)
     const int most = std::min(a.experts, slots);
     p.many = slots >= 4 * most;
     p.out_tiles = (a.dim + (p.many ? 31 : 15)) / (p.many ? 32 : 16);
-    const char* v = getenv("SP");
-    const int sp = v ? atoi(v) : 2;
-    p.out_parts = std::max(1, std::min((sp * num_cus() + p.out_tiles - 1) / p.out_tiles, most * (a.hidden_pad / 128) / 32));
+    // A workgroup a CU, each wave with four blocks of k at least.  More parts cost more to
+    // join than they help (7 tokens of 64 experts, top 6, 2048 x 1024: 19.1 us in two
+    // parts, 20.1 in four, 23.6 in eight, 28 in one).
+    p.out_parts = std::max(1, std::min((num_cus() + p.out_tiles - 1) / p.out_tiles, most * (a.hidden_pad / 128) / 32));
     return p;
 }
 
@@ -817,11 +834,11 @@ void allow_lds(const void* kernel, size_t lds)
     if (lds > 64 * 1024) GRAFT_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
 }
 
-template <int FORMAT, class T, int G, int NT, int CT, int WAVES>
+template <int FORMAT, class T, int G, int NT, int CT>
 void hidden_launch(const LayerArgs& a, hipStream_t s)
 {
     const unsigned most = (unsigned)std::min(a.experts, a.tokens * a.topk);
-    layer_hidden_kernel<FORMAT, T, G, NT, CT, WAVES><<<dim3(a.hidden_pad / (16 * NT), most), WAVES * 64, 0, s>>>(a);
+    layer_hidden_kernel<FORMAT, T, G, NT, CT><<<dim3(a.hidden_pad / (16 * NT), most), kHiddenWaves * 64, 0, s>>>(a);
     GRAFT_LAUNCH_CHECK();
 }
 
@@ -851,12 +868,12 @@ void products(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
     constexpr int CT = sizeof(T) == 4 ? 4 : 2;
     if (p.many) {
-        if (a.gated) hidden_launch<FORMAT, T, 2, 2, CT, 8>(a, s);
-        else hidden_launch<FORMAT, T, 1, 4, CT, 8>(a, s);
+        if (a.gated) hidden_launch<FORMAT, T, 2, 1, CT>(a, s);
+        else hidden_launch<FORMAT, T, 1, 2, CT>(a, s);
         out_launch<FORMAT, T, 2, CT, 8, 2>(a, p, s);
     } else {
-        if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1, 4>(a, s);
-        else hidden_launch<FORMAT, T, 1, 1, 1, 4>(a, s);
+        if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1>(a, s);
+        else hidden_launch<FORMAT, T, 1, 1, 1>(a, s);
         out_launch<FORMAT, T, 1, 1, 8, 3>(a, p, s);
     }
 }
