@@ -281,11 +281,14 @@ __device__ __forceinline__ void plan(const LayerArgs& a, const int* expert, int*
 }
 
 // LDS of the routing kernel: sums of its waves, then scores and keys, then the plan's
-// counts, in one place; the slots' experts; the logits.
+// counts, in one place; the slots' experts; the logits, if there is room for them: they
+// are read token by token if not.
+constexpr int kLdsBytes = 160 * 1024 - 64;  // with what the kernel declares itself
 struct RouteLds {
     int experts_at, logits_at, size;
+    bool logits;
 };
-__host__ __device__ inline RouteLds route_lds(const LayerArgs& a, int waves, int tiles, int logits)
+__host__ __device__ inline RouteLds route_lds(const LayerArgs& a, int waves, int tiles)
 {
     int scores = 0;
     with_lanes(a, [&](auto, auto P) { scores = waves * 64 * 4 * (a.groups > 1 ? 2 * decltype(P)::value + 1 : decltype(P)::value); });
@@ -294,10 +297,10 @@ __host__ __device__ inline RouteLds route_lds(const LayerArgs& a, int waves, int
     l.experts_at = sums > scores ? sums : scores;
     if (counts > l.experts_at) l.experts_at = counts;
     l.logits_at = l.experts_at + a.tokens * a.topk * 4;
-    l.size = l.logits_at + logits * 4;
+    l.logits = l.logits_at + a.tokens * a.experts * 4 <= kLdsBytes;
+    l.size = l.logits_at + (l.logits ? a.tokens * a.experts * 4 : 0);
     return l;
 }
-constexpr int kLogitsInLds = 16384;  // more of them are read token by token
 constexpr int kRouteParts = 8;
 
 // Logits of 16 experts over a part of k that the waves share out; the tokens' terms on
@@ -317,10 +320,10 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
     const int blocks = a.dim_pad / 128, parts = gridDim.y;
     const int kb0 = blocks * blockIdx.y / parts, kb1 = blocks * (blockIdx.y + 1) / parts;
     const bool alone = gridDim.x * parts == 1;
-    const RouteLds at = route_lds(a, waves, MT, 0);
+    const RouteLds at = route_lds(a, waves, MT);
     int* const expert = reinterpret_cast<int*>(lds + at.experts_at);
     const int all = a.tokens * a.experts;
-    float* const logits = all <= kLogitsInLds ? reinterpret_cast<float*>(lds + at.logits_at) : nullptr;
+    float* const logits = at.logits ? reinterpret_cast<float*>(lds + at.logits_at) : nullptr;
     f4 acc[MT];
 #pragma unroll
     for (int j = 0; j < MT; j++) acc[j] = f4zero();
@@ -856,8 +859,7 @@ template <class T, class R, int MT>
 void route_launch(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
     const unsigned groups = (a.experts + 15) / 16;
-    const int logits = a.tokens * a.experts;
-    const size_t lds = route_lds(a, p.route_waves, MT, logits <= kLogitsInLds ? logits : 0).size;
+    const size_t lds = route_lds(a, p.route_waves, MT).size;
     allow_lds((const void*)layer_route_kernel<T, R, MT>, lds);
     layer_route_kernel<T, R, MT><<<dim3(groups, p.route_parts), p.route_waves * 64, lds, s>>>(a);
     GRAFT_LAUNCH_CHECK();

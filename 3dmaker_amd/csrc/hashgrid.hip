@@ -441,21 +441,22 @@ __global__ void zero_tickets_kernel(uint32_t* t) { t[threadIdx.x] = 0; }
 
 struct Tickets {
     uint32_t* p = nullptr;
+    bool in_graphs = false;
     Tickets() = default;
     Tickets(const Tickets&) = delete;
     Tickets& operator=(const Tickets&) = delete;
     ~Tickets()
     {
-        if (p) (void)hipFree(p);
+        if (p && !in_graphs) (void)hipFree(p);  // graphs may outlive the thread
     }
     uint32_t* get(hipStream_t s)
     {
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        const bool capturing = hipStreamIsCapturing(s, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
+        if (capturing) (void)hipGetLastError();
+        in_graphs |= capturing;
         if (!p) {
-            hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-            if (hipStreamIsCapturing(s, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
-                (void)hipGetLastError();
-                throw std::runtime_error("the first call of this kind on a stream cannot be captured: make one before");
-            }
+            if (capturing) throw std::runtime_error("the first call of this kind on a stream cannot be captured: make one before");
             uint32_t* fresh = nullptr;
             GRAFT_HIP_CHECK(hipMalloc(&fresh, kStreamTickets * sizeof(uint32_t)));
             p = fresh;

@@ -35,6 +35,8 @@ class Layer:
             if gap > 1e-4:
                 break
             x = R.randn(g, T, D).to(S.DT[code])
+        else:
+            self.indices, self.weights, _ = self.routes(x)
         self.x = R.strided(x, pad_x, shift)
         self.buf = torch.full((shift + T * (D + pad_o) + 5,), -7.0, dtype=S.DT[code], device="cuda")
         self.out = self.buf[shift:shift + T * (D + pad_o)].view(T, D + pad_o)
@@ -90,6 +92,16 @@ def test_activations(act, gated, fmt):
 def test_routes(T, E, k, route):
     for bias in (False, True):
         Layer(T, E, k, 64, 40, act=2, gated=True, fmt=1, code=2, bias=bias, seed=3, **route).check()
+
+
+@pytest.mark.parametrize("T,E,k,route", [
+    (16, 1024, 4, dict(numGroups=8, topGroups=4, scoreType=1)), (64, 1024, 32, dict(numGroups=64, topGroups=9, groupScore=1)),
+    (40, 512, 20, dict(numGroups=64, topGroups=32)), (64, 300, 2, {}), (64, 1024, 1, dict(scoreType=1)),
+    (6, 64, 24, {}), (11, 64, 3, dict(numGroups=32, topGroups=7)), (13, 128, 6, dict(numGroups=64, topGroups=20, groupScore=1)),
+    (64, 8, 8, {}), (1, 1024, 32, dict(numGroups=2, topGroups=1))])
+def test_routes_of_many_experts_groups_and_picks(T, E, k, route):
+    """Every width of a token's lanes; logits that have room beside scores and keys in LDS, and such as have not."""
+    Layer(T, E, k, 160, 24, fmt=1, code=1, router=1, seed=12, **route).check()
 
 
 @pytest.mark.parametrize("code", [0, 1, 2])
