@@ -32,7 +32,7 @@ struct LayerArgs {
     int tokens, experts, topk, dim, hidden, activation;
     int groups, kept, group_best;
     float scale;
-    bool sigmoid, renorm, gated, vec_x, vec_router, vec_out;
+    bool sigmoid, renorm, gated, fp4, vec_x, vec_router, vec_out;
     int scale_shift;          // rows of a scale, as a shift
     int dim_pad, hidden_pad;  // filled up to whole blocks of 128
     // scratch
@@ -63,6 +63,16 @@ __device__ __forceinline__ void split(float v, __bf16 (&t)[N])
         v = __builtin_isinf(v) ? 0.0f : v - cut;
     }
     t[N - 1] = (__bf16)v;
+}
+
+// Where eight consecutive k, k % 8 == 0, of a block of 128 stand among a token's terms
+// or a slot's activations: the order in which the lanes load them beside the weights,
+// so that a load of 16 rows takes 64 consecutive bytes of each.  Lane quarter `quad`
+// has bytes 16 quad .. 16 quad + 15 of 64 of a row of weights: 16 k of e4m3, 32 of fp4.
+__device__ __forceinline__ int place_of(int k, bool fp4)
+{
+    const int in = k & 127;
+    return k - in + (fp4 ? (in / 8 % 4) * 32 + in / 32 * 8 : (in / 64 * 2 + in / 8 % 2) * 32 + in / 16 % 4 * 8);
 }
 
 // Eight consecutive elements, zero from the n-th on.
@@ -354,7 +364,7 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
             if (kb % gridDim.x == blockIdx.x && t < a.tokens) {
 #pragma unroll
                 for (int m = 0; m < X; m++)
-                    *reinterpret_cast<bf16x8*>(a.xs + ((long long)t * X + m) * a.dim_pad + k) = x[m];
+                    *reinterpret_cast<bf16x8*>(a.xs + ((long long)t * X + m) * a.dim_pad + place_of(k, a.fp4)) = x[m];
             }
         }
     }
@@ -412,8 +422,8 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
 // the experts' products
 // ---------------------------------------------------------------------------
 
-// A lane's 32 of the 128 k of a row: those from 32 quad on, eight to a matrix
-// instruction.
+// A lane's 32 of the 128 k of a row, eight to a matrix instruction: which eight is
+// place_of's order.
 template <int FORMAT>
 struct Piece;
 
@@ -423,8 +433,8 @@ struct Piece<EXPERT_FP8> {
     int byte;
     __device__ __forceinline__ void load(const uint8_t* row, const uint8_t* scales, int kb, int quad)
     {
-        v[0] = *reinterpret_cast<const i4v*>(row + kb * 128 + quad * 32);
-        v[1] = *reinterpret_cast<const i4v*>(row + kb * 128 + quad * 32 + 16);
+        v[0] = *reinterpret_cast<const i4v*>(row + kb * 128 + quad * 16);
+        v[1] = *reinterpret_cast<const i4v*>(row + kb * 128 + 64 + quad * 16);
         byte = scales[kb];
     }
     __device__ __forceinline__ bf16x8 operator()(int q) const
@@ -508,7 +518,7 @@ struct Values {
 #pragma unroll
         for (int j = 0; j < CT; j++)
 #pragma unroll
-            for (int q = 0; q < 4; q++) t[j][q] = *reinterpret_cast<const bf16x8*>(from[j] + kb * 128 + q * 8);
+            for (int q = 0; q < 4; q++) t[j][q] = *reinterpret_cast<const bf16x8*>(from[j] + kb * 128 + q * 32);
     }
 };
 
@@ -579,7 +589,7 @@ __global__ __launch_bounds__(kHiddenWaves * 64) void layer_hidden_kernel(LayerAr
 #pragma unroll
         for (int j = 0; j < CT; j++) {
             const int token = (slot[j] >= 0 ? slot[j] : a.slots[first]) / a.topk;
-            x[j] = a.xs + ((long long)token * X + (slot[j] >= 0 ? mine.term : 0)) * a.dim_pad + quad * 32;
+            x[j] = a.xs + ((long long)token * X + (slot[j] >= 0 ? mine.term : 0)) * a.dim_pad + quad * 8;
         }
         if (VALUES > 1 && wave < blocks) v[0].load(x, wave);
         for (int kb = wave; kb < blocks;) {
@@ -625,7 +635,7 @@ __global__ __launch_bounds__(kHiddenWaves * 64) void layer_hidden_kernel(LayerAr
 #pragma unroll
                     for (int t = 0; t < A; t++) o[t][i] = s[t];
                 }
-                __bf16* to = a.acts + (long long)slot[j] * A * a.hidden_pad + row;
+                __bf16* to = a.acts + (long long)slot[j] * A * a.hidden_pad + place_of(row & ~7, FORMAT == EXPERT_FP4) + (row & 4);
 #pragma unroll
                 for (int t = 0; t < A; t++) *reinterpret_cast<Vec<__bf16, 4>*>(to + (long long)t * a.hidden_pad) = o[t];
             }
@@ -703,7 +713,7 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
             for (int j = 0; j < CT; j++) {
                 const int slot = slot_of(c, j);
                 act[j] = a.acts + ((long long)(slot >= 0 ? slot : list[first[c.at]]) * A + (slot >= 0 ? mine.term : 0)) * a.hidden_pad +
-                         quad * 32;
+                         quad * 8;
             }
         }
 #pragma unroll
@@ -923,6 +933,7 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     a.sigmoid = o.route.scoreType == ROUTE_SIGMOID;
     a.renorm = o.route.renormalize != 0;
     a.gated = o.gated != 0;
+    a.fp4 = o.weightFormat == EXPERT_FP4;
     const int bytes = data_bytes(o.dataType);
     a.vec_x = aligned16(t.x) && o.strideX * bytes % 16 == 0;
     a.vec_router = aligned16(t.router) && (long long)o.dim * data_bytes(o.routerType) % 16 == 0;
