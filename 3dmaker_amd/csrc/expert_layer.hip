@@ -39,7 +39,8 @@ struct LayerArgs {
     float *logits, *weights;  // [parts][tokens][experts], [slots]
     int* active;              // number of experts that some token takes, and which
     int *first, *slots;       // where their slots begin in the list of slots, and its end
-    __bf16 *xs, *acts;        // [tokens][terms][dim_pad], [slots][terms][hidden_pad]
+    __bf16 *xs, *acts;        // [tokens][terms][dim_pad], [slots][terms][hidden_pad] or fragments
+    __bf16* frags;            // [fragments][dim_pad / 128][4][64][8]
     float* sums;              // [parts][tiles][tokens][columns of a tile], of more than one part
     uint32_t *route_ticket, *out_tickets;
     int out_tiles;
@@ -422,22 +423,30 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
 // the experts' products
 // ---------------------------------------------------------------------------
 
-// A lane's 32 of the 128 k of a row, eight to a matrix instruction: which eight is
-// place_of's order.
+// A wave's copies of weights: 16 rows by 64 bytes each, four consecutive lanes a row, so
+// that the vector memory unit takes 16 cycles for them.  A load in the order of the
+// matrix instruction, whose consecutive lanes have rows of their own, takes it 64,
+// which was what bounded these kernels.  Piece p of row r goes to place p ^ key(r) of
+// the row's four: a quarter of a 16-byte read from LDS then meets each bank once.
+constexpr int kCopyBytes = 1024;
+__device__ __forceinline__ int copy_key(int row) { return -(row >> 2) & 3; }
+
+// A lane's 32 of the 128 k of a row, from the copies of a block; eight to a matrix
+// instruction: which eight is place_of's order.
 template <int FORMAT>
 struct Piece;
 
 template <>
 struct Piece<EXPERT_FP8> {
+    static constexpr int kCopies = 2;
     i4v v[2];
-    int byte;
-    __device__ __forceinline__ void load(const uint8_t* row, const uint8_t* scales, int kb, int quad)
+    __device__ __forceinline__ void read(const uint8_t* lds, int at)
     {
-        v[0] = *reinterpret_cast<const i4v*>(row + kb * 128 + quad * 16);
-        v[1] = *reinterpret_cast<const i4v*>(row + kb * 128 + 64 + quad * 16);
-        byte = scales[kb];
+        v[0] = *reinterpret_cast<const i4v*>(lds + at);
+        v[1] = *reinterpret_cast<const i4v*>(lds + at + kCopyBytes);
     }
-    __device__ __forceinline__ bf16x8 operator()(int q) const
+    static __device__ __forceinline__ int scale(const uint8_t* scales, int kb, int) { return scales[kb]; }
+    __device__ __forceinline__ bf16x8 operator()(int q, int byte) const
     {
         return widen(v[q >> 1][2 * (q & 1)], v[q >> 1][2 * (q & 1) + 1], scale_of(byte));
     }
@@ -445,14 +454,11 @@ struct Piece<EXPERT_FP8> {
 
 template <>
 struct Piece<EXPERT_FP4> {
+    static constexpr int kCopies = 1;
     i4v v;
-    int byte;
-    __device__ __forceinline__ void load(const uint8_t* row, const uint8_t* scales, int kb, int quad)
-    {
-        v = *reinterpret_cast<const i4v*>(row + kb * 64 + quad * 16);
-        byte = scales[kb * 4 + quad];
-    }
-    __device__ __forceinline__ bf16x8 operator()(int q) const
+    __device__ __forceinline__ void read(const uint8_t* lds, int at) { v = *reinterpret_cast<const i4v*>(lds + at); }
+    static __device__ __forceinline__ int scale(const uint8_t* scales, int kb, int quad) { return scales[kb * 4 + quad]; }
+    __device__ __forceinline__ bf16x8 operator()(int q, int byte) const
     {
         const float scale = byte == 255 ? __builtin_bit_cast(float, 0x7fc00000) : scale_of(byte);
         const uint32_t w = (uint32_t)v[q];
@@ -503,36 +509,82 @@ struct Columns {
     }
 };
 
-// 128 of k: a wave's F fragments of weights, and its CT of tokens or hidden
-// activations.
-template <int FORMAT, int F>
-struct Weights {
-    Piece<FORMAT> w[F];
-};
-
+// 128 of k of a wave's CT fragments of tokens or hidden activations, from where the
+// lane's are: 32 elements to a row of STEP.  With one fragment they are in rows; with
+// several, which cost more than the weights, as fragments: the lanes' pieces of 16
+// bytes one behind the other, 1 KB to a load.
 template <int CT>
 struct Values {
+    static constexpr int kStep = CT == 1 ? 32 : 512, kBlock = 4 * kStep;  // to the next load's, to the next block's
     bf16x8 t[CT][4];
-    __device__ __forceinline__ void load(const __bf16* const (&from)[CT], int kb)
+    __device__ __forceinline__ void load(const __bf16* const (&from)[CT], int kb, int used)
     {
 #pragma unroll
         for (int j = 0; j < CT; j++)
+            if (j == 0 || j < used)
 #pragma unroll
-            for (int q = 0; q < 4; q++) t[j][q] = *reinterpret_cast<const bf16x8*>(from[j] + kb * 128 + q * 32);
+                for (int q = 0; q < 4; q++) t[j][q] = *reinterpret_cast<const bf16x8*>(from[j] + (long long)kb * kBlock + q * kStep);
     }
 };
 
+// Fragments of an expert's slots, the n-th active one's, whose slots begin at `first`:
+// the first fragment's number.  No two experts' meet: the sum of ceil(c / SLOTS) over
+// the first n of them is less than first / SLOTS + n.
+template <int SLOTS>
+__device__ __forceinline__ int fragment_of(int first, int n) { return first / SLOTS + n; }
+
+// The scales of F fragments of weights.  They are loaded behind the copies of those:
+// when they are there, so are the copies.
+template <int FORMAT, int F>
+struct Scales {
+    int byte[F];
+    __device__ __forceinline__ void load(const uint8_t* const (&from)[F], int kb, int quad)
+    {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int f = 0; f < F; f++) byte[f] = Piece<FORMAT>::scale(from[f], kb, quad);
+    }
+    __device__ __forceinline__ void arrive()
+    {
+#pragma unroll
+        for (int f = 0; f < F; f++) asm volatile("" : "+v"(byte[f])::"memory");
+    }
+};
+
+// lds: the copies of the block, those of a fragment behind the other's; at: the lane's
+// place in a copy.
 template <int FORMAT, int F, int CT>
-__device__ __forceinline__ void multiply(f4 (&acc)[F][CT], const Weights<FORMAT, F>& w, const Values<CT>& v)
+__device__ __forceinline__ void multiply(f4 (&acc)[F][CT], const uint8_t* lds, int at, const Scales<FORMAT, F>& s, const Values<CT>& v)
 {
+    Piece<FORMAT> w[F];
+#pragma unroll
+    for (int f = 0; f < F; f++) w[f].read(lds + f * (Piece<FORMAT>::kCopies * kCopyBytes), at);
 #pragma unroll
     for (int q = 0; q < 4; q++)
 #pragma unroll
         for (int f = 0; f < F; f++) {
-            const bf16x8 b = w.w[f](q);
+            const bf16x8 b = w[f](q, s.byte[f]);
 #pragma unroll
             for (int j = 0; j < CT; j++) acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, v.t[j][q], acc[f][j], 0, 0, 0);
         }
+}
+
+// Tokens' terms as fragments, block by block.
+template <class T>
+__global__ __launch_bounds__(256) void layer_gather_kernel(LayerArgs a)
+{
+    constexpr int X = Terms<T>::kX, kSlots = Columns<X>::kSlots;
+    const int n = blockIdx.y, kb = blockIdx.x, lane = threadIdx.x & 63, q = threadIdx.x >> 6;
+    if (n >= a.active[0]) return;
+    const int first = a.first[n], count = a.first[n + 1] - first;
+    const Columns<X> mine(lane & 15);
+    __bf16* to = a.frags + ((long long)fragment_of<kSlots>(first, n) * gridDim.x + kb) * 2048 + threadIdx.x * 8;
+    for (int s0 = 0; s0 < count; s0 += kSlots, to += gridDim.x * 2048) {
+        if (mine.slot >= kSlots || s0 + mine.slot >= count) continue;
+        const int token = a.slots[first + s0 + mine.slot] / a.topk;
+        *reinterpret_cast<bf16x8*>(to) = *reinterpret_cast<const bf16x8*>(
+            a.xs + ((long long)token * X + mine.term) * a.dim_pad + kb * 128 + q * 32 + (lane >> 4) * 8);
+    }
 }
 
 // The hidden activations of 16 NT rows (with their gate's: G 2) for the slots of an
@@ -548,19 +600,29 @@ constexpr int kHiddenWaves = 4;
 template <int FORMAT, class T, int G, int NT, int CT>
 __global__ __launch_bounds__(kHiddenWaves * 64) void layer_hidden_kernel(LayerArgs a)
 {
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass needs the kernel's name alone
     constexpr int WAVES = kHiddenWaves;
     constexpr int X = Terms<T>::kX, A = Terms<T>::kA, F = G * NT, kSlots = Columns<X>::kSlots;
-    __shared__ f4 sums[WAVES][F][CT][64];
+    constexpr int kCopies = Piece<FORMAT>::kCopies, kBlock = F * kCopies * kCopyBytes;
+    constexpr int kSums = WAVES * F * CT * 1024, kRings = WAVES * 2 * kBlock;
+    // One array: with two, the compiler waits for all copies before each LDS read.
+    __shared__ __attribute__((aligned(128))) uint8_t lds[kSums > kRings ? kSums : kRings];
+    f4(*const sums)[F][CT][64] = reinterpret_cast<f4(*)[F][CT][64]>(lds);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int col = lane & 15, quad = lane >> 4, n0 = blockIdx.x * 16 * NT, n = blockIdx.y;
     // one round trip for all four; behind the active experts they are of no use
     const int number = a.active[0], e = a.active[1 + n], first = a.first[n], count = a.first[n + 1] - first;
     if (n >= number) return;
-    const uint8_t *W[F], *S[F];
+    uint8_t* const ring = lds + wave * 2 * kBlock;
+    const int pitch = (int)pitch_of<FORMAT>(a.dim_pad), rows = min(16 * NT, max(a.hidden - n0, 0));
+    const uint32_t from = (lane >> 2) * pitch + ((lane & 3) ^ copy_key(lane >> 2)) * 16, at = col * 64 + (quad ^ copy_key(col)) * 16;
+    const uint8_t* const w = row_of<FORMAT>(a.w1, e, G * a.hidden, a.dim_pad, min(n0, a.hidden));
+    const auto w0 = __builtin_amdgcn_make_buffer_rsrc((void*)w, 0, rows * pitch, 0x00020000);
+    const auto w1 = __builtin_amdgcn_make_buffer_rsrc((void*)(w + (G - 1) * (long long)a.hidden * pitch), 0, rows * pitch, 0x00020000);
+    const uint8_t* S[F];
 #pragma unroll
     for (int f = 0; f < F; f++) {
         const int row = min(n0 + f % NT * 16 + col, a.hidden - 1) + f / NT * a.hidden;
-        W[f] = row_of<FORMAT>(a.w1, e, G * a.hidden, a.dim_pad, row);
         S[f] = scales_of<FORMAT>(a.s1, e, G * a.hidden, a.dim_pad, row, a.scale_shift);
     }
     const int blocks = a.dim_pad / 128;
@@ -576,41 +638,50 @@ __global__ __launch_bounds__(kHiddenWaves * 64) void layer_hidden_kernel(LayerAr
 #pragma unroll
             for (int f = 0; f < F; f++) acc[f][j] = f4zero();
         }
-        // Weights of the next block are under way, and values, which are in the L2, where
-        // they cost no wave its place.
-        constexpr int VALUES = CT == 1 ? 2 : 1;
-        Weights<FORMAT, F> b[2];
-        Values<CT> v[VALUES];
-        auto load_weights = [&](Weights<FORMAT, F>& to, int kb) {
+        const int used = (min(count - s0, kSlots * CT) + kSlots - 1) / kSlots;
+        Scales<FORMAT, F> scales[2];
+        Values<CT> v[2];
+        auto load_weights = [&](int d, Scales<FORMAT, F>& to, int kb) {
 #pragma unroll
-            for (int f = 0; f < F; f++) to.w[f].load(W[f], S[f], kb, quad);
+            for (int f = 0; f < F; f++)
+#pragma unroll
+                for (int h = 0; h < kCopies; h++)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                        f < NT ? w0 : w1, (__attribute__((address_space(3))) void*)(ring + d * kBlock + (f * kCopies + h) * kCopyBytes), 16,
+                        from + f % NT * 16 * pitch + (kb * kCopies + h) * 64, 0, 0, 0);
+            to.load(S, kb, quad);
         };
-        if (wave < blocks) load_weights(b[0], wave);  // they need no slots
+        if (wave < blocks) load_weights(0, scales[0], wave);  // they need no slots
 #pragma unroll
         for (int j = 0; j < CT; j++) {
-            const int token = (slot[j] >= 0 ? slot[j] : a.slots[first]) / a.topk;
-            x[j] = a.xs + ((long long)token * X + (slot[j] >= 0 ? mine.term : 0)) * a.dim_pad + quad * 8;
+            if (CT == 1) {
+                const int token = (slot[j] >= 0 ? slot[j] : a.slots[first]) / a.topk;
+                x[j] = a.xs + ((long long)token * X + (slot[j] >= 0 ? mine.term : 0)) * a.dim_pad + quad * 8;
+            } else x[j] = a.frags + (long long)(fragment_of<kSlots>(first, n) + s0 / kSlots + j) * blocks * 2048 + lane * 8;
         }
-        if (VALUES > 1 && wave < blocks) v[0].load(x, wave);
+        if (wave < blocks) v[0].load(x, wave, used);
         for (int kb = wave; kb < blocks;) {
             each<2>([&](auto D) {
                 constexpr int d = decltype(D)::value;
                 if (kb >= blocks) return;
-                const bool more = kb + WAVES < blocks;
-                if (VALUES == 1) v[0].load(x, kb);
-                else if (more) v[(d + 1) % VALUES].load(x, kb + WAVES);
-                if (more) load_weights(b[1 - d], kb + WAVES);
-                multiply(acc, b[d], v[d % VALUES]);
-                kb += WAVES;
+                const int next = kb + WAVES;
+                __builtin_amdgcn_s_waitcnt(kLdsDone);  // reads of the place that is copied to
+                if (next < blocks) {
+                    v[1 - d].load(x, next, used);
+                    load_weights(1 - d, scales[1 - d], next);
+                }
+                scales[d].arrive();
+                multiply(acc, ring + d * kBlock, at, scales[d], v[d]);
+                kb = next;
             });
         }
-        if (s0 > 0) __syncthreads();
+        __syncthreads();  // sums take the rings' place
 #pragma unroll
         for (int f = 0; f < F; f++)
 #pragma unroll
             for (int j = 0; j < CT; j++) sums[wave][f][j][lane] = acc[f][j];
         __syncthreads();
-        const int used = min(WAVES, blocks);
+        const int joined = min(WAVES, blocks);
 #pragma unroll
         for (int f = 0; f < NT; f++)
 #pragma unroll
@@ -621,7 +692,7 @@ __global__ __launch_bounds__(kHiddenWaves * 64) void layer_hidden_kernel(LayerAr
                 for (int g = 0; g < G; g++) {
                     h[g] = f4zero();
                     for (int u = 0; u < X; u++)
-                        for (int w = 0; w < used; w++) h[g] += sums[w][g * NT + f][j][lane + u * kSlots];
+                        for (int w = 0; w < joined; w++) h[g] += sums[w][g * NT + f][j][lane + u * kSlots];
                 }
                 const int row = n0 + f * 16 + quad * 4;
                 Vec<__bf16, 4> o[A];
@@ -635,27 +706,43 @@ __global__ __launch_bounds__(kHiddenWaves * 64) void layer_hidden_kernel(LayerAr
 #pragma unroll
                     for (int t = 0; t < A; t++) o[t][i] = s[t];
                 }
-                __bf16* to = a.acts + (long long)slot[j] * A * a.hidden_pad + place_of(row & ~7, FORMAT == EXPERT_FP4) + (row & 4);
+                const int k = place_of(row & ~7, FORMAT == EXPERT_FP4);
+                if (CT == 1) {
+                    __bf16* to = a.acts + (long long)slot[j] * A * a.hidden_pad + k + (row & 4);
 #pragma unroll
-                for (int t = 0; t < A; t++) *reinterpret_cast<Vec<__bf16, 4>*>(to + (long long)t * a.hidden_pad) = o[t];
+                    for (int t = 0; t < A; t++) *reinterpret_cast<Vec<__bf16, 4>*>(to + (long long)t * a.hidden_pad) = o[t];
+                } else {
+                    constexpr int kOut = Columns<A>::kSlots;
+                    const int i = s0 + j * kSlots + mine.slot;
+                    __bf16* to = a.acts + (long long)(fragment_of<kOut>(first, n) + i / kOut) * a.hidden_pad * 16 + k / 32 * 512 +
+                                 (k / 8 % 4 * 16 + i % kOut) * 8 + (row & 4);
+#pragma unroll
+                    for (int t = 0; t < A; t++) *reinterpret_cast<Vec<__bf16, 4>*>(to + t * kOut * 8) = o[t];
+                }
             }
+        if (s0 + kSlots * CT < count) __syncthreads();
     }
+#endif
 }
 
 // 16 NT columns of the outputs for all tokens and a part of the active experts' k, which
 // its waves share out in runs of one expert's.  Their sums go, weighted, to the
 // tokens' in the wave's part of LDS; those are joined in wave order, and the parts in
 // their order by the workgroup of a tile that is last.
-template <int FORMAT, class T, int NT, int CT, int WAVES, int DEPTH>
-__global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
+constexpr int kOutWaves = 8;
+
+template <int FORMAT, class T, int NT, int CT>
+__global__ __launch_bounds__(kOutWaves * 64) void layer_out_kernel(LayerArgs a)
 {
-    constexpr int A = Terms<T>::kA, kSlots = Columns<A>::kSlots;
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    __shared__ bool last;
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass needs the kernel's name alone
+    constexpr int WAVES = kOutWaves, A = Terms<T>::kA, kSlots = Columns<A>::kSlots;
+    constexpr int kCopies = Piece<FORMAT>::kCopies, kBlock = NT * kCopies * kCopyBytes;
+    extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int col = lane & 15, quad = lane >> 4, d0 = blockIdx.x * 16 * NT;
     const int slots = a.tokens * a.topk, most = min(a.experts, slots);
-    f4* const sums = reinterpret_cast<f4*>(lds);  // [waves][tokens][4 NT]
+    uint8_t* const ring = lds + wave * 2 * kBlock;
+    f4* const sums = reinterpret_cast<f4*>(lds + WAVES * 2 * kBlock);  // [waves][tokens][4 NT]
     int* const active = reinterpret_cast<int*>(sums + WAVES * a.tokens * 4 * NT);
     int *const first = active + most, *const list = first + most + 1;
     float* const weights = reinterpret_cast<float*>(list + slots);  // in LDS as well: a load would wait for all that are ahead
@@ -671,6 +758,9 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
     int row[NT];
 #pragma unroll
     for (int f = 0; f < NT; f++) row[f] = min(d0 + f * 16 + col, a.dim - 1);
+    const int pitch = (int)pitch_of<FORMAT>(a.hidden_pad), rows = min(16 * NT, a.dim - d0);
+    const uint32_t copy_from = (lane >> 2) * pitch + ((lane & 3) ^ copy_key(lane >> 2)) * 16;
+    const int at = col * 64 + (quad ^ copy_key(col)) * 16;
     const Columns<A> mine(col);
 
     // Block kb, from .. to - 1, of expert `at`, for its slots from s0 on.
@@ -695,30 +785,43 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
         const int f0 = first[c.at], i = c.s0 + j * kSlots + mine.slot;
         return mine.slot < kSlots && i < first[c.at + 1] - f0 ? list[f0 + i] : -1;
     };
-    struct Part {
-        Weights<FORMAT, NT> w;
-        Values<CT> v;
-    };
-    const uint8_t *W[NT], *S[NT];
+    Scales<FORMAT, NT> scales[2];
+    __amdgpu_buffer_rsrc_t W;
+    const uint8_t* S[NT];
     const __bf16* act[CT];
-    auto load = [&](Part& b, const Cursor& c) {
+    int used = 1;
+    auto load_weights = [&](int d, Scales<FORMAT, NT>& to, const Cursor& c) {
         if (c.first_of_run()) {
             const int e = __builtin_amdgcn_readfirstlane(active[c.at]);
+            W = __builtin_amdgcn_make_buffer_rsrc((void*)row_of<FORMAT>(a.w2, e, a.dim, a.hidden_pad, d0), 0, rows * pitch, 0x00020000);
 #pragma unroll
-            for (int f = 0; f < NT; f++) {
-                W[f] = row_of<FORMAT>(a.w2, e, a.dim, a.hidden_pad, row[f]);
-                S[f] = scales_of<FORMAT>(a.s2, e, a.dim, a.hidden_pad, row[f], a.scale_shift);
-            }
-#pragma unroll
-            for (int j = 0; j < CT; j++) {
-                const int slot = slot_of(c, j);
-                act[j] = a.acts + ((long long)(slot >= 0 ? slot : list[first[c.at]]) * A + (slot >= 0 ? mine.term : 0)) * a.hidden_pad +
-                         quad * 8;
-            }
+            for (int f = 0; f < NT; f++) S[f] = scales_of<FORMAT>(a.s2, e, a.dim, a.hidden_pad, row[f], a.scale_shift);
         }
 #pragma unroll
-        for (int f = 0; f < NT; f++) b.w.w[f].load(W[f], S[f], c.kb, quad);
-        b.v.load(act, c.kb);
+        for (int f = 0; f < NT; f++)
+#pragma unroll
+            for (int h = 0; h < kCopies; h++)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    W, (__attribute__((address_space(3))) void*)(ring + d * kBlock + (f * kCopies + h) * kCopyBytes), 16,
+                    copy_from + f * 16 * pitch + (c.kb * kCopies + h) * 64, 0, 0, 0);
+        to.load(S, c.kb, quad);
+    };
+    auto load_values = [&](Values<CT>& v, const Cursor& c) {
+        if (c.first_of_run()) {
+#pragma unroll
+            for (int j = 0; j < CT; j++) {
+                if (CT == 1) {
+                    const int slot = slot_of(c, j);
+                    act[j] = a.acts + ((long long)(slot >= 0 ? slot : list[first[c.at]]) * A + (slot >= 0 ? mine.term : 0)) * a.hidden_pad +
+                             quad * 8;
+                } else {
+                    const int f0 = __builtin_amdgcn_readfirstlane(first[c.at]), n = __builtin_amdgcn_readfirstlane(first[c.at + 1]) - f0;
+                    act[j] = a.acts + (long long)(fragment_of<kSlots>(f0, c.at) + c.s0 / kSlots + j) * a.hidden_pad * 16 + lane * 8;
+                    used = (min(n - c.s0, kSlots * CT) + kSlots - 1) / kSlots;
+                }
+            }
+        }
+        v.load(act, c.kb, used);
     };
     f4 own[NT][CT];
     auto finish_run = [&](const Cursor& c) {
@@ -748,33 +851,30 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
         }
     };
     if (begin < end) {
-        Part b[DEPTH];
+        Values<CT> v[2];
         Cursor ahead = enter(begin / blocks), now = ahead;
-#pragma unroll
-        for (int d = 0; d + 1 < DEPTH; d++)
-            if (ahead.valid()) {
-                load(b[d], ahead);
-                advance(ahead);
-            }
-        bool more = true;
-        while (more) {
-            each<DEPTH>([&](auto D) {
+        auto load = [&](int d, Values<CT>& values, Scales<FORMAT, NT>& to) {
+            load_values(values, ahead);
+            load_weights(d, to, ahead);
+            advance(ahead);
+        };
+        load(0, v[0], scales[0]);
+        while (now.valid()) {
+            each<2>([&](auto D) {
                 constexpr int d = decltype(D)::value;
-                if (!more) return;
-                if (ahead.valid()) {
-                    load(b[(d + DEPTH - 1) % DEPTH], ahead);
-                    advance(ahead);
-                }
+                if (!now.valid()) return;
+                __builtin_amdgcn_s_waitcnt(kLdsDone);  // reads of the place that is copied to
+                if (ahead.valid()) load(1 - d, v[1 - d], scales[1 - d]);
                 if (now.first_of_run()) {
 #pragma unroll
                     for (int j = 0; j < CT; j++)
 #pragma unroll
                         for (int f = 0; f < NT; f++) own[f][j] = f4zero();
                 }
-                multiply(own, b[d].w, b[d].v);
+                scales[d].arrive();
+                multiply(own, ring + d * kBlock, at, scales[d], v[d]);
                 if (now.last_of_run()) finish_run(now);
                 advance(now);
-                more = now.valid();
             });
         }
     }
@@ -807,7 +907,7 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
                 store_past(parts + blockIdx.y * plane + i * 4 + j, v[j]);
         }
     }
-    if (gridDim.y == 1 || !is_last(a.out_tickets + blockIdx.x, gridDim.y, &last)) return;
+    if (gridDim.y == 1 || !is_last(a.out_tickets + blockIdx.x, gridDim.y, reinterpret_cast<bool*>(lds))) return;  // a ring's place
     for (int i = threadIdx.x; i < pieces; i += WAVES * 64) {
         f4 v = f4zero();
         for (unsigned p = 0; p < gridDim.y; p++)
@@ -816,6 +916,7 @@ __global__ __launch_bounds__(WAVES * 64) void layer_out_kernel(LayerArgs a)
                 v[j] += load_past(parts + p * plane + i * 4 + j);
         store(i, v);
     }
+#endif
 }
 
 // What a call launches, by its sizes.
@@ -855,13 +956,14 @@ void hidden_launch(const LayerArgs& a, hipStream_t s)
     GRAFT_LAUNCH_CHECK();
 }
 
-template <int FORMAT, class T, int NT, int CT, int WAVES, int DEPTH>
+template <int FORMAT, class T, int NT, int CT>
 void out_launch(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
     const int slots = a.tokens * a.topk, most = std::min(a.experts, slots);
-    const size_t lds = (size_t)WAVES * a.tokens * 64 * NT + (size_t)(2 * most + 1 + 2 * slots) * 4;
-    allow_lds((const void*)layer_out_kernel<FORMAT, T, NT, CT, WAVES, DEPTH>, lds);
-    layer_out_kernel<FORMAT, T, NT, CT, WAVES, DEPTH><<<dim3(p.out_tiles, p.out_parts), WAVES * 64, lds, s>>>(a);
+    const size_t lds = kOutWaves * ((size_t)2 * NT * Piece<FORMAT>::kCopies * kCopyBytes + (size_t)a.tokens * 64 * NT) +
+                       (size_t)(2 * most + 1 + 2 * slots) * 4;
+    allow_lds((const void*)layer_out_kernel<FORMAT, T, NT, CT>, lds);
+    layer_out_kernel<FORMAT, T, NT, CT><<<dim3(p.out_tiles, p.out_parts), kOutWaves * 64, lds, s>>>(a);
     GRAFT_LAUNCH_CHECK();
 }
 
@@ -880,13 +982,15 @@ void products(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
     constexpr int CT = sizeof(T) == 4 ? 4 : 2;
     if (p.many) {
+        layer_gather_kernel<T><<<dim3(a.dim_pad / 128, std::min(a.experts, a.tokens * a.topk)), 256, 0, s>>>(a);
+        GRAFT_LAUNCH_CHECK();
         if (a.gated) hidden_launch<FORMAT, T, 2, 1, CT>(a, s);
         else hidden_launch<FORMAT, T, 1, 2, CT>(a, s);
-        out_launch<FORMAT, T, 2, CT, 8, 2>(a, p, s);
+        out_launch<FORMAT, T, 2, CT>(a, p, s);
     } else {
         if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1>(a, s);
         else hidden_launch<FORMAT, T, 1, 1, 1>(a, s);
-        out_launch<FORMAT, T, 1, 1, 8, 3>(a, p, s);
+        out_launch<FORMAT, T, 1, 1>(a, p, s);
     }
 }
 
@@ -952,7 +1056,10 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     const size_t x_terms = o.dataType == DATA_F32 ? 3 : o.dataType == DATA_BF16 ? 1 : 2, a_terms = o.dataType == DATA_F32 ? 3 : 2;
     const size_t at_logits = take((size_t)p.route_parts * tokens * a.experts * 4), at_weights = take((size_t)slots * 4);
     const size_t at_active = take((size_t)(most + 1) * 4), at_first = take((size_t)(most + 1) * 4), at_slots = take((size_t)slots * 4);
-    const size_t at_xs = take((size_t)tokens * x_terms * a.dim_pad * 2), at_acts = take((size_t)slots * a_terms * a.hidden_pad * 2);
+    const size_t at_xs = take((size_t)tokens * x_terms * a.dim_pad * 2);
+    auto fragments = [&](size_t terms) { return (size_t)(slots / (16 / terms) + most); };
+    const size_t at_acts = take(p.many ? fragments(a_terms) * a.hidden_pad * 32 : (size_t)slots * a_terms * a.hidden_pad * 2);
+    const size_t at_frags = take(p.many ? fragments(x_terms) * a.dim_pad * 32 : 0);
     const bool split = p.out_parts > 1;
     const size_t at_sums = take(split ? (size_t)p.out_parts * p.out_tiles * tokens * (p.many ? 32 : 16) * 4 : 0);
     const size_t at_tickets = take(split ? (size_t)p.out_tiles * 4 : 0);
@@ -965,6 +1072,7 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     a.slots = (int*)(ws + at_slots);
     a.xs = (__bf16*)(ws + at_xs);
     a.acts = (__bf16*)(ws + at_acts);
+    a.frags = (__bf16*)(ws + at_frags);
     if (split) {
         a.sums = (float*)(ws + at_sums);
         a.out_tickets = (uint32_t*)(ws + at_tickets);
