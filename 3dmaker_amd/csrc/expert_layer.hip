@@ -312,13 +312,14 @@ __host__ __device__ inline RouteLds route_lds(const LayerArgs& a, int waves, int
     l.size = l.logits_at + (l.logits ? a.tokens * a.experts * 4 : 0);
     return l;
 }
-constexpr int kRouteParts = 8;
 
 // Logits of 16 experts over a part of k that the waves share out; the tokens' terms on
 // the way; routing and plan by the workgroup that is last.  Products of terms are
-// exact; those of 2^-24 of a product and less are left out.  A part is four blocks of
-// k, a quarter of one for each of 16 waves, while that makes no more than 128
-// workgroups: one round trip, and the splitting of fp32 numbers spread.
+// exact; those of 2^-24 of a product and less are left out.  Bound by round trips.  A
+// part is two blocks of k, a quarter of one for each of eight waves, while that makes
+// no more than 128 workgroups, so that reading and splitting tokens is spread (64 fp32
+// tokens of 4096 by 8 experts: 14.2 us, 19.9 with four blocks, 13.0 with one; 27 of
+// 2048 by 128: 15.6, 16.5 and 17.3).
 template <class T, class R, int MT>
 __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
 {
@@ -393,19 +394,22 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
         if (threadIdx.x == 0) *a.route_ticket = 0;
         if (logits) {  // all parts' loads together
             for (int i0 = threadIdx.x; i0 < all; i0 += 4 * blockDim.x) {
-                float z[4][kRouteParts];
+                float v[4] = {};
+                for (int p0 = 0; p0 < parts; p0 += 8) {
+                    float z[4][8];
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+#pragma unroll
+                        for (int p = 0; p < 8; p++)
+                            z[u][p] = load_past(a.logits + min(p0 + p, parts - 1) * all + min(i0 + u * (int)blockDim.x, all - 1));
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+#pragma unroll
+                        for (int p = 0; p < 8; p++) v[u] += p0 + p < parts ? z[u][p] : 0.0f;
+                }
 #pragma unroll
                 for (int u = 0; u < 4; u++)
-#pragma unroll
-                    for (int p = 0; p < kRouteParts; p++)
-                        z[u][p] = load_past(a.logits + min(p, parts - 1) * all + min(i0 + u * (int)blockDim.x, all - 1));
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    float v = z[u][0];
-#pragma unroll
-                    for (int p = 1; p < kRouteParts; p++) v += p < parts ? z[u][p] : 0.0f;
-                    if (i0 + u * (int)blockDim.x < all) logits[i0 + u * blockDim.x] = v;
-                }
+                    if (i0 + u * (int)blockDim.x < all) logits[i0 + u * blockDim.x] = v[u];
             }
             __syncthreads();
         }
@@ -930,7 +934,7 @@ LayerPlan layer_plan(const LayerArgs& a)
 {
     LayerPlan p{};
     const int slots = a.tokens * a.topk, blocks = a.dim_pad / 128, groups = (a.experts + 15) / 16;
-    p.route_parts = std::max(1, std::min({blocks / 4, 128 / groups, kRouteParts}));
+    p.route_parts = std::max(1, std::min({blocks / 2, 128 / groups, 32}));
     p.route_waves = std::min(kRouteWaves, std::max(4 * ((blocks + p.route_parts - 1) / p.route_parts), a.tokens));
     const int most = std::min(a.experts, slots);
     p.many = slots >= 4 * most;
