@@ -4,8 +4,8 @@
  * matrices with a scale for each block of 128, the gather and combine of the
  * experts' rows, and the norms, gate and residual around a block; forward and
  * backward.  For serving, 4-bit matrices with a scale for each block of 32, and
- * the whole layer of experts for few tokens in one call.  No counterpart exists in the reference, whose heads are single
- * MLPs of at most 128 (modules/TinyMLP).
+ * the whole layer of experts for few tokens in one call.  No counterpart exists in
+ * the reference, whose heads are single MLPs of at most 128 (modules/TinyMLP).
  *
  * Conventions are those of tinymlp_abi.h: device pointers unless stated, a
  * trailing stream, void launchers that report through tinymlp_last_error()
@@ -272,7 +272,7 @@ typedef struct ExpertLayerOption {
  * weights' values and the tokens' are exact, a is held in 16 bits more than a
  * 16-bit token (in all of fp32 for fp32 tokens), sums are fp32, and out is rounded
  * once.  A token none of whose experts is available (NaN among its logits) gets
- * zeros.  out and x do not overlap. */
+ * zeros.  out may be x.  A stream's first call cannot be captured into a graph. */
 void launchExpertLayer(const ExpertLayerOption* opt, const void* d_x, const void* d_router, const float* d_bias,
                        const uint8_t* d_w1, const uint8_t* d_w1Scales, const uint8_t* d_w2, const uint8_t* d_w2Scales,
                        void* d_out, int numTokens, hipStream_t stream);
