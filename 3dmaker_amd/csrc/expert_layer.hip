@@ -449,7 +449,8 @@ struct Piece<EXPERT_FP8> {
         v[0] = *reinterpret_cast<const i4v*>(lds + at);
         v[1] = *reinterpret_cast<const i4v*>(lds + at + kCopyBytes);
     }
-    static __device__ __forceinline__ int scale(const uint8_t* scales, int kb, int) { return scales[kb]; }
+    static __device__ __forceinline__ int four_scales(const uint8_t* scales, int kb) { return *(const int*)(scales + (kb & ~3)); }
+    static __device__ __forceinline__ int shift(int kb, int) { return 8 * (kb & 3); }
     __device__ __forceinline__ bf16x8 operator()(int q, int byte) const
     {
         return widen(v[q >> 1][2 * (q & 1)], v[q >> 1][2 * (q & 1) + 1], scale_of(byte));
@@ -461,7 +462,8 @@ struct Piece<EXPERT_FP4> {
     static constexpr int kCopies = 1;
     i4v v;
     __device__ __forceinline__ void read(const uint8_t* lds, int at) { v = *reinterpret_cast<const i4v*>(lds + at); }
-    static __device__ __forceinline__ int scale(const uint8_t* scales, int kb, int quad) { return scales[kb * 4 + quad]; }
+    static __device__ __forceinline__ int four_scales(const uint8_t* scales, int kb) { return *(const int*)(scales + kb * 4); }
+    static __device__ __forceinline__ int shift(int, int quad) { return 8 * quad; }
     __device__ __forceinline__ bf16x8 operator()(int q, int byte) const
     {
         const float scale = byte == 255 ? __builtin_bit_cast(float, 0x7fc00000) : scale_of(byte);
@@ -488,6 +490,16 @@ __device__ __forceinline__ const uint8_t* scales_of(const uint8_t* s, int e, int
 {
     return s + ((long long)e * ((rows + (1 << shift) - 1) >> shift) + (row >> shift)) * scale_pitch_of<FORMAT>(pad);
 }
+
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass does not know the type
+// Rows of weights, with zeros behind them; the same for all lanes.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t weights_from(const uint8_t* p, int bytes)
+{
+    const uint64_t at = (uint64_t)p;
+    const uint32_t low = __builtin_amdgcn_readfirstlane((uint32_t)at), high = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)high << 32 | low), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+#endif
 
 __device__ __forceinline__ float activate(int kind, float v)
 {
@@ -521,13 +533,12 @@ template <int CT>
 struct Values {
     static constexpr int kStep = CT == 1 ? 32 : 512, kBlock = 4 * kStep;  // to the next load's, to the next block's
     bf16x8 t[CT][4];
-    __device__ __forceinline__ void load(const __bf16* const (&from)[CT], int kb, int used)
+    __device__ __forceinline__ void load(const __bf16* const (&from)[CT], int kb)
     {
 #pragma unroll
         for (int j = 0; j < CT; j++)
-            if (j == 0 || j < used)
 #pragma unroll
-                for (int q = 0; q < 4; q++) t[j][q] = *reinterpret_cast<const bf16x8*>(from[j] + (long long)kb * kBlock + q * kStep);
+            for (int q = 0; q < 4; q++) t[j][q] = *reinterpret_cast<const bf16x8*>(from[j] + (long long)kb * kBlock + q * kStep);
     }
 };
 
@@ -537,40 +548,66 @@ struct Values {
 template <int SLOTS>
 __device__ __forceinline__ int fragment_of(int first, int n) { return first / SLOTS + n; }
 
-// The scales of F fragments of weights.  They are loaded behind the copies of those:
-// when they are there, so are the copies.
+// The blocks of a wave, one under way ahead of the one that is worked on, in two
+// places: first(place), then load(place) and work(place) while more() says so, and
+// end(place).  What is under way is the same on every path to a wait: where loads
+// depend on a condition, the compiler has the wait for the older block wait for them.
+template <class More, class First, class Load, class Work, class End>
+__device__ __forceinline__ void in_two_places(More&& more, First&& first, Load&& load, Work&& work, End&& end)
+{
+    const std::integral_constant<int, 0> a;
+    const std::integral_constant<int, 1> b;
+    first(a);
+    while (true) {
+        if (!more()) {
+            end(a);
+            return;
+        }
+        load(b);
+        work(a);
+        if (!more()) {
+            end(b);
+            return;
+        }
+        load(a);
+        work(b);
+    }
+}
+
+// The scales of F fragments of weights, four bytes at a time.  They are loaded behind
+// the copies of those: when they are there, so are the copies.
 template <int FORMAT, int F>
 struct Scales {
-    int byte[F];
-    __device__ __forceinline__ void load(const uint8_t* const (&from)[F], int kb, int quad)
+    int four[F];
+    __device__ __forceinline__ void load(const uint8_t* const (&from)[F], int kb)
     {
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int f = 0; f < F; f++) byte[f] = Piece<FORMAT>::scale(from[f], kb, quad);
+        for (int f = 0; f < F; f++) four[f] = Piece<FORMAT>::four_scales(from[f], kb);
     }
     __device__ __forceinline__ void arrive()
     {
 #pragma unroll
-        for (int f = 0; f < F; f++) asm volatile("" : "+v"(byte[f])::"memory");
+        for (int f = 0; f < F; f++) asm volatile("" : "+v"(four[f])::"memory");
     }
 };
 
 // lds: the copies of the block, those of a fragment behind the other's; at: the lane's
-// place in a copy.
+// place in a copy; shift: to its scale.
 template <int FORMAT, int F, int CT>
-__device__ __forceinline__ void multiply(f4 (&acc)[F][CT], const uint8_t* lds, int at, const Scales<FORMAT, F>& s, const Values<CT>& v)
+__device__ __forceinline__ void multiply(f4 (&acc)[F][CT], const uint8_t* lds, int at, const Scales<FORMAT, F>& s, int shift,
+                                         const Values<CT>& v)
 {
     Piece<FORMAT> w[F];
 #pragma unroll
     for (int f = 0; f < F; f++) w[f].read(lds + f * (Piece<FORMAT>::kCopies * kCopyBytes), at);
 #pragma unroll
-    for (int q = 0; q < 4; q++)
+    for (int u = 0; u < 4 * F; u++) {  // with few fragments of values the weights' in turn, so that sums wait less for each other
+        const int f = CT > 1 ? u / 4 : u % F, q = CT > 1 ? u % 4 : u / F;
+        const bf16x8 b = w[f](q, s.four[f] >> shift & 255);
 #pragma unroll
-        for (int f = 0; f < F; f++) {
-            const bf16x8 b = w[f](q, s.byte[f]);
-#pragma unroll
-            for (int j = 0; j < CT; j++) acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, v.t[j][q], acc[f][j], 0, 0, 0);
-        }
+        for (int j = 0; j < CT; j++) acc[f][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, v.t[j][q], acc[f][j], 0, 0, 0);
+    }
 }
 
 // Tokens' terms as fragments, block by block.
@@ -602,7 +639,7 @@ __global__ __launch_bounds__(256) void layer_gather_kernel(LayerArgs a)
 constexpr int kHiddenWaves = 4;
 
 template <int FORMAT, class T, int G, int NT, int CT>
-__global__ __launch_bounds__(kHiddenWaves * 64) void layer_hidden_kernel(LayerArgs a)
+__global__ __launch_bounds__(kHiddenWaves * 64, CT == 4 ? 2 : CT == 2 ? 3 : 4) void layer_hidden_kernel(LayerArgs a)
 {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass needs the kernel's name alone
     constexpr int WAVES = kHiddenWaves;
@@ -615,14 +652,15 @@ __global__ __launch_bounds__(kHiddenWaves * 64) void layer_hidden_kernel(LayerAr
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int col = lane & 15, quad = lane >> 4, n0 = blockIdx.x * 16 * NT, n = blockIdx.y;
     // one round trip for all four; behind the active experts they are of no use
-    const int number = a.active[0], e = a.active[1 + n], first = a.first[n], count = a.first[n + 1] - first;
-    if (n >= number) return;
+    const int number = a.active[0], at_e = a.active[1 + n], at_first = a.first[n], at_end = a.first[n + 1];
+    if (n >= __builtin_amdgcn_readfirstlane(number)) return;
+    const int e = __builtin_amdgcn_readfirstlane(at_e), first = __builtin_amdgcn_readfirstlane(at_first);
+    const int count = __builtin_amdgcn_readfirstlane(at_end) - first;
     uint8_t* const ring = lds + wave * 2 * kBlock;
     const int pitch = (int)pitch_of<FORMAT>(a.dim_pad), rows = min(16 * NT, max(a.hidden - n0, 0));
     const uint32_t from = (lane >> 2) * pitch + ((lane & 3) ^ copy_key(lane >> 2)) * 16, at = col * 64 + (quad ^ copy_key(col)) * 16;
     const uint8_t* const w = row_of<FORMAT>(a.w1, e, G * a.hidden, a.dim_pad, min(n0, a.hidden));
-    const auto w0 = __builtin_amdgcn_make_buffer_rsrc((void*)w, 0, rows * pitch, 0x00020000);
-    const auto w1 = __builtin_amdgcn_make_buffer_rsrc((void*)(w + (G - 1) * (long long)a.hidden * pitch), 0, rows * pitch, 0x00020000);
+    const __amdgpu_buffer_rsrc_t w0 = weights_from(w, rows * pitch), w1 = weights_from(w + (G - 1) * (long long)a.hidden * pitch, rows * pitch);
     const uint8_t* S[F];
 #pragma unroll
     for (int f = 0; f < F; f++) {
@@ -638,46 +676,59 @@ __global__ __launch_bounds__(kHiddenWaves * 64) void layer_hidden_kernel(LayerAr
 #pragma unroll
         for (int j = 0; j < CT; j++) {
             const int i = s0 + j * kSlots + mine.slot;
-            slot[j] = mine.slot < kSlots && i < count ? a.slots[first + i] : -1;
+            const bool there = mine.slot < kSlots && i < count;
+            slot[j] = a.slots[first + (there ? i : 0)];
+            const int token = slot[j] / a.topk;
+            if (CT == 1) x[j] = a.xs + ((long long)token * X + (there ? mine.term : 0)) * a.dim_pad + quad * 8;
+            else {
+                const int j1 = min(j, (count - s0 - 1) / kSlots);  // behind the last fragment: that once more
+                x[j] = a.frags + (long long)(fragment_of<kSlots>(first, n) + s0 / kSlots + j1) * blocks * 2048 + lane * 8;
+            }
+            if (!there) slot[j] = -1;
 #pragma unroll
             for (int f = 0; f < F; f++) acc[f][j] = f4zero();
         }
-        const int used = (min(count - s0, kSlots * CT) + kSlots - 1) / kSlots;
+        // Four fragments of values leave no registers for those of two blocks.
+        constexpr bool kOne = CT == 4;
         Scales<FORMAT, F> scales[2];
-        Values<CT> v[2];
-        auto load_weights = [&](int d, Scales<FORMAT, F>& to, int kb) {
-#pragma unroll
-            for (int f = 0; f < F; f++)
-#pragma unroll
-                for (int h = 0; h < kCopies; h++)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                        f < NT ? w0 : w1, (__attribute__((address_space(3))) void*)(ring + d * kBlock + (f * kCopies + h) * kCopyBytes), 16,
-                        from + f % NT * 16 * pitch + (kb * kCopies + h) * 64, 0, 0, 0);
-            to.load(S, kb, quad);
-        };
-        if (wave < blocks) load_weights(0, scales[0], wave);  // they need no slots
-#pragma unroll
-        for (int j = 0; j < CT; j++) {
-            if (CT == 1) {
-                const int token = (slot[j] >= 0 ? slot[j] : a.slots[first]) / a.topk;
-                x[j] = a.xs + ((long long)token * X + (slot[j] >= 0 ? mine.term : 0)) * a.dim_pad + quad * 8;
-            } else x[j] = a.frags + (long long)(fragment_of<kSlots>(first, n) + s0 / kSlots + j) * blocks * 2048 + lane * 8;
-        }
-        if (wave < blocks) v[0].load(x, wave, used);
-        for (int kb = wave; kb < blocks;) {
-            each<2>([&](auto D) {
+        Values<CT> v[kOne ? 1 : 2];
+        if (wave < blocks) {
+            int ahead = wave, now = wave;
+            auto weights = [&](auto D) {
                 constexpr int d = decltype(D)::value;
-                if (kb >= blocks) return;
-                const int next = kb + WAVES;
                 __builtin_amdgcn_s_waitcnt(kLdsDone);  // reads of the place that is copied to
-                if (next < blocks) {
-                    v[1 - d].load(x, next, used);
-                    load_weights(1 - d, scales[1 - d], next);
-                }
+#pragma unroll
+                for (int f = 0; f < F; f++)
+#pragma unroll
+                    for (int h = 0; h < kCopies; h++)
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                            f < NT ? w0 : w1, (__attribute__((address_space(3))) void*)(ring + d * kBlock + (f * kCopies + h) * kCopyBytes),
+                            16, from + f % NT * 16 * pitch + (ahead * kCopies + h) * 64, 0, 0, 0);
+                scales[d].load(S, ahead);
+                ahead += WAVES;
+            };
+            auto work = [&](auto D) {
+                constexpr int d = decltype(D)::value;
                 scales[d].arrive();
-                multiply(acc, ring + d * kBlock, at, scales[d], v[d]);
-                kb = next;
-            });
+                multiply(acc, ring + d * kBlock, at, scales[d], Piece<FORMAT>::shift(now, quad), v[kOne ? 0 : d]);
+                now += WAVES;
+            };
+            in_two_places(
+                [&] { return ahead < blocks; },
+                [&](auto D) {
+                    if (!kOne) v[0].load(x, ahead);
+                    weights(D);
+                },
+                [&](auto D) {
+                    if (kOne) v[0].load(x, now);
+                    else v[decltype(D)::value].load(x, ahead);
+                    weights(D);
+                },
+                work,
+                [&](auto D) {
+                    if (kOne) v[0].load(x, now);
+                    work(D);
+                });
         }
         __syncthreads();  // sums take the rings' place
 #pragma unroll
@@ -793,11 +844,10 @@ __global__ __launch_bounds__(kOutWaves * 64) void layer_out_kernel(LayerArgs a)
     __amdgpu_buffer_rsrc_t W;
     const uint8_t* S[NT];
     const __bf16* act[CT];
-    int used = 1;
     auto load_weights = [&](int d, Scales<FORMAT, NT>& to, const Cursor& c) {
         if (c.first_of_run()) {
             const int e = __builtin_amdgcn_readfirstlane(active[c.at]);
-            W = __builtin_amdgcn_make_buffer_rsrc((void*)row_of<FORMAT>(a.w2, e, a.dim, a.hidden_pad, d0), 0, rows * pitch, 0x00020000);
+            W = weights_from(row_of<FORMAT>(a.w2, e, a.dim, a.hidden_pad, d0), rows * pitch);
 #pragma unroll
             for (int f = 0; f < NT; f++) S[f] = scales_of<FORMAT>(a.s2, e, a.dim, a.hidden_pad, row[f], a.scale_shift);
         }
@@ -808,7 +858,7 @@ __global__ __launch_bounds__(kOutWaves * 64) void layer_out_kernel(LayerArgs a)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     W, (__attribute__((address_space(3))) void*)(ring + d * kBlock + (f * kCopies + h) * kCopyBytes), 16,
                     copy_from + f * 16 * pitch + (c.kb * kCopies + h) * 64, 0, 0, 0);
-        to.load(S, c.kb, quad);
+        to.load(S, c.kb);
     };
     auto load_values = [&](Values<CT>& v, const Cursor& c) {
         if (c.first_of_run()) {
@@ -820,12 +870,12 @@ __global__ __launch_bounds__(kOutWaves * 64) void layer_out_kernel(LayerArgs a)
                              quad * 8;
                 } else {
                     const int f0 = __builtin_amdgcn_readfirstlane(first[c.at]), n = __builtin_amdgcn_readfirstlane(first[c.at + 1]) - f0;
-                    act[j] = a.acts + (long long)(fragment_of<kSlots>(f0, c.at) + c.s0 / kSlots + j) * a.hidden_pad * 16 + lane * 8;
-                    used = (min(n - c.s0, kSlots * CT) + kSlots - 1) / kSlots;
+                    const int j1 = min(j, (n - c.s0 - 1) / kSlots);  // behind the last fragment: that once more
+                    act[j] = a.acts + (long long)(fragment_of<kSlots>(f0, c.at) + c.s0 / kSlots + j1) * a.hidden_pad * 16 + lane * 8;
                 }
             }
         }
-        v.load(act, c.kb, used);
+        v.load(act, c.kb);
     };
     f4 own[NT][CT];
     auto finish_run = [&](const Cursor& c) {
@@ -857,30 +907,27 @@ __global__ __launch_bounds__(kOutWaves * 64) void layer_out_kernel(LayerArgs a)
     if (begin < end) {
         Values<CT> v[2];
         Cursor ahead = enter(begin / blocks), now = ahead;
-        auto load = [&](int d, Values<CT>& values, Scales<FORMAT, NT>& to) {
-            load_values(values, ahead);
-            load_weights(d, to, ahead);
+        auto load = [&](auto D) {
+            constexpr int d = decltype(D)::value;
+            __builtin_amdgcn_s_waitcnt(kLdsDone);  // reads of the place that is copied to
+            load_values(v[d], ahead);
+            load_weights(d, scales[d], ahead);
             advance(ahead);
         };
-        load(0, v[0], scales[0]);
-        while (now.valid()) {
-            each<2>([&](auto D) {
-                constexpr int d = decltype(D)::value;
-                if (!now.valid()) return;
-                __builtin_amdgcn_s_waitcnt(kLdsDone);  // reads of the place that is copied to
-                if (ahead.valid()) load(1 - d, v[1 - d], scales[1 - d]);
-                if (now.first_of_run()) {
+        auto work = [&](auto D) {
+            constexpr int d = decltype(D)::value;
+            if (now.first_of_run()) {
 #pragma unroll
-                    for (int j = 0; j < CT; j++)
+                for (int j = 0; j < CT; j++)
 #pragma unroll
-                        for (int f = 0; f < NT; f++) own[f][j] = f4zero();
-                }
-                scales[d].arrive();
-                multiply(own, ring + d * kBlock, at, scales[d], v[d]);
-                if (now.last_of_run()) finish_run(now);
-                advance(now);
-            });
-        }
+                    for (int f = 0; f < NT; f++) own[f][j] = f4zero();
+            }
+            scales[d].arrive();
+            multiply(own, ring + d * kBlock, at, scales[d], Piece<FORMAT>::shift(now.kb, quad), v[d]);
+            if (now.last_of_run()) finish_run(now);
+            advance(now);
+        };
+        in_two_places([&] { return ahead.valid(); }, load, load, work, work);
     }
     __syncthreads();
     const int pieces = a.tokens * 4 * NT;
