@@ -10,7 +10,15 @@
 // so that nothing is rounded to 8 bits on the way.
 //
 // Three launches: routing (the last workgroup to have its logits ready routes all
-// tokens), the hidden activations, the outputs.
+// tokens), the hidden activations, the outputs; one more to gather tokens where experts
+// have many slots each.
+//
+// Measured, us for routing, hidden activations, outputs: 7 bf16 tokens, top 6 of 64,
+// gated 2048 x 1024 fp4: 9, 20.5, 16.7 (107 MB of weights at 2.3 TB/s in all); 27
+// tokens, top 8 of 128, gated 2048 x 768 fp8: 16, 52, 34 (498 MB, 5.8 TB/s in the
+// products); 64 fp32 tokens, top 2 of 8, 4096 x 2048 fp8: 14 and 5 for the gathering,
+// 31, 29 (134 MB: there the three terms of values, five times the weights' bytes from
+// the L2, and registers for two waves a SIMD bound it).
 #include "product.h"
 #include "route_math.h"
 
@@ -430,7 +438,9 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
 // A wave's copies of weights: 16 rows by 64 bytes each, four consecutive lanes a row, so
 // that the vector memory unit takes 16 cycles for them.  A load in the order of the
 // matrix instruction, whose consecutive lanes have rows of their own, takes it 64,
-// which was what bounded these kernels.  Piece p of row r goes to place p ^ key(r) of
+// which bounded these kernels (7 tokens, top 6 of 64, 2048 x 1024 fp4: 26 and 19 us
+// for hidden activations and outputs, 20.6 and 16.9 this way; 27 tokens, top 8 of 128,
+// 2048 x 768 fp8: 55 and 40, 52 and 35).  Piece p of row r goes to place p ^ key(r) of
 // the row's four: a quarter of a 16-byte read from LDS then meets each bank once.
 constexpr int kCopyBytes = 1024;
 __device__ __forceinline__ int copy_key(int row) { return -(row >> 2) & 3; }
@@ -632,10 +642,9 @@ __global__ __launch_bounds__(256) void layer_gather_kernel(LayerArgs a)
 // active expert, as many at a time as CT fragments have: waves share out k, and their
 // sums are joined in LDS in wave order.  A lane whose column has no slot works on the
 // first one's for nothing.  Bound by the weights' trips from memory, of which many
-// waves a CU have more under way than few that look far ahead: four waves of two blocks
-// in registers took 53.7 us where four of four took 61.1 and eight of two 67.1 (27
-// tokens, top 4 of 128, 1024 x 1536 fp8), and 25.7, 27.9 and 29.3 (7 tokens, top 6 of
-// 64, 2048 x 1024 fp4).
+// waves a CU have more under way than few that look far ahead: four waves with two
+// blocks in LDS took 20.6 us where four blocks took 22.7 and six 25.2 (7 tokens, top 6
+// of 64, 2048 x 1024 fp4), 52.2, 68.8 and 98 (27 tokens, top 8 of 128, 2048 x 768 fp8).
 constexpr int kHiddenWaves = 4;
 
 template <int FORMAT, class T, int G, int NT, int CT>
@@ -783,7 +792,8 @@ __global__ __launch_bounds__(kHiddenWaves * 64, CT == 4 ? 2 : CT == 2 ? 3 : 4) v
 // 16 NT columns of the outputs for all tokens and a part of the active experts' k, which
 // its waves share out in runs of one expert's.  Their sums go, weighted, to the
 // tokens' in the wave's part of LDS; those are joined in wave order, and the parts in
-// their order by the workgroup of a tile that is last.
+// their order by the workgroup of a tile that is last.  Bound as the hidden activations'
+// kernel is: 16.7 us for 36 MB, 34 for 166 MB (4.9 TB/s).
 constexpr int kOutWaves = 8;
 
 template <int FORMAT, class T, int NT, int CT>
@@ -984,7 +994,11 @@ LayerPlan layer_plan(const LayerArgs& a)
     p.route_parts = std::max(1, std::min({blocks / 2, 128 / groups, 32}));
     p.route_waves = std::min(kRouteWaves, std::max(4 * ((blocks + p.route_parts - 1) / p.route_parts), a.tokens));
     const int most = std::min(a.experts, slots);
-    p.many = slots >= 4 * most;
+    // Fragments cost a launch and the gathering, and pay where experts have many slots (64
+    // tokens, top 2, gated 2048 x 1024 fp8, us as fragments and as rows: 8 slots an expert
+    // fp32 tokens 63 and 70, bf16 51 and 49, with fp4 weights 42 and 45; 16 slots 50 and 61,
+    // 37 and 38, 36 and 41; 4 slots 87 and 80, 72 and 61, 64 and 56).
+    p.many = slots >= 8 * most;
     p.out_tiles = (a.dim + (p.many ? 31 : 15)) / (p.many ? 32 : 16);
     // A workgroup a CU, each wave with four blocks of k at least.  More parts cost more to
     // join than they help (7 tokens of 64 experts, top 6, 2048 x 1024: 19.1 us in two
