@@ -347,7 +347,9 @@ void check_clip(const GradTensor* tensors, int count, float max_norm, int non_fi
     }
 }
 
-constexpr int kMostWorkgroups = 1024;  // of a launch
+// Of a launch: four a CU (400,000,003 bf16 elements in 390 tensors, four launches: 516
+// us for norm and clipping, 4.2 and 5.0 TB/s; with 1,024 over all of them 851).
+constexpr int kMostWorkgroups = 1024;
 
 void add_to(GradTable& t, const GradTensor& g, long long pieces)
 {
@@ -384,7 +386,9 @@ int in_tables(const GradTensor* tensors, int count, F&& f)
 }
 
 // The whole list in one workgroup's hands where it is short: up to kSmallPieces of a
-// wave.
+// wave, 4 KB each (norm and clipping of four tensors, us by one workgroup and by two
+// launches of many: 32 KB in all 3.5 and 5.4, 128 KB 4.6 and 5.4, 192 KB 5.6 and 5.5; of
+// 40 tensors of 3 KB, a piece each, 7.3 and 6.1).
 constexpr int kSmallPieces = 32;
 bool small_table(const GradTensor* tensors, int count, GradTable& t)
 {
