@@ -120,12 +120,11 @@ private:
 // calling thread's, kept until that ends.
 Workspace& stream_workspace(hipStream_t s);
 
-// Counters of (current device, stream), kStreamTickets of them, zero: a kernel that
-// counts its workgroups with one leaves it zero again, so that the stream's next
-// finds it so.  Kept as the workspace is, of which they are no part; made by the
-// first call, which cannot be one under capture.
-constexpr int kStreamTickets = 16;
-uint32_t* stream_tickets(hipStream_t s);
+// A counter of (current device, stream), zero: a kernel that counts its workgroups
+// with it leaves it zero again, so that the stream's next finds it so.  Kept as the
+// workspace is, of which it is no part; made by the first call, which cannot be one
+// under capture.
+uint32_t* stream_ticket(hipStream_t s);
 
 // One Workspace per (device, stream) that its callers work on, for callers that
 // have another way: calls of several threads and streams each find their

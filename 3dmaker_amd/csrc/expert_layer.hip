@@ -1128,7 +1128,7 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     const bool split = p.out_parts > 1;
     const size_t at_sums = take(split ? (size_t)p.out_parts * p.out_tiles * tokens * (p.many ? 32 : 16) * 4 : 0);
     const size_t at_tickets = take(split ? (size_t)p.out_tiles * 4 : 0);
-    a.route_ticket = stream_tickets(s);
+    a.route_ticket = stream_ticket(s);
     char* ws = (char*)stream_workspace(s).get(size);
     a.logits = (float*)(ws + at_logits);
     a.weights = (float*)(ws + at_weights);

@@ -1,7 +1,8 @@
 // Internal interface of the mixture-of-experts operators (route.hip,
 // fp8_quant.hip, fp8_product.hip, fp4_quant.hip, fp4_product.hip,
-// expert_rows.hip, expert_layer.hip, norm_gate.hip); the options are those of experts_abi.h.  Every function checks its arguments before its
-// first device call and throws std::runtime_error.
+// expert_rows.hip, expert_layer.hip, norm_gate.hip); the options are those of
+// experts_abi.h.  Every function checks its arguments before its first device call
+// and throws std::runtime_error.
 #pragma once
 
 #include "common.h"

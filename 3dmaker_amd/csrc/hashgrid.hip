@@ -437,15 +437,15 @@ Workspace& stream_workspace(hipStream_t s)
 
 namespace {
 
-__global__ void zero_tickets_kernel(uint32_t* t) { t[threadIdx.x] = 0; }
+__global__ void zero_ticket_kernel(uint32_t* t) { *t = 0; }
 
-struct Tickets {
+struct Ticket {
     uint32_t* p = nullptr;
     bool in_graphs = false;
-    Tickets() = default;
-    Tickets(const Tickets&) = delete;
-    Tickets& operator=(const Tickets&) = delete;
-    ~Tickets()
+    Ticket() = default;
+    Ticket(const Ticket&) = delete;
+    Ticket& operator=(const Ticket&) = delete;
+    ~Ticket()
     {
         if (p && !in_graphs) (void)hipFree(p);  // graphs may outlive the thread
     }
@@ -458,9 +458,9 @@ struct Tickets {
         if (!p) {
             if (capturing) throw std::runtime_error("the first call of this kind on a stream cannot be captured: make one before");
             uint32_t* fresh = nullptr;
-            GRAFT_HIP_CHECK(hipMalloc(&fresh, kStreamTickets * sizeof(uint32_t)));
+            GRAFT_HIP_CHECK(hipMalloc(&fresh, sizeof(uint32_t)));
             p = fresh;
-            hipLaunchKernelGGL(zero_tickets_kernel, dim3(1), dim3(kStreamTickets), 0, s, p);
+            hipLaunchKernelGGL(zero_ticket_kernel, dim3(1), dim3(1), 0, s, p);
             GRAFT_LAUNCH_CHECK();
         }
         return p;
@@ -469,16 +469,16 @@ struct Tickets {
 
 }  // namespace
 
-uint32_t* stream_tickets(hipStream_t s)
+uint32_t* stream_ticket(hipStream_t s)
 {
     int dev = 0;
     GRAFT_HIP_CHECK(hipGetDevice(&dev));
     if (s == hipStreamPerThread) {
-        thread_local std::map<int, Tickets> own;
+        thread_local std::map<int, Ticket> own;
         return own[dev].get(s);
     }
     std::lock_guard<std::mutex> lk(g_ws_mu);
-    static auto* all = new std::map<std::pair<int, hipStream_t>, Tickets>();  // outlives static destructors
+    static auto* all = new std::map<std::pair<int, hipStream_t>, Ticket>();  // outlives static destructors
     return (*all)[{dev, s}].get(s);
 }
 

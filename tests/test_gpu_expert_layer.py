@@ -271,3 +271,34 @@ def test_beside_the_blocks_other_operators():
     assert torch.equal(idx.cpu(), L.indices)
     rel = float((got.double() - out.double()).norm() / out.double().norm())
     assert 1e-3 < rel < 2.0 ** -4 * 2  # two quantisings, each within 2^-4 of a value
+
+
+def test_most_slots():
+    """64 tokens that all take 32 of 64 experts (the most LDS that the outputs need), and all of 32."""
+    for E, fmt, code in ((64, 0, 0), (32, 0, 2), (32, 1, 1)):
+        Layer(64, E, 32, 140, 136, act=2, gated=True, fmt=fmt, code=code, seed=80 + E).check()
+
+
+@pytest.mark.parametrize("T,E,gated", [(2, 9, False), (64, 9, False), (64, 8, True)])
+def test_weights_beyond_2_gib(T, E, gated):
+    """The last expert's matrices begin 2 GiB behind the first's (the gated form's first matrix does); dim and hidden are the
+    largest."""
+    D, H, code, last = 16384, 16384, 2, E - 1
+    P = pkg()
+    g = R.gen(90)
+    w = []
+    for rows in (2 * H if gated else H, D):
+        q = torch.zeros(E, rows, P.fp8_pitch(D), dtype=torch.uint8, device="cuda")
+        s = torch.full((E, rows // 128, P.fp8_scale_pitch(D)), 127, dtype=torch.uint8, device="cuda")
+        q[last], s[last], _, _ = R.run_quantize(R.randn(g, rows, D) / 128, 128)
+        w.append((q, s, {last: R.values(q[last], s[last], D, 128)}))
+    x = R.randn(g, T, D).to(S.DT[code])
+    router, bias = torch.zeros(E, D, device="cuda"), torch.zeros(E, device="cuda")
+    bias[last] = 1.0
+    out = torch.full((T, D), -7.0, dtype=S.DT[code], device="cuda")
+    o = S.layer_option(E, 1, D, H, 1, gated, 0, 128, code, 0)
+    R.launch("launchExpertLayer", C.byref(o), x, router, bias, w[0][0], w[0][1], w[1][0], w[1][1], out, T, R.stream())
+    # one expert, renormalised: its weight is 1 to a rounding
+    for t in range(0, T, 21):
+        want, bound = S.layer(x[t:t + 1], torch.full((1, 1), last), torch.ones(1, 1), w[0][2], w[1][2], H, 1, gated, code)
+        assert bool((out[t].double() - want[0]).abs().le(bound[0] + 2.0 ** -23 * want[0].abs()).all())
