@@ -679,21 +679,19 @@ __global__ __launch_bounds__(kHiddenWaves * 64, CT == 4 ? 2 : CT == 2 ? 3 : 4) v
     const int blocks = a.dim_pad / 128;
     const Columns<X> mine(col);
     for (int s0 = 0; s0 < count; s0 += kSlots * CT) {
-        int slot[CT];
+        int slot = 0;  // of rows
         const __bf16* x[CT];
         f4 acc[F][CT];
 #pragma unroll
         for (int j = 0; j < CT; j++) {
-            const int i = s0 + j * kSlots + mine.slot;
-            const bool there = mine.slot < kSlots && i < count;
-            slot[j] = a.slots[first + (there ? i : 0)];
-            const int token = slot[j] / a.topk;
-            if (CT == 1) x[j] = a.xs + ((long long)token * X + (there ? mine.term : 0)) * a.dim_pad + quad * 8;
-            else {
+            if (CT == 1) {
+                const bool there = mine.slot < kSlots && s0 + mine.slot < count;
+                slot = a.slots[first + (there ? s0 + mine.slot : 0)];
+                x[j] = a.xs + ((long long)(slot / a.topk) * X + (there ? mine.term : 0)) * a.dim_pad + quad * 8;
+            } else {
                 const int j1 = min(j, (count - s0 - 1) / kSlots);  // behind the last fragment: that once more
                 x[j] = a.frags + (long long)(fragment_of<kSlots>(first, n) + s0 / kSlots + j1) * blocks * 2048 + lane * 8;
             }
-            if (!there) slot[j] = -1;
 #pragma unroll
             for (int f = 0; f < F; f++) acc[f][j] = f4zero();
         }
@@ -720,6 +718,7 @@ __global__ __launch_bounds__(kHiddenWaves * 64, CT == 4 ? 2 : CT == 2 ? 3 : 4) v
                 constexpr int d = decltype(D)::value;
                 scales[d].arrive();
                 multiply(acc, ring + d * kBlock, at, scales[d], Piece<FORMAT>::shift(now, quad), v[kOne ? 0 : d]);
+                if (kOne) __builtin_amdgcn_sched_barrier(0);  // the next values' loads stay behind: they have these' registers
                 now += WAVES;
             };
             in_two_places(
@@ -746,44 +745,36 @@ __global__ __launch_bounds__(kHiddenWaves * 64, CT == 4 ? 2 : CT == 2 ? 3 : 4) v
             for (int j = 0; j < CT; j++) sums[wave][f][j][lane] = acc[f][j];
         __syncthreads();
         const int joined = min(WAVES, blocks);
+        for (int c = wave; c < NT * CT; c += WAVES) {
+            const int f = c / CT, j = c % CT, i = s0 + j * kSlots + mine.slot;
+            if (mine.slot >= kSlots || i >= count || mine.term > 0) continue;
+            f4 h[G];
 #pragma unroll
-        for (int f = 0; f < NT; f++)
-#pragma unroll
-            for (int j = 0; j < CT; j++) {
-                if ((f * CT + j) % WAVES != wave || slot[j] < 0 || mine.term > 0) continue;
-                f4 h[G];
-#pragma unroll
-                for (int g = 0; g < G; g++) {
-                    h[g] = f4zero();
-                    for (int u = 0; u < X; u++)
-                        for (int w = 0; w < joined; w++) h[g] += sums[w][g * NT + f][j][lane + u * kSlots];
-                }
-                const int row = n0 + f * 16 + quad * 4;
-                Vec<__bf16, 4> o[A];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float v = activate(a.activation, h[0][i]);
-                    if (G == 2) v *= h[G - 1][i];
-                    if (row + i >= a.hidden) v = 0.0f;
-                    __bf16 s[A];
-                    split(v, s);
-#pragma unroll
-                    for (int t = 0; t < A; t++) o[t][i] = s[t];
-                }
-                const int k = place_of(row & ~7, FORMAT == EXPERT_FP4);
-                if (CT == 1) {
-                    __bf16* to = a.acts + (long long)slot[j] * A * a.hidden_pad + k + (row & 4);
-#pragma unroll
-                    for (int t = 0; t < A; t++) *reinterpret_cast<Vec<__bf16, 4>*>(to + (long long)t * a.hidden_pad) = o[t];
-                } else {
-                    constexpr int kOut = Columns<A>::kSlots;
-                    const int i = s0 + j * kSlots + mine.slot;
-                    __bf16* to = a.acts + (long long)(fragment_of<kOut>(first, n) + i / kOut) * a.hidden_pad * 16 + k / 32 * 512 +
-                                 (k / 8 % 4 * 16 + i % kOut) * 8 + (row & 4);
-#pragma unroll
-                    for (int t = 0; t < A; t++) *reinterpret_cast<Vec<__bf16, 4>*>(to + t * kOut * 8) = o[t];
-                }
+            for (int g = 0; g < G; g++) {
+                h[g] = f4zero();
+                for (int u = 0; u < X; u++)
+                    for (int w = 0; w < joined; w++) h[g] += sums[w][g * NT + f][j][lane + u * kSlots];
             }
+            const int row = n0 + f * 16 + quad * 4;
+            Vec<__bf16, 4> o[A];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float v = activate(a.activation, h[0][r]);
+                if (G == 2) v *= h[G - 1][r];
+                if (row + r >= a.hidden) v = 0.0f;
+                __bf16 s[A];
+                split(v, s);
+#pragma unroll
+                for (int t = 0; t < A; t++) o[t][r] = s[t];
+            }
+            const int k = place_of(row & ~7, FORMAT == EXPERT_FP4);
+            constexpr int kOut = Columns<A>::kSlots;
+            __bf16* const to = CT == 1 ? a.acts + (long long)slot * A * a.hidden_pad + k + (row & 4)
+                                       : a.acts + (long long)(fragment_of<kOut>(first, n) + i / kOut) * a.hidden_pad * 16 +
+                                             k / 32 * 512 + (k / 8 % 4 * 16 + i % kOut) * 8 + (row & 4);
+#pragma unroll
+            for (int t = 0; t < A; t++) *reinterpret_cast<Vec<__bf16, 4>*>(to + (CT == 1 ? (long long)t * a.hidden_pad : t * kOut * 8)) = o[t];
+        }
         if (s0 + kSlots * CT < count) __syncthreads();
     }
 #endif
