@@ -302,3 +302,28 @@ def test_weights_beyond_2_gib(T, E, gated):
     for t in range(0, T, 21):
         want, bound = S.layer(x[t:t + 1], torch.full((1, 1), last), torch.ones(1, 1), w[0][2], w[1][2], H, 1, gated, code)
         assert bool((out[t].double() - want[0]).abs().le(bound[0] + 2.0 ** -23 * want[0].abs()).all())
+
+
+@pytest.mark.parametrize("T,E,k,code,fmt", [(64, 8, 2, 0, 0), (64, 1024, 4, 2, 1), (64, 64, 32, 1, 0)])
+def test_captured_with_much_lds(T, E, k, code, fmt):
+    """Kernels that ask for more than 64 KB of LDS, many slots an expert and many experts, replayed on other tokens."""
+    L = Layer(T, E, k, 192, 136, act=3, code=code, fmt=fmt, seed=95)
+    tokens = [L.x.clone(), torch.roll(L.x, 5, 0)]
+    want = []
+    for x in tokens:
+        L.x.copy_(x)
+        want.append(L.run().clone())
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        L.run(s.cuda_stream)
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            L.run(s.cuda_stream)
+        for rep in range(5):
+            L.x.copy_(tokens[rep % 2])
+            L.out.fill_(-7)
+            graph.replay()
+            s.synchronize()
+            assert torch.equal(L.out, want[rep % 2]), rep
