@@ -6,7 +6,7 @@
 // exact, and go to v_mfma_f32_16x16x32_bf16 as 16 rows by 32 of k; an expert's slots
 // (a token's place for it) are its 16 columns, few or many, at the same cost.  Tokens
 // and a_j are split into as many bf16 terms as they need (16-bit tokens are exact in
-// one or two, fp32 ones in three; a_j has two, 16 bits, or three under fp32 tokens),
+// one or two, fp32 ones in three; a_j has two, 17 bits, or three under fp32 tokens),
 // so that nothing is rounded to 8 bits on the way.
 //
 // Three launches: routing (the last workgroup to have its logits ready routes all
@@ -60,16 +60,19 @@ struct Terms {
     static constexpr int kA = sizeof(T) == 4 ? 3 : 2;                                  // of a hidden activation
 };
 
-// v as N bf16 numbers: the first N - 1 cut, so that what is left over is exact, the
-// last rounded.  An infinity is the first alone, a NaN also the last.
+// v as N bf16 numbers, each what is nearest to what those before it leave, which is
+// exact: two keep 17 bits of v, three all of an fp32 number.  Where rounding would
+// give an infinity for a finite v, the first is cut.  An infinity is the first alone,
+// a NaN also the last.
 template <int N>
 __device__ __forceinline__ void split(float v, __bf16 (&t)[N])
 {
 #pragma unroll
     for (int i = 0; i < N - 1; i++) {
-        const float cut = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);
-        t[i] = (__bf16)cut;
-        v = __builtin_isinf(v) ? 0.0f : v - cut;
+        float near = (float)(__bf16)v;
+        if (__builtin_isinf(near)) near = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);
+        t[i] = (__bf16)near;
+        v = __builtin_isinf(v) ? 0.0f : v - near;
     }
     t[N - 1] = (__bf16)v;
 }
@@ -323,7 +326,9 @@ __host__ __device__ inline RouteLds route_lds(const LayerArgs& a, int waves, int
 
 // Logits of 16 experts over a part of k that the waves share out; the tokens' terms on
 // the way; routing and plan by the workgroup that is last.  Products of terms are
-// exact; those of 2^-24 of a product and less are left out.  Bound by round trips.  A
+// exact; a second term is at most 2^-8 of its number and a third 2^-17, so that the
+// products that are left out come to 2^-24 of the whole one at most, of either sign.
+// Bound by round trips.  A
 // part is two blocks of k, a quarter of one for each of eight waves, while that makes
 // no more than 128 workgroups, so that reading and splitting tokens is spread (64 fp32
 // tokens of 4096 by 8 experts: 14.2 us, 19.9 with four blocks, 13.0 with one; 27 of
