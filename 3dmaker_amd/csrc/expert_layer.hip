@@ -23,6 +23,7 @@
 #include "route_math.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace graft {
 
@@ -70,9 +71,9 @@ __device__ __forceinline__ void split(float v, __bf16 (&t)[N])
 #pragma unroll
     for (int i = 0; i < N - 1; i++) {
         float near = (float)(__bf16)v;
-        if (__builtin_isinf(near)) near = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);
+        if (i == 0 && __builtin_isinf(near)) near = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);
         t[i] = (__bf16)near;
-        v = __builtin_isinf(v) ? 0.0f : v - near;
+        v = i == 0 && __builtin_isinf(near) ? 0.0f : v - near;
     }
     t[N - 1] = (__bf16)v;
 }
@@ -103,6 +104,14 @@ __device__ __forceinline__ void load8(T (&v)[8], const T* p, int n, bool vec)
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = j < n ? p[j] : (T)0.0f;
     }
+}
+
+// v but for its infinities, which are zero.
+__device__ __forceinline__ bf16x8 finite8(bf16x8 v)
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = __builtin_isinf((float)v[i]) ? (__bf16)0.0f : v[i];
+    return v;
 }
 
 template <class T, int N = Terms<T>::kX>
@@ -350,9 +359,12 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
     const int all = a.tokens * a.experts;
     float* const logits = at.logits ? reinterpret_cast<float*>(lds + at.logits_at) : nullptr;
     f4 acc[MT];
+    const R* r = (const R*)a.router + (long long)min(e0 + col, a.experts - 1) * a.dim;
 #pragma unroll
     for (int j = 0; j < MT; j++) acc[j] = f4zero();
-    const R* r = (const R*)a.router + (long long)min(e0 + col, a.experts - 1) * a.dim;
+    auto load_x = [&](T(&w)[8], int j, int k) {
+        load8(w, (const T*)a.x + min(j * 16 + col, a.tokens - 1) * a.stride_x + k, a.dim - k, a.vec_x);
+    };
     for (int u = 4 * kb0 + wave; u < 4 * kb1; u += waves) {  // a quarter of a block at a time
         const int kb = u / 4, k = kb * 128 + quad * 32 + u % 4 * 8;
         R v[8];
@@ -361,8 +373,7 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
         T w[MT][8];
 #pragma unroll
         for (int j = 0; j < MT; j++)
-            if (j * 16 < a.tokens)
-                load8(w[j], (const T*)a.x + min(j * 16 + col, a.tokens - 1) * a.stride_x + k, a.dim - k, a.vec_x);
+            if (j * 16 < a.tokens) load_x(w[j], j, k);
         split8(v, y);
 #pragma unroll
         for (int j = 0; j < MT; j++) {
@@ -380,6 +391,36 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
 #pragma unroll
                 for (int m = 0; m < X; m++)
                     *reinterpret_cast<bf16x8*>(a.xs + ((long long)t * X + m) * a.dim_pad + place_of(k, a.fp4)) = x[m];
+            }
+        }
+    }
+    // An infinity, which is a first term, makes a NaN with the other operand's second term
+    // where that is zero or of the other sign: then all of it again, where it meets the
+    // first term alone.
+    if constexpr (X * Y > 1) {
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+            const bool nan = __builtin_isnan(acc[j][0]) || __builtin_isnan(acc[j][1]) || __builtin_isnan(acc[j][2]) || __builtin_isnan(acc[j][3]);
+            if (!__any(nan)) continue;
+            acc[j] = f4zero();
+#pragma unroll 1
+            for (int u = 4 * kb0 + wave; u < 4 * kb1; u += waves) {
+                const int k = u / 4 * 128 + quad * 32 + u % 4 * 8;
+                R v[8];
+                T w[8];
+                bf16x8 x[X], y[Y];
+                load8(v, r + k, a.dim - k, a.vec_router);
+                load_x(w, j, k);
+                split8(v, y);
+                split8(w, x);
+                const bf16x8 first_x = finite8(x[0]), first_y = finite8(y[0]);
+#pragma unroll
+                for (int m = 0; m < X; m++)
+#pragma unroll
+                    for (int n = 0; n < Y; n++)
+                        if (m + n < 3)
+                            acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(n == 0 && m > 0 ? first_y : y[n],
+                                                                             m == 0 && n > 0 ? first_x : x[m], acc[j], 0, 0, 0);
             }
         }
     }

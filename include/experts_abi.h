@@ -270,8 +270,12 @@ typedef struct ExpertLayerOption {
  * 2 H) x D] and W2 [E x D x H] as the quantising launchers write them (scale
  * bytes of EXPERT_FP8 17 to 246).  Neither x nor a is quantised: products of the
  * weights' values and the tokens' are exact, a is held in 17 significant bits (in
- * all 24 of fp32 for fp32 tokens), sums are fp32, and out is rounded once.  A token none of whose experts is available (NaN among its logits) gets
- * zeros.  out may be x.  A stream's first call cannot be captured into a graph. */
+ * all 24 of fp32 for fp32 tokens), sums are fp32, and out is rounded once; of fp32
+ * numbers what lies below 2^-133 is lost.  Infinities count as they do in these
+ * formulas: a logit that one makes infinite is the largest finite number or makes
+ * its expert unavailable, as for launchRouteExperts.  A token none of whose experts
+ * is available (NaN among its logits) gets zeros.  out may be x.  A stream's first
+ * call cannot be captured into a graph. */
 void launchExpertLayer(const ExpertLayerOption* opt, const void* d_x, const void* d_router, const float* d_bias,
                        const uint8_t* d_w1, const uint8_t* d_w1Scales, const uint8_t* d_w2, const uint8_t* d_w2Scales,
                        void* d_out, int numTokens, hipStream_t stream);
