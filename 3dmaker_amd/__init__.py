@@ -21,7 +21,7 @@ __all__ = [
     "LIB_PATH", "lib", "launch", "MLPOption", "MLPGridOptions", "HashGrid", "Net",
     "OUT_ACT_NONE", "OUT_ACT_SIGMOID", "ptr", "check", "RouteOption", "Fp8QuantOption", "Fp8ProductOption", "NormGateOption",
     "Fp4QuantOption", "Fp4ProductOption", "ExpertLayerOption", "GradTensor", "FP4_SCALE_FLOOR", "FP4_SCALE_COVER",
-    "EXPERT_FP8", "EXPERT_FP4", "EXPERT_LINEAR", "EXPERT_RELU", "EXPERT_SILU", "EXPERT_GELU", "EXPERT_LAYER_TOKENS",
+    "EXPERT_FP8", "EXPERT_FP4", "EXPERT_LINEAR", "EXPERT_RELU", "EXPERT_SILU", "EXPERT_GELU", "EXPERT_LAYER_TOKENS", "EXPERT_HIDDEN_F32",
     "GRAD_NORM_2", "GRAD_NORM_MAX", "GRAD_NONFINITE_KEEP", "GRAD_NONFINITE_ZERO", "fp4_pitch", "fp4_scale_pitch",
     "DATA_F32", "DATA_F16", "DATA_BF16", "ROUTE_SOFTMAX", "ROUTE_SIGMOID", "PRODUCT_DENSE", "PRODUCT_ROWS", "PRODUCT_SUM", "PRODUCT_EXACT", "COMBINE_ROWS_F32",
     "NORM_NONE", "NORM_RMS", "NORM_LAYER", "fp8_pitch", "fp8_scale_pitch", "Float3", "Uint3", "NerfOptions", "Nerf", "NerfTrainer", "NtrConfig", "NtrStats",
@@ -41,6 +41,7 @@ FP4_SCALE_FLOOR, FP4_SCALE_COVER = 0, 1
 EXPERT_FP8, EXPERT_FP4 = 0, 1
 EXPERT_LINEAR, EXPERT_RELU, EXPERT_SILU, EXPERT_GELU = 0, 1, 2, 3
 EXPERT_LAYER_TOKENS = 64
+EXPERT_HIDDEN_F32 = 0x100
 
 # include/grad_abi.h
 GRAD_NORM_2, GRAD_NORM_MAX = 0, 1

@@ -6,7 +6,7 @@
 // exact, and go to v_mfma_f32_16x16x32_bf16 as 16 rows by 32 of k; an expert's slots
 // (a token's place for it) are its 16 columns, few or many, at the same cost.  Tokens
 // and a_j are split into as many bf16 terms as they need (16-bit tokens are exact in
-// one or two, fp32 ones in three; a_j has two, 17 bits, or three under fp32 tokens),
+// one or two, fp32 ones in three; a_j has two, 17 bits, or three, all of fp32),
 // so that nothing is rounded to 8 bits on the way.
 //
 // Three launches: routing (the last workgroup to have its logits ready routes all
@@ -58,8 +58,13 @@ struct LayerArgs {
 template <class T>
 struct Terms {
     static constexpr int kX = sizeof(T) == 4 ? 3 : std::is_same_v<T, __bf16> ? 1 : 2;  // of a token or a router's row
-    static constexpr int kA = sizeof(T) == 4 ? 3 : 2;                                  // of a hidden activation
 };
+
+// Of a hidden activation, A below: two under 16-bit tokens, three under fp32 ones and on
+// request (us with two and with three: 27 tokens, top 8 of 128, gated 2048 x 768 fp8 107
+// and 115; 64, top 2 of 8, gated 2048 x 1024 fp8 37.7 and 40.4; 7, top 6 of 64, fp4 45
+// and 46).
+constexpr int a_terms_of(bool f32) { return f32 ? 3 : 2; }
 
 // v as N bf16 numbers, each what is nearest to what those before it leave, which is
 // exact: two keep 17 bits of v, three all of an fp32 number.  Where rounding would
@@ -693,12 +698,12 @@ __global__ __launch_bounds__(256) void layer_gather_kernel(LayerArgs a)
 // of 64, 2048 x 1024 fp4), 52.2, 68.8 and 98 (27 tokens, top 8 of 128, 2048 x 768 fp8).
 constexpr int kHiddenWaves = 4;
 
-template <int FORMAT, class T, int G, int NT, int CT>
+template <int FORMAT, class T, int A, int G, int NT, int CT>
 __global__ __launch_bounds__(kHiddenWaves * 64, CT == 4 ? 2 : CT == 2 ? 3 : 4) void layer_hidden_kernel(LayerArgs a)
 {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass needs the kernel's name alone
     constexpr int WAVES = kHiddenWaves;
-    constexpr int X = Terms<T>::kX, A = Terms<T>::kA, F = G * NT, kSlots = Columns<X>::kSlots;
+    constexpr int X = Terms<T>::kX, F = G * NT, kSlots = Columns<X>::kSlots;
     constexpr int kCopies = Piece<FORMAT>::kCopies, kBlock = F * kCopies * kCopyBytes;
     constexpr int kSums = WAVES * F * CT * 1024, kRings = WAVES * 2 * kBlock;
     // One array: with two, the compiler waits for all copies before each LDS read.
@@ -833,11 +838,11 @@ __global__ __launch_bounds__(kHiddenWaves * 64, CT == 4 ? 2 : CT == 2 ? 3 : 4) v
 // kernel is: 16.7 us for 36 MB, 34 for 166 MB (4.9 TB/s).
 constexpr int kOutWaves = 8;
 
-template <int FORMAT, class T, int NT, int CT>
+template <int FORMAT, class T, int A, int NT, int CT>
 __global__ __launch_bounds__(kOutWaves * 64) void layer_out_kernel(LayerArgs a)
 {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass needs the kernel's name alone
-    constexpr int WAVES = kOutWaves, A = Terms<T>::kA, kSlots = Columns<A>::kSlots;
+    constexpr int WAVES = kOutWaves, kSlots = Columns<A>::kSlots;
     constexpr int kCopies = Piece<FORMAT>::kCopies, kBlock = NT * kCopies * kCopyBytes;
     extern __shared__ __attribute__((aligned(128))) uint8_t lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -1050,22 +1055,22 @@ void allow_lds(const void* kernel, size_t lds)
     if (lds > 64 * 1024) GRAFT_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
 }
 
-template <int FORMAT, class T, int G, int NT, int CT>
+template <int FORMAT, class T, int A, int G, int NT, int CT>
 void hidden_launch(const LayerArgs& a, hipStream_t s)
 {
     const unsigned most = (unsigned)std::min(a.experts, a.tokens * a.topk);
-    layer_hidden_kernel<FORMAT, T, G, NT, CT><<<dim3(a.hidden_pad / (16 * NT), most), kHiddenWaves * 64, 0, s>>>(a);
+    layer_hidden_kernel<FORMAT, T, A, G, NT, CT><<<dim3(a.hidden_pad / (16 * NT), most), kHiddenWaves * 64, 0, s>>>(a);
     GRAFT_LAUNCH_CHECK();
 }
 
-template <int FORMAT, class T, int NT, int CT>
+template <int FORMAT, class T, int A, int NT, int CT>
 void out_launch(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
     const int slots = a.tokens * a.topk, most = std::min(a.experts, slots);
     const size_t lds = kOutWaves * ((size_t)2 * NT * Piece<FORMAT>::kCopies * kCopyBytes + (size_t)a.tokens * 64 * NT) +
                        (size_t)(2 * most + 1 + 2 * slots) * 4;
-    allow_lds((const void*)layer_out_kernel<FORMAT, T, NT, CT>, lds);
-    layer_out_kernel<FORMAT, T, NT, CT><<<dim3(p.out_tiles, p.out_parts), kOutWaves * 64, lds, s>>>(a);
+    allow_lds((const void*)layer_out_kernel<FORMAT, T, A, NT, CT>, lds);
+    layer_out_kernel<FORMAT, T, A, NT, CT><<<dim3(p.out_tiles, p.out_parts), kOutWaves * 64, lds, s>>>(a);
     GRAFT_LAUNCH_CHECK();
 }
 
@@ -1079,20 +1084,20 @@ void route_launch(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
     GRAFT_LAUNCH_CHECK();
 }
 
-template <int FORMAT, class T>
+template <int FORMAT, class T, int A>
 void products(const LayerArgs& a, const LayerPlan& p, hipStream_t s)
 {
-    constexpr int CT = sizeof(T) == 4 ? 4 : 2;
+    constexpr int CT = Terms<T>::kX == 3 ? 4 : 2;  // fragments: 20 slots of three terms, 16 or 32 of fewer
     if (p.many) {
         layer_gather_kernel<T><<<dim3(a.dim_pad / 128, std::min(a.experts, a.tokens * a.topk)), 256, 0, s>>>(a);
         GRAFT_LAUNCH_CHECK();
-        if (a.gated) hidden_launch<FORMAT, T, 2, 1, CT>(a, s);
-        else hidden_launch<FORMAT, T, 1, 2, CT>(a, s);
-        out_launch<FORMAT, T, 2, CT>(a, p, s);
+        if (a.gated) hidden_launch<FORMAT, T, A, 2, 1, CT>(a, s);
+        else hidden_launch<FORMAT, T, A, 1, 2, CT>(a, s);
+        out_launch<FORMAT, T, A, 2, A == 3 ? 4 : 2>(a, p, s);
     } else {
-        if (a.gated) hidden_launch<FORMAT, T, 2, 1, 1>(a, s);
-        else hidden_launch<FORMAT, T, 1, 1, 1>(a, s);
-        out_launch<FORMAT, T, 1, 1>(a, p, s);
+        if (a.gated) hidden_launch<FORMAT, T, A, 2, 1, 1>(a, s);
+        else hidden_launch<FORMAT, T, A, 1, 1, 1>(a, s);
+        out_launch<FORMAT, T, A, 1, 1>(a, p, s);
     }
 }
 
@@ -1108,7 +1113,9 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     require(o.weightFormat == EXPERT_FP8 || o.weightFormat == EXPERT_FP4, "unknown weightFormat");
     require(o.scaleRows == 1 || (o.scaleRows == 128 && o.weightFormat == EXPERT_FP8),
             "scaleRows must be 1, or 128 with EXPERT_FP8");
-    require_type(o.dataType);
+    const int type = o.dataType & ~EXPERT_HIDDEN_F32;
+    const bool hidden_f32 = type == DATA_F32 || (o.dataType & EXPERT_HIDDEN_F32);
+    require_type(type);
     require_type(o.routerType);
     require(o.strideX >= o.dim && o.strideOut >= o.dim, "strides must be at least dim");
     if (tokens == 0) return;
@@ -1140,7 +1147,7 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
     a.renorm = o.route.renormalize != 0;
     a.gated = o.gated != 0;
     a.fp4 = o.weightFormat == EXPERT_FP4;
-    const int bytes = data_bytes(o.dataType);
+    const int bytes = data_bytes(type);
     a.vec_x = aligned16(t.x) && o.strideX * bytes % 16 == 0;
     a.vec_router = aligned16(t.router) && (long long)o.dim * data_bytes(o.routerType) % 16 == 0;
     a.vec_out = aligned16(out) && o.strideOut * bytes % 16 == 0;
@@ -1155,7 +1162,7 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
         size += round_up<size_t>(n, 256);
         return at;
     };
-    const size_t x_terms = o.dataType == DATA_F32 ? 3 : o.dataType == DATA_BF16 ? 1 : 2, a_terms = o.dataType == DATA_F32 ? 3 : 2;
+    const size_t x_terms = type == DATA_F32 ? 3 : type == DATA_BF16 ? 1 : 2, a_terms = a_terms_of(hidden_f32);
     const size_t at_logits = take((size_t)p.route_parts * tokens * a.experts * 4), at_weights = take((size_t)slots * 4);
     const size_t at_active = take((size_t)(most + 1) * 4), at_first = take((size_t)(most + 1) * 4), at_slots = take((size_t)slots * 4);
     const size_t at_xs = take((size_t)tokens * x_terms * a.dim_pad * 2);
@@ -1180,14 +1187,20 @@ void expert_layer(const ExpertLayerOption& o, const ExpertLayerTensors& t, void*
         a.out_tickets = (uint32_t*)(ws + at_tickets);
         a.out_tiles = p.out_tiles;
     }
-    with_type(o.dataType, [&](auto x) {
+    with_type(type, [&](auto x) {
         using T = decltype(x);
         with_type(o.routerType, [&](auto r) {
             if (tokens <= 16) route_launch<T, decltype(r), 1>(a, p, s);
             else route_launch<T, decltype(r), 4>(a, p, s);
         });
-        if (o.weightFormat == EXPERT_FP8) products<EXPERT_FP8, T>(a, p, s);
-        else products<EXPERT_FP4, T>(a, p, s);
+        auto of_format = [&](auto f) {
+            constexpr int F = decltype(f)::value;
+            if constexpr (sizeof(T) == 4) products<F, T, a_terms_of(true)>(a, p, s);
+            else if (hidden_f32) products<F, T, a_terms_of(true)>(a, p, s);
+            else products<F, T, a_terms_of(false)>(a, p, s);
+        };
+        if (o.weightFormat == EXPERT_FP8) of_format(std::integral_constant<int, EXPERT_FP8>{});
+        else of_format(std::integral_constant<int, EXPERT_FP4>{});
     });
 }
 

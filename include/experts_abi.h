@@ -256,12 +256,16 @@ typedef struct ExpertLayerOption {
     int gated;            /* nonzero: W1 has 2 H rows, the activation's and those that it is multiplied by */
     int weightFormat;     /* EXPERT_FP8 or EXPERT_FP4 */
     int scaleRows;        /* rows of a matrix that share a scale: EXPERT_FP8 1 or 128, EXPERT_FP4 1 */
-    int dataType;         /* DATA_*, of x and out */
+    int dataType;         /* DATA_*, of x and out, and EXPERT_HIDDEN_F32 */
     int routerType;       /* DATA_*, of the router */
     long long strideX, strideOut; /* between rows */
 } ExpertLayerOption;
 
 #define EXPERT_LAYER_TOKENS 64
+
+/* Or'ed to dataType: the hidden activations of 16-bit tokens are held in all of
+ * fp32, as those of fp32 tokens always are. */
+#define EXPERT_HIDDEN_F32 0x100
 
 /* out[t] = sum_j w_j W2_e a(W1_e x[t]) over the experts e = e_j and weights w_j
  * that launchRouteExperts gives for the logits x router^T (and d_bias, nullable):
@@ -270,7 +274,7 @@ typedef struct ExpertLayerOption {
  * 2 H) x D] and W2 [E x D x H] as the quantising launchers write them (scale
  * bytes of EXPERT_FP8 17 to 246).  Neither x nor a is quantised: products of the
  * weights' values and the tokens' are exact, a is held in 17 significant bits (in
- * all 24 of fp32 for fp32 tokens), sums are fp32, and out is rounded once; of fp32
+ * all 24 of fp32 for fp32 tokens and with EXPERT_HIDDEN_F32), sums are fp32, and out is rounded once; of fp32
  * numbers what lies below 2^-133 is lost.  Infinities count as they do in these
  * formulas: a logit that one makes infinite is the largest finite number or makes
  * its expert unavailable, as for launchRouteExperts.  A token none of whose experts

@@ -8,8 +8,11 @@ torch = pytest.importorskip("torch")
 
 import experts_ref as R  # noqa: E402
 import serving_ref as S  # noqa: E402
+from helpers import pkg  # noqa: E402
+from test_gpu_expert_layer import Layer  # noqa: E402
 
 pytestmark = pytest.mark.gpu
+EXACT = pkg().EXPERT_HIDDEN_F32
 
 
 def quantized(w):
@@ -52,6 +55,59 @@ def test_hidden_values(T, code):
     off = 0.0 if code == 0 else 2.0 ** -17
     bound = off + S.HALF[code] * (want + off) + S.TINY[code]
     assert bool((got - want).abs().le(bound).all()), float((got - want).abs().max() * 2 ** 17)
+
+
+@pytest.mark.parametrize("T", [1, 7, 40])
+@pytest.mark.parametrize("code", [0, 1, 2])
+def test_hidden_values_in_fp32(T, code):
+    """On request nothing of them is lost, and no other result changes."""
+    n = 96
+    x, w1, w2, want = hidden_values(T, n, code)
+    o = S.layer_option(1, 1, n, 2 * n, act=0, code=code | EXACT)
+    got = run(x, torch.zeros(1, n, device="cuda"), w1, w2, o)
+    assert torch.equal(got, want.to(got.dtype).expand(T, n))
+
+
+@pytest.mark.parametrize("T,E,k,D,H,act,gated,fmt", [
+    (1, 8, 2, 64, 96, 1, False, 0), (7, 16, 4, 300, 200, 2, True, 1), (11, 4, 2, 136, 140, 3, False, 0),
+    (33, 5, 2, 260, 72, 2, True, 1), (64, 4, 2, 136, 264, 0, True, 0), (64, 16, 1, 384, 130, 3, False, 1)])
+@pytest.mark.parametrize("code", [1, 2])
+def test_layers_in_fp32(T, E, k, D, H, act, gated, fmt, code):
+    """Against 64 bits with hidden values of 24 bits: tokens widened to fp32 are the same tokens, whose bound counts that."""
+    L = Layer(T, E, k, D, H, act=act, gated=gated, fmt=fmt, code=code, seed=11)
+    L.o.dataType |= EXACT
+    got = L.run()
+    want, bound = S.layer(L.x, L.indices, L.weights, L.w1[2], L.w2[2], H, act, gated, 0)
+    dz = float(((D / 8 + 16) * 2.0 ** -24 * (L.x.double().abs() @ L.router.double().abs().t())).max())
+    bound = bound + (4 * dz + 16 * 2.0 ** -24) * L.magnitude()
+    assert bool((got.double() - want).abs().le(bound + S.HALF[code] * (want.abs() + bound) + S.TINY[code]).all())
+    assert torch.equal(got, L.run())
+
+
+def test_layers_in_fp32_captured():
+    """Many slots an expert and few, on a stream of its own, replayed on other tokens."""
+    for T, E in ((40, 4), (9, 16)):
+        L = Layer(T, E, 2, 264, 136, act=2, gated=True, code=2, seed=12)
+        L.o.dataType |= EXACT
+        tokens = [L.x.clone(), torch.roll(L.x, 3, 0)]
+        want = []
+        for x in tokens:
+            L.x.copy_(x)
+            want.append(L.run().clone())
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            L.run(s.cuda_stream)
+            s.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                L.run(s.cuda_stream)
+            for rep in range(4):
+                L.x.copy_(tokens[rep % 2])
+                L.out.fill_(-7)
+                graph.replay()
+                s.synchronize()
+                assert torch.equal(L.out, want[rep % 2]), rep
 
 
 def test_logits():
