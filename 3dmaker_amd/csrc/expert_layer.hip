@@ -1049,10 +1049,12 @@ LayerPlan layer_plan(const LayerArgs& a)
     return p;
 }
 
-// More dynamic LDS than any kernel may have has to be asked for.
+// More dynamic LDS than any kernel may have has to be asked for.  The limit is the
+// kernel's, not the call's: all ask for the same, so that none lowers what another
+// thread's launch, or a captured one, needs.
 void allow_lds(const void* kernel, size_t lds)
 {
-    if (lds > 64 * 1024) GRAFT_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    if (lds > 64 * 1024) GRAFT_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes));
 }
 
 template <int FORMAT, class T, int A, int G, int NT, int CT>
