@@ -459,9 +459,11 @@ struct Ticket {
             if (capturing) throw std::runtime_error("the first call of this kind on a stream cannot be captured: make one before");
             uint32_t* fresh = nullptr;
             GRAFT_HIP_CHECK(hipMalloc(&fresh, sizeof(uint32_t)));
+            hipLaunchKernelGGL(zero_ticket_kernel, dim3(1), dim3(1), 0, s, fresh);
+            const hipError_t launched = hipGetLastError();
+            if (launched != hipSuccess) (void)hipFree(fresh);  // the next call makes one
+            GRAFT_HIP_CHECK(launched);
             p = fresh;
-            hipLaunchKernelGGL(zero_ticket_kernel, dim3(1), dim3(1), 0, s, p);
-            GRAFT_LAUNCH_CHECK();
         }
         return p;
     }

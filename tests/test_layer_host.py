@@ -1,5 +1,5 @@
 """What launchExpertLayer asks of the HIP runtime, call by call, with a runtime of the test's own under the library (no GPU):
-limits of dynamic LDS, which belong to a kernel and not to a call."""
+limits of dynamic LDS, which belong to a kernel and not to a call, and the stream's counter when its clearing fails."""
 import os
 import subprocess
 import sys
@@ -96,4 +96,18 @@ for tokens, experts, topk, kw in ((64, 8, 2, {}), (40, 8, 2, {}), (33, 8, 2, {})
     assert call(tokens, experts, topk, **kw) == ""
 assert number("launches").value > 0 and number("beyond").value == 0
 assert number("lowered").value == 0, number("lowered").value
+""")
+
+
+def test_a_counter_that_could_not_be_cleared(tmp_path):
+    """The call says so, and the next one of that stream clears it."""
+    run(tmp_path, r"""
+number("fail_at").value = 0
+assert "the test's" in call(4, 8, 2)
+assert number("launches").value == 1 and number("held").value == 0
+assert call(4, 8, 2) == ""
+launched = (C.c_void_p * 256).in_dll(R, "launched")
+assert number("launches").value == 5 and launched[1] == launched[0]
+assert call(4, 8, 2) == ""  # and clears it once
+assert number("launches").value == 8 and launched[0] not in launched[2:8]
 """)
