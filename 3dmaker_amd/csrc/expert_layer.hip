@@ -69,16 +69,16 @@ constexpr int a_terms_of(bool f32) { return f32 ? 3 : 2; }
 // v as N bf16 numbers, each what is nearest to what those before it leave, which is
 // exact: two keep 17 bits of v, three all of an fp32 number.  Where rounding would
 // give an infinity for a finite v, the first is cut.  An infinity is the first alone,
-// a NaN also the last.
-template <int N>
+// a NaN also the last.  Not SAFE: infinities, and what rounds to them, become NaN.
+template <bool SAFE = true, int N>
 __device__ __forceinline__ void split(float v, __bf16 (&t)[N])
 {
 #pragma unroll
     for (int i = 0; i < N - 1; i++) {
         float near = (float)(__bf16)v;
-        if (i == 0 && __builtin_isinf(near)) near = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);
+        if (SAFE && i == 0 && __builtin_isinf(near)) near = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);
         t[i] = (__bf16)near;
-        v = i == 0 && __builtin_isinf(near) ? 0.0f : v - near;
+        v = SAFE && i == 0 && __builtin_isinf(near) ? 0.0f : v - near;
     }
     t[N - 1] = (__bf16)v;
 }
@@ -119,14 +119,14 @@ __device__ __forceinline__ bf16x8 finite8(bf16x8 v)
     return v;
 }
 
-template <class T, int N = Terms<T>::kX>
+template <bool SAFE, class T, int N = Terms<T>::kX>
 __device__ __forceinline__ void split8(const T (&v)[8], bf16x8 (&t)[N])
 {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         __bf16 s[N];
         if constexpr (N == 1) s[0] = v[i];
-        else split((float)v[i], s);
+        else split<SAFE>((float)v[i], s);
 #pragma unroll
         for (int u = 0; u < N; u++) t[u][i] = s[u];
     }
@@ -370,8 +370,14 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
     auto load_x = [&](T(&w)[8], int j, int k) {
         load8(w, (const T*)a.x + min(j * 16 + col, a.tokens - 1) * a.stride_x + k, a.dim - k, a.vec_x);
     };
+    auto store_x = [&](const bf16x8(&x)[X], int j, int k) {  // each workgroup of a part stores some blocks of the terms
+        const int t = j * 16 + col;
+        if (k / 128 % gridDim.x != blockIdx.x || t >= a.tokens) return;
+#pragma unroll
+        for (int m = 0; m < X; m++) *reinterpret_cast<bf16x8*>(a.xs + ((long long)t * X + m) * a.dim_pad + place_of(k, a.fp4)) = x[m];
+    };
     for (int u = 4 * kb0 + wave; u < 4 * kb1; u += waves) {  // a quarter of a block at a time
-        const int kb = u / 4, k = kb * 128 + quad * 32 + u % 4 * 8;
+        const int k = u / 4 * 128 + quad * 32 + u % 4 * 8;
         R v[8];
         bf16x8 y[Y];
         load8(v, r + k, a.dim - k, a.vec_router);
@@ -379,34 +385,31 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
 #pragma unroll
         for (int j = 0; j < MT; j++)
             if (j * 16 < a.tokens) load_x(w[j], j, k);
-        split8(v, y);
+        split8<false>(v, y);
 #pragma unroll
         for (int j = 0; j < MT; j++) {
             if (j * 16 >= a.tokens) break;
-            const int t = j * 16 + col;
             bf16x8 x[X];
-            split8(w[j], x);
+            split8<false>(w[j], x);
 #pragma unroll
             for (int m = 0; m < X; m++)
 #pragma unroll
                 for (int n = 0; n < Y; n++)
                     if (m + n < 3) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[n], x[m], acc[j], 0, 0, 0);
-            // each workgroup of a part stores some blocks of the terms
-            if (kb % gridDim.x == blockIdx.x && t < a.tokens) {
-#pragma unroll
-                for (int m = 0; m < X; m++)
-                    *reinterpret_cast<bf16x8*>(a.xs + ((long long)t * X + m) * a.dim_pad + place_of(k, a.fp4)) = x[m];
-            }
+            store_x(x, j, k);
         }
     }
-    // An infinity, which is a first term, makes a NaN with the other operand's second term
-    // where that is zero or of the other sign: then all of it again, where it meets the
-    // first term alone.
+    // An infinity has become a NaN, which it would also with the other operand's second
+    // term where that is zero or of the other sign.  Where there is a NaN all of it again,
+    // infinities as first terms, which meet the other operand's first term alone.
     if constexpr (X * Y > 1) {
+        float any = 0.0f;
+#pragma unroll
+        for (int j = 0; j < MT; j++) any += (acc[j][0] + acc[j][1]) + (acc[j][2] + acc[j][3]);
+        const bool again = __any(__builtin_isnan(any));
 #pragma unroll
         for (int j = 0; j < MT; j++) {
-            const bool nan = __builtin_isnan(acc[j][0]) || __builtin_isnan(acc[j][1]) || __builtin_isnan(acc[j][2]) || __builtin_isnan(acc[j][3]);
-            if (!__any(nan)) continue;
+            if (!again || j * 16 >= a.tokens) break;
             acc[j] = f4zero();
 #pragma unroll 1
             for (int u = 4 * kb0 + wave; u < 4 * kb1; u += waves) {
@@ -416,8 +419,8 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
                 bf16x8 x[X], y[Y];
                 load8(v, r + k, a.dim - k, a.vec_router);
                 load_x(w, j, k);
-                split8(v, y);
-                split8(w, x);
+                split8<true>(v, y);
+                split8<true>(w, x);
                 const bf16x8 first_x = finite8(x[0]), first_y = finite8(y[0]);
 #pragma unroll
                 for (int m = 0; m < X; m++)
@@ -426,6 +429,7 @@ __global__ __launch_bounds__(kRouteThreads) void layer_route_kernel(LayerArgs a)
                         if (m + n < 3)
                             acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(n == 0 && m > 0 ? first_y : y[n],
                                                                              m == 0 && n > 0 ? first_x : x[m], acc[j], 0, 0, 0);
+                store_x(x, j, k);
             }
         }
     }
