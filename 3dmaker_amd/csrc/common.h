@@ -121,7 +121,8 @@ private:
 Workspace& stream_workspace(hipStream_t s);
 
 // A counter of (current device, stream), zero: a kernel that counts its workgroups
-// with it leaves it zero again, so that the stream's next finds it so.  Kept as the
+// with it leaves it zero again, so that the stream's next finds it so (a later kernel of
+// the call clears it once more, in case others counted at the same time).  Kept as the
 // workspace is, of which it is no part; made by the first call, which cannot be one
 // under capture.
 uint32_t* stream_ticket(hipStream_t s);

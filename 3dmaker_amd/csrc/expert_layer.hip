@@ -985,6 +985,9 @@ __global__ __launch_bounds__(kOutWaves * 64) void layer_out_kernel(LayerArgs a)
         };
         in_two_places([&] { return ahead.valid(); }, load, load, work, work);
     }
+    // Zero already, unless calls that share the counter ran at once, against the rules:
+    // then at least the stream's next one finds it so.
+    if (blockIdx.x + blockIdx.y + threadIdx.x == 0) *a.route_ticket = 0;
     __syncthreads();
     const int pieces = a.tokens * 4 * NT;
     auto store = [&](int i, f4 v) {
