@@ -232,19 +232,36 @@ __global__ __launch_bounds__(kGradThreads) void grad_norm_kernel(GradArgs a)
     if (threadIdx.x == 0) *a.norm_out = n;
 }
 
+// What gradients are multiplied by: max / n, as v 2^e where it is below the normal
+// numbers, whose few bits would be those of every gradient.
+struct Factor {
+    float v;
+    int e;
+    __device__ __forceinline__ Factor(float max_norm, float n)
+    {
+        v = n > max_norm ? max_norm / n : 1.0f;
+        e = 0;
+        if (v < 0x1p-126f && max_norm > 0.0f) {
+            int max_e, n_e;
+            v = frexpf(max_norm, &max_e) * 0.5f / frexpf(n, &n_e);  // at most 1: products stay finite
+            e = max_e + 1 - n_e;
+        }
+    }
+};
+
 template <int THREADS, class T>
-__device__ __forceinline__ void clip_piece(const void* data, void* out, long long n, uint32_t piece, float factor, bool zero)
+__device__ __forceinline__ void clip_piece(const void* data, void* out, long long n, uint32_t piece, Factor factor, bool zero)
 {
     constexpr int N = Span<T>::N;
     const Span<T> t(data, n);
     T* const to = (T*)out - t.lo;
-    auto scaled = [&](T v) { return zero ? (T)0.0f : (T)((float)v * factor); };
+    auto scaled = [&](T v) { return zero ? (T)0.0f : (T)ldexpf((float)v * factor.v, factor.e); };
     auto one = [&](long long at, int, T v) { to[at] = scaled(v); };
     if (((uintptr_t)to & 15) == 0) {
         for_parts<THREADS>(
             t, piece,
             [&](long long at, Vec<T, N> v) {
-                if (factor != 1.0f || zero) {
+                if (factor.v != 1.0f || zero) {
 #pragma unroll
                     for (int j = 0; j < N; j++) v[j] = scaled(v[j]);
                 }
@@ -266,10 +283,10 @@ template <int THREADS>
 __device__ __forceinline__ void clip_all(const GradTable& t, const GradArgs& a, float n, uint32_t worker, uint32_t workers)
 {
     const bool finite = magnitude(n) < 0x7f800000u, zero = !finite && a.zero;
-    const float factor = finite && n > a.max_norm ? a.max_norm / n : 1.0f;
+    const Factor factor(a.max_norm, finite ? n : 0.0f);
     for_pieces<true>(t, worker, workers, [&](int i, uint32_t piece) {
         void* const out = t.out[i];
-        if (out == t.data[i] && factor == 1.0f && !zero) return;
+        if (out == t.data[i] && factor.v == 1.0f && !zero) return;
         with_type_of(t.type[i], [&](auto z) { clip_piece<THREADS, decltype(z)>(t.data[i], out, t.n[i], piece, factor, zero); });
     });
 }

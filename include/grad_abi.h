@@ -39,7 +39,7 @@ typedef struct GradTensor {
  * does a norm beyond fp32.  count 0..65536. */
 void launchGradNorm(const GradTensor* tensors, int count, int norm, float gradScale, float* d_norm, hipStream_t stream);
 
-/* g = g * min(1, maxNorm / *d_norm), each element rounded once to its type.  d_norm
+/* g = g * min(1, maxNorm / *d_norm) in fp32, rounded to g's type.  d_norm
  * is launchGradNorm's, or what ranks that hold parts of the gradients have made of
  * theirs.  In place nothing is written where the factor is 1.  maxNorm >= 0.
  * A tensor that is written may not overlap another of the list. */
