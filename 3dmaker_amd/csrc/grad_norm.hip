@@ -329,15 +329,21 @@ void check_list(const GradTensor* tensors, int count)
     }
 }
 
+void check_norm_pointer(const float* d_norm)
+{
+    require(d_norm, "null argument");
+    require(((uintptr_t)d_norm & 3) == 0, "d_norm must be aligned to its elements");
+}
+
 void check_norm(int norm, float scale, const float* d_norm)
 {
     require(norm == GRAD_NORM_2 || norm == GRAD_NORM_MAX, "unknown norm");
     require(std::isfinite(scale) && scale > 0.0f, "gradScale must be finite and above 0");
-    require(d_norm, "null argument");
+    check_norm_pointer(d_norm);
 }
 
-// Nothing that is written is another tensor's.
-void check_clip(const GradTensor* tensors, int count, float max_norm, int non_finite)
+// Nothing that is written is another tensor's, or the norm's.
+void check_clip(const GradTensor* tensors, int count, float max_norm, int non_finite, const float* d_norm, bool norm_written)
 {
     require(max_norm >= 0.0f, "maxNorm must be >= 0");
     require(non_finite == GRAD_NONFINITE_KEEP || non_finite == GRAD_NONFINITE_ZERO, "unknown nonFinite");
@@ -346,7 +352,7 @@ void check_clip(const GradTensor* tensors, int count, float max_norm, int non_fi
         bool written;
     };
     std::vector<Range> all;
-    all.reserve(2 * count);
+    all.reserve(2 * (size_t)count);
     for (int i = 0; i < count; i++) {
         const GradTensor& t = tensors[i];
         if (t.n == 0) continue;
@@ -355,6 +361,10 @@ void check_clip(const GradTensor* tensors, int count, float max_norm, int non_fi
         all.push_back({in, in + size, in_place});
         if (!in_place) all.push_back({out, out + size, true});
     }
+    check_norm_pointer(d_norm);
+    const uintptr_t norm_lo = (uintptr_t)d_norm, norm_hi = norm_lo + sizeof(float);
+    for (const Range& t : all)
+        require(norm_hi <= t.lo || t.hi <= norm_lo || !(norm_written || t.written), "d_norm overlaps a tensor");
     auto before = [](const Range& a, const Range& b) { return a.lo < b.lo; };
     if (!std::is_sorted(all.begin(), all.end(), before)) std::sort(all.begin(), all.end(), before);
     uintptr_t read = 0, written = 0;  // where those so far end
@@ -475,8 +485,7 @@ void grad_norm(const GradTensor* tensors, int count, int norm_kind, float scale,
 void grad_clip(const GradTensor* tensors, int count, float max_norm, int non_finite, const float* d_norm, hipStream_t s)
 {
     check_list(tensors, count);
-    check_clip(tensors, count, max_norm, non_finite);
-    require(d_norm, "null argument");
+    check_clip(tensors, count, max_norm, non_finite, d_norm, false);
     GradArgs a{};
     a.max_norm = max_norm;
     a.zero = non_finite == GRAD_NONFINITE_ZERO;
@@ -489,7 +498,7 @@ void grad_norm_clip(const GradTensor* tensors, int count, int norm_kind, float s
 {
     check_list(tensors, count);
     check_norm(norm_kind, scale, d_norm);
-    check_clip(tensors, count, max_norm, non_finite);
+    check_clip(tensors, count, max_norm, non_finite, d_norm, true);
     GradArgs a{};
     a.top = norm_kind == GRAD_NORM_MAX;
     a.scale = scale;

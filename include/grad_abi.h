@@ -42,11 +42,12 @@ void launchGradNorm(const GradTensor* tensors, int count, int norm, float gradSc
 /* g = g * min(1, maxNorm / *d_norm) in fp32, rounded to g's type.  d_norm
  * is launchGradNorm's, or what ranks that hold parts of the gradients have made of
  * theirs.  In place nothing is written where the factor is 1.  maxNorm >= 0.
- * A tensor that is written may not overlap another of the list. */
+ * A tensor that is written may not overlap another of the list, or d_norm. */
 void launchGradClip(const GradTensor* tensors, int count, float maxNorm, int nonFinite, const float* d_norm,
                     hipStream_t stream);
 
-/* Both in one call: *d_norm is the norm before clipping. */
+/* Both in one call: *d_norm, which is no part of any tensor, is the norm before
+ * clipping. */
 void launchGradNormClip(const GradTensor* tensors, int count, int norm, float gradScale, float maxNorm, int nonFinite,
                         float* d_norm, hipStream_t stream);
 
