@@ -1,6 +1,6 @@
 """A field over 3D points whose capacity is a mixture of experts, trained with the block's operators.
 
-    python examples/expert_field.py [--steps 200] [--tokens 8192] [--max-norm 1.0]
+    python examples/expert_field.py [--steps 200] [--tokens 8192] [--max-norm 1.0] [--answer-bits 4]
 
 Points are embedded as sines and cosines (D features); one residual block
 
@@ -11,7 +11,7 @@ and a linear map to colours follow; the loss is the mean squared error against a
 products run in 8 bits with a scale for each block of 128, forward and backward; master weights and Adam are fp32.
 Everything but the embedding, the colour map and Adam goes through the launchers of include/experts_abi.h; with a largest
 norm the gradients are clipped by those of include/grad_abi.h.  A few points at a time are answered by the whole layer in
-one call (ExpertBlock.answer).
+one call (ExpertBlock.answer), from weights in 8 bits or in 4, which the run ends with.
 """
 from __future__ import annotations
 
@@ -63,6 +63,18 @@ def product(a, a_scales, b, b_scales, out, m, n, k, experts, grouping, scale_row
                            outType=P.DATA_F32 if out.dtype == torch.float32 else TYPE, outStride=out.stride(-2))
     P.launch("launchFp8Product", C.byref(o), a, a_scales, b, b_scales, offsets, out, stream())
     return out
+
+
+class Fp4:
+    """All experts' matrices [experts, rows, cols] as e2m1 values with a scale for each 32 columns."""
+
+    def __init__(self, w):
+        E, rows, cols = w.shape
+        self.q = empty(E, rows, P.fp4_pitch(cols), dtype=torch.uint8)
+        self.s = empty(E, rows, P.fp4_scale_pitch(cols), dtype=torch.uint8)
+        o = P.Fp4QuantOption(rows=rows, cols=cols, batch=E, scaleRule=P.FP4_SCALE_COVER, srcType=CODES[w.dtype], slotsPerRow=0,
+                             srcRows=rows, srcStride=w.stride(1), srcBatchStride=w.stride(0))
+        P.launch("launchFp4Quantize", C.byref(o), w, None, self.q, self.s, stream())
 
 
 class ExpertBlock:
@@ -117,10 +129,13 @@ class ExpertBlock:
         P.launch("launchNormGateResidual", C.byref(o), x, self.f, self.gate, p["norm_out"], None, None, None, y, None, T, stream())
         return y
 
-    def prepare(self):
-        """The weights' 8-bit form for answer(), once after training."""
-        self.w1.quantize(self.p["w1"])
-        self.w2.quantize(self.p["w2"])
+    def prepare(self, bits=8):
+        """The weights' form for answer(), in 8 bits or 4, once after training."""
+        self.bits = bits
+        if bits == 4:
+            self.served = Fp4(self.p["w1"]), Fp4(self.p["w2"])
+        else:
+            self.served = self.w1.quantize(self.p["w1"]), self.w2.quantize(self.p["w2"])
 
     def answer(self, x):
         """forward() for up to 64 rows: the layer of experts in one call, neither tokens nor hidden activations quantised."""
@@ -129,8 +144,10 @@ class ExpertBlock:
         o = self.norm_option(P.NORM_NONE, P.NORM_RMS, 0, 1.0)
         P.launch("launchNormGateResidual", C.byref(o), x, None, None, None, None, p["norm_in"], None, None, h, T, stream())
         o = P.ExpertLayerOption(route=self.route_option(), dim=D, hidden=self.hidden, activation=P.EXPERT_RELU, gated=0,
-                                weightFormat=P.EXPERT_FP8, scaleRows=128, dataType=TYPE, routerType=P.DATA_F32, strideX=D, strideOut=D)
-        P.launch("launchExpertLayer", C.byref(o), h, p["router"], None, self.w1.q, self.w1.s, self.w2.q, self.w2.s, f, T, stream())
+                                weightFormat=P.EXPERT_FP4 if self.bits == 4 else P.EXPERT_FP8, scaleRows=1 if self.bits == 4 else 128,
+                                dataType=TYPE, routerType=P.DATA_F32, strideX=D, strideOut=D)
+        w1, w2 = self.served
+        P.launch("launchExpertLayer", C.byref(o), h, p["router"], None, w1.q, w1.s, w2.q, w2.s, f, T, stream())
         o = self.norm_option(P.NORM_RMS, P.NORM_NONE, T, 1.0)
         P.launch("launchNormGateResidual", C.byref(o), x, f, p["gate"].to(DT), p["norm_out"], None, None, None, y, None, T, stream())
         return y
@@ -194,8 +211,14 @@ def clip(grads, max_norm, loss_scale):
     return norm
 
 
-def train(steps=200, tokens=8192, dim=256, hidden=512, experts=8, topk=2, lr=2e-3, loss_scale=1024.0, verbose=True, max_norm=None):
-    """The losses of the steps."""
+def colours(block, head, points):
+    """The field's colours at up to 64 points, by the block's answers."""
+    return block.answer(embed(points, block.dim).to(DT)).float() @ head.t()
+
+
+def train(steps=200, tokens=8192, dim=256, hidden=512, experts=8, topk=2, lr=2e-3, loss_scale=1024.0, verbose=True, max_norm=None,
+          answer_bits=None):
+    """The losses of the steps; with answer_bits also of 64 points that the trained block answers with weights of so many."""
     block = ExpertBlock(dim, hidden, experts, topk)
     g = torch.Generator(device="cuda")
     g.manual_seed(1)
@@ -219,6 +242,12 @@ def train(steps=200, tokens=8192, dim=256, hidden=512, experts=8, topk=2, lr=2e-
             t.addcdiv_(m[n] / (1 - 0.9 ** step), (v[n] / (1 - 0.99 ** step)).sqrt() + 1e-8, value=-lr)
         if verbose and (step == 1 or step % 50 == 0):
             print(f"step {step} loss {float(losses[-1]):.5f}", flush=True)
+    if answer_bits:
+        block.prepare(answer_bits)
+        points = torch.rand(P.EXPERT_LAYER_TOKENS, 3, generator=g, device="cuda")
+        losses.append((colours(block, params["head"], points) - scene(points)).square().mean())
+        if verbose:
+            print(f"{len(points)} points answered with weights of {answer_bits} bits: loss {float(losses[-1]):.5f}", flush=True)
     return [float(x) for x in losses]
 
 
@@ -227,5 +256,6 @@ if __name__ == "__main__":
     ap.add_argument("--steps", type=int, default=200)
     ap.add_argument("--tokens", type=int, default=8192)
     ap.add_argument("--max-norm", type=float, default=None)
+    ap.add_argument("--answer-bits", type=int, choices=[4, 8], default=8)
     a = ap.parse_args()
-    train(a.steps, a.tokens, max_norm=a.max_norm)
+    train(a.steps, a.tokens, max_norm=a.max_norm, answer_bits=a.answer_bits)

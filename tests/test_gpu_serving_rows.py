@@ -64,3 +64,30 @@ def test_answers(D, H, E, k, T):
     w1 = torch.stack([R.values(q, s, D, 128) for q, s in zip(block.w1.q, block.w1.s)])
     w2 = torch.stack([R.values(q, s, H, 128) for q, s in zip(block.w2.q, block.w2.s)])
     check_answers(block, x, block.answer(x), w1, w2)
+
+
+@pytest.mark.parametrize("T", [1, 33])
+def test_answers_from_four_bits(T):
+    D, H, E, k = 192, 320, 5, 2
+    M, block, g = trained(D, H, E, k, T)
+    block.prepare(4)
+    (w1, w2), x = block.served, R.randn(g, T, D).half()
+    v1 = torch.stack([S.values4(q, s, D) for q, s in zip(w1.q, w1.s)])
+    v2 = torch.stack([S.values4(q, s, H) for q, s in zip(w2.q, w2.s)])
+    for w, v in ((block.p["w1"], v1), (block.p["w2"], v2)):  # as quantised to 64 bits
+        assert all(torch.equal(S.quantize4(a, 1)[0] * torch.exp2(S.quantize4(a, 1)[1].double() - 127).repeat_interleave(32, 1)
+                               [:, :a.shape[1]], b) for a, b in zip(w, v))
+    y = block.answer(x)
+    check_answers(block, x, y, v1, v2)
+    points = torch.rand(T, 3, generator=g, device="cuda")
+    head = R.randn(g, 3, D)
+    assert torch.equal(M.colours(block, head, points), block.answer(M.embed(points, D).half()).float() @ head.t())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_training_that_ends_with_answers(bits):
+    from test_gpu_expert_field import example
+    kind = dict(steps=2, tokens=256, dim=64, hidden=128, experts=4, verbose=False)
+    M = example()
+    plain, losses = M.train(**kind), M.train(answer_bits=bits, **kind)
+    assert losses[:-1] == plain and len(losses) == 3 and math.isfinite(losses[-1])
