@@ -174,7 +174,9 @@ void launchFp8Product(const Fp8ProductOption* opt, const uint8_t* d_a, const uin
  * power of two 2^(byte - 127): [rows x scale pitch], scale pitch = blocks of the
  * filled row, a multiple of 4.  Both start at a multiple of 16 (bytes) and 4
  * (scales).  A scale is at least 2^-126; byte 255 is a block of NaN, which any
- * infinity or NaN in it makes of a block.
+ * infinity or NaN in it makes of a block.  These are the values and scales of the
+ * OCP microscaling formats but for scale byte 0 (2^-127 there), which no matrix given
+ * to the launchers below may have.
  */
 
 /* 2^(floor(log2 max) - 2) of the block's largest magnitude (the rule of the OCP
@@ -272,7 +274,8 @@ typedef struct ExpertLayerOption {
  *   a(h) = act(h), or gated act(h[0..H-1]) * h[H..2H-1]
  * for 0..EXPERT_LAYER_TOKENS tokens.  router [E x D] without gaps; W1 [E x (H or
  * 2 H) x D] and W2 [E x D x H] as the quantising launchers write them (scale
- * bytes of EXPERT_FP8 17 to 246).  Neither x nor a is quantised: products of the
+ * bytes of EXPERT_FP8 17 to 246, of EXPERT_FP4 1 to 252 and 255: within these the
+ * weights' values are bf16 numbers).  Neither x nor a is quantised: products of the
  * weights' values and the tokens' are exact, a is held in 17 significant bits (in
  * all 24 of fp32 for fp32 tokens and with EXPERT_HIDDEN_F32), sums are fp32, and out is rounded once; of fp32
  * numbers what lies below 2^-133 is lost.  Infinities count as they do in these

@@ -1,9 +1,13 @@
 /*
- * C-ABI of the gradients' global norm and its clipping on MI355X (gfx950), for the
- * parameters of any of the library's networks: a step runs it between the
- * backward and the Adam launchers (tinymlp_abi.h), whose lossScale is gradScale
- * here.  No counterpart exists in the reference, whose optimizer takes the
- * gradients as they are.
+ * C-ABI of the gradients' global norm and its clipping on MI355X (gfx950), for
+ * gradients that lie in arrays of the caller's: those of the backward launchers of
+ * tinymlp_abi.h and experts_abi.h, and of the TinyMLP and TinyMLPHashGrid classes
+ * (w_grad, b_grad and, where the table's gradient is an array, hashtable_grads).
+ * A step runs it between the backward and the Adam launchers (tinymlp_abi.h), whose
+ * lossScale is gradScale here.  The training steps of InstantNerf and NerfTrainer
+ * do not clip: their binned scatter updates the table as its sums complete, without
+ * an array of its gradients.  No counterpart exists in the reference, whose
+ * optimizer takes the gradients as they are.
  *
  * Conventions are those of experts_abi.h: a trailing stream, errors through
  * tinymlp_last_error() before any device call, scratch by (device, stream), the
