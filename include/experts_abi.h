@@ -275,15 +275,16 @@ typedef struct ExpertLayerOption {
  * for 0..EXPERT_LAYER_TOKENS tokens.  router [E x D] without gaps; W1 [E x (H or
  * 2 H) x D] and W2 [E x D x H] as the quantising launchers write them (scale
  * bytes of EXPERT_FP8 17 to 246, of EXPERT_FP4 1 to 252 and 255: within these the
- * weights' values are bf16 numbers).  Neither x nor a is quantised: products of the
- * weights' values and the tokens' are exact, a is held in 17 significant bits (in
- * all 24 of fp32 for fp32 tokens and with EXPERT_HIDDEN_F32), sums are fp32, in an order that goes by the
- * call's sizes and the number of experts that are taken, and out is rounded once; of
- * fp32 numbers what lies below 2^-133 is lost.  Infinities count as they do in these
- * formulas: a logit that one makes infinite is the largest finite number or makes
- * its expert unavailable, as for launchRouteExperts.  A token none of whose experts
- * is available (NaN among its logits) gets zeros.  out may be x.  A stream's first
- * call cannot be captured into a graph. */
+ * weights' values are bf16 numbers).  Neither x nor a is quantised: products of
+ * the weights' values and the tokens' are exact, a is held in 17 significant bits
+ * (in all 24 of fp32 for fp32 tokens and with EXPERT_HIDDEN_F32), sums are fp32,
+ * in an order that goes by the call's sizes and the number of experts that are
+ * taken, and out is rounded once; of fp32 numbers what lies below 2^-133 is lost.
+ * Infinities count as they do in these formulas: a logit that one makes infinite
+ * is the largest finite number or makes its expert unavailable, as for
+ * launchRouteExperts.  A token none of whose experts is available (NaN among its
+ * logits) gets zeros.  out may be x.  A stream's first call cannot be captured into
+ * a graph. */
 void launchExpertLayer(const ExpertLayerOption* opt, const void* d_x, const void* d_router, const float* d_bias,
                        const uint8_t* d_w1, const uint8_t* d_w1Scales, const uint8_t* d_w2, const uint8_t* d_w2Scales,
                        void* d_out, int numTokens, hipStream_t stream);
